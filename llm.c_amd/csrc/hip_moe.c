@@ -147,6 +147,11 @@ static hipStream_t device_stream(int dev)
 	return s;
 }
 
+void *moe_device_stream(int dev)
+{
+	return device_stream(dev);
+}
+
 static size_t row_bytes(int wtype, size_t n)
 {
 	if (wtype == HIP_MOE_Q4_K || wtype == HIP_MOE_Q6_K)

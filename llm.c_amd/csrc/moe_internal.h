@@ -229,6 +229,8 @@ int moe_err_word(const struct hip_moe_layer *L, const uint32_t **word);
 
 /* Record an error message for hip_moe_last_error (and print it). */
 void moe_set_error(const char *msg);
+/* the library's stream of a device (a hipStream_t), NULL with an error */
+void *moe_device_stream(int dev);
 
 /* Static device scratch of the allocation-free decode entry point
  * (moe_decode.hip): MOE_STATIC_SCRATCH_BYTES per device, looked up and
