@@ -17,11 +17,11 @@
  *
  * Exactness.  Codes are small integers, exact in f16, and stay unscaled in the
  * operands: a key group's scale multiplies its partial scores in fp32, a value
- * row's scale its probability.  A key code q enters as the subnormal q * 2^-18
- * (its bits in place, nothing around them) and its surplus of 8 a channel leaves
- * through the accumulator's start (-8 sum of the query's channels); a value code
- * enters as 16 + q (its bits or'ed into the mantissa of 16.0) less 24, since over
- * many cached rows a surplus would outweigh the sum.  A query row is scaled by a power of two (its largest value into [2^13, 2^14))
+ * row's scale its probability.  A code q enters as the subnormal q * 2^-18 (its
+ * bits in place, nothing around them: a shift and a mask for two).  The keys'
+ * surplus of 8 a channel leaves through the accumulator's start (-8 sum of the
+ * query's channels), the values' by a subtraction, exact as well, since over many
+ * cached rows a surplus would outweigh the sum.  A query row is scaled by a power of two (its largest value into [2^13, 2^14))
  * and, from fp32, split into two f16 parts of together 22 bits; f16 and bf16
  * queries are exact in one.  The probability times the value scale is scaled
  * by a power of two that keeps the largest below 2^15, and split in two as
@@ -40,28 +40,38 @@ __device__ static inline half8_t as_half8(u32 a, u32 b, u32 c, u32 d)
 	return __builtin_bit_cast(half8_t, v);
 }
 
-/* a word's codes, in their order, as f16 with the mantissa's upper four bits:
- * code * 2^-18, or with base = 0x4c004c00 16 + code */
-__device__ static inline half8_t kv_word(u32 w, u32 base)
+/* a word's codes, in their order, as f16 with the mantissa's upper four bits
+ * and nothing else: code * 2^-18, a subnormal */
+__device__ static inline half8_t kv_word(u32 w)
 {
 	const u32 m = 0x03c003c0u; /* the codes whose lowest bits are 6 and 22 */
-	return as_half8((w << 4 & m) | base, (w & m) | base, (w >> 4 & m) | base,
-			(kv_rotr(w, 8) & m) | base);
+	return as_half8(w << 4 & m, w & m, w >> 4 & m, kv_rotr(w, 8) & m);
 }
 
 #define KV_CODE_STEP (1.0f / (1 << 18))
 
-/* the largest over the four lanes that share a query row */
+/* the lane's value and those of the three others that share its query row, put
+ * together by fn.  The swaps exchange the odd rows of 16 lanes (the upper 32)
+ * of the first register with the even ones (the lower) of the second, so of a
+ * value and its copy both then hold both.  (In assembly: the builtin hands out its
+ * first result twice.  The s_nop are the two wait states after a VALU write.) */
+template <class Fn> __device__ static inline float over_row(float v, Fn fn)
+{
+	float w = v;
+	asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+	w = v = fn(v, w);
+	asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+	return fn(v, w);
+}
+
 __device__ static inline float row_max(float v)
 {
-	v = fmaxf(v, __shfl_xor(v, 16, WAVE));
-	return fmaxf(v, __shfl_xor(v, 32, WAVE));
+	return over_row(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 __device__ static inline float row_sum(float v)
 {
-	v += __shfl_xor(v, 16, WAVE);
-	return v + __shfl_xor(v, 32, WAVE);
+	return over_row(v, [](float a, float b) { return a + b; });
 }
 
 /* 2^n, n within -126 .. 127 */
@@ -70,19 +80,18 @@ __device__ static inline float pow2(int n)
 	return __builtin_bit_cast(float, (u32)(n + 127) << 23);
 }
 
-/* the exponent e of v = m 2^e, 0.5 <= m < 1 (finite, not 0) */
-__device__ static inline int exponent(float v)
+/* 2^(x - ref), 0 for a maximum (x or ref) that nothing was seen for */
+__device__ static inline float weight(float x, float ref)
 {
-	return __builtin_amdgcn_frexp_expf(v);
+	return __builtin_amdgcn_exp2f(x - (ref == -__builtin_inff() ? 0.0f : ref));
 }
 
-/* the rows that a tile of query rows sees: the lane's row, and all of them */
+/* the cached rows that the lane's query row sees, and the tile's rows */
 struct kv_span {
-	int lo, hi;         /* cached rows of the lane's query row */
-	int first, last;    /* of all rows of the tile */
-	int inner0, inner1; /* seen by every row of the tile */
-	size_t at;          /* the row's index among the batch's rows, and its head */
-	int head;
+	int lo, hi;         /* of the lane's query row */
+	int first, last;    /* of some row of the tile */
+	int inner0, inner1; /* of every row of the tile */
+	int row, head;      /* the row among the batch's rows, and its head */
 	bool valid;
 };
 
@@ -91,14 +100,13 @@ __device__ static inline kv_span kv_rows_of(const kv_seq &sq, int tile, int G, i
 {
 	kv_span r;
 	const int base = sq.len - sq.n, all = sq.n * G;
-	const int mine = tile * KV_ROWS + lane % 16;
-	const int i0 = tile * KV_ROWS / G, i1 = (min(tile * KV_ROWS + KV_ROWS, all) - 1) / G;
-	const int i = min(mine, all - 1) / G;
+	const int mine = tile * KV_ROWS + lane % 16, kept = min(mine, all - 1), i = kept / G;
+	const int i0 = __builtin_amdgcn_readlane(i, 0), i1 = __builtin_amdgcn_readlane(i, 15);
 	r.valid = mine < all;
 	r.hi = base + i + 1;
 	r.lo = window ? max(0, r.hi - window) : 0;
-	r.at = sq.row + i;
-	r.head = kv_head * G + min(mine, all - 1) % G;
+	r.row = sq.row + i;
+	r.head = kv_head * G + kept - i * G;
 	r.last = base + i1 + 1;
 	r.first = window ? max(0, base + i0 + 1 - window) : 0;
 	r.inner0 = window ? max(0, r.last - window) : 0;
@@ -106,32 +114,196 @@ __device__ static inline kv_span kv_rows_of(const kv_seq &sq, int tile, int G, i
 	return r;
 }
 
+/* a tile of the cache in registers: the lane's share, as the layout has it */
+template <int D> struct kv_keys {
+	typedef kv_tile<D> L;
+	u32 w[2][L::G];        /* rows lane % 16 of each half */
+	_Float16 d[2][4][L::G]; /* scales of rows 4 (lane / 16) + j of each half */
+	__device__ inline void load(const uint8_t *tile, int lane)
+	{
+#pragma unroll
+		for (int h = 0; h < 2; h++) {
+			typedef uint32_t words __attribute__((ext_vector_type(L::P)));
+#pragma unroll
+			for (int g = 0; g < L::G; g += L::P) {
+				const words x = ((const words *)tile)[(h * (L::G / L::P) + g / L::P) * 64 + lane];
+#pragma unroll
+				for (int u = 0; u < L::P; u++)
+					w[h][g + u] = x[u];
+			}
+			const half8_t *s = (const half8_t *)(tile + L::K_SCALES) + (16 * h + 4 * (lane / 16)) * L::G / 8;
+#pragma unroll
+			for (int u = 0; u < L::G / 2; u++) {
+				const half8_t x = s[u];
+#pragma unroll
+				for (int j = 0; j < 8; j++)
+					d[h][(8 * u + j) / L::G][(8 * u + j) % L::G] = x[j];
+			}
+		}
+	}
+};
+
+template <int D> struct kv_values {
+	typedef kv_tile<D> L;
+	u32 w[D / 16]; /* channels 16 c + lane % 16 */
+	__device__ inline void load(const uint8_t *tile, int lane)
+	{
+		const u32x4 *p = (const u32x4 *)(tile + L::V_CODES) + lane;
+#pragma unroll
+		for (int c = 0; c < D / 64; c++) {
+			const u32x4 x = p[64 * c];
+#pragma unroll
+			for (int u = 0; u < 4; u++)
+				w[4 * c + u] = x[u];
+		}
+	}
+};
+
+/* value scales of the lane's eight rows */
+__device__ static inline half8_t kv_value_scales(const uint8_t *scales, int lane)
+{
+	const half4_t *p = (const half4_t *)scales + lane / 16;
+	const half4_t a = p[0], b = p[4];
+	return half8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+/* a query row in f16 parts, and what belongs to it */
+template <int D, int QP> struct kv_query {
+	half8_t f[QP][D / 32];
+	float start[D / 32]; /* of the accumulators: -8 steps times the group's sum */
+	float rs;            /* a score times this is a logit in powers of two; > 0 */
+	template <int TY> __device__ inline void load(const typename kv_type<TY>::t *x, float scale, int part)
+	{
+		float v[D / 32][8], top = 0.0f;
+#pragma unroll
+		for (int g = 0; g < D / 32; g++) {
+			const kv_vec<TY, 8> w = *(const kv_vec<TY, 8> *)(x + 32 * g + 8 * part);
+#pragma unroll
+			for (int j = 0; j < 8; j++) {
+				v[g][j] = kv_type<TY>::get(w.v[j]);
+				top = fmaxf(top, fabsf(v[g][j]));
+			}
+		}
+		top = row_max(top);
+		int e = 14 - __builtin_amdgcn_frexp_expf(top);
+		e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 126) : 0;
+		/* a negative scale turns the query around, 0 makes it 0 */
+		const float sc = scale > 0.0f ? pow2(e) : scale < 0.0f ? -pow2(e) : 0.0f;
+		rs = (scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / KV_CODE_STEP) * pow2(-e);
+#pragma unroll
+		for (int g = 0; g < D / 32; g++) {
+			float sum = 0.0f;
+#pragma unroll
+			for (int j = 0; j < 8; j++) {
+				const float y = v[g][j] * sc;
+				const _Float16 hi = (_Float16)y;
+				f[0][g][j] = hi;
+				sum += (float)hi;
+				if (QP > 1) {
+					const _Float16 lo = (_Float16)(y - (float)hi);
+					f[QP - 1][g][j] = lo;
+					sum += (float)lo;
+				}
+			}
+			start[g] = -8.0f * KV_CODE_STEP * row_sum(sum);
+		}
+	}
+};
+
+/* scores of 32 cached rows: 4 part + j of each half */
+template <int D, int QP>
+__device__ static inline void kv_scores(const kv_keys<D> &k, const kv_query<D, QP> &q, float *x)
+{
+#pragma unroll
+	for (int h = 0; h < 2; h++) {
+#pragma unroll
+		for (int g = 0; g < D / 32; g++) {
+			floatx4 acc = (floatx4)q.start[g];
+			const half8_t kf = kv_word(k.w[h][g]);
+#pragma unroll
+			for (int p = 0; p < QP; p++)
+				acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q.f[p][g], acc, 0, 0, 0);
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+				x[4 * h + j] = g ? fmaf((float)k.d[h][j][g], acc[j], x[4 * h + j])
+						 : (float)k.d[h][j][g] * acc[j];
+		}
+	}
+}
+
 /*
- * One workgroup: a tile of query rows over `chunk` tiles of the cache, dealt to
- * its four waves one by one; the waves' results meet in LDS.  With more than
- * one workgroup along the cache each leaves its maximum, sum and unnormalised
- * output in ws for k_kv_merge.
+ * The running softmax of a query row.  ref is its reference in powers of two: a
+ * probability is 2^(logit - ref), and ref is the largest logit so far plus the
+ * exponent of the value scales that came with it, less 15, so that probability
+ * times value scale stays below 2^15 (f16's largest is 2^16) and mostly far
+ * above f16's smallest; sums and outputs carry the same factor, which the
+ * division at the end takes out.
  */
+struct kv_soft {
+	float ref, sum;
+};
+
+/* probabilities times value scales of 32 cached rows, in f16 parts; returns what
+ * the output so far is multiplied by */
+template <int PP>
+__device__ static inline float kv_softmax(kv_soft &s, const float *x, const half8_t dv, float rs,
+					  half8_t (&pf)[PP])
+{
+	float top = x[0], big = fabsf((float)dv[0]);
+#pragma unroll
+	for (int j = 1; j < 8; j++) {
+		top = fmaxf(top, x[j]);
+		big = fmaxf(big, fabsf((float)dv[j]));
+	}
+	/* scales of nothing but zeros: exponent 0 */
+	const float next = fmaxf(s.ref, row_max(fmaf(top, rs, (float)(__builtin_amdgcn_frexp_expf(big) - 15))));
+	const float back = weight(s.ref, next);
+	s.ref = next;
+	const float ref = next == -__builtin_inff() ? 0.0f : next;
+	float sum = 0.0f;
+#pragma unroll
+	for (int j = 0; j < 8; j++) {
+		const float p = __builtin_amdgcn_exp2f(fmaf(x[j], rs, -ref));
+		sum += p;
+		const float w = fmaf((float)dv[j], p, 0.0f); /* fma: takes the f16 as it is */
+		const _Float16 hi = (_Float16)w;
+		pf[0][j] = hi;
+		if (PP > 1)
+			pf[PP - 1][j] = (_Float16)fmaf((float)hi, -1.0f, w);
+	}
+	s.sum = s.sum * back + sum;
+	return back;
+}
+
+/*
+ * Few query rows: one workgroup takes a tile of them over `chunk` tiles of the
+ * cache, dealt to its four waves one by one; the waves' results meet in LDS.
+ * With more than one workgroup along the cache each leaves its reference, sum
+ * and unnormalised output in ws for k_kv_merge.  A wave loads a tile's keys
+ * while it still works on the values of the tile before, and the values while
+ * it works on the keys.
+ */
+/* two waves a SIMD, so that nothing is kept in accumulation registers and moved;
+ * heads of 256 do not fit */
 template <int D, int TY>
-__global__ __launch_bounds__(KV_NT) void k_kv_attn(
+__global__ __launch_bounds__(KV_NT) __attribute__((amdgpu_waves_per_eu(D < 256 ? 2 : 1)))
+void k_kv_attn(
 	kv_args a, const typename kv_type<TY>::t *q, size_t q_stride, int G,
 	typename kv_type<TY>::t *out, size_t out_stride, float scale, int window, float *ws,
-	int row_tiles, int chunk, int splits)
+	int row_tiles, int chunk)
 {
 	typedef kv_type<TY> T;
 	typedef kv_tile<D> L;
 	constexpr int QP = TY == HIP_KV_F32 ? 2 : 1, PP = TY == HIP_KV_BF16 ? 1 : 2;
 	constexpr int CT = D / 16; /* channel tiles of O^T */
 	__shared__ float s_o[KV_WAVES][KV_ROWS][D + 4];
-	__shared__ float s_m[KV_WAVES][KV_ROWS], s_l[KV_WAVES][KV_ROWS];
+	__shared__ float s_ref[KV_WAVES][KV_ROWS], s_sum[KV_WAVES][KV_ROWS];
+	__shared__ int s_row[KV_ROWS], s_head[KV_ROWS];
 
-	const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, part = lane / 16;
-	int b = blockIdx.x;
-	const int kv_head = b % a.kv_heads;
-	b /= a.kv_heads;
-	const int split = b % splits;
-	b /= splits;
-	const int rt = b % row_tiles, s = b / row_tiles;
+	const int lane = threadIdx.x % WAVE, part = lane / 16;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+	const int kv_head = blockIdx.x % a.kv_heads, rt = blockIdx.x / a.kv_heads;
+	const int split = blockIdx.y, splits = gridDim.y, s = blockIdx.z;
 	const kv_seq sq = kv_sequence(a, s);
 	if (rt * KV_ROWS >= sq.n * G)
 		return;
@@ -141,136 +313,68 @@ __global__ __launch_bounds__(KV_NT) void k_kv_attn(
 	if (split > 0 && t0 >= t1)
 		return;
 
-	/* the query row: its parts, and the sums that start the accumulators */
-	half8_t qf[QP][L::G];
-	float qsum[L::G], rs;
-	{
-		float v[L::G][8], top = 0.0f;
-		const typename T::t *x = q + r.at * q_stride + (size_t)r.head * D;
-#pragma unroll
-		for (int g = 0; g < L::G; g++) {
-			const kv_vec<TY, 8> w = *(const kv_vec<TY, 8> *)(x + 32 * g + 8 * part);
-#pragma unroll
-			for (int j = 0; j < 8; j++) {
-				v[g][j] = T::get(w.v[j]);
-				top = fmaxf(top, fabsf(v[g][j]));
-			}
+	/* the wave's tiles t0 + wave, + 4, ..; a lane holds the page of one of the
+	 * next 64.  A page outside the pool: its first tile, with every row hidden */
+	const int shift = a.page_shift - 5, n = a.pages ? (t1 - t0 - wave + KV_WAVES - 1) / KV_WAVES : 0;
+	int page = -1;
+	bool lost = false;
+	const auto tile_of = [&](int i) -> const uint8_t * {
+		const int t = t0 + wave + i * KV_WAVES;
+		if (i % WAVE == 0) {
+			const int tl = t + lane * KV_WAVES;
+			page = tl < t1 ? a.table[s * a.table_stride + (tl >> shift)] : -1;
 		}
-		top = row_max(top);
-		int e = 14 - exponent(top);
-		e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 126) : 0;
-		const float sc = pow2(e);
-		rs = scale * (1.44269504088896341f / KV_CODE_STEP) * pow2(-e);
-#pragma unroll
-		for (int g = 0; g < L::G; g++) {
-			float sum = 0.0f;
-#pragma unroll
-			for (int j = 0; j < 8; j++) {
-				const float y = v[g][j] * sc;
-				const _Float16 hi = (_Float16)y;
-				qf[0][g][j] = hi;
-				sum += (float)hi;
-				if (QP > 1) {
-					const _Float16 lo = (_Float16)(y - (float)hi);
-					qf[QP - 1][g][j] = lo;
-					sum += (float)lo;
-				}
-			}
-			qsum[g] = -8.0f * KV_CODE_STEP * row_sum(sum);
-		}
+		const int id = __builtin_amdgcn_readlane(page, i % WAVE);
+		lost = (u32)id >= (u32)a.pages;
+		const size_t at = lost ? 0 : ((((size_t)id * a.kv_heads + kv_head) << shift) + (t & ((1 << shift) - 1)));
+		return a.pool + at * L::BYTES;
+	};
+	kv_keys<D> k;
+	kv_values<D> v;
+	half8_t dv;
+	if (n > 0) {
+		const uint8_t *tile = tile_of(0);
+		k.load(tile, lane);
+		dv = kv_value_scales(tile + L::V_SCALES, lane);
+		v.load(tile, lane);
+	} else if (!a.pages && lane == 0) {
+		kv_error(a, HIP_KV_ERR_PAGE);
+	}
+	kv_query<D, QP> qr;
+	qr.template load<TY>(q + (size_t)r.row * q_stride + (size_t)r.head * D, scale, part);
+	if (threadIdx.x < KV_ROWS) {
+		s_row[threadIdx.x] = r.valid ? r.row : -1;
+		s_head[threadIdx.x] = r.hi > r.lo ? r.head : ~r.head;
 	}
 
 	floatx4 o[CT];
 #pragma unroll
 	for (int c = 0; c < CT; c++)
 		o[c] = (floatx4)0.0f;
-	float m = -__builtin_inff(), l = 0.0f;
-	int pe = -1000; /* probabilities are multiplied by 2^pe; unset */
+	kv_soft soft = {-__builtin_inff(), 0.0f};
 
-	for (int t = t0 + wave; t < t1; t += KV_WAVES) {
-		const uint8_t *tile = kv_tile_at<D>(a, s, kv_head, t);
-		if (!tile) {
-			if (lane == 0)
-				kv_error(a, HIP_KV_ERR_PAGE);
-			continue;
-		}
-		float x[8], dv[8];
-#pragma unroll
-		for (int h = 0; h < 2; h++) {
-			u32 kw[L::G];
-			_Float16 kd[4][L::G];
-#pragma unroll
-			for (int g = 0; g < L::G; g++)
-				kw[g] = ((const u32 *)tile)[((h * (L::G / L::P) + g / L::P) * 64 + lane) * L::P +
-							     g % L::P];
-#pragma unroll
-			for (int j = 0; j < 4; j++) {
-				const int row = 16 * h + 4 * part + j;
-				dv[4 * h + j] = (float)((const _Float16 *)(tile + L::V_SCALES))[row];
-#pragma unroll
-				for (int g = 0; g < L::G; g++)
-					kd[j][g] = ((const _Float16 *)(tile + L::K_SCALES))[row * L::G + g];
-				x[4 * h + j] = 0.0f;
-			}
-#pragma unroll
-			for (int g = 0; g < L::G; g++) {
-				floatx4 acc = (floatx4)qsum[g];
-				const half8_t kf = kv_word(kw[g], 0);
-#pragma unroll
-				for (int p = 0; p < QP; p++)
-					acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[p][g], acc, 0, 0, 0);
-#pragma unroll
-				for (int j = 0; j < 4; j++)
-					x[4 * h + j] = fmaf((float)kd[j][g], acc[j], x[4 * h + j]);
-			}
-		}
-		const bool edge = t * KV_TILE < r.inner0 || (t + 1) * KV_TILE > r.inner1;
-		float top = -__builtin_inff(), big = 0.0f;
-#pragma unroll
-		for (int j = 0; j < 8; j++) {
-			x[j] *= rs;
-			if (edge) {
-				const int at = t * KV_TILE + 16 * (j / 4) + 4 * part + j % 4;
-				if (at < r.lo || at >= r.hi)
-					x[j] = -__builtin_inff();
-				if (at < r.first || at >= r.last)
-					dv[j] = 0.0f;
-			}
-			top = fmaxf(top, x[j]);
-			big = fmaxf(big, fabsf(dv[j]));
-		}
-		top = fmaxf(m, row_max(top));
-		const float base = top == -__builtin_inff() ? 0.0f : top;
-		const float alpha = __builtin_amdgcn_exp2f(m - base);
-		float back = alpha;
-		m = top;
-		/* the probabilities' scale: the same in all lanes, since the value
-		 * scales are; lowered when a larger one comes */
-		big = row_max(big);
-		const int e = big > 0.0f ? 15 - exponent(big) : 100;
-		if (pe == -1000) {
-			pe = min(e, 100) - 1;
-		} else if (e < pe) {
-			back *= pow2(max(e - 1 - pe, -126));
-			pe = e - 1;
-		}
-		const float ps = pow2(pe);
-		float sum = 0.0f, w[8];
-#pragma unroll
-		for (int j = 0; j < 8; j++) {
-			const float p = __builtin_amdgcn_exp2f(x[j] - base);
-			sum += p;
-			w[j] = edge && p == 0.0f ? 0.0f : p * (dv[j] * ps);
-		}
-		l = l * alpha + sum;
+	for (int i = 0; i < n; i++) {
+		const int t = t0 + wave + i * KV_WAVES;
+		const bool hidden = lost, more = i + 1 < n;
+		const uint8_t *next = more ? tile_of(i + 1) : NULL;
+		float x[8];
 		half8_t pf[PP];
+		kv_scores<D, QP>(k, qr, x);
+		if (more)
+			k.load(next, lane);
+		if (hidden || t * KV_TILE < r.inner0 || (t + 1) * KV_TILE > r.inner1) {
+			const int lo = hidden ? 0x7fffffff : r.lo;
 #pragma unroll
-		for (int j = 0; j < 8; j++) {
-			const _Float16 hi = (_Float16)w[j];
-			pf[0][j] = hi;
-			if (PP > 1)
-				pf[PP - 1][j] = (_Float16)(w[j] - (float)hi);
+			for (int j = 0; j < 8; j++) {
+				const int at = t * KV_TILE + 16 * (j / 4) + 4 * part + j % 4;
+				const bool hide = at < lo || at >= r.hi;
+				x[j] = hide ? -__builtin_inff() : x[j];
+				dv[j] = hide ? (_Float16)0.0f : dv[j];
+			}
+			if (hidden && lane == 0)
+				kv_error(a, HIP_KV_ERR_PAGE);
 		}
+		const float back = kv_softmax<PP>(soft, x, dv, qr.rs, pf);
 		if (__ballot(back != 1.0f)) {
 #pragma unroll
 			for (int c = 0; c < CT; c++)
@@ -278,110 +382,130 @@ __global__ __launch_bounds__(KV_NT) void k_kv_attn(
 		}
 #pragma unroll
 		for (int c = 0; c < CT; c++) {
-			const u32 vw = ((const u32 *)(tile + L::V_CODES))[(c / 4 * 64 + lane) * 4 + c % 4];
-			const half8_t vf = kv_word(vw, 0x4c004c00u) - (half8_t)(_Float16)24.0f;
+			const half8_t vf = kv_word(v.w[c]) - (half8_t)(_Float16)(8.0f * KV_CODE_STEP);
 #pragma unroll
 			for (int p = 0; p < PP; p++)
 				o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[p], o[c], 0, 0, 0);
 		}
+		if (more) {
+			dv = kv_value_scales(next + L::V_SCALES, lane);
+			v.load(next, lane);
+		}
 	}
 
-	/* the waves' results: to one maximum, then added in wave order */
-	l = row_sum(l);
+	/* the waves' results: to one reference, then added in wave order */
+	const float sum = KV_CODE_STEP * row_sum(soft.sum); /* the outputs' own factor */
 	if (part == 0) {
-		s_m[wave][lane] = m;
-		s_l[wave][lane] = l;
+		s_ref[wave][lane] = soft.ref;
+		s_sum[wave][lane] = sum;
 	}
 	__syncthreads();
-	float top = s_m[0][lane % 16];
+	float ref = s_ref[0][lane % 16];
 #pragma unroll
 	for (int w = 1; w < KV_WAVES; w++)
-		top = fmaxf(top, s_m[w][lane % 16]);
-	const float back = top == -__builtin_inff() ? 0.0f : top;
-	float factor = pe == -1000 ? 0.0f : __builtin_amdgcn_exp2f(m - back) * pow2(-pe);
+		ref = fmaxf(ref, s_ref[w][lane % 16]);
+	const float factor = weight(soft.ref, ref);
+	if (r.valid) {
 #pragma unroll
-	for (int c = 0; c < CT; c++)
-#pragma unroll
-		for (int j = 0; j < 4; j++)
-			s_o[wave][lane % 16][16 * c + 4 * part + j] = pe == -1000 ? 0.0f : o[c][j] * factor;
+		for (int c = 0; c < CT; c++)
+			*(floatx4 *)&s_o[wave][lane % 16][16 * c + 4 * part] = o[c] * factor;
+	}
 	__syncthreads();
 	const size_t slot = ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
+	float *to = ws + slot * KV_ROWS * (D + 2);
 	for (int at = threadIdx.x; at < KV_ROWS * D / 4; at += KV_NT) {
-		const int row = at / (D / 4), c = at % (D / 4) * 4;
-		const kv_span z = kv_rows_of(sq, rt, G, kv_head, window, row);
-		if (!z.valid)
-			continue;
-		float high = s_m[0][row], den = 0.0f, y[4] = {};
+		const int i = at / (D / 4), c = at % (D / 4) * 4, row = s_row[i];
+		if (row < 0)
+			break; /* the rows behind are not there either */
+		float high = s_ref[0][i], den = 0.0f;
 #pragma unroll
 		for (int w = 1; w < KV_WAVES; w++)
-			high = fmaxf(high, s_m[w][row]);
-		const float zero = high == -__builtin_inff() ? 0.0f : high;
+			high = fmaxf(high, s_ref[w][i]);
+		floatx4 y = (floatx4)0.0f;
 #pragma unroll
 		for (int w = 0; w < KV_WAVES; w++) {
-			den += s_l[w][row] * __builtin_amdgcn_exp2f(s_m[w][row] - zero);
-#pragma unroll
-			for (int u = 0; u < 4; u++)
-				y[u] += s_o[w][row][c + u];
+			den += s_sum[w][i] * weight(s_ref[w][i], high);
+			y += *(const floatx4 *)&s_o[w][i][c];
 		}
 		if (splits == 1) {
-			kv_vec<TY, 4> v;
+			kv_vec<TY, 4> z;
+			const int head = s_head[i];
 #pragma unroll
 			for (int u = 0; u < 4; u++)
-				v.v[u] = T::put(z.hi > z.lo ? y[u] / den : 0.0f);
-			*(kv_vec<TY, 4> *)(out + z.at * out_stride + (size_t)z.head * D + c) = v;
+				z.v[u] = T::put(head >= 0 ? y[u] / den : 0.0f);
+			*(kv_vec<TY, 4> *)(out + row * out_stride + (size_t)(head < 0 ? ~head : head) * D + c) = z;
 			continue;
 		}
-		float *to = ws + slot * KV_ROWS * (D + 2);
-		*(floatx4 *)(to + row * D + c) = floatx4{y[0], y[1], y[2], y[3]};
+		*(floatx4 *)(to + i * D + c) = y;
 		if (c == 0) {
-			to[KV_ROWS * D + 2 * row] = high;
-			to[KV_ROWS * D + 2 * row + 1] = den;
+			to[KV_ROWS * D + 2 * i] = high;
+			to[KV_ROWS * D + 2 * i + 1] = den;
 		}
 	}
 }
 
-/* the workgroups' results of one tile of query rows, added in their order */
+/*
+ * The workgroups' results of one query row: D / 4 threads take its channels,
+ * KV_NT / (D / 4) of them share the workgroups along the cache, and are added
+ * in their order.
+ */
 template <int D, int TY>
 __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename kv_type<TY>::t *out,
 						     size_t out_stride, int window, const float *ws,
 						     int row_tiles, int chunk, int splits)
 {
 	typedef kv_type<TY> T;
-	int b = blockIdx.x;
-	const int kv_head = b % a.kv_heads;
-	b /= a.kv_heads;
-	const int rt = b % row_tiles, s = b / row_tiles;
+	constexpr int CH = D / 4, PARTS = KV_NT / CH;
+	__shared__ floatx4 s_y[PARTS][CH];
+	__shared__ float s_ref[PARTS], s_sum[PARTS];
+	const int kv_head = blockIdx.x % a.kv_heads, mine = blockIdx.x / a.kv_heads, s = blockIdx.y;
 	const kv_seq sq = kv_sequence(a, s);
-	if (rt * KV_ROWS >= sq.n * G)
+	if (mine >= sq.n * G)
 		return;
-	const float *part = ws + ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits *
-					 KV_ROWS * (D + 2);
-	for (int at = threadIdx.x; at < KV_ROWS * D / 4; at += KV_NT) {
-		const int row = at / (D / 4), c = at % (D / 4) * 4;
-		const kv_span z = kv_rows_of(sq, rt, G, kv_head, window, row);
-		if (!z.valid)
-			continue;
-		const int tiles = (max(z.last, 0) + KV_TILE - 1) / KV_TILE - z.first / KV_TILE;
-		const int n = min(splits, max(1, (tiles + chunk - 1) / chunk));
-		float m = -__builtin_inff(), l = 0.0f;
-		floatx4 y = (floatx4)0.0f;
-		for (int i = 0; i < n; i++) {
-			const float *p = part + (size_t)i * KV_ROWS * (D + 2);
-			m = fmaxf(m, p[KV_ROWS * D + 2 * row]);
-		}
-		const float base = m == -__builtin_inff() ? 0.0f : m;
-		for (int i = 0; i < n; i++) {
-			const float *p = part + (size_t)i * KV_ROWS * (D + 2);
-			const float f = __builtin_amdgcn_exp2f(p[KV_ROWS * D + 2 * row] - base);
-			l += p[KV_ROWS * D + 2 * row + 1] * f;
-			y += *(const floatx4 *)(p + row * D + c) * f;
-		}
-		kv_vec<TY, 4> v;
-#pragma unroll
-		for (int u = 0; u < 4; u++)
-			v.v[u] = T::put(z.hi > z.lo ? y[u] / l : 0.0f);
-		*(kv_vec<TY, 4> *)(out + z.at * out_stride + (size_t)z.head * D + c) = v;
+	const int rt = mine / KV_ROWS, i = mine / G, base = sq.len - sq.n;
+	const int i0 = rt * KV_ROWS / G, i1 = (min(rt * KV_ROWS + KV_ROWS, sq.n * G) - 1) / G;
+	const int first = window ? max(0, base + i0 + 1 - window) : 0, last = max(base + i1 + 1, 0);
+	const int tiles = (last + KV_TILE - 1) / KV_TILE - first / KV_TILE;
+	const int n = min(splits, max(1, (tiles + chunk - 1) / chunk));
+	const float *p = ws + (((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits) * KV_ROWS * (D + 2);
+	const int at = mine % KV_ROWS, c = threadIdx.x % CH, part = threadIdx.x / CH;
+	constexpr size_t STEP = KV_ROWS * (D + 2);
+
+	float ref = -__builtin_inff(), sum = 0.0f;
+	for (int u = part; u < n; u += PARTS)
+		ref = fmaxf(ref, p[u * STEP + KV_ROWS * D + 2 * at]);
+	floatx4 y = (floatx4)0.0f;
+	for (int u = part; u < n; u += PARTS) {
+		const float *x = p + u * STEP;
+		const float f = weight(x[KV_ROWS * D + 2 * at], ref);
+		sum += x[KV_ROWS * D + 2 * at + 1] * f;
+		y += *(const floatx4 *)(x + at * D + 4 * c) * f;
 	}
+	s_y[part][c] = y;
+	if (c == 0) {
+		s_ref[part] = ref;
+		s_sum[part] = sum;
+	}
+	__syncthreads();
+	if (part)
+		return;
+#pragma unroll
+	for (int u = 1; u < PARTS; u++)
+		ref = fmaxf(ref, s_ref[u]);
+	sum = 0.0f;
+	y = (floatx4)0.0f;
+#pragma unroll
+	for (int u = 0; u < PARTS; u++) {
+		const float f = weight(s_ref[u], ref);
+		sum += s_sum[u] * f;
+		y += s_y[u][c] * f;
+	}
+	kv_vec<TY, 4> z;
+#pragma unroll
+	for (int u = 0; u < 4; u++)
+		z.v[u] = T::put(base + i >= 0 ? y[u] / sum : 0.0f);
+	*(kv_vec<TY, 4> *)(out + (size_t)(sq.row + i) * out_stride + (size_t)(kv_head * G + mine - i * G) * D +
+			   4 * c) = z;
 }
 
 extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int window, kv_plan *p)
@@ -413,14 +537,15 @@ extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const vo
 			      int window, void *ws, const kv_plan *p, void *stream)
 {
 	const int G = heads / a->kv_heads;
-	const size_t wgs = (size_t)a->nseq * a->kv_heads * p->row_tiles;
+	const dim3 grid((unsigned)(a->kv_heads * p->row_tiles), (unsigned)p->splits, (unsigned)a->nseq);
+	const dim3 rows((unsigned)(a->kv_heads * a->max_rows * G), (unsigned)a->nseq);
 	KV_DISPATCH_HEAD(head_len, D, KV_DISPATCH_TYPE(type, TY, {
 		typedef kv_type<TY>::t t;
-		k_kv_attn<D, TY><<<dim3((unsigned)(wgs * p->splits)), KV_NT, 0, (hipStream_t)stream>>>(
+		k_kv_attn<D, TY><<<grid, KV_NT, 0, (hipStream_t)stream>>>(
 			*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window, (float *)ws,
-			p->row_tiles, p->chunk, p->splits);
+			p->row_tiles, p->chunk);
 		if (p->splits > 1)
-			k_kv_merge<D, TY><<<dim3((unsigned)wgs), KV_NT, 0, (hipStream_t)stream>>>(
+			k_kv_merge<D, TY><<<rows, KV_NT, 0, (hipStream_t)stream>>>(
 				*a, G, (t *)out, out_stride, window, (const float *)ws, p->row_tiles,
 				p->chunk, p->splits);
 	}))
