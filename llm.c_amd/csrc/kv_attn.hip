@@ -290,7 +290,7 @@ __global__ __launch_bounds__(KV_NT) __attribute__((amdgpu_waves_per_eu(D < 256 ?
 void k_kv_attn(
 	kv_args a, const typename kv_type<TY>::t *q, size_t q_stride, int G,
 	typename kv_type<TY>::t *out, size_t out_stride, float scale, int window, float *ws,
-	int row_tiles, int chunk)
+	int row_tiles, int chunk, int nrows)
 {
 	typedef kv_type<TY> T;
 	typedef kv_tile<D> L;
@@ -412,7 +412,7 @@ void k_kv_attn(
 	}
 	__syncthreads();
 	const size_t slot = ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
-	float *to = ws + slot * KV_ROWS * (D + 2);
+	float *to = ws + slot * nrows * (D + 4);
 	for (int at = threadIdx.x; at < KV_ROWS * D / 4; at += KV_NT) {
 		const int i = at / (D / 4), c = at % (D / 4) * 4, row = s_row[i];
 		if (row < 0)
@@ -436,10 +436,10 @@ void k_kv_attn(
 			*(kv_vec<TY, 4> *)(out + row * out_stride + (size_t)(head < 0 ? ~head : head) * D + c) = z;
 			continue;
 		}
-		*(floatx4 *)(to + i * D + c) = y;
+		*(floatx4 *)(to + i * (D + 4) + c) = y;
 		if (c == 0) {
-			to[KV_ROWS * D + 2 * i] = high;
-			to[KV_ROWS * D + 2 * i + 1] = den;
+			to[i * (D + 4) + D] = high;
+			to[i * (D + 4) + D + 1] = den;
 		}
 	}
 }
@@ -452,7 +452,7 @@ void k_kv_attn(
 template <int D, int TY>
 __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename kv_type<TY>::t *out,
 						     size_t out_stride, int window, const float *ws,
-						     int row_tiles, int chunk, int splits)
+						     int row_tiles, int chunk, int splits, int nrows)
 {
 	typedef kv_type<TY> T;
 	constexpr int CH = D / 4, PARTS = KV_NT / CH;
@@ -467,19 +467,20 @@ __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename k
 	const int first = window ? max(0, base + i0 + 1 - window) : 0, last = max(base + i1 + 1, 0);
 	const int tiles = (last + KV_TILE - 1) / KV_TILE - first / KV_TILE;
 	const int n = min(splits, max(1, (tiles + chunk - 1) / chunk));
-	const float *p = ws + (((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits) * KV_ROWS * (D + 2);
-	const int at = mine % KV_ROWS, c = threadIdx.x % CH, part = threadIdx.x / CH;
-	constexpr size_t STEP = KV_ROWS * (D + 2);
+	const float *p = ws + (((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits) * nrows * (D + 4) +
+			 mine % KV_ROWS * (D + 4);
+	const int c = threadIdx.x % CH, part = threadIdx.x / CH;
+	const size_t STEP = nrows * (D + 4);
 
 	float ref = -__builtin_inff(), sum = 0.0f;
 	for (int u = part; u < n; u += PARTS)
-		ref = fmaxf(ref, p[u * STEP + KV_ROWS * D + 2 * at]);
+		ref = fmaxf(ref, p[u * STEP + D]);
 	floatx4 y = (floatx4)0.0f;
 	for (int u = part; u < n; u += PARTS) {
 		const float *x = p + u * STEP;
-		const float f = weight(x[KV_ROWS * D + 2 * at], ref);
-		sum += x[KV_ROWS * D + 2 * at + 1] * f;
-		y += *(const floatx4 *)(x + at * D + 4 * c) * f;
+		const float f = weight(x[D], ref);
+		sum += x[D + 1] * f;
+		y += *(const floatx4 *)(x + 4 * c) * f;
 	}
 	s_y[part][c] = y;
 	if (c == 0) {
@@ -508,6 +509,14 @@ __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename k
 			   4 * c) = z;
 }
 
+/*
+ * Along the cache: as many workgroups as the chip holds at once (256 CUs; two,
+ * four or one wave a SIMD by the registers of the head length), each with a tile
+ * for every wave at least; of a long cache, pieces of at most KV_CHUNK tiles,
+ * so that sequences of different lengths fill the chip evenly.
+ */
+#define KV_CHUNK 32
+
 extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int window, kv_plan *p)
 {
 	const int G = heads / a->kv_heads;
@@ -516,20 +525,29 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	if (window && (long)window + KV_ROWS < a->max_len)
 		tiles = ((long)window + KV_ROWS + KV_TILE - 2) / KV_TILE + 1;
 	tiles = tiles < all ? tiles : all;
-	p->row_tiles = (int)(((long)a->max_rows * G + KV_ROWS - 1) / KV_ROWS);
+	const long rows = (long)a->max_rows * G;
+	p->row_tiles = (int)((rows + KV_ROWS - 1) / KV_ROWS);
+	p->rows = (int)(rows < KV_ROWS ? rows : KV_ROWS);
 	const size_t wgs = (size_t)a->nseq * a->kv_heads * p->row_tiles;
-	/* along the cache: enough workgroups to fill the chip, each with a tile
-	 * for every wave at least */
-	const long want = wgs ? (long)((1024 + wgs - 1) / wgs) : 1;
-	const long most = (all + KV_WAVES - 1) / KV_WAVES;
-	const long splits = want < most ? want : most > 1 ? most : 1;
-	long chunk = (tiles + splits - 1) / splits;
-	chunk = (chunk + KV_WAVES - 1) / KV_WAVES * KV_WAVES;
-	p->chunk = (int)(chunk < KV_WAVES ? KV_WAVES : chunk);
+	const size_t room = head_len == 64 ? 1024 : head_len == 128 ? 512 : 256;
+	const auto cut = [&](long n) {
+		long splits = wgs ? (long)(room / wgs) : 1;
+		splits = splits < 1 ? 1 : splits;
+		long chunk = (n + splits - 1) / splits;
+		if (wgs >= room / 8 && chunk > KV_CHUNK && p->row_tiles == 1)
+			chunk = KV_CHUNK;
+		return chunk < KV_WAVES ? (long)KV_WAVES : chunk;
+	};
+	p->chunk = (int)cut(tiles);
 	p->splits = (int)((tiles + p->chunk - 1) / p->chunk);
 	p->splits = p->splits < 1 ? 1 : p->splits;
-	/* without regard to the window, so that one workspace serves any */
-	p->ws = splits > 1 ? wgs * splits * KV_ROWS * (head_len + 2) * sizeof(float) : 0;
+	/* without regard to the window, so that one workspace serves any: pieces by
+	 * room, or of KV_CHUNK tiles, and none below KV_WAVES */
+	const long by_room = wgs ? (long)(room / wgs) : 1, by_chunk = (all + KV_CHUNK - 1) / KV_CHUNK;
+	const long few = (all + KV_WAVES - 1) / KV_WAVES;
+	long most = p->row_tiles == 1 && by_chunk > by_room ? by_chunk : by_room;
+	most = most < few ? most : few;
+	p->ws = most > 1 ? wgs * most * p->rows * (head_len + 4) * sizeof(float) : 0;
 }
 
 extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const void *q,
@@ -543,11 +561,11 @@ extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const vo
 		typedef kv_type<TY>::t t;
 		k_kv_attn<D, TY><<<grid, KV_NT, 0, (hipStream_t)stream>>>(
 			*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window, (float *)ws,
-			p->row_tiles, p->chunk);
+			p->row_tiles, p->chunk, p->rows);
 		if (p->splits > 1)
 			k_kv_merge<D, TY><<<rows, KV_NT, 0, (hipStream_t)stream>>>(
 				*a, G, (t *)out, out_stride, window, (const float *)ws, p->row_tiles,
-				p->chunk, p->splits);
+				p->chunk, p->splits, p->rows);
 	}))
 	return (int)hipGetLastError();
 }
