@@ -30,9 +30,12 @@
  */
 #include "kv_device.h"
 
+#include <type_traits>
+
 #define KV_NT 256
 #define KV_WAVES (KV_NT / WAVE)
 #define KV_ROWS 16 /* query rows of a tile */
+#define KV_SPLITS 1024 /* pieces of a cache, at most */
 
 __device__ static inline half8_t as_half8(u32 a, u32 b, u32 c, u32 d)
 {
@@ -118,7 +121,11 @@ __device__ static inline kv_span kv_rows_of(const kv_seq &sq, int tile, int G, i
 template <int D> struct kv_keys {
 	typedef kv_tile<D> L;
 	u32 w[2][L::G];        /* rows lane % 16 of each half */
-	_Float16 d[2][4][L::G]; /* scales of rows 4 (lane / 16) + j of each half */
+	u32x4 d[2][L::G / 2];  /* scales of rows 4 (lane / 16) + j of each half */
+	__device__ inline float scale(int h, int j, int g) const
+	{
+		return (float)__builtin_bit_cast(half8_t, d[h][(j * L::G + g) / 8])[(j * L::G + g) % 8];
+	}
 	__device__ inline void load(const uint8_t *tile, int lane)
 	{
 #pragma unroll
@@ -131,14 +138,10 @@ template <int D> struct kv_keys {
 				for (int u = 0; u < L::P; u++)
 					w[h][g + u] = x[u];
 			}
-			const half8_t *s = (const half8_t *)(tile + L::K_SCALES) + (16 * h + 4 * (lane / 16)) * L::G / 8;
+			const u32x4 *s = (const u32x4 *)(tile + L::K_SCALES) + (16 * h + 4 * (lane / 16)) * L::G / 8;
 #pragma unroll
-			for (int u = 0; u < L::G / 2; u++) {
-				const half8_t x = s[u];
-#pragma unroll
-				for (int j = 0; j < 8; j++)
-					d[h][(8 * u + j) / L::G][(8 * u + j) % L::G] = x[j];
-			}
+			for (int u = 0; u < L::G / 2; u++)
+				d[h][u] = s[u];
 		}
 	}
 };
@@ -160,85 +163,108 @@ template <int D> struct kv_values {
 };
 
 /* value scales of the lane's eight rows */
-__device__ static inline half8_t kv_value_scales(const uint8_t *scales, int lane)
+__device__ static inline u32x4 kv_value_scales(const uint8_t *scales, int lane)
 {
-	const half4_t *p = (const half4_t *)scales + lane / 16;
-	const half4_t a = p[0], b = p[4];
-	return half8_t{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+	const u32x2 *p = (const u32x2 *)scales + lane / 16;
+	const u32x2 a = p[0], b = p[4];
+	return u32x4{a.x, a.y, b.x, b.y};
 }
 
-/* a query row in f16 parts, and what belongs to it */
+/*
+ * A tile of query rows as the products take it, in LDS for all waves: part p of
+ * group g of the lane's row at f[p][g][lane], and what the accumulators start
+ * with, -8 steps times the group's sum.
+ */
 template <int D, int QP> struct kv_query {
-	half8_t f[QP][D / 32];
-	float start[D / 32]; /* of the accumulators: -8 steps times the group's sum */
-	float rs;            /* a score times this is a logit in powers of two; > 0 */
-	template <int TY> __device__ inline void load(const typename kv_type<TY>::t *x, float scale, int part)
-	{
-		float v[D / 32][8], top = 0.0f;
-#pragma unroll
-		for (int g = 0; g < D / 32; g++) {
-			const kv_vec<TY, 8> w = *(const kv_vec<TY, 8> *)(x + 32 * g + 8 * part);
-#pragma unroll
-			for (int j = 0; j < 8; j++) {
-				v[g][j] = kv_type<TY>::get(w.v[j]);
-				top = fmaxf(top, fabsf(v[g][j]));
-			}
-		}
-		top = row_max(top);
-		int e = 14 - __builtin_amdgcn_frexp_expf(top);
-		e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 126) : 0;
-		/* a negative scale turns the query around, 0 makes it 0 */
-		const float sc = scale > 0.0f ? pow2(e) : scale < 0.0f ? -pow2(e) : 0.0f;
-		rs = (scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / KV_CODE_STEP) * pow2(-e);
-#pragma unroll
-		for (int g = 0; g < D / 32; g++) {
-			float sum = 0.0f;
-#pragma unroll
-			for (int j = 0; j < 8; j++) {
-				const float y = v[g][j] * sc;
-				const _Float16 hi = (_Float16)y;
-				f[0][g][j] = hi;
-				sum += (float)hi;
-				if (QP > 1) {
-					const _Float16 lo = (_Float16)(y - (float)hi);
-					f[QP - 1][g][j] = lo;
-					sum += (float)lo;
-				}
-			}
-			start[g] = -8.0f * KV_CODE_STEP * row_sum(sum);
-		}
-	}
+	half8_t f[QP][D / 32][WAVE];
+	float start[D / 32][16];
 };
+
+/* The groups wave, wave + waves, .. of the lane's row x into LDS (of one row of
+ * 16 lanes a quarter each: part); returns what a score is multiplied by to be a
+ * logit in powers of two (above 0).  The caller synchronises. */
+template <int D, int QP, int TY>
+__device__ static inline float kv_load_query(kv_query<D, QP> &q, const typename kv_type<TY>::t *x,
+					     float scale, int lane, int wave, int waves)
+{
+	typedef kv_type<TY> T;
+	const int part = lane / 16;
+	float top = 0.0f;
+	kv_vec<TY, 8> w[D / 32];
+#pragma unroll
+	for (int g = 0; g < D / 32; g++)
+		w[g] = *(const kv_vec<TY, 8> *)(x + 32 * g + 8 * part);
+#pragma unroll
+	for (int g = 0; g < D / 32; g++)
+#pragma unroll
+		for (int j = 0; j < 8; j++)
+			top = fmaxf(top, fabsf(T::get(w[g].v[j])));
+	top = row_max(top);
+	int e = 14 - __builtin_amdgcn_frexp_expf(top);
+	e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 126) : 0;
+	/* a negative scale turns the query around, 0 makes it 0 */
+	const float sc = scale > 0.0f ? pow2(e) : scale < 0.0f ? -pow2(e) : 0.0f;
+#pragma unroll
+	for (int g = 0; g < D / 32; g++) {
+		if (g % waves != wave)
+			continue;
+		half8_t f[QP];
+		float sum = 0.0f;
+#pragma unroll
+		for (int j = 0; j < 8; j++) {
+			const float y = T::get(w[g].v[j]) * sc;
+			f[0][j] = (_Float16)y;
+			sum += (float)f[0][j];
+			if (QP > 1) {
+				f[QP - 1][j] = (_Float16)fmaf((float)f[0][j], -1.0f, y);
+				sum += (float)f[QP - 1][j];
+			}
+		}
+#pragma unroll
+		for (int p = 0; p < QP; p++)
+			q.f[p][g][lane] = f[p];
+		sum = row_sum(sum);
+		if (part == 0)
+			q.start[g][lane] = -8.0f * KV_CODE_STEP * sum;
+	}
+	return (scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / KV_CODE_STEP) * pow2(-e);
+}
 
 /* scores of 32 cached rows: 4 part + j of each half */
 template <int D, int QP>
-__device__ static inline void kv_scores(const kv_keys<D> &k, const kv_query<D, QP> &q, float *x)
+__device__ static inline void kv_scores(const kv_keys<D> &k, const kv_query<D, QP> &q, int lane, float *x)
 {
 #pragma unroll
-	for (int h = 0; h < 2; h++) {
+	for (int g = 0; g < D / 32; g++) {
+		half8_t f[QP];
 #pragma unroll
-		for (int g = 0; g < D / 32; g++) {
-			floatx4 acc = (floatx4)q.start[g];
+		for (int p = 0; p < QP; p++)
+			f[p] = q.f[p][g][lane];
+		const floatx4 start = (floatx4)q.start[g][lane % 16];
+#pragma unroll
+		for (int h = 0; h < 2; h++) {
+			floatx4 acc = start;
 			const half8_t kf = kv_word(k.w[h][g]);
 #pragma unroll
 			for (int p = 0; p < QP; p++)
-				acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q.f[p][g], acc, 0, 0, 0);
+				acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, f[p], acc, 0, 0, 0);
 #pragma unroll
 			for (int j = 0; j < 4; j++)
-				x[4 * h + j] = g ? fmaf((float)k.d[h][j][g], acc[j], x[4 * h + j])
-						 : (float)k.d[h][j][g] * acc[j];
+				x[4 * h + j] = fmaf(k.scale(h, j, g), acc[j], g ? x[4 * h + j] : 0.0f);
 		}
 	}
 }
 
 /*
  * The running softmax of a query row.  ref is its reference in powers of two: a
- * probability is 2^(logit - ref), and ref is the largest logit so far plus the
- * exponent of the value scales that came with it, less 15, so that probability
- * times value scale stays below 2^15 (f16's largest is 2^16) and mostly far
- * above f16's smallest; sums and outputs carry the same factor, which the
- * division at the end takes out.
+ * probability is 2^(logit - ref), and ref the largest logit plus the exponent of
+ * the value scales that come with it, less KV_REF, so that probability times value
+ * scale stays below 2^KV_REF.  It stays as it is until the product would reach
+ * 2^15 (f16's largest is 2^16): most tiles then leave the output alone.  Sums and
+ * outputs carry the same factor, which the division at the end takes out.
  */
+#define KV_REF 9.0f
+
 struct kv_soft {
 	float ref, sum;
 };
@@ -255,8 +281,9 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
 		top = fmaxf(top, x[j]);
 		big = fmaxf(big, fabsf((float)dv[j]));
 	}
-	/* scales of nothing but zeros: exponent 0 */
-	const float next = fmaxf(s.ref, row_max(fmaf(top, rs, (float)(__builtin_amdgcn_frexp_expf(big) - 15))));
+	/* (scales of nothing but zeros: exponent 0) */
+	const float high = row_max(fmaf(top, rs, (float)__builtin_amdgcn_frexp_expf(big)));
+	const float next = high - s.ref > 15.0f ? high - KV_REF : s.ref;
 	const float back = weight(s.ref, next);
 	s.ref = next;
 	const float ref = next == -__builtin_inff() ? 0.0f : next;
@@ -283,10 +310,10 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
  * while it still works on the values of the tile before, and the values while
  * it works on the keys.
  */
-/* two waves a SIMD, so that nothing is kept in accumulation registers and moved;
+/* three waves a SIMD, so that nothing is kept in accumulation registers and moved;
  * heads of 256 do not fit */
 template <int D, int TY>
-__global__ __launch_bounds__(KV_NT) __attribute__((amdgpu_waves_per_eu(D < 256 ? 2 : 1)))
+__global__ __launch_bounds__(KV_NT) __attribute__((amdgpu_waves_per_eu(D < 256 ? 3 : 1)))
 void k_kv_attn(
 	kv_args a, const typename kv_type<TY>::t *q, size_t q_stride, int G,
 	typename kv_type<TY>::t *out, size_t out_stride, float scale, int window, float *ws,
@@ -299,6 +326,7 @@ void k_kv_attn(
 	__shared__ float s_o[KV_WAVES][KV_ROWS][D + 4];
 	__shared__ float s_ref[KV_WAVES][KV_ROWS], s_sum[KV_WAVES][KV_ROWS];
 	__shared__ int s_row[KV_ROWS], s_head[KV_ROWS];
+	__shared__ kv_query<D, QP> s_q;
 
 	const int lane = threadIdx.x % WAVE, part = lane / 16;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
@@ -331,21 +359,22 @@ void k_kv_attn(
 	};
 	kv_keys<D> k;
 	kv_values<D> v;
-	half8_t dv;
+	u32x4 vd;
 	if (n > 0) {
 		const uint8_t *tile = tile_of(0);
 		k.load(tile, lane);
-		dv = kv_value_scales(tile + L::V_SCALES, lane);
+		vd = kv_value_scales(tile + L::V_SCALES, lane);
 		v.load(tile, lane);
 	} else if (!a.pages && lane == 0) {
 		kv_error(a, HIP_KV_ERR_PAGE);
 	}
-	kv_query<D, QP> qr;
-	qr.template load<TY>(q + (size_t)r.row * q_stride + (size_t)r.head * D, scale, part);
+	const float rs = kv_load_query<D, QP, TY>(s_q, q + (size_t)r.row * q_stride + (size_t)r.head * D,
+						  scale, lane, wave, KV_WAVES);
 	if (threadIdx.x < KV_ROWS) {
 		s_row[threadIdx.x] = r.valid ? r.row : -1;
 		s_head[threadIdx.x] = r.hi > r.lo ? r.head : ~r.head;
 	}
+	__syncthreads();
 
 	floatx4 o[CT];
 #pragma unroll
@@ -353,14 +382,16 @@ void k_kv_attn(
 		o[c] = (floatx4)0.0f;
 	kv_soft soft = {-__builtin_inff(), 0.0f};
 
-	for (int i = 0; i < n; i++) {
+	const auto step = [&](int i, auto more) {
 		const int t = t0 + wave + i * KV_WAVES;
-		const bool hidden = lost, more = i + 1 < n;
-		const uint8_t *next = more ? tile_of(i + 1) : NULL;
+		const bool hidden = lost;
+		const uint8_t *next = NULL;
+		if constexpr (more.value)
+			next = tile_of(i + 1);
 		float x[8];
-		half8_t pf[PP];
-		kv_scores<D, QP>(k, qr, x);
-		if (more)
+		half8_t pf[PP], dv = __builtin_bit_cast(half8_t, vd);
+		kv_scores<D, QP>(k, s_q, lane, x);
+		if constexpr (more.value)
 			k.load(next, lane);
 		if (hidden || t * KV_TILE < r.inner0 || (t + 1) * KV_TILE > r.inner1) {
 			const int lo = hidden ? 0x7fffffff : r.lo;
@@ -374,7 +405,7 @@ void k_kv_attn(
 			if (hidden && lane == 0)
 				kv_error(a, HIP_KV_ERR_PAGE);
 		}
-		const float back = kv_softmax<PP>(soft, x, dv, qr.rs, pf);
+		const float back = kv_softmax<PP>(soft, x, dv, rs, pf);
 		if (__ballot(back != 1.0f)) {
 #pragma unroll
 			for (int c = 0; c < CT; c++)
@@ -387,11 +418,15 @@ void k_kv_attn(
 			for (int p = 0; p < PP; p++)
 				o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[p], o[c], 0, 0, 0);
 		}
-		if (more) {
-			dv = kv_value_scales(next + L::V_SCALES, lane);
+		if constexpr (more.value) {
+			vd = kv_value_scales(next + L::V_SCALES, lane);
 			v.load(next, lane);
 		}
-	}
+	};
+	for (int i = 0; i < n - 1; i++)
+		step(i, std::true_type());
+	if (n > 0)
+		step(n - 1, std::false_type());
 
 	/* the waves' results: to one reference, then added in wave order */
 	const float sum = KV_CODE_STEP * row_sum(soft.sum); /* the outputs' own factor */
@@ -445,9 +480,9 @@ void k_kv_attn(
 }
 
 /*
- * The workgroups' results of one query row: D / 4 threads take its channels,
- * KV_NT / (D / 4) of them share the workgroups along the cache, and are added
- * in their order.
+ * The pieces' results of one query row: first their weights, then D / 4 threads
+ * take the row's channels, KV_NT / (D / 4) times over, each its share of the
+ * pieces.
  */
 template <int D, int TY>
 __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename kv_type<TY>::t *out,
@@ -457,7 +492,7 @@ __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename k
 	typedef kv_type<TY> T;
 	constexpr int CH = D / 4, PARTS = KV_NT / CH;
 	__shared__ floatx4 s_y[PARTS][CH];
-	__shared__ float s_ref[PARTS], s_sum[PARTS];
+	__shared__ float s_w[KV_SPLITS], s_ref[KV_WAVES], s_sum[KV_WAVES];
 	const int kv_head = blockIdx.x % a.kv_heads, mine = blockIdx.x / a.kv_heads, s = blockIdx.y;
 	const kv_seq sq = kv_sequence(a, s);
 	if (mine >= sq.n * G)
@@ -470,37 +505,53 @@ __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename k
 	const float *p = ws + (((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits) * nrows * (D + 4) +
 			 mine % KV_ROWS * (D + 4);
 	const int c = threadIdx.x % CH, part = threadIdx.x / CH;
-	const size_t STEP = nrows * (D + 4);
+	const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+	const size_t step = nrows * (D + 4);
 
-	float ref = -__builtin_inff(), sum = 0.0f;
-	for (int u = part; u < n; u += PARTS)
-		ref = fmaxf(ref, p[u * STEP + D]);
+	/* every piece's reference and sum, then its weight */
+	constexpr int PER = KV_SPLITS / KV_NT;
+	float r[PER], l[PER], ref = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+	for (int u = 0; u < PER; u++) {
+		const int at = threadIdx.x + u * KV_NT;
+		r[u] = at < n ? p[at * step + D] : -__builtin_inff();
+		l[u] = at < n ? p[at * step + D + 1] : 0.0f;
+		ref = fmaxf(ref, r[u]);
+	}
+	for (int o = WAVE / 2; o > 0; o >>= 1)
+		ref = fmaxf(ref, __shfl_xor(ref, o, WAVE));
+	if (lane == 0)
+		s_ref[wave] = ref;
+	__syncthreads();
+#pragma unroll
+	for (int u = 0; u < KV_WAVES; u++)
+		ref = fmaxf(ref, s_ref[u]);
+#pragma unroll
+	for (int u = 0; u < PER; u++) {
+		const float f = weight(r[u], ref);
+		s_w[threadIdx.x + u * KV_NT] = f;
+		sum += l[u] * f;
+	}
+	for (int o = WAVE / 2; o > 0; o >>= 1)
+		sum += __shfl_xor(sum, o, WAVE);
+	if (lane == 0)
+		s_sum[wave] = sum;
+	__syncthreads();
 	floatx4 y = (floatx4)0.0f;
-	for (int u = part; u < n; u += PARTS) {
-		const float *x = p + u * STEP;
-		const float f = weight(x[D], ref);
-		sum += x[D + 1] * f;
-		y += *(const floatx4 *)(x + 4 * c) * f;
-	}
+#pragma unroll 8
+	for (int u = part; u < n; u += PARTS)
+		y += *(const floatx4 *)(p + u * step + 4 * c) * s_w[u];
 	s_y[part][c] = y;
-	if (c == 0) {
-		s_ref[part] = ref;
-		s_sum[part] = sum;
-	}
 	__syncthreads();
 	if (part)
 		return;
 #pragma unroll
 	for (int u = 1; u < PARTS; u++)
-		ref = fmaxf(ref, s_ref[u]);
-	sum = 0.0f;
-	y = (floatx4)0.0f;
+		y += s_y[u][c];
+	sum = s_sum[0];
 #pragma unroll
-	for (int u = 0; u < PARTS; u++) {
-		const float f = weight(s_ref[u], ref);
-		sum += s_sum[u] * f;
-		y += s_y[u][c] * f;
-	}
+	for (int u = 1; u < KV_WAVES; u++)
+		sum += s_sum[u];
 	kv_vec<TY, 4> z;
 #pragma unroll
 	for (int u = 0; u < 4; u++)
@@ -536,6 +587,8 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 		long chunk = (n + splits - 1) / splits;
 		if (wgs >= room / 8 && chunk > KV_CHUNK && p->row_tiles == 1)
 			chunk = KV_CHUNK;
+		if (chunk < (n + KV_SPLITS - 1) / KV_SPLITS)
+			chunk = (n + KV_SPLITS - 1) / KV_SPLITS;
 		return chunk < KV_WAVES ? (long)KV_WAVES : chunk;
 	};
 	p->chunk = (int)cut(tiles);
@@ -547,6 +600,7 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	const long few = (all + KV_WAVES - 1) / KV_WAVES;
 	long most = p->row_tiles == 1 && by_chunk > by_room ? by_chunk : by_room;
 	most = most < few ? most : few;
+	most = most < KV_SPLITS ? most : KV_SPLITS;
 	p->ws = most > 1 ? wgs * most * p->rows * (head_len + 4) * sizeof(float) : 0;
 }
 
