@@ -17,8 +17,8 @@
  *
  * Exactness.  Codes are small integers, exact in f16, and stay unscaled in the
  * operands: a key group's scale multiplies its partial scores in fp32, a value
- * row's scale its probability.  A code q enters as the subnormal q * 2^-18 (its
- * bits in place, nothing around them: a shift and a mask for two).  The keys'
+ * row's scale its probability.  A code enters as a subnormal, its bits
+ * where they lie and nothing around them (a mask for two).  The keys'
  * surplus of 8 a channel leaves through the accumulator's start (-8 sum of the
  * query's channels), the values' by a subtraction, exact as well, since over many
  * cached rows a surplus would outweigh the sum.  A query row is scaled by a power of two (its largest value into [2^13, 2^14))
@@ -43,15 +43,41 @@ __device__ static inline half8_t as_half8(u32 a, u32 b, u32 c, u32 d)
 	return __builtin_bit_cast(half8_t, v);
 }
 
-/* a word's codes, in their order, as f16 with the mantissa's upper four bits
- * and nothing else: code * 2^-18, a subnormal */
+/*
+ * A word's codes, in their order, as f16 with the mantissa's bits where they lie
+ * and nothing else, subnormals: code * 2^-22 for codes 0, 1, 4 and 5, code * 2^-18
+ * for the others.  One turn and four masks for eight; the other operand has 16
+ * times the value where the code has the smaller step.
+ */
 __device__ static inline half8_t kv_word(u32 w)
 {
-	const u32 m = 0x03c003c0u; /* the codes whose lowest bits are 6 and 22 */
-	return as_half8(w << 4 & m, w & m, w >> 4 & m, kv_rotr(w, 8) & m);
+	const u32 r = kv_rotr(w, 8);
+	return as_half8(w & 0x003c003cu, w & 0x03c003c0u, r & 0x003c003cu, r & 0x03c003c0u);
 }
 
 #define KV_CODE_STEP (1.0f / (1 << 18))
+
+/* whether code j has the smaller step */
+__device__ static constexpr bool kv_small(int j)
+{
+	return j % 4 < 2;
+}
+
+/* a word's codes less 8, in the same steps */
+__device__ static inline half8_t kv_word8(u32 w)
+{
+	const _Float16 a = (_Float16)(8.0f * KV_CODE_STEP / 16.0f), b = (_Float16)(8.0f * KV_CODE_STEP);
+	return kv_word(w) - half8_t{a, a, b, b, a, a, b, b};
+}
+
+/* x = hi + lo in f16; the products with the hidden -1 stay fused with the
+ * conversions */
+__device__ static inline _Float16 rest(float x, _Float16 hi)
+{
+	float minus = -1.0f;
+	asm("" : "+s"(minus));
+	return (_Float16)fmaf((float)hi, minus, x);
+}
 
 /* the lane's value and those of the three others that share its query row, put
  * together by fn.  The swaps exchange the odd rows of 16 lanes (the upper 32)
@@ -177,7 +203,7 @@ __device__ static inline u32x4 kv_value_scales(const uint8_t *scales, int lane)
  */
 template <int D, int QP> struct kv_query {
 	half8_t f[QP][D / 32][WAVE];
-	float start[D / 32][16];
+	floatx4 start[D / 32][16];
 };
 
 /* The groups wave, wave + waves, .. of the lane's row x into LDS (of one row of
@@ -200,8 +226,8 @@ __device__ static inline float kv_load_query(kv_query<D, QP> &q, const typename 
 		for (int j = 0; j < 8; j++)
 			top = fmaxf(top, fabsf(T::get(w[g].v[j])));
 	top = row_max(top);
-	int e = 14 - __builtin_amdgcn_frexp_expf(top);
-	e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 126) : 0;
+	int e = 10 - __builtin_amdgcn_frexp_expf(top);
+	e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 122) : 0;
 	/* a negative scale turns the query around, 0 makes it 0 */
 	const float sc = scale > 0.0f ? pow2(e) : scale < 0.0f ? -pow2(e) : 0.0f;
 #pragma unroll
@@ -212,20 +238,18 @@ __device__ static inline float kv_load_query(kv_query<D, QP> &q, const typename 
 		float sum = 0.0f;
 #pragma unroll
 		for (int j = 0; j < 8; j++) {
-			const float y = T::get(w[g].v[j]) * sc;
-			f[0][j] = (_Float16)y;
-			sum += (float)f[0][j];
-			if (QP > 1) {
-				f[QP - 1][j] = (_Float16)fmaf((float)f[0][j], -1.0f, y);
-				sum += (float)f[QP - 1][j];
-			}
+			const float y = T::get(w[g].v[j]) * (kv_small(j) ? 16.0f * sc : sc);
+			float z = (float)(f[0][j] = (_Float16)y);
+			if (QP > 1)
+				z += (float)(f[QP - 1][j] = rest(y, f[0][j]));
+			sum += kv_small(j) ? z * (1.0f / 16.0f) : z;
 		}
 #pragma unroll
 		for (int p = 0; p < QP; p++)
 			q.f[p][g][lane] = f[p];
 		sum = row_sum(sum);
 		if (part == 0)
-			q.start[g][lane] = -8.0f * KV_CODE_STEP * sum;
+			q.start[g][lane] = (floatx4)(-8.0f * KV_CODE_STEP * sum);
 	}
 	return (scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / KV_CODE_STEP) * pow2(-e);
 }
@@ -240,7 +264,7 @@ __device__ static inline void kv_scores(const kv_keys<D> &k, const kv_query<D, Q
 #pragma unroll
 		for (int p = 0; p < QP; p++)
 			f[p] = q.f[p][g][lane];
-		const floatx4 start = (floatx4)q.start[g][lane % 16];
+		const floatx4 start = q.start[g][lane % 16];
 #pragma unroll
 		for (int h = 0; h < 2; h++) {
 			floatx4 acc = start;
@@ -260,17 +284,20 @@ __device__ static inline void kv_scores(const kv_keys<D> &k, const kv_query<D, Q
  * probability is 2^(logit - ref), and ref the largest logit plus the exponent of
  * the value scales that come with it, less KV_REF, so that probability times value
  * scale stays below 2^KV_REF.  It stays as it is until the product would reach
- * 2^15 (f16's largest is 2^16): most tiles then leave the output alone.  Sums and
- * outputs carry the same factor, which the division at the end takes out.
+ * 2^KV_TOP (16 times that is below f16's largest): most tiles then leave the output
+ * alone.  Sums and outputs carry the same factor, which the division at the end
+ * takes out.
  */
-#define KV_REF 9.0f
+#define KV_REF 5.0f
+#define KV_TOP 11.0f
 
 struct kv_soft {
 	float ref, sum;
 };
 
-/* probabilities times value scales of 32 cached rows, in f16 parts; returns what
- * the output so far is multiplied by */
+/* probabilities times value scales of 32 cached rows, in f16 parts, 16 times that
+ * where the codes have the smaller step; returns what the output so far is
+ * multiplied by */
 template <int PP>
 __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half8_t dv, float rs,
 					  half8_t (&pf)[PP])
@@ -283,28 +310,29 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
 	}
 	/* (scales of nothing but zeros: exponent 0) */
 	const float high = row_max(fmaf(top, rs, (float)__builtin_amdgcn_frexp_expf(big)));
-	const float next = high - s.ref > 15.0f ? high - KV_REF : s.ref;
+	const float next = high - s.ref > KV_TOP ? high - KV_REF : s.ref;
 	const float back = weight(s.ref, next);
 	s.ref = next;
-	const float ref = next == -__builtin_inff() ? 0.0f : next;
-	float sum = 0.0f;
+	const float ref = next == -__builtin_inff() ? 0.0f : next, ref16 = ref - 4.0f;
+	float sum = 0.0f, sum16 = 0.0f;
 #pragma unroll
 	for (int j = 0; j < 8; j++) {
-		const float p = __builtin_amdgcn_exp2f(fmaf(x[j], rs, -ref));
-		sum += p;
-		const float w = fmaf((float)dv[j], p, 0.0f); /* fma: takes the f16 as it is */
-		const _Float16 hi = (_Float16)w;
-		pf[0][j] = hi;
+		const float p = __builtin_amdgcn_exp2f(fmaf(x[j], rs, kv_small(j) ? -ref16 : -ref));
+		(kv_small(j) ? sum16 : sum) += p;
+		float w = fmaf((float)dv[j], p, 0.0f); /* fma: takes the f16 as it is */
 		if (PP > 1)
-			pf[PP - 1][j] = (_Float16)fmaf((float)hi, -1.0f, w);
+			asm("" : "+v"(w)); /* once, not once for each part */
+		pf[0][j] = (_Float16)w;
+		if (PP > 1)
+			pf[PP - 1][j] = rest(w, pf[0][j]);
 	}
-	s.sum = s.sum * back + sum;
+	s.sum = s.sum * back + fmaf(sum16, 1.0f / 16.0f, sum);
 	return back;
 }
 
 /*
  * Few query rows: one workgroup takes a tile of them over `chunk` tiles of the
- * cache, dealt to its four waves one by one; the waves' results meet in LDS.
+ * cache, dealt to its waves one by one; the waves' results meet in LDS.
  * With more than one workgroup along the cache each leaves its reference, sum
  * and unnormalised output in ws for k_kv_merge.  A wave loads a tile's keys
  * while it still works on the values of the tile before, and the values while
@@ -312,8 +340,8 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
  */
 /* three waves a SIMD, so that nothing is kept in accumulation registers and moved;
  * heads of 256 do not fit */
-template <int D, int TY>
-__global__ __launch_bounds__(KV_NT) __attribute__((amdgpu_waves_per_eu(D < 256 ? 3 : 1)))
+template <int D, int TY, int NW>
+__global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(D < 256 ? 3 : 1)))
 void k_kv_attn(
 	kv_args a, const typename kv_type<TY>::t *q, size_t q_stride, int G,
 	typename kv_type<TY>::t *out, size_t out_stride, float scale, int window, float *ws,
@@ -323,8 +351,8 @@ void k_kv_attn(
 	typedef kv_tile<D> L;
 	constexpr int QP = TY == HIP_KV_F32 ? 2 : 1, PP = TY == HIP_KV_BF16 ? 1 : 2;
 	constexpr int CT = D / 16; /* channel tiles of O^T */
-	__shared__ float s_o[KV_WAVES][KV_ROWS][D + 4];
-	__shared__ float s_ref[KV_WAVES][KV_ROWS], s_sum[KV_WAVES][KV_ROWS];
+	__shared__ float s_o[NW][KV_ROWS][D + 4];
+	__shared__ float s_ref[NW][KV_ROWS], s_sum[NW][KV_ROWS];
 	__shared__ int s_row[KV_ROWS], s_head[KV_ROWS];
 	__shared__ kv_query<D, QP> s_q;
 
@@ -343,13 +371,13 @@ void k_kv_attn(
 
 	/* the wave's tiles t0 + wave, + 4, ..; a lane holds the page of one of the
 	 * next 64.  A page outside the pool: its first tile, with every row hidden */
-	const int shift = a.page_shift - 5, n = a.pages ? (t1 - t0 - wave + KV_WAVES - 1) / KV_WAVES : 0;
+	const int shift = a.page_shift - 5, n = a.pages ? (t1 - t0 - wave + NW - 1) / NW : 0;
 	int page = -1;
 	bool lost = false;
 	const auto tile_of = [&](int i) -> const uint8_t * {
-		const int t = t0 + wave + i * KV_WAVES;
+		const int t = t0 + wave + i * NW;
 		if (i % WAVE == 0) {
-			const int tl = t + lane * KV_WAVES;
+			const int tl = t + lane * NW;
 			page = tl < t1 ? a.table[s * a.table_stride + (tl >> shift)] : -1;
 		}
 		const int id = __builtin_amdgcn_readlane(page, i % WAVE);
@@ -369,7 +397,7 @@ void k_kv_attn(
 		kv_error(a, HIP_KV_ERR_PAGE);
 	}
 	const float rs = kv_load_query<D, QP, TY>(s_q, q + (size_t)r.row * q_stride + (size_t)r.head * D,
-						  scale, lane, wave, KV_WAVES);
+						  scale, lane, wave, NW);
 	if (threadIdx.x < KV_ROWS) {
 		s_row[threadIdx.x] = r.valid ? r.row : -1;
 		s_head[threadIdx.x] = r.hi > r.lo ? r.head : ~r.head;
@@ -383,7 +411,7 @@ void k_kv_attn(
 	kv_soft soft = {-__builtin_inff(), 0.0f};
 
 	const auto step = [&](int i, auto more) {
-		const int t = t0 + wave + i * KV_WAVES;
+		const int t = t0 + wave + i * NW;
 		const bool hidden = lost;
 		const uint8_t *next = NULL;
 		if constexpr (more.value)
@@ -413,7 +441,7 @@ void k_kv_attn(
 		}
 #pragma unroll
 		for (int c = 0; c < CT; c++) {
-			const half8_t vf = kv_word(v.w[c]) - (half8_t)(_Float16)(8.0f * KV_CODE_STEP);
+			const half8_t vf = kv_word8(v.w[c]);
 #pragma unroll
 			for (int p = 0; p < PP; p++)
 				o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[p], o[c], 0, 0, 0);
@@ -437,7 +465,7 @@ void k_kv_attn(
 	__syncthreads();
 	float ref = s_ref[0][lane % 16];
 #pragma unroll
-	for (int w = 1; w < KV_WAVES; w++)
+	for (int w = 1; w < NW; w++)
 		ref = fmaxf(ref, s_ref[w][lane % 16]);
 	const float factor = weight(soft.ref, ref);
 	if (r.valid) {
@@ -448,17 +476,17 @@ void k_kv_attn(
 	__syncthreads();
 	const size_t slot = ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
 	float *to = ws + slot * nrows * (D + 4);
-	for (int at = threadIdx.x; at < KV_ROWS * D / 4; at += KV_NT) {
+	for (int at = threadIdx.x; at < KV_ROWS * D / 4; at += (NW * WAVE)) {
 		const int i = at / (D / 4), c = at % (D / 4) * 4, row = s_row[i];
 		if (row < 0)
 			break; /* the rows behind are not there either */
 		float high = s_ref[0][i], den = 0.0f;
 #pragma unroll
-		for (int w = 1; w < KV_WAVES; w++)
+		for (int w = 1; w < NW; w++)
 			high = fmaxf(high, s_ref[w][i]);
 		floatx4 y = (floatx4)0.0f;
 #pragma unroll
-		for (int w = 0; w < KV_WAVES; w++) {
+		for (int w = 0; w < NW; w++) {
 			den += s_sum[w][i] * weight(s_ref[w][i], high);
 			y += *(const floatx4 *)&s_o[w][i][c];
 		}
@@ -561,12 +589,18 @@ __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename k
 }
 
 /*
- * Along the cache: as many workgroups as the chip holds at once (256 CUs; two,
- * four or one wave a SIMD by the registers of the head length), each with a tile
- * for every wave at least; of a long cache, pieces of at most KV_CHUNK tiles,
- * so that sequences of different lengths fill the chip evenly.
+ * Along the cache.  A workgroup of KV_MANY waves (three a SIMD: all that their
+ * registers allow) takes a row tile's whole cache while that leaves each wave
+ * KV_SHORT tiles or fewer: pieces would need a second launch to add them up
+ * (16 sequences x 1100 rows, 32 heads on 8: 9.9 us against 12.0 + 4.1 us; 16 heads
+ * x 1024 rows: 8.1 against 5.8 + 4.5).  Longer caches are cut into pieces for
+ * workgroups of four waves, as many as the chip holds at once (256 CUs; two or one
+ * wave a SIMD by the registers of the head length), and of many sequences into
+ * pieces of at most KV_CHUNK tiles, so that different lengths fill the chip evenly.
  */
 #define KV_CHUNK 32
+#define KV_MANY 12
+#define KV_SHORT 6
 
 extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int window, kv_plan *p)
 {
@@ -581,26 +615,26 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	p->rows = (int)(rows < KV_ROWS ? rows : KV_ROWS);
 	const size_t wgs = (size_t)a->nseq * a->kv_heads * p->row_tiles;
 	const size_t room = head_len == 64 ? 1024 : head_len == 128 ? 512 : 256;
-	const auto cut = [&](long n) {
-		long splits = wgs ? (long)(room / wgs) : 1;
-		splits = splits < 1 ? 1 : splits;
-		long chunk = (n + splits - 1) / splits;
-		if (wgs >= room / 8 && chunk > KV_CHUNK && p->row_tiles == 1)
-			chunk = KV_CHUNK;
-		if (chunk < (n + KV_SPLITS - 1) / KV_SPLITS)
-			chunk = (n + KV_SPLITS - 1) / KV_SPLITS;
-		return chunk < KV_WAVES ? (long)KV_WAVES : chunk;
-	};
-	p->chunk = (int)cut(tiles);
+	const long by_room = wgs < room ? (long)(room / wgs) : 1;
+	p->waves = head_len < 256 && p->row_tiles == 1 && tiles <= KV_MANY * KV_SHORT ? KV_MANY : KV_WAVES;
+	long chunk = (tiles + by_room - 1) / by_room;
+	if (wgs >= room / 8 && chunk > KV_CHUNK && p->row_tiles == 1)
+		chunk = KV_CHUNK;
+	if (chunk < (tiles + KV_SPLITS - 1) / KV_SPLITS)
+		chunk = (tiles + KV_SPLITS - 1) / KV_SPLITS;
+	if (p->waves == KV_MANY)
+		chunk = tiles;
+	p->chunk = (int)(chunk < KV_WAVES ? KV_WAVES : chunk);
 	p->splits = (int)((tiles + p->chunk - 1) / p->chunk);
 	p->splits = p->splits < 1 ? 1 : p->splits;
 	/* without regard to the window, so that one workspace serves any: pieces by
 	 * room, or of KV_CHUNK tiles, and none below KV_WAVES */
-	const long by_room = wgs ? (long)(room / wgs) : 1, by_chunk = (all + KV_CHUNK - 1) / KV_CHUNK;
-	const long few = (all + KV_WAVES - 1) / KV_WAVES;
+	const long by_chunk = (all + KV_CHUNK - 1) / KV_CHUNK, few = (all + KV_WAVES - 1) / KV_WAVES;
 	long most = p->row_tiles == 1 && by_chunk > by_room ? by_chunk : by_room;
 	most = most < few ? most : few;
 	most = most < KV_SPLITS ? most : KV_SPLITS;
+	if (head_len < 256 && p->row_tiles == 1 && all <= KV_MANY * KV_SHORT)
+		most = 1;
 	p->ws = most > 1 ? wgs * most * p->rows * (head_len + 4) * sizeof(float) : 0;
 }
 
@@ -613,9 +647,16 @@ extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const vo
 	const dim3 rows((unsigned)(a->kv_heads * a->max_rows * G), (unsigned)a->nseq);
 	KV_DISPATCH_HEAD(head_len, D, KV_DISPATCH_TYPE(type, TY, {
 		typedef kv_type<TY>::t t;
-		k_kv_attn<D, TY><<<grid, KV_NT, 0, (hipStream_t)stream>>>(
-			*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window, (float *)ws,
-			p->row_tiles, p->chunk, p->rows);
+		/* (heads of 256 have no room for KV_MANY waves) */
+		constexpr int MANY = D < 256 ? KV_MANY : KV_WAVES;
+		if (p->waves == KV_MANY)
+			k_kv_attn<D, TY, MANY><<<grid, MANY * WAVE, 0, (hipStream_t)stream>>>(
+				*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window,
+				(float *)ws, p->row_tiles, p->chunk, p->rows);
+		else
+			k_kv_attn<D, TY, KV_WAVES><<<grid, KV_NT, 0, (hipStream_t)stream>>>(
+				*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window,
+				(float *)ws, p->row_tiles, p->chunk, p->rows);
 		if (p->splits > 1)
 			k_kv_merge<D, TY><<<rows, KV_NT, 0, (hipStream_t)stream>>>(
 				*a, G, (t *)out, out_stride, window, (const float *)ws, p->row_tiles,

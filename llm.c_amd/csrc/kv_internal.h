@@ -41,6 +41,7 @@ int kv_launch_read(const kv_args *a, int head_len, int type, void *k, void *v, s
 typedef struct kv_plan {
 	int row_tiles; /* tiles of query rows of one (sequence, kv head) */
 	int rows;      /* query rows of a tile, at most */
+	int waves;     /* of a workgroup */
 	int chunk;     /* cache tiles of one workgroup */
 	int splits;    /* workgroups along the cache */
 	size_t ws;     /* bytes of partial results, whatever the window */

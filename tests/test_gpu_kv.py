@@ -12,9 +12,10 @@ codes up to 15, against a largest value of 8 in the group, within 2^-24 * 32 *
 probabilities of 22 bits and the sums over cached rows, or 2^-11 where the
 probabilities are rounded to f16 (bf16 outputs).  A probability times its row's
 value scale is held in f16 parts scaled by a power of two that takes the
-largest value scale dmax into [2^13, 2^15); below f16's smallest normal the last
-part is off by half of 2^-24, which a code of up to 8 multiplies: n cached rows
-add n * 2^-25 * 8 / 2^13 * dmax = n * 2^-35 dmax, whatever the probabilities.
+largest such product into [2^4, 2^11) (its bound into [2^5, 2^11), an exponent
+above); below f16's smallest normal the last part is off by half of 2^-24, which a
+code of up to 8 multiplies: n cached rows add n * 2^-25 * 8 / 2^4 = n * 2^-26
+times the largest value scale dmax, whatever their probabilities.
 Over whole outputs of fp32 the roundings are independent: relative L2 error
 within 4e-6, and within 2^-23 of the largest logit's size more: fp32 holds a
 logit (its sum, its scaling, its distance to the maximum) to half a step, 2^-24
@@ -350,7 +351,7 @@ def check_attention(dev, c, H, ty, window, rng, scale=None, qscale=1.0, pad=0, c
     d = np.abs(c.pool.bytes[..., 34 * D:].view(np.float16).astype(np.float64))
     dmax = d[np.isfinite(d)].max()
     tol = np.abs(want) * ref.HALF_STEP[ty] + mass * (2 * size[..., None] * 2.0 ** -17 + F)
-    tol += max(c.lens) * 2.0 ** -35 * dmax
+    tol += max(c.lens) * 2.0 ** -26 * dmax
     if ty == F16:
         tol += 2.0 ** -25
     err = np.abs(got - want)
