@@ -206,20 +206,16 @@ template <int D, int QP> struct kv_query {
 	floatx4 start[D / 32][16];
 };
 
-/* The groups wave, wave + waves, .. of the lane's row x into LDS (of one row of
- * 16 lanes a quarter each: part); returns what a score is multiplied by to be a
- * logit in powers of two (above 0).  The caller synchronises. */
+/* The groups wave, wave + waves, .. of the lane's row into LDS, from w, the lane's
+ * quarter of each group; returns what a score is multiplied by to be a logit in
+ * powers of two (above 0).  The caller synchronises. */
 template <int D, int QP, int TY>
-__device__ static inline float kv_load_query(kv_query<D, QP> &q, const typename kv_type<TY>::t *x,
-					     float scale, int lane, int wave, int waves)
+__device__ static inline float kv_put_query(kv_query<D, QP> &q, const kv_vec<TY, 8> (&w)[D / 32], float scale,
+					    int lane, int wave, int waves)
 {
 	typedef kv_type<TY> T;
 	const int part = lane / 16;
 	float top = 0.0f;
-	kv_vec<TY, 8> w[D / 32];
-#pragma unroll
-	for (int g = 0; g < D / 32; g++)
-		w[g] = *(const kv_vec<TY, 8> *)(x + 32 * g + 8 * part);
 #pragma unroll
 	for (int g = 0; g < D / 32; g++)
 #pragma unroll
@@ -360,6 +356,16 @@ void k_kv_attn(
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
 	const int kv_head = blockIdx.x % a.kv_heads, rt = blockIdx.x / a.kv_heads;
 	const int split = blockIdx.y, splits = gridDim.y, s = blockIdx.z;
+	/* the wave's tiles t0 + wave, + NW, ..; a lane holds the page of one of the
+	 * next 64.  Without a window the first lot needs no length, only the table's
+	 * bound, and is on its way before the length is known */
+	const int shift = a.page_shift - 5;
+	const int32_t *table = a.table + s * a.table_stride;
+	int page = -1;
+	if (!window) {
+		const int at = (split * chunk + wave + lane * NW) >> shift;
+		page = at < a.table_stride ? table[at] : -1;
+	}
 	const kv_seq sq = kv_sequence(a, s);
 	if (rt * KV_ROWS >= sq.n * G)
 		return;
@@ -368,17 +374,19 @@ void k_kv_attn(
 	const int t1 = min(t0 + chunk, (max(r.last, 0) + KV_TILE - 1) / KV_TILE);
 	if (split > 0 && t0 >= t1)
 		return;
+	kv_vec<TY, 8> qv[L::G];
+#pragma unroll
+	for (int g = 0; g < L::G; g++)
+		qv[g] = *(const kv_vec<TY, 8> *)(q + (size_t)r.row * q_stride + (size_t)r.head * D + 32 * g + 8 * part);
 
-	/* the wave's tiles t0 + wave, + 4, ..; a lane holds the page of one of the
-	 * next 64.  A page outside the pool: its first tile, with every row hidden */
-	const int shift = a.page_shift - 5, n = a.pages ? (t1 - t0 - wave + NW - 1) / NW : 0;
-	int page = -1;
+	/* (a page outside the pool: its first tile, with every row hidden) */
+	const int n = a.pages ? (t1 - t0 - wave + NW - 1) / NW : 0;
 	bool lost = false;
 	const auto tile_of = [&](int i) -> const uint8_t * {
 		const int t = t0 + wave + i * NW;
-		if (i % WAVE == 0) {
+		if (i % WAVE == 0 && (i || window)) {
 			const int tl = t + lane * NW;
-			page = tl < t1 ? a.table[s * a.table_stride + (tl >> shift)] : -1;
+			page = tl < t1 ? table[tl >> shift] : -1;
 		}
 		const int id = __builtin_amdgcn_readlane(page, i % WAVE);
 		lost = (u32)id >= (u32)a.pages;
@@ -396,8 +404,7 @@ void k_kv_attn(
 	} else if (!a.pages && lane == 0) {
 		kv_error(a, HIP_KV_ERR_PAGE);
 	}
-	const float rs = kv_load_query<D, QP, TY>(s_q, q + (size_t)r.row * q_stride + (size_t)r.head * D,
-						  scale, lane, wave, NW);
+	const float rs = kv_put_query<D, QP, TY>(s_q, qv, scale, lane, wave, NW);
 	if (threadIdx.x < KV_ROWS) {
 		s_row[threadIdx.x] = r.valid ? r.row : -1;
 		s_head[threadIdx.x] = r.hi > r.lo ? r.head : ~r.head;
@@ -457,11 +464,9 @@ void k_kv_attn(
 		step(n - 1, std::false_type());
 
 	/* the waves' results: to one reference, then added in wave order */
-	const float sum = KV_CODE_STEP * row_sum(soft.sum); /* the outputs' own factor */
-	if (part == 0) {
+	float sum = KV_CODE_STEP * row_sum(soft.sum); /* the outputs' own factor */
+	if (part == 0)
 		s_ref[wave][lane] = soft.ref;
-		s_sum[wave][lane] = sum;
-	}
 	__syncthreads();
 	float ref = s_ref[0][lane % 16];
 #pragma unroll
@@ -472,22 +477,21 @@ void k_kv_attn(
 #pragma unroll
 		for (int c = 0; c < CT; c++)
 			*(floatx4 *)&s_o[wave][lane % 16][16 * c + 4 * part] = o[c] * factor;
+		if (part == 0)
+			s_sum[wave][lane] = sum * factor;
 	}
 	__syncthreads();
 	const size_t slot = ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
 	float *to = ws + slot * nrows * (D + 4);
-	for (int at = threadIdx.x; at < KV_ROWS * D / 4; at += (NW * WAVE)) {
+	for (int at = threadIdx.x; at < KV_ROWS * D / 4; at += NW * WAVE) {
 		const int i = at / (D / 4), c = at % (D / 4) * 4, row = s_row[i];
 		if (row < 0)
 			break; /* the rows behind are not there either */
-		float high = s_ref[0][i], den = 0.0f;
+		float den = s_sum[0][i];
+		floatx4 y = *(const floatx4 *)&s_o[0][i][c];
 #pragma unroll
-		for (int w = 1; w < NW; w++)
-			high = fmaxf(high, s_ref[w][i]);
-		floatx4 y = (floatx4)0.0f;
-#pragma unroll
-		for (int w = 0; w < NW; w++) {
-			den += s_sum[w][i] * weight(s_ref[w][i], high);
+		for (int w = 1; w < NW; w++) {
+			den += s_sum[w][i];
 			y += *(const floatx4 *)&s_o[w][i][c];
 		}
 		if (splits == 1) {
@@ -501,6 +505,10 @@ void k_kv_attn(
 		}
 		*(floatx4 *)(to + i * (D + 4) + c) = y;
 		if (c == 0) {
+			float high = s_ref[0][i];
+#pragma unroll
+			for (int w = 1; w < NW; w++)
+				high = fmaxf(high, s_ref[w][i]);
 			to[i * (D + 4) + D] = high;
 			to[i * (D + 4) + D + 1] = den;
 		}
