@@ -103,6 +103,21 @@ __device__ static inline float row_sum(float v)
 	return over_row(v, [](float a, float b) { return a + b; });
 }
 
+/* the same of the two lanes l and l + 32 */
+__device__ static inline float half_max(float v)
+{
+	float w = v;
+	asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+	return fmaxf(v, w);
+}
+
+__device__ static inline float half_sum(float v)
+{
+	float w = v;
+	asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
+	return v + w;
+}
+
 /* 2^n, n within -126 .. 127 */
 __device__ static inline float pow2(int n)
 {
@@ -124,13 +139,14 @@ struct kv_span {
 	bool valid;
 };
 
+template <int ROWS = KV_ROWS>
 __device__ static inline kv_span kv_rows_of(const kv_seq &sq, int tile, int G, int kv_head, int window,
 					    int lane)
 {
 	kv_span r;
 	const int base = sq.len - sq.n, all = sq.n * G;
-	const int mine = tile * KV_ROWS + lane % 16, kept = min(mine, all - 1), i = kept / G;
-	const int i0 = __builtin_amdgcn_readlane(i, 0), i1 = __builtin_amdgcn_readlane(i, 15);
+	const int mine = tile * ROWS + lane % ROWS, kept = min(mine, all - 1), i = kept / G;
+	const int i0 = __builtin_amdgcn_readlane(i, 0), i1 = __builtin_amdgcn_readlane(i, ROWS - 1);
 	r.valid = mine < all;
 	r.hi = base + i + 1;
 	r.lo = window ? max(0, r.hi - window) : 0;
@@ -206,48 +222,64 @@ template <int D, int QP> struct kv_query {
 	floatx4 start[D / 32][16];
 };
 
-/* The groups wave, wave + waves, .. of the lane's row into LDS, from w, the lane's
- * quarter of each group; returns what a score is multiplied by to be a logit in
- * powers of two (above 0).  The caller synchronises. */
+/* what a query row whose largest value is top is multiplied by, and its scores
+ * then, to be logits in powers of two (the latter above 0) */
+struct kv_factor {
+	float query, score;
+};
+
+__device__ static inline kv_factor kv_query_factor(float top, float scale)
+{
+	int e = 10 - __builtin_amdgcn_frexp_expf(top);
+	e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 122) : 0;
+	/* a negative scale turns the query around, 0 makes it 0 */
+	return {scale > 0.0f ? pow2(e) : scale < 0.0f ? -pow2(e) : 0.0f,
+		(scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / KV_CODE_STEP) * pow2(-e)};
+}
+
+/* eight channels of a query row in f16 parts, and their sum */
+template <int QP, int TY>
+__device__ static inline float kv_split8(const kv_vec<TY, 8> &w, float factor, half8_t (&f)[QP])
+{
+	float sum = 0.0f;
+#pragma unroll
+	for (int j = 0; j < 8; j++) {
+		const float y = kv_type<TY>::get(w.v[j]) * (kv_small(j) ? 16.0f * factor : factor);
+		float z = (float)(f[0][j] = (_Float16)y);
+		if (QP > 1)
+			z += (float)(f[QP - 1][j] = rest(y, f[0][j]));
+		sum += kv_small(j) ? z * (1.0f / 16.0f) : z;
+	}
+	return sum;
+}
+
+/* The groups g % waves == wave of a tile of query rows into LDS, from w, the lane's
+ * quarter of each group of its row; returns the scores' factor.  The caller
+ * synchronises. */
 template <int D, int QP, int TY>
 __device__ static inline float kv_put_query(kv_query<D, QP> &q, const kv_vec<TY, 8> (&w)[D / 32], float scale,
 					    int lane, int wave, int waves)
 {
-	typedef kv_type<TY> T;
-	const int part = lane / 16;
 	float top = 0.0f;
 #pragma unroll
 	for (int g = 0; g < D / 32; g++)
 #pragma unroll
 		for (int j = 0; j < 8; j++)
-			top = fmaxf(top, fabsf(T::get(w[g].v[j])));
-	top = row_max(top);
-	int e = 10 - __builtin_amdgcn_frexp_expf(top);
-	e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 122) : 0;
-	/* a negative scale turns the query around, 0 makes it 0 */
-	const float sc = scale > 0.0f ? pow2(e) : scale < 0.0f ? -pow2(e) : 0.0f;
+			top = fmaxf(top, fabsf(kv_type<TY>::get(w[g].v[j])));
+	const kv_factor f = kv_query_factor(row_max(top), scale);
 #pragma unroll
 	for (int g = 0; g < D / 32; g++) {
 		if (g % waves != wave)
 			continue;
-		half8_t f[QP];
-		float sum = 0.0f;
-#pragma unroll
-		for (int j = 0; j < 8; j++) {
-			const float y = T::get(w[g].v[j]) * (kv_small(j) ? 16.0f * sc : sc);
-			float z = (float)(f[0][j] = (_Float16)y);
-			if (QP > 1)
-				z += (float)(f[QP - 1][j] = rest(y, f[0][j]));
-			sum += kv_small(j) ? z * (1.0f / 16.0f) : z;
-		}
+		half8_t z[QP];
+		const float sum = row_sum(kv_split8<QP, TY>(w[g], f.query, z));
 #pragma unroll
 		for (int p = 0; p < QP; p++)
-			q.f[p][g][lane] = f[p];
-		sum = row_sum(sum);
-		if (part == 0)
+			q.f[p][g][lane] = z[p];
+		if (lane < 16)
 			q.start[g][lane] = (floatx4)(-8.0f * KV_CODE_STEP * sum);
 	}
-	return (scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / KV_CODE_STEP) * pow2(-e);
+	return f.score;
 }
 
 /* scores of 32 cached rows: 4 part + j of each half */
@@ -291,36 +323,39 @@ struct kv_soft {
 	float ref, sum;
 };
 
-/* probabilities times value scales of 32 cached rows, in f16 parts, 16 times that
- * where the codes have the smaller step; returns what the output so far is
- * multiplied by */
-template <int PP>
-__device__ static inline float kv_softmax(kv_soft &s, const float *x, const half8_t dv, float rs,
-					  half8_t (&pf)[PP])
+/* probabilities times value scales of the lane's N cached rows (8 of 4 lanes, 16
+ * of 2), in f16 parts, 16 times that where the codes have the smaller step: rows
+ * 4 i + j are codes 4 (i / (N / 8)) + j of step i % (N / 8).  Returns what the output
+ * so far is multiplied by. */
+template <int N, int PP>
+__device__ static inline float kv_softmax(kv_soft &s, const float *x, const _Float16 *dv, float rs,
+					  half8_t (&pf)[N / 8][PP])
 {
 	float top = x[0], big = fabsf((float)dv[0]);
 #pragma unroll
-	for (int j = 1; j < 8; j++) {
+	for (int j = 1; j < N; j++) {
 		top = fmaxf(top, x[j]);
 		big = fmaxf(big, fabsf((float)dv[j]));
 	}
 	/* (scales of nothing but zeros: exponent 0) */
-	const float high = row_max(fmaf(top, rs, (float)__builtin_amdgcn_frexp_expf(big)));
+	const float most = fmaf(top, rs, (float)__builtin_amdgcn_frexp_expf(big));
+	const float high = N == 8 ? row_max(most) : half_max(most);
 	const float next = high - s.ref > KV_TOP ? high - KV_REF : s.ref;
 	const float back = weight(s.ref, next);
 	s.ref = next;
 	const float ref = next == -__builtin_inff() ? 0.0f : next, ref16 = ref - 4.0f;
 	float sum = 0.0f, sum16 = 0.0f;
 #pragma unroll
-	for (int j = 0; j < 8; j++) {
+	for (int j = 0; j < N; j++) {
 		const float p = __builtin_amdgcn_exp2f(fmaf(x[j], rs, kv_small(j) ? -ref16 : -ref));
 		(kv_small(j) ? sum16 : sum) += p;
-		float w = fmaf((float)dv[j], p, 0.0f); /* fma: takes the f16 as it is */
+		float w = fmaf((float)dv[j], p, 0.0f); /* fma: takes an f16 as it is */
 		if (PP > 1)
 			asm("" : "+v"(w)); /* once, not once for each part */
-		pf[0][j] = (_Float16)w;
+		const int h = j / 4 % (N / 8), at = j / 4 / (N / 8) * 4 + j % 4;
+		pf[h][0][at] = (_Float16)w;
 		if (PP > 1)
-			pf[PP - 1][j] = rest(w, pf[0][j]);
+			pf[h][PP - 1][at] = rest(w, pf[h][0][at]);
 	}
 	s.sum = s.sum * back + fmaf(sum16, 1.0f / 16.0f, sum);
 	return back;
@@ -424,7 +459,11 @@ void k_kv_attn(
 		if constexpr (more.value)
 			next = tile_of(i + 1);
 		float x[8];
-		half8_t pf[PP], dv = __builtin_bit_cast(half8_t, vd);
+		_Float16 dv[8];
+		half8_t pf[1][PP];
+#pragma unroll
+		for (int j = 0; j < 8; j++)
+			dv[j] = __builtin_bit_cast(half8_t, vd)[j];
 		kv_scores<D, QP>(k, s_q, lane, x);
 		if constexpr (more.value)
 			k.load(next, lane);
@@ -440,7 +479,7 @@ void k_kv_attn(
 			if (hidden && lane == 0)
 				kv_error(a, HIP_KV_ERR_PAGE);
 		}
-		const float back = kv_softmax<PP>(soft, x, dv, rs, pf);
+		const float back = kv_softmax<8, PP>(soft, x, dv, rs, pf);
 		if (__ballot(back != 1.0f)) {
 #pragma unroll
 			for (int c = 0; c < CT; c++)
@@ -451,7 +490,7 @@ void k_kv_attn(
 			const half8_t vf = kv_word8(v.w[c]);
 #pragma unroll
 			for (int p = 0; p < PP; p++)
-				o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[p], o[c], 0, 0, 0);
+				o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[0][p], o[c], 0, 0, 0);
 		}
 		if constexpr (more.value) {
 			vd = kv_value_scales(next + L::V_SCALES, lane);
@@ -597,6 +636,263 @@ __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename k
 }
 
 /*
+ * Many query rows: tiles of 32 of them on v_mfma_f32_32x32x16_f16, which needs half
+ * the instructions and whose lanes hold 16 scores of one query row: the row's
+ * statistics cost half as much a score, and a tile's codes are made f16 once for 32
+ * rows.  The layout serves it as it is: lane l (c = l / 32) takes row l % 32 of the
+ * keys, 8-channel parts c and 2 + c of a group in two steps; the scores of cached
+ * rows 8 i + 4 c + (0 .. 3), i < 4, come out in it, of which i = 0 and 2 are the rows
+ * of value words c, i = 1 and 3 those of words 2 + c.  Row 16 e + m of channel tile
+ * 2 b + u is channel 64 b + 16 (2 e + u) + m, so that a lane's words lie together.
+ *
+ * A workgroup's four waves share 32 query rows and deal the cache's tiles among
+ * them, and the row tiles that see most come first: even the last workgroups are
+ * short.
+ */
+#define KV_WIDE 32
+
+template <int D> struct kv_keys32 {
+	typedef kv_tile<D> L;
+	u32 w[2][L::G];       /* part c and 2 + c of row lane % 32 */
+	u32x4 d[4][L::G / 2]; /* scales of rows 8 i + 4 c + j */
+	__device__ inline void load(const uint8_t *tile, int lane)
+	{
+		typedef uint32_t words __attribute__((ext_vector_type(L::P)));
+		const int c = lane / 32, r = lane % 32;
+#pragma unroll
+		for (int h = 0; h < 2; h++)
+#pragma unroll
+			for (int g = 0; g < L::G; g += L::P) {
+				const words x = ((const words *)tile)[(r / 16 * (L::G / L::P) + g / L::P) * 64 +
+								      16 * (2 * h + c) + r % 16];
+#pragma unroll
+				for (int u = 0; u < L::P; u++)
+					w[h][g + u] = x[u];
+			}
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+#pragma unroll
+			for (int u = 0; u < L::G / 2; u++)
+				d[i][u] = ((const u32x4 *)(tile + L::K_SCALES))[(8 * i + 4 * c) * L::G / 8 + u];
+	}
+	__device__ inline float scale(int i, int j, int g) const
+	{
+		return (float)__builtin_bit_cast(half8_t, d[i][(j * L::G + g) / 8])[(j * L::G + g) % 8];
+	}
+};
+
+template <int D> struct kv_values32 {
+	u32x2 w[D / 64][2]; /* parts c and 2 + c of rows 16 e + m of channel tiles 2 b and 2 b + 1 */
+	u32x2 d[4];         /* scales of rows 8 i + 4 c + j */
+	__device__ inline void load(const uint8_t *tile, int lane)
+	{
+		typedef kv_tile<D> L;
+		const int c = lane / 32, e = lane / 16 % 2, m = lane % 16;
+#pragma unroll
+		for (int b = 0; b < D / 64; b++)
+#pragma unroll
+			for (int h = 0; h < 2; h++)
+				w[b][h] = ((const u32x2 *)(tile + L::V_CODES))[(64 * b + 16 * (2 * h + c) + m) * 2 + e];
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+			d[i] = ((const u32x2 *)(tile + L::V_SCALES))[2 * i + c];
+	}
+	__device__ inline _Float16 scale(int i, int j) const
+	{
+		return __builtin_bit_cast(half4_t, d[i])[j];
+	}
+};
+
+template <int D, int TY>
+__global__ __launch_bounds__(KV_NT) __attribute__((amdgpu_waves_per_eu(2)))
+void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride, int G,
+		    typename kv_type<TY>::t *out, size_t out_stride, float scale, int window, int row_tiles)
+{
+	typedef kv_type<TY> T;
+	typedef kv_tile<D> L;
+	constexpr int QP = TY == HIP_KV_F32 ? 2 : 1, PP = TY == HIP_KV_BF16 ? 1 : 2;
+	constexpr int CT = D / 32;
+	/* the queries' parts, [part][group][step][lane], then the waves' outputs */
+	__shared__ union {
+		half8_t q[QP][L::G][2][WAVE];
+		float o[KV_WAVES][KV_WIDE][D + 4];
+	} sh;
+	__shared__ float s_ref[KV_WAVES][KV_WIDE], s_sum[KV_WAVES][KV_WIDE];
+	__shared__ int s_row[KV_WIDE], s_head[KV_WIDE];
+
+	const int lane = threadIdx.x % WAVE, part = lane / 32;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+	const int kv_head = blockIdx.x % a.kv_heads, s = blockIdx.z;
+	const int rt = row_tiles - 1 - (int)(blockIdx.x / a.kv_heads);
+	const kv_seq sq = kv_sequence(a, s);
+	if (rt * KV_WIDE >= sq.n * G)
+		return;
+	const kv_span r = kv_rows_of<KV_WIDE>(sq, rt, G, kv_head, window, lane);
+	const int t0 = r.first / KV_TILE, t1 = (max(r.last, 0) + KV_TILE - 1) / KV_TILE;
+	float rs;
+	{
+		/* the lane's parts 2 h + c of each group, of which the wave puts its own
+		 * share of the groups into LDS */
+		kv_vec<TY, 8> w[2 * L::G];
+#pragma unroll
+		for (int u = 0; u < 2 * L::G; u++)
+			w[u] = *(const kv_vec<TY, 8> *)(q + (size_t)r.row * q_stride + (size_t)r.head * D +
+							32 * (u / 2) + 8 * (u % 2 * 2 + part));
+		float top = 0.0f;
+#pragma unroll
+		for (int u = 0; u < 2 * L::G; u++)
+#pragma unroll
+			for (int j = 0; j < 8; j++)
+				top = fmaxf(top, fabsf(T::get(w[u].v[j])));
+		const kv_factor f = kv_query_factor(half_max(top), scale);
+		rs = f.score;
+#pragma unroll
+		for (int u = 0; u < 2 * L::G; u++) {
+			if (u % KV_WAVES != wave)
+				continue;
+			half8_t z[QP];
+			kv_split8<QP, TY>(w[u], f.query, z);
+#pragma unroll
+			for (int p = 0; p < QP; p++)
+				sh.q[p][u / 2][u % 2][lane] = z[p];
+		}
+	}
+	if (threadIdx.x < KV_WIDE) {
+		s_row[threadIdx.x] = r.valid ? r.row : -1;
+		s_head[threadIdx.x] = r.hi > r.lo ? r.head : ~r.head;
+	}
+
+	const int shift = a.page_shift - 5;
+	const int32_t *table = a.table + s * a.table_stride;
+	const int n = a.pages ? (t1 - t0 - wave + KV_WAVES - 1) / KV_WAVES : 0;
+	int page = -1;
+	bool lost = false;
+	const auto tile_of = [&](int i) -> const uint8_t * {
+		const int t = t0 + wave + i * KV_WAVES;
+		if (i % WAVE == 0) {
+			const int tl = t + lane * KV_WAVES;
+			page = tl < t1 ? table[tl >> shift] : -1;
+		}
+		const int id = __builtin_amdgcn_readlane(page, i % WAVE);
+		lost = (u32)id >= (u32)a.pages;
+		const size_t at = lost ? 0 : ((((size_t)id * a.kv_heads + kv_head) << shift) + (t & ((1 << shift) - 1)));
+		return a.pool + at * L::BYTES;
+	};
+	kv_keys32<D> k;
+	kv_values32<D> v;
+	if (n > 0) {
+		const uint8_t *tile = tile_of(0);
+		k.load(tile, lane);
+		v.load(tile, lane);
+	} else if (!a.pages && lane == 0) {
+		kv_error(a, HIP_KV_ERR_PAGE);
+	}
+	floatx16 o[CT];
+#pragma unroll
+	for (int c = 0; c < CT; c++)
+		o[c] = (floatx16)0.0f;
+	kv_soft soft = {-__builtin_inff(), 0.0f};
+	__syncthreads();
+
+	for (int i = 0; i < n; i++) {
+		const int t = t0 + wave + i * KV_WAVES;
+		const bool hidden = lost;
+		const uint8_t *next = tile_of(min(i + 1, n - 1));
+		float x[16];
+		_Float16 dv[16];
+#pragma unroll
+		for (int g = 0; g < L::G; g++) {
+			floatx16 acc = (floatx16)0.0f;
+#pragma unroll
+			for (int h = 0; h < 2; h++) {
+				const half8_t kf = kv_word8(k.w[h][g]);
+#pragma unroll
+				for (int p = 0; p < QP; p++)
+					acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, sh.q[p][g][h][lane], acc, 0, 0, 0);
+			}
+#pragma unroll
+			for (int j = 0; j < 16; j++)
+				x[j] = fmaf(k.scale(j / 4, j % 4, g), acc[j], g ? x[j] : 0.0f);
+		}
+		k.load(next, lane);
+#pragma unroll
+		for (int j = 0; j < 16; j++)
+			dv[j] = v.scale(j / 4, j % 4);
+		if (hidden || t * KV_TILE < r.inner0 || (t + 1) * KV_TILE > r.inner1) {
+			const int lo = hidden ? 0x7fffffff : r.lo;
+#pragma unroll
+			for (int j = 0; j < 16; j++) {
+				const int at = t * KV_TILE + 8 * (j / 4) + 4 * part + j % 4;
+				const bool hide = at < lo || at >= r.hi;
+				x[j] = hide ? -__builtin_inff() : x[j];
+				dv[j] = hide ? (_Float16)0.0f : dv[j];
+			}
+			if (hidden && lane == 0)
+				kv_error(a, HIP_KV_ERR_PAGE);
+		}
+		half8_t pf[2][PP];
+		const float back = kv_softmax<16, PP>(soft, x, dv, rs, pf);
+		if (__ballot(back != 1.0f)) {
+#pragma unroll
+			for (int c = 0; c < CT; c++)
+				o[c] *= back;
+		}
+#pragma unroll
+		for (int c = 0; c < CT; c++)
+#pragma unroll
+			for (int h = 0; h < 2; h++) {
+				const half8_t vf = kv_word8(v.w[c / 2][h][c % 2]);
+#pragma unroll
+				for (int p = 0; p < PP; p++)
+					o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[h][p], o[c], 0, 0, 0);
+			}
+		v.load(next, lane);
+	}
+
+	/* the waves' results: to one reference, then added in wave order */
+	const float sum = KV_CODE_STEP * half_sum(soft.sum);
+	if (part == 0)
+		s_ref[wave][lane] = soft.ref;
+	__syncthreads();
+	float ref = s_ref[0][lane % 32];
+#pragma unroll
+	for (int w = 1; w < KV_WAVES; w++)
+		ref = fmaxf(ref, s_ref[w][lane % 32]);
+	const float factor = weight(soft.ref, ref);
+	if (part == 0)
+		s_sum[wave][lane] = sum * factor;
+#pragma unroll
+	for (int c = 0; c < CT; c++)
+#pragma unroll
+		for (int i = 0; i < 4; i++) {
+			floatx4 y;
+#pragma unroll
+			for (int j = 0; j < 4; j++)
+				y[j] = o[c][4 * i + j] * factor;
+			*(floatx4 *)&sh.o[wave][lane % 32][64 * (c / 2) + 16 * (i / 2 * 2 + c % 2) +
+							    8 * (i % 2) + 4 * part] = y;
+		}
+	__syncthreads();
+	for (int at = threadIdx.x; at < KV_WIDE * D / 4; at += KV_NT) {
+		const int i = at / (D / 4), c = at % (D / 4) * 4, row = s_row[i], head = s_head[i];
+		if (row < 0)
+			break;
+		float den = s_sum[0][i];
+		floatx4 y = *(const floatx4 *)&sh.o[0][i][c];
+#pragma unroll
+		for (int w = 1; w < KV_WAVES; w++) {
+			den += s_sum[w][i];
+			y += *(const floatx4 *)&sh.o[w][i][c];
+		}
+		kv_vec<TY, 4> z;
+#pragma unroll
+		for (int u = 0; u < 4; u++)
+			z.v[u] = T::put(head >= 0 ? y[u] / den : 0.0f);
+		*(kv_vec<TY, 4> *)(out + row * out_stride + (size_t)(head < 0 ? ~head : head) * D + c) = z;
+	}
+}
+
+/*
  * Along the cache.  A workgroup of KV_MANY waves (three a SIMD: all that their
  * registers allow) takes a row tile's whole cache while that leaves each wave
  * KV_SHORT tiles or fewer: pieces would need a second launch to add them up
@@ -622,6 +918,13 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	p->row_tiles = (int)((rows + KV_ROWS - 1) / KV_ROWS);
 	p->rows = (int)(rows < KV_ROWS ? rows : KV_ROWS);
 	const size_t wgs = (size_t)a->nseq * a->kv_heads * p->row_tiles;
+	p->wide = head_len < 256 && rows >= 2 * KV_WIDE && wgs >= 512;
+	if (p->wide) {
+		p->row_tiles = (int)((rows + KV_WIDE - 1) / KV_WIDE);
+		p->splits = 1;
+		p->ws = 0;
+		return;
+	}
 	const size_t room = head_len == 64 ? 1024 : head_len == 128 ? 512 : 256;
 	const long by_room = wgs < room ? (long)(room / wgs) : 1;
 	p->waves = head_len < 256 && p->row_tiles == 1 && tiles <= KV_MANY * KV_SHORT ? KV_MANY : KV_WAVES;
@@ -655,6 +958,13 @@ extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const vo
 	const dim3 rows((unsigned)(a->kv_heads * a->max_rows * G), (unsigned)a->nseq);
 	KV_DISPATCH_HEAD(head_len, D, KV_DISPATCH_TYPE(type, TY, {
 		typedef kv_type<TY>::t t;
+		constexpr int WIDE = D < 256 ? D : 128; /* heads of 256 have no registers for it */
+		if (p->wide) {
+			k_kv_attn_wide<WIDE, TY><<<grid, KV_NT, 0, (hipStream_t)stream>>>(
+				*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window,
+				p->row_tiles);
+			return (int)hipGetLastError();
+		}
 		/* (heads of 256 have no room for KV_MANY waves) */
 		constexpr int MANY = D < 256 ? KV_MANY : KV_WAVES;
 		if (p->waves == KV_MANY)

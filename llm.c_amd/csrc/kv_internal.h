@@ -40,6 +40,7 @@ int kv_launch_read(const kv_args *a, int head_len, int type, void *k, void *v, s
 /* how an attention call is cut up, from the host's bounds alone */
 typedef struct kv_plan {
 	int row_tiles; /* tiles of query rows of one (sequence, kv head) */
+	int wide;      /* tiles of 32 query rows */
 	int rows;      /* query rows of a tile, at most */
 	int waves;     /* of a workgroup */
 	int chunk;     /* cache tiles of one workgroup */

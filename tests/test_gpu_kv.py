@@ -388,6 +388,28 @@ def test_attention_long(dev, ty, D, KH, H, rows, lens, window):
     check_attention(dev, c, H, ty, window, rng, qscale=2.0)
 
 
+@pytest.mark.parametrize("ty,D,KH,H,rows,lens,page,window", (
+    (F32, 64, 16, 16, [270] * 4, [270, 300, 333, 1000], 32, 0),
+    (F16, 128, 4, 16, [130] * 9, [130, 131, 160, 700, 130, 65, 10, 400, 223], 64, 0),
+    (BF16, 128, 16, 32, [131] * 4, [131, 290, 500, 140], 32, 100),
+    (F32, 256, 8, 16, [140] * 8, [140, 141, 200, 300, 139, 150, 160, 170], 64, 0),
+    (F32, 128, 8, 32, [530] * 4, [530, 531, 900, 300], 256, 0),
+    (BF16, 128, 16, 64, [515, 20, 0, 511], [700, 20, 0, 1300], 128, 300),
+    (F16, 64, 16, 48, [700, 701], [700, 1111], 64, 0),
+    (BF16, 64, 16, 16, [1025] * 4, [1025, 1030, 1100, 1500], 64, 50),
+))
+def test_attention_of_many_rows(dev, ty, D, KH, H, rows, lens, page, window):
+    """Calls with enough query rows to fill the chip, against a sample of them:
+    the first and last rows of sequences and of tiles, and others."""
+    rng = np.random.default_rng(sum(lens))
+    c = Case(dev, rng, rows, lens, page, KH, D)
+    start = c.start[:-1]
+    at = np.concatenate([start, start + 1, start + 15, start + 16, start + 64, c.start[1:] - 1,
+                         rng.integers(0, c.T, 6)])
+    check = sorted({int(i) for i in at if 0 <= i < c.T})
+    check_attention(dev, c, H, ty, window, rng, qscale=2.0, pad=8, check=check)
+
+
 @pytest.mark.parametrize("qscale,scale", ((1e-20, 1.0), (1e-38, 1.0), (30.0, None), (1e6, 1e-7), (1.0, 0.0),
                                           (1.0, -0.1)))
 def test_attention_sizes_of_queries(dev, qscale, scale):
