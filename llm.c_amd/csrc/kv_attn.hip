@@ -63,11 +63,16 @@ __device__ static constexpr bool kv_small(int j)
 	return j % 4 < 2;
 }
 
-/* a word's codes less 8, in the same steps */
-__device__ static inline half8_t kv_word8(u32 w)
+/* 8 in the steps of a word's codes, and the codes less that */
+__device__ static inline half8_t kv_surplus8()
 {
 	const _Float16 a = (_Float16)(8.0f * KV_CODE_STEP / 16.0f), b = (_Float16)(8.0f * KV_CODE_STEP);
-	return kv_word(w) - half8_t{a, a, b, b, a, a, b, b};
+	return half8_t{a, a, b, b, a, a, b, b};
+}
+
+__device__ static inline half8_t kv_word8(u32 w)
+{
+	return kv_word(w) - kv_surplus8();
 }
 
 /* x = hi + lo in f16; the products with the hidden -1 stay fused with the
@@ -79,43 +84,44 @@ __device__ static inline _Float16 rest(float x, _Float16 hi)
 	return (_Float16)fmaf((float)hi, minus, x);
 }
 
-/* the lane's value and those of the three others that share its query row, put
- * together by fn.  The swaps exchange the odd rows of 16 lanes (the upper 32)
- * of the first register with the even ones (the lower) of the second, so of a
- * value and its copy both then hold both.  (In assembly: the builtin hands out its
- * first result twice.  The s_nop are the two wait states after a VALU write.) */
-template <class Fn> __device__ static inline float over_row(float v, Fn fn)
+/* v and its copy after an exchange of the odd rows of 16 lanes (SPAN 16; the
+ * upper 32 lanes, SPAN 32) of the one with the even rows (the lower) of the other:
+ * both lanes of a pair that far apart then hold both of their values */
+template <int SPAN> __device__ static inline float2 swapped(float v)
 {
-	float w = v;
-	asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(v), "+v"(w));
-	w = v = fn(v, w);
-	asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
-	return fn(v, w);
+	const u32 u = __builtin_bit_cast(u32, v);
+	const auto t = SPAN == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false)
+				  : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+	const u32 x = t[0], y = t[1];
+	return make_float2(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
 }
 
+/* the largest (the sum) over the four lanes l % 16 that share a query row */
 __device__ static inline float row_max(float v)
 {
-	return over_row(v, [](float a, float b) { return fmaxf(a, b); });
+	float2 t = swapped<16>(v);
+	t = swapped<32>(fmaxf(t.x, t.y));
+	return fmaxf(t.x, t.y);
 }
 
 __device__ static inline float row_sum(float v)
 {
-	return over_row(v, [](float a, float b) { return a + b; });
+	float2 t = swapped<16>(v);
+	t = swapped<32>(t.x + t.y);
+	return t.x + t.y;
 }
 
-/* the same of the two lanes l and l + 32 */
+/* the same of the two lanes l % 32 */
 __device__ static inline float half_max(float v)
 {
-	float w = v;
-	asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
-	return fmaxf(v, w);
+	const float2 t = swapped<32>(v);
+	return fmaxf(t.x, t.y);
 }
 
 __device__ static inline float half_sum(float v)
 {
-	float w = v;
-	asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(v), "+v"(w));
-	return v + w;
+	const float2 t = swapped<32>(v);
+	return t.x + t.y;
 }
 
 /* 2^n, n within -126 .. 127 */
@@ -284,8 +290,9 @@ __device__ static inline float kv_put_query(kv_query<D, QP> &q, const kv_vec<TY,
 
 /* scores of 32 cached rows: 4 part + j of each half */
 template <int D, int QP>
-__device__ static inline void kv_scores(const kv_keys<D> &k, const kv_query<D, QP> &q, int lane, float *x)
+__device__ static inline floatx8 kv_scores(const kv_keys<D> &k, const kv_query<D, QP> &q, int lane)
 {
+	floatx8 x;
 #pragma unroll
 	for (int g = 0; g < D / 32; g++) {
 		half8_t f[QP];
@@ -305,6 +312,7 @@ __device__ static inline void kv_scores(const kv_keys<D> &k, const kv_query<D, Q
 				x[4 * h + j] = fmaf(k.scale(h, j, g), acc[j], g ? x[4 * h + j] : 0.0f);
 		}
 	}
+	return x;
 }
 
 /*
@@ -328,15 +336,24 @@ struct kv_soft {
  * 4 i + j are codes 4 (i / (N / 8)) + j of step i % (N / 8).  Returns what the output
  * so far is multiplied by. */
 template <int N, int PP>
-__device__ static inline float kv_softmax(kv_soft &s, const float *x, const _Float16 *dv, float rs,
+__device__ static inline float kv_softmax(kv_soft &s, const float *x, const half4_t *dv, float rs,
 					  half8_t (&pf)[N / 8][PP])
 {
-	float top = x[0], big = fabsf((float)dv[0]);
+	float top = x[0];
 #pragma unroll
-	for (int j = 1; j < N; j++) {
+	for (int j = 1; j < N; j++)
 		top = fmaxf(top, x[j]);
-		big = fmaxf(big, fabsf((float)dv[j]));
+	/* f16 without their sign order as whole numbers do */
+	ushort2_t most2 = {0, 0};
+#pragma unroll
+	for (int i = 0; i < N / 4; i++) {
+		const u32x2 w = __builtin_bit_cast(u32x2, dv[i]);
+		const u32 a = w.x & 0x7fff7fffu, b = w.y & 0x7fff7fffu; /* (bit_cast takes no element) */
+		most2 = __builtin_elementwise_max(most2, __builtin_bit_cast(ushort2_t, a));
+		most2 = __builtin_elementwise_max(most2, __builtin_bit_cast(ushort2_t, b));
 	}
+	const unsigned short most1 = most2.x > most2.y ? most2.x : most2.y;
+	const float big = (float)__builtin_bit_cast(_Float16, most1);
 	/* (scales of nothing but zeros: exponent 0) */
 	const float most = fmaf(top, rs, (float)__builtin_amdgcn_frexp_expf(big));
 	const float high = N == 8 ? row_max(most) : half_max(most);
@@ -349,7 +366,7 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const _Flo
 	for (int j = 0; j < N; j++) {
 		const float p = __builtin_amdgcn_exp2f(fmaf(x[j], rs, kv_small(j) ? -ref16 : -ref));
 		(kv_small(j) ? sum16 : sum) += p;
-		float w = fmaf((float)dv[j], p, 0.0f); /* fma: takes an f16 as it is */
+		float w = fmaf((float)dv[j / 4][j % 4], p, 0.0f); /* fma: takes an f16 as it is */
 		if (PP > 1)
 			asm("" : "+v"(w)); /* once, not once for each part */
 		const int h = j / 4 % (N / 8), at = j / 4 / (N / 8) * 4 + j % 4;
@@ -458,13 +475,12 @@ void k_kv_attn(
 		const uint8_t *next = NULL;
 		if constexpr (more.value)
 			next = tile_of(i + 1);
-		float x[8];
-		_Float16 dv[8];
+		const half8_t vd8 = __builtin_bit_cast(half8_t, vd);
+		half4_t dv[2] = {vd8.lo, vd8.hi};
 		half8_t pf[1][PP];
-#pragma unroll
-		for (int j = 0; j < 8; j++)
-			dv[j] = __builtin_bit_cast(half8_t, vd)[j];
-		kv_scores<D, QP>(k, s_q, lane, x);
+		floatx8 x = kv_scores<D, QP>(k, s_q, lane);
+		/* the scales are used up before their registers are loaded again */
+		asm volatile("" : "+v"(x) : : "memory");
 		if constexpr (more.value)
 			k.load(next, lane);
 		if (hidden || t * KV_TILE < r.inner0 || (t + 1) * KV_TILE > r.inner1) {
@@ -474,12 +490,12 @@ void k_kv_attn(
 				const int at = t * KV_TILE + 16 * (j / 4) + 4 * part + j % 4;
 				const bool hide = at < lo || at >= r.hi;
 				x[j] = hide ? -__builtin_inff() : x[j];
-				dv[j] = hide ? (_Float16)0.0f : dv[j];
+				dv[j / 4][j % 4] = hide ? (_Float16)0.0f : dv[j / 4][j % 4];
 			}
 			if (hidden && lane == 0)
 				kv_error(a, HIP_KV_ERR_PAGE);
 		}
-		const float back = kv_softmax<8, PP>(soft, x, dv, rs, pf);
+		const float back = kv_softmax<8, PP>(soft, (const float *)&x, dv, rs, pf);
 		if (__ballot(back != 1.0f)) {
 #pragma unroll
 			for (int c = 0; c < CT; c++)
@@ -655,6 +671,7 @@ template <int D> struct kv_keys32 {
 	typedef kv_tile<D> L;
 	u32 w[2][L::G];       /* part c and 2 + c of row lane % 32 */
 	u32x4 d[4][L::G / 2]; /* scales of rows 8 i + 4 c + j */
+	u32 own[L::G / 2];    /* of row lane % 32 */
 	__device__ inline void load(const uint8_t *tile, int lane)
 	{
 		typedef uint32_t words __attribute__((ext_vector_type(L::P)));
@@ -674,6 +691,21 @@ template <int D> struct kv_keys32 {
 #pragma unroll
 			for (int u = 0; u < L::G / 2; u++)
 				d[i][u] = ((const u32x4 *)(tile + L::K_SCALES))[(8 * i + 4 * c) * L::G / 8 + u];
+#pragma unroll
+		for (int u = 0; u < L::G / 2; u++)
+			own[u] = ((const u32 *)(tile + L::K_SCALES))[r * L::G / 2 + u];
+	}
+	/* the row's scales, and again with a 64th of them: the operand that
+	 * kv_attn_wide's surplus is multiplied with */
+	__device__ inline half8_t scales8() const
+	{
+		u32 w[4] = {};
+#pragma unroll
+		for (int u = 0; u < L::G / 2; u++) {
+			w[u] = own[u];
+			w[2 + u] = __builtin_bit_cast(u32, __builtin_bit_cast(half2_t, own[u]) * (half2_t)(_Float16)0.015625f);
+		}
+		return as_half8(w[0], w[1], w[2], w[3]);
 	}
 	__device__ inline float scale(int i, int j, int g) const
 	{
@@ -696,10 +728,6 @@ template <int D> struct kv_values32 {
 #pragma unroll
 		for (int i = 0; i < 4; i++)
 			d[i] = ((const u32x2 *)(tile + L::V_SCALES))[2 * i + c];
-	}
-	__device__ inline _Float16 scale(int i, int j) const
-	{
-		return __builtin_bit_cast(half4_t, d[i])[j];
 	}
 };
 
@@ -730,6 +758,7 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 	const kv_span r = kv_rows_of<KV_WIDE>(sq, rt, G, kv_head, window, lane);
 	const int t0 = r.first / KV_TILE, t1 = (max(r.last, 0) + KV_TILE - 1) / KV_TILE;
 	float rs;
+	half8_t surplus = (half8_t)(_Float16)0.0f;
 	{
 		/* the lane's parts 2 h + c of each group, of which the wave puts its own
 		 * share of the groups into LDS */
@@ -747,14 +776,23 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 		const kv_factor f = kv_query_factor(half_max(top), scale);
 		rs = f.score;
 #pragma unroll
-		for (int u = 0; u < 2 * L::G; u++) {
-			if (u % KV_WAVES != wave)
-				continue;
-			half8_t z[QP];
-			kv_split8<QP, TY>(w[u], f.query, z);
+		for (int u = 0; u < L::G; u++) {
+			float sum = 0.0f;
 #pragma unroll
-			for (int p = 0; p < QP; p++)
-				sh.q[p][u / 2][u % 2][lane] = z[p];
+			for (int h = 0; h < 2; h++) {
+				half8_t z[QP];
+				sum += kv_split8<QP, TY>(w[2 * u + h], f.query, z);
+#pragma unroll
+				for (int p = 0; p < QP; p++)
+					if (u % KV_WAVES == wave)
+						sh.q[p][u][h][lane] = z[p];
+			}
+			/* in two f16 parts, of 11 bits and of the rest times 64 */
+			sum = -8.0f * KV_CODE_STEP * half_sum(sum);
+			if (part == 0) {
+				surplus[u] = (_Float16)sum;
+				surplus[4 + u] = (_Float16)(64.0f * (sum - (float)surplus[u]));
+			}
 		}
 	}
 	if (threadIdx.x < KV_WIDE) {
@@ -787,7 +825,12 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 	} else if (!a.pages && lane == 0) {
 		kv_error(a, HIP_KV_ERR_PAGE);
 	}
-	floatx16 o[CT];
+	/* For bf16 outputs the values' surplus of 8 leaves at the end, as 8 times the
+	 * sum of the (rounded) probabilities times scales: it outweighs the output by
+	 * up to 3 times the root of the rows that matter, which fp32 sums have to
+	 * spare over bf16's 8 bits. */
+	constexpr bool LATE = TY == HIP_KV_BF16;
+	floatx16 o[CT], late = (floatx16)0.0f;
 #pragma unroll
 	for (int c = 0; c < CT; c++)
 		o[c] = (floatx16)0.0f;
@@ -798,26 +841,28 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 		const int t = t0 + wave + i * KV_WAVES;
 		const bool hidden = lost;
 		const uint8_t *next = tile_of(min(i + 1, n - 1));
-		float x[16];
-		_Float16 dv[16];
+		half4_t dv[4];
+		floatx16 x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k.scales8(), surplus, (floatx16)0.0f, 0, 0, 0);
 #pragma unroll
 		for (int g = 0; g < L::G; g++) {
 			floatx16 acc = (floatx16)0.0f;
 #pragma unroll
 			for (int h = 0; h < 2; h++) {
-				const half8_t kf = kv_word8(k.w[h][g]);
+				const half8_t kf = kv_word(k.w[h][g]);
 #pragma unroll
 				for (int p = 0; p < QP; p++)
 					acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, sh.q[p][g][h][lane], acc, 0, 0, 0);
 			}
 #pragma unroll
 			for (int j = 0; j < 16; j++)
-				x[j] = fmaf(k.scale(j / 4, j % 4, g), acc[j], g ? x[j] : 0.0f);
+				x[j] = fmaf(k.scale(j / 4, j % 4, g), acc[j], x[j]);
 		}
+		/* the scales are used up before their registers are loaded again */
+		asm volatile("" : "+v"(x) : : "memory");
 		k.load(next, lane);
 #pragma unroll
-		for (int j = 0; j < 16; j++)
-			dv[j] = v.scale(j / 4, j % 4);
+		for (int j = 0; j < 4; j++)
+			dv[j] = __builtin_bit_cast(half4_t, v.d[j]);
 		if (hidden || t * KV_TILE < r.inner0 || (t + 1) * KV_TILE > r.inner1) {
 			const int lo = hidden ? 0x7fffffff : r.lo;
 #pragma unroll
@@ -825,14 +870,15 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 				const int at = t * KV_TILE + 8 * (j / 4) + 4 * part + j % 4;
 				const bool hide = at < lo || at >= r.hi;
 				x[j] = hide ? -__builtin_inff() : x[j];
-				dv[j] = hide ? (_Float16)0.0f : dv[j];
+				dv[j / 4][j % 4] = hide ? (_Float16)0.0f : dv[j / 4][j % 4];
 			}
 			if (hidden && lane == 0)
 				kv_error(a, HIP_KV_ERR_PAGE);
 		}
 		half8_t pf[2][PP];
-		const float back = kv_softmax<16, PP>(soft, x, dv, rs, pf);
+		const float back = kv_softmax<16, PP>(soft, (const float *)&x, dv, rs, pf);
 		if (__ballot(back != 1.0f)) {
+			late *= back;
 #pragma unroll
 			for (int c = 0; c < CT; c++)
 				o[c] *= back;
@@ -841,13 +887,22 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 		for (int c = 0; c < CT; c++)
 #pragma unroll
 			for (int h = 0; h < 2; h++) {
-				const half8_t vf = kv_word8(v.w[c / 2][h][c % 2]);
+				const u32 w = v.w[c / 2][h][c % 2];
+				const half8_t vf = LATE ? kv_word(w) : kv_word8(w);
 #pragma unroll
 				for (int p = 0; p < PP; p++)
 					o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[h][p], o[c], 0, 0, 0);
 			}
+		if (LATE)
+#pragma unroll
+			for (int h = 0; h < 2; h++)
+				late = __builtin_amdgcn_mfma_f32_32x32x16_f16(kv_surplus8(), pf[h][0], late, 0, 0, 0);
 		v.load(next, lane);
 	}
+	if (LATE)
+#pragma unroll
+		for (int c = 0; c < CT; c++)
+			o[c] -= late;
 
 	/* the waves' results: to one reference, then added in wave order */
 	const float sum = KV_CODE_STEP * half_sum(soft.sum);
