@@ -49,6 +49,13 @@ __device__ static inline double2 kv_turn(const hip_rope &R, int pos, int i)
 	return make_double2(c * R.mag, s * R.mag);
 }
 
+/* A row's (cos, sin) in LDS, by pair: one place is left free after eight, so that
+ * lanes that each read eight or four in a row do not meet in the same banks */
+__host__ __device__ static inline int kv_slot(int pair)
+{
+	return pair + (pair >> 3);
+}
+
 /* 16 bytes of values */
 template <int TY> struct kv_wide {
 	static constexpr int N = 16 / sizeof(typename kv_type<TY>::t);
@@ -59,8 +66,8 @@ template <int TY> struct kv_wide {
  * cs and sn belong to channel c's pair */
 __device__ static inline float kv_turned(float own, float other, bool first, double2 t)
 {
-	const double a = (double)own * t.x, b = (double)other * t.y;
-	return (float)(first ? a - b : a + b);
+	const double b = (double)other * t.y;
+	return (float)fma((double)own, t.x, first ? -b : b);
 }
 
 /* The vector x[c0 ..] of a head row with what its turn needs: in HALVES, where half
@@ -92,7 +99,7 @@ template <int TY> struct kv_turn_in {
 			for (int u = 0; u < N; u += 2) {
 				if (c0 + u >= rot)
 					continue;
-				const double2 t = turns[(c0 + u) / 2];
+				const double2 t = turns[kv_slot((c0 + u) / 2)];
 				const float a = y[u], b = y[u + 1];
 				y[u] = kv_turned(a, b, true, t);
 				y[u + 1] = kv_turned(b, a, false, t);
@@ -101,13 +108,13 @@ template <int TY> struct kv_turn_in {
 			const bool first = c0 < half;
 #pragma unroll
 			for (int u = 0; u < N; u++)
-				y[u] = kv_turned(y[u], T::get(other.v[u]), first, turns[(first ? c0 : c0 - half) + u]);
+				y[u] = kv_turned(y[u], T::get(other.v[u]), first, turns[kv_slot((first ? c0 : c0 - half) + u)]);
 		} else {
 			for (int u = 0; u < N && c0 + u < rot; u++) {
 				const int c = c0 + u;
 				const bool first = c < half;
 				y[u] = kv_turned(y[u], T::get(x[first ? c + half : c - half]), first,
-						 turns[first ? c : c - half]);
+						 turns[kv_slot(first ? c : c - half)]);
 			}
 		}
 	}
@@ -132,14 +139,14 @@ __global__ __launch_bounds__(KV_NT) void k_kv_rope(
 	int heads_per)
 {
 	typedef kv_type<TY> T;
-	extern __shared__ double2 turns[]; /* [rows][rot / 2] */
-	const int half = (int)R.rot / 2, r0 = blockIdx.x * per, n = min(per, rows - r0);
+	extern __shared__ double2 turns[]; /* [rows][kv_slot(rot / 2)] */
+	const int half = (int)R.rot / 2, slots = kv_slot(half), r0 = blockIdx.x * per, n = min(per, rows - r0);
 	const bool pairs = R.layout == HIP_ROPE_PAIRS;
 	x += (size_t)blockIdx.y * heads_per * head_len;
 	out += (size_t)blockIdx.y * heads_per * head_len;
 	heads = min(heads_per, heads - (int)blockIdx.y * heads_per);
 	for (int at = threadIdx.x; at < n * half; at += KV_NT)
-		turns[at] = kv_turn(R, pos[r0 + at / half], at % half);
+		turns[at / half * slots + kv_slot(at % half)] = kv_turn(R, pos[r0 + at / half], at % half);
 	__syncthreads();
 	if (VEC) {
 		constexpr int N = kv_wide<TY>::N;
@@ -153,7 +160,7 @@ __global__ __launch_bounds__(KV_NT) void k_kv_rope(
 			const int c = v * N, c0 = pairs || c < half ? c : c + half;
 			const typename T::t *xr = x + (size_t)(r0 + r) * x_stride + h * head_len + c0;
 			typename T::t *yr = out + (size_t)(r0 + r) * out_stride + h * head_len + c0;
-			const double2 *t = turns + r * half;
+			const double2 *t = turns + r * slots;
 			vec a = *(const vec *)xr;
 			if (pairs) {
 #pragma unroll
@@ -161,7 +168,7 @@ __global__ __launch_bounds__(KV_NT) void k_kv_rope(
 					if (c + u >= 2 * half)
 						continue;
 					const float y1 = T::get(a.v[u]), y2 = T::get(a.v[u + 1]);
-					const double2 z = t[(c + u) / 2];
+					const double2 z = t[kv_slot((c + u) / 2)];
 					a.v[u] = T::put(kv_turned(y1, y2, true, z));
 					a.v[u + 1] = T::put(kv_turned(y2, y1, false, z));
 				}
@@ -170,8 +177,8 @@ __global__ __launch_bounds__(KV_NT) void k_kv_rope(
 #pragma unroll
 				for (int u = 0; u < N; u++) {
 					const float y1 = T::get(a.v[u]), y2 = T::get(b.v[u]);
-					a.v[u] = T::put(kv_turned(y1, y2, true, t[c + u]));
-					b.v[u] = T::put(kv_turned(y2, y1, false, t[c + u]));
+					a.v[u] = T::put(kv_turned(y1, y2, true, t[kv_slot(c + u)]));
+					b.v[u] = T::put(kv_turned(y2, y1, false, t[kv_slot(c + u)]));
 				}
 				*(vec *)(yr + half) = b;
 			}
@@ -179,9 +186,9 @@ __global__ __launch_bounds__(KV_NT) void k_kv_rope(
 		}
 		return;
 	}
-	const int slots = half + (head_len - 2 * half), all = n * heads * slots;
+	const int own = half + (head_len - 2 * half), all = n * heads * own;
 	for (int at = threadIdx.x; at < all; at += KV_NT) {
-		const int i = at % slots, h = at / slots % heads, r = at / slots / heads;
+		const int i = at % own, h = at / own % heads, r = at / own / heads;
 		const typename T::t *xr = x + (size_t)(r0 + r) * x_stride + h * head_len;
 		typename T::t *yr = out + (size_t)(r0 + r) * out_stride + h * head_len;
 		if (i >= half) { /* a channel that passes */
@@ -190,8 +197,8 @@ __global__ __launch_bounds__(KV_NT) void k_kv_rope(
 		}
 		const int c1 = pairs ? 2 * i : i, c2 = pairs ? 2 * i + 1 : i + half;
 		const float a = T::get(xr[c1]), b = T::get(xr[c2]);
-		yr[c1] = T::put(kv_turned(a, b, true, turns[r * half + i]));
-		yr[c2] = T::put(kv_turned(b, a, false, turns[r * half + i]));
+		yr[c1] = T::put(kv_turned(a, b, true, turns[r * slots + kv_slot(i)]));
+		yr[c2] = T::put(kv_turned(b, a, false, turns[r * slots + kv_slot(i)]));
 	}
 }
 
@@ -199,63 +206,76 @@ __global__ __launch_bounds__(KV_NT) void k_kv_rope(
 /* storing rows                                                           */
 /* ---------------------------------------------------------------------- */
 
-/* the scale of a group whose smallest and largest values are lo and hi */
-__device__ static inline _Float16 kv_scale(float lo, float hi)
+/* A value's bits turned left by one order values by size, the negative one of two
+ * equal last, and NaN behind all */
+__device__ static inline u32 kv_key(float v)
 {
-	const float m = hi > -lo ? hi : lo;
-	return (_Float16)fminf(fmaxf(m * -0.125f, -65504.0f), 65504.0f);
+	return kv_rotr(__builtin_bit_cast(u32, v), 31);
 }
 
-/* floor(x / d + 8.5) within 0 .. 15, exactly: the quotient's estimate is
- * put right by the sign of x - (q - 8.5) d, which one fma has (the product
- * holds 16 bits).  inv is 1 / |d|. */
-__device__ static inline u32 kv_code(float x, float d, float inv)
-{
-	const float y = d < 0.0f ? -x : x, w = fabsf(d);
-	float q = floorf(fminf(fmaxf(y * inv, -8.5f), 8.5f) + 8.5f);
-	q = fmaf(8.5f - q, w, y) < 0.0f ? q - 1.0f : fmaf(7.5f - q, w, y) >= 0.0f ? q + 1.0f : q;
-	return w == 0.0f ? 8 : (u32)fminf(fmaxf(q, 0.0f), 15.0f);
-}
-
-/* the smallest (the largest) of the LANES lanes around this one: within 16 lanes
- * by mirrored halves, which after the first steps hold equal values */
-template <int CTRL> __device__ static inline float kv_dpp(float v)
-{
-	return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
-}
-
-template <int LANES, class Fn> __device__ static inline float kv_over(float v, Fn fn)
+/* the largest key of the LANES lanes around this one: within 16 lanes by mirrored
+ * halves, which after the first steps hold equal values */
+template <int LANES> __device__ static inline u32 kv_most(u32 v)
 {
 	if (LANES > 1)
-		v = fn(v, kv_dpp<0xb1>(v)); /* lane ^ 1 */
+		v = max(v, (u32)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, true)); /* lane ^ 1 */
 	if (LANES > 2)
-		v = fn(v, kv_dpp<0x4e>(v)); /* lane ^ 2 */
+		v = max(v, (u32)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, true)); /* lane ^ 2 */
 	if (LANES > 4)
-		v = fn(v, kv_dpp<0x141>(v)); /* 7 - lane of 8 */
+		v = max(v, (u32)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true)); /* 7 - lane of 8 */
 	if (LANES > 8)
-		v = fn(v, kv_dpp<0x140>(v)); /* 15 - lane of 16 */
-	if (LANES > 16)
-		v = fn(v, __shfl_xor(v, 16, WAVE));
-	if (LANES > 32)
-		v = fn(v, __shfl_xor(v, 32, WAVE));
+		v = max(v, (u32)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true)); /* 15 - lane of 16 */
+	if (LANES > 16) {
+		const auto t = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+		v = max((u32)t[0], (u32)t[1]);
+	}
+	if (LANES > 32) {
+		const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+		v = max((u32)t[0], (u32)t[1]);
+	}
 	return v;
 }
 
-/* the scale of the group of values that LANES lanes hold N each of; NaN if one of
- * them is */
-template <int LANES, int N> __device__ static inline _Float16 kv_group(const float *y)
+/*
+ * The scale of a group of values that LANES lanes hold N each of, and the lane's
+ * codes floor(y / d + 8.5) within 0 .. 15, exactly.  In fp32, y * (1 / d) + 8.5 is
+ * within 2^-19 of what it stands for (2^-24 of 1 / d, times 8.1 at most, and half a
+ * step of 16); where a value lies that near to a border the lanes look again, by the
+ * sign of y - (q - 8.5) d, which one fma has (the product holds 16 bits).
+ */
+template <int LANES, int N> __device__ static inline _Float16 kv_encode(const float *y, u32 *codes)
 {
-	float lo = y[0], hi = y[0], any = 0.0f;
+	u32 key = kv_key(y[0]);
+#pragma unroll
+	for (int u = 1; u < N; u++)
+		key = max(key, kv_key(y[u]));
+	const float m = __builtin_bit_cast(float, kv_rotr(kv_most<LANES>(key), 1)) * -0.125f;
+	const _Float16 d = (_Float16)(fabsf(m) > 65504.0f ? copysignf(65504.0f, m) : m);
+	const float df = (float)d, inv = df == 0.0f ? 0.0f : 1.0f / df;
+	float q[N], off = 0.0f;
 #pragma unroll
 	for (int u = 0; u < N; u++) {
-		lo = fminf(lo, y[u]);
-		hi = fmaxf(hi, y[u]);
-		any = y[u] != y[u] ? y[u] : any;
+		const float t = fmaf(y[u], inv, 8.5f);
+		q[u] = floorf(t);
+		off = fmaxf(off, fabsf(t - q[u] - 0.5f));
 	}
-	lo = kv_over<LANES>(lo, [](float a, float b) { return fminf(a, b); });
-	hi = kv_over<LANES>(hi, [](float a, float b) { return fmaxf(a, b); });
-	any = kv_over<LANES>(any, [](float a, float b) { return a + b; });
-	return any == any ? kv_scale(lo, hi) : (_Float16)__builtin_nanf("");
+	if (__ballot(off > 0.5f - 0x1p-18f)) {
+		const float w = fabsf(df);
+#pragma unroll
+		for (int u = 0; u < N; u++) {
+			const float v = df < 0.0f ? -y[u] : y[u];
+			const float below = fmaf(8.5f - q[u], w, v), above = fmaf(7.5f - q[u], w, v);
+			q[u] += (above >= 0.0f ? 1.0f : 0.0f) - (below < 0.0f ? 1.0f : 0.0f);
+		}
+		/* (a scale of 0 stands for 0: code 8) */
+#pragma unroll
+		for (int u = 0; u < N; u++)
+			q[u] = w > 0.0f ? q[u] : 8.0f;
+	}
+#pragma unroll
+	for (int u = 0; u < N; u++)
+		codes[u] = (u32)__builtin_amdgcn_fmed3f(q[u], 0.0f, 15.0f);
+	return d;
 }
 
 /*
@@ -281,9 +301,9 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 	constexpr int HP = WAVE / HL;                 /* heads of a wave's step */
 	constexpr int GL = 32 / N;                    /* lanes of a key group */
 	typedef typename kv_wide<TY>::vec vec;
-	extern __shared__ double2 turns[]; /* [most][rot / 2], then the codes [per][most][D] */
-	const int half = (int)R.rot / 2;
-	uint8_t *codes = (uint8_t *)(turns + most * half);
+	extern __shared__ double2 turns[]; /* [most][kv_slot(rot / 2)], then the codes [per][most][D] */
+	const int half = (int)R.rot / 2, slots = kv_slot(half);
+	uint8_t *codes = (uint8_t *)(turns + most * slots);
 
 	const int groups = (a.kv_heads + per - 1) / per;
 	const int hg = blockIdx.x % groups, tb = blockIdx.x / groups % tiles;
@@ -298,10 +318,6 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 	const int q0 = q ? (int)((long)heads * h0 / a.kv_heads) : 0;
 	const int q1 = q ? (int)((long)heads * h1 / a.kv_heads) : 0;
 	const bool pairs = R.layout == HIP_ROPE_PAIRS;
-	for (int at = threadIdx.x; at < n * half; at += KV_APPEND_NT) {
-		const int r = at / half;
-		turns[at] = kv_turn(R, pos ? pos[row0 + r] : lo + r, at % half);
-	}
 	/* the page: one for the tile */
 	const int shift = a.page_shift - 5, id = a.table[s * a.table_stride + (t >> shift)];
 	uint8_t *const page = (u32)id < (u32)a.pages
@@ -309,9 +325,8 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 	const size_t head_bytes = (size_t)L::BYTES << shift;
 	if (!page && threadIdx.x == 0)
 		kv_error(a, HIP_KV_ERR_PAGE);
-	__syncthreads();
 
-	const int wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), lane = threadIdx.x % WAVE;
 	const int sub = lane / HL, c0 = lane % HL * N;
 	const int ks = page ? (h1 - h0 + HP - 1) / HP : 0, steps = ks + (q1 - q0 + HP - 1) / HP;
 	constexpr int NW = KV_APPEND_NT / WAVE;
@@ -342,13 +357,18 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 	item next;
 	if (wave < n * steps)
 		next = fetch(wave);
+	for (int at = threadIdx.x; at < n * half; at += KV_APPEND_NT) {
+		const int r = at / half;
+		turns[r * slots + kv_slot(at % half)] = kv_turn(R, pos ? pos[row0 + r] : lo + r, at % half);
+	}
+	__syncthreads();
 	for (int at = wave; at < n * steps; at += NW) {
 		const item z = next;
 		if (at + NW < n * steps)
 			next = fetch(at + NW);
 		const int i = z.i;
 		float y[N];
-		z.in.turn(z.x, c0, 2 * half, pairs, turns + i * half, y);
+		z.in.turn(z.x, c0, 2 * half, pairs, turns + i * slots, y);
 		if (at % steps >= ks) {
 			vec o;
 #pragma unroll
@@ -360,14 +380,18 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 		}
 		uint8_t *const tile = page + z.h * head_bytes;
 		const int r = r0 + i;
-		_Float16 d = kv_group<GL, N>(y);
-		float df = (float)d, inv = df == 0.0f ? 0.0f : 1.0f / fabsf(df);
-		u32 w = 0;
+		u32 z4[N], w = 0;
+		_Float16 d = kv_encode<GL, N>(y, z4);
 #pragma unroll
 		for (int u = 0; u < N; u++)
-			w |= kv_rotr(kv_code(y[u], df, inv), 32 - kv_bit((c0 + u) % 8));
-		if (N == 4)
+			w |= z4[u] << kv_bit(u);
+		if (N == 8)
+			w |= z4[N - 1] >> 2; /* code 7 wraps */
+		if (N == 4) { /* codes 0 .. 3 and, of the next lane, 4 .. 7 */
+			if (c0 % 8)
+				w = kv_rotr(w, 24);
 			w |= (u32)__builtin_amdgcn_mov_dpp((int)w, 0xb1, 0xf, 0xf, true);
+		}
 		if (c0 % 8 == 0)
 			((u32 *)tile)[L::k_word(r, c0)] = w;
 		if (c0 % 32 == 0)
@@ -376,14 +400,11 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 #pragma unroll
 		for (int u = 0; u < N; u++)
 			y[u] = T::get(z.val.v[u]);
-		d = kv_group<HL, N>(y);
-		df = (float)d;
-		inv = df == 0.0f ? 0.0f : 1.0f / fabsf(df);
-		uint8_t b[N];
+		d = kv_encode<HL, N>(y, z4);
+		u32 *to = (u32 *)&codes[((z.h - h0) * most + i) * D + c0];
 #pragma unroll
-		for (int u = 0; u < N; u++)
-			b[u] = (uint8_t)kv_code(y[u], df, inv);
-		__builtin_memcpy(__builtin_assume_aligned(&codes[((z.h - h0) * most + i) * D + c0], N), b, N);
+		for (int u = 0; u < N; u += 4)
+			to[u / 4] = z4[u] | z4[u + 1] << 8 | z4[u + 2] << 16 | z4[u + 3] << 24;
 		if (c0 == 0)
 			((_Float16 *)(tile + L::V_SCALES))[r] = d;
 	}
@@ -496,7 +517,7 @@ extern "C" int kv_launch_rope(int type, const void *x, size_t x_stride, void *ou
 	while (heads_per > 4 && rows * ((heads + heads_per - 1) / heads_per) < 512)
 		heads_per = (heads_per + 1) / 2;
 	const dim3 grid((unsigned)((rows + per - 1) / per), (unsigned)((heads + heads_per - 1) / heads_per));
-	const size_t lds = per * (R->rot / 2) * sizeof(double2);
+	const size_t lds = per * kv_slot((int)R->rot / 2) * sizeof(double2);
 	KV_DISPATCH_TYPE(type, TY, {
 		typedef kv_type<TY>::t t;
 		const size_t n = kv_wide<TY>::N;
@@ -522,14 +543,14 @@ extern "C" int kv_launch_append(const kv_args *a, int head_len, int type, const 
 	const hip_rope none = {0, HIP_ROPE_PAIRS, NULL, 1.0};
 	const int tiles = kv_tiles_of(a->max_rows), most = a->max_rows < KV_TILE ? a->max_rows : KV_TILE;
 	/* all kv heads a workgroup (32 KB of codes at most) where the tiles alone
-	 * are two a CU; else fewer, down to one */
+	 * are four a CU; else fewer, down to one */
 	int per = 1;
 	const int top = 32768 / (KV_TILE * head_len);
-	while (per < top && per < a->kv_heads && (size_t)a->nseq * tiles * a->kv_heads / (2 * per) >= 512)
+	while (per < top && per < a->kv_heads && (size_t)a->nseq * tiles * a->kv_heads / (2 * per) >= 1024)
 		per *= 2;
 	per = per < a->kv_heads ? per : a->kv_heads;
 	const size_t grid = (size_t)a->nseq * tiles * ((a->kv_heads + per - 1) / per);
-	const size_t lds = (size_t)most * ((R ? R->rot / 2 * sizeof(double2) : 0) + (size_t)per * head_len);
+	const size_t lds = (size_t)most * ((R ? kv_slot((int)R->rot / 2) * sizeof(double2) : 0) + (size_t)per * head_len);
 	KV_DISPATCH_HEAD(head_len, D, KV_DISPATCH_TYPE(type, TY, {
 		typedef kv_type<TY>::t t;
 		k_kv_append<D, TY><<<dim3((unsigned)grid), KV_APPEND_NT, lds, (hipStream_t)stream>>>(
