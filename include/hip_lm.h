@@ -169,6 +169,18 @@ typedef struct hip_lm_batch hip_lm_batch;
 
 hip_lm_batch *hip_lm_batch_new(hip_lm *M, size_t nseq);
 
+/*
+ * The same with the caches in 4 bits (hip_kv.h: 138 bytes a row, kv head and layer
+ * instead of 1024, so that 7.4 times the sequences or context fit): a step's q/k/v
+ * rows go through hip_kv_append_dev and hip_kv_attn_dev, and every other call takes
+ * the batch as it is.  A key is off by up to a sixteenth of the largest of its 32
+ * neighbours (an eighth where the largest have both signs), a value of its row's
+ * largest: picks change, and logits of random weights move by a tenth.  The caches
+ * keep every row: steps past the context return 0 instead of rotating.  q and k turn
+ * by angles of 64 bits.
+ */
+hip_lm_batch *hip_lm_batch_new_kv4(hip_lm *M, size_t nseq);
+
 /* One step: toks[nseq] in, logits[nseq][vocab] (host, optional) and the
  * greedy picks next[nseq] (optional) out.  Synchronous. */
 int hip_lm_batch_decode(hip_lm_batch *B, const int *toks, float *logits, int *next);

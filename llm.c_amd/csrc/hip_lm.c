@@ -14,6 +14,7 @@
  * counters from the device, so generate captures a step once per shape
  * (with and without the lm_head) and replays it.
  */
+#include "hip_kv.h"
 #include "hip_lm.h"
 #include "lm_internal.h"
 #include "moe_internal.h"
@@ -985,6 +986,137 @@ static int rows_product(hip_lm *M, const uint8_t *W, int N, int K, const float *
 	return 1;
 }
 
+/* A batch's caches in 4 bits (hip_kv.h): a pool of pages for each layer, sequence
+ * s's the pages s * stride .. of it, in order */
+#define KV4_PAGE 64
+struct lm_kv4 {
+	uint8_t *d_pool; /* [L] pools of pool_bytes */
+	size_t pool_bytes, pages, stride;
+	int32_t *d_table, *d_len; /* [S][stride], [S] */
+	double *d_freq;           /* [HL / 2] */
+	double mag;
+	uint32_t *err;            /* the batch's step error word */
+	void *d_ws, *d_pf_ws; /* of the steps' attention, and of the prompts' */
+	size_t ws, pf_ws;
+};
+
+static void kv4_free(struct lm_kv4 *k)
+{
+	if (!k)
+		return;
+	void *bufs[] = {k->d_pool, k->d_table, k->d_len, k->d_freq, k->d_ws, k->d_pf_ws};
+	for (size_t i = 0; i < sizeof(bufs) / sizeof(bufs[0]); i++)
+		hipFree(bufs[i]);
+	free(k);
+}
+
+/* sequences z .. z + nseq - 1 of the pool of layer l, T rows each, up to max_len */
+static void kv4_args(const hip_lm *M, const struct lm_kv4 *k, size_t l, size_t z, size_t nseq, size_t T,
+		     size_t max_len, hip_kv_cache *c, hip_kv_batch *b)
+{
+	*c = (hip_kv_cache){k->d_pool + l * k->pool_bytes, k->pages, KV4_PAGE, M->KH, M->HL, k->err};
+	*b = (hip_kv_batch){nseq, nseq * T, T, max_len, NULL, k->d_len + z, k->d_table + z * k->stride,
+			    k->stride};
+}
+
+/* the caches of S sequences and their steps' workspace, on the current device; the
+ * device finds errors into *err */
+static struct lm_kv4 *kv4_new(const hip_lm *M, size_t S, uint32_t *err)
+{
+	struct lm_kv4 *k = calloc(1, sizeof(*k));
+	double freq[LM_HLEN / 2];
+	int32_t *table = NULL;
+	if (!k) {
+		lm_err("lm_batch_new_kv4: out of host memory");
+		return NULL;
+	}
+	k->err = err;
+	k->stride = (M->C + KV4_PAGE - 1) / KV4_PAGE;
+	k->pages = S * k->stride;
+	k->pool_bytes = k->pages * hip_kv_page_bytes(KV4_PAGE, M->KH, M->HL);
+	if (!hip_rope_freqs(M->HL, M->theta, HIP_ROPE_PLAIN, 1.0, 0.0, 0.0, 0.0, freq, &k->mag))
+		goto fail;
+	table = malloc(k->pages * sizeof(*table));
+	if (!table) {
+		lm_err("lm_batch_new_kv4: out of host memory");
+		goto fail;
+	}
+	for (size_t i = 0; i < k->pages; i++)
+		table[i] = (int32_t)i;
+	HIPCHK(hipMalloc((void **)&k->d_pool, M->L * k->pool_bytes), "hipMalloc(4-bit caches)");
+	HIPCHK(hipMalloc((void **)&k->d_table, k->pages * sizeof(*table)), "hipMalloc(page table)");
+	HIPCHK(hipMemcpy(k->d_table, table, k->pages * sizeof(*table), hipMemcpyHostToDevice),
+	       "copy page table");
+	HIPCHK(hipMalloc((void **)&k->d_len, S * sizeof(int32_t)), "hipMalloc(lengths)");
+	HIPCHK(hipMemset(k->d_len, 0, S * sizeof(int32_t)), "clear lengths");
+	HIPCHK(hipMalloc((void **)&k->d_freq, sizeof(freq)), "hipMalloc(frequencies)");
+	HIPCHK(hipMemcpy(k->d_freq, freq, M->HL / 2 * sizeof(double), hipMemcpyHostToDevice),
+	       "copy frequencies");
+	hip_kv_cache c;
+	hip_kv_batch b;
+	kv4_args(M, k, 0, 0, S, 1, M->C, &c, &b);
+	k->ws = hip_kv_attn_ws(&c, &b, M->H);
+	if (k->ws)
+		HIPCHK(hipMalloc(&k->d_ws, k->ws), "hipMalloc(attention pieces)");
+	free(table);
+	return k;
+fail:
+	free(table);
+	kv4_free(k);
+	return NULL;
+}
+
+/*
+ * The rows qkv [nseq * T][EQ + 2 EKV] of sequences z .. of layer l: q and k
+ * normalised (OLMoE) and turned, k and v stored, and the attention of q over the
+ * caches into out [nseq * T][EQ].  The lengths with these rows, at most max_len, are
+ * in k->d_len.
+ */
+static int kv4_attention(hip_lm *M, struct lm_kv4 *k, size_t l, size_t z, size_t nseq, size_t T,
+			 size_t max_len, float *qkv, float *out, void *ws, size_t ws_bytes, hipStream_t s)
+{
+	const struct lm_layer *y = &M->ly[l];
+	const size_t NQKV = M->EQ + 2 * M->EKV;
+	const hip_rope R = {M->HL, HIP_ROPE_PAIRS, k->d_freq, k->mag};
+	hip_kv_cache c;
+	hip_kv_batch b;
+	kv4_args(M, k, l, z, nseq, T, max_len, &c, &b);
+	if (y->q_norm)
+		LCHK(lm_launch_qk_norm(qkv, y->q_norm, y->k_norm, (int)M->EQ, (int)M->EKV, (int)(nseq * T), s),
+		     "q/k norms");
+	return hip_kv_append_dev(&c, &b, &R, HIP_KV_F32, qkv + M->EQ, qkv + M->EQ + M->EKV, NQKV, NULL, qkv,
+				 NQKV, M->H, qkv, NQKV, s) &&
+	       hip_kv_attn_dev(&c, &b, HIP_KV_F32, qkv, NQKV, M->H, out, M->EQ,
+			       M->arch == HIP_LM_OLMOE ? 1.0f / M->scale : M->scale, M->window, ws, ws_bytes, s);
+}
+
+/* the workspace of the attention of S prompts of T rows, nseq of them and the rest
+ * (which may be cut into more pieces) at a time.  The last prompts' launches ended
+ * with the call that made them, and no graph names it. */
+static int kv4_prefill_ws(const hip_lm *M, struct lm_kv4 *k, size_t S, size_t nseq, size_t T,
+			  size_t max_len)
+{
+	hip_kv_cache c;
+	hip_kv_batch b;
+	kv4_args(M, k, 0, 0, nseq, T, max_len, &c, &b);
+	size_t ws = hip_kv_attn_ws(&c, &b, M->H);
+	if (S % nseq) {
+		kv4_args(M, k, 0, 0, S % nseq, T, max_len, &c, &b);
+		const size_t rest = hip_kv_attn_ws(&c, &b, M->H);
+		ws = ws > rest ? ws : rest;
+	}
+	if (ws <= k->pf_ws)
+		return 1;
+	hipFree(k->d_pf_ws);
+	k->d_pf_ws = NULL;
+	k->pf_ws = 0;
+	HIPCHK(hipMalloc(&k->d_pf_ws, ws), "hipMalloc(attention pieces)");
+	k->pf_ws = ws;
+	return 1;
+fail:
+	return 0;
+}
+
 /*
  * olmoe_prefill / llama_prefill (olmoe.c:409-508, llama.c:458-564) of nseq
  * sequences at once: T ids each (sequence z's at d_ids + z * T, its cache
@@ -995,12 +1127,14 @@ static int rows_product(hip_lm *M, const uint8_t *W, int N, int K, const float *
  * product with the residual, rms_norm, the MoE layer at nseq * T tokens),
  * then each sequence's last row: the final rms_norm, the lm_head product
  * into logits [nseq][V] and the greedy pick into btok[z] and, when tokens
- * is not NULL, tokens[z * tstride].  Enqueued on `s`; the caller advances
- * the position and cache size by T.
+ * is not NULL, tokens[z * tstride].  With kv4 the caches are in 4 bits instead
+ * (kc and vc are not read): sequences z0 .. of kv4, whose lengths have the new rows
+ * already.  Enqueued on `s`; the caller advances the position and cache size by T.
  */
 static int enqueue_prefill(hip_lm *M, int size, int pos, size_t T, size_t nseq,
-			   const int *d_ids, float *kc, float *vc, size_t cstride, float *logits,
-			   int *btok, int *tokens, int tstride, hipStream_t s)
+			   const int *d_ids, float *kc, float *vc, size_t cstride,
+			   struct lm_kv4 *kv4, size_t z0, float *logits, int *btok, int *tokens,
+			   int tstride, hipStream_t s)
 {
 	const int wt = M->wtype, E = (int)M->E, NQKV = (int)(M->EQ + 2 * M->EKV);
 	const int n = (int)(T * nseq);
@@ -1017,7 +1151,11 @@ static int enqueue_prefill(hip_lm *M, int size, int pos, size_t T, size_t nseq,
 		}
 		if (!rows_product(M, y->wqkv, NQKV, E, M->d_pf_x, n, NULL, M->d_pf_qkv, s))
 			goto out;
-		if (lm_launch_pf_qk(M->d_pf_qkv, y->q_norm, y->k_norm, M->d_freq, kc + co, vc + co,
+		if (kv4) {
+			if (!kv4_attention(M, kv4, l, z0, nseq, T, (size_t)size + T, M->d_pf_qkv,
+					   M->d_pf_attn, kv4->d_pf_ws, kv4->pf_ws, s))
+				goto out;
+		} else if (lm_launch_pf_qk(M->d_pf_qkv, y->q_norm, y->k_norm, M->d_freq, kc + co, vc + co,
 				    M->d_pf_q, (int)M->H, (int)M->KH, (int)M->C, size, pos, (int)T,
 				    (int)nseq, cstride, s) != 0 ||
 		    lm_launch_pf_attn(M->d_pf_q, kc + co, vc + co, M->d_pf_attn, (int)M->H,
@@ -1102,7 +1240,7 @@ int hip_lm_prefill(hip_lm *M, const int *prompt, size_t n, float *logits, int *n
 	HIPCHK(hipStreamSynchronize(M->stream), "synchronize");
 	HIPCHK(hipMemcpy(M->d_prompt, prompt, n * sizeof(int), hipMemcpyHostToDevice),
 	       "copy prompt");
-	if (!enqueue_prefill(M, M->st.size, M->st.pos, n, 1, M->d_prompt, M->d_kc, M->d_vc, 0,
+	if (!enqueue_prefill(M, M->st.size, M->st.pos, n, 1, M->d_prompt, M->d_kc, M->d_vc, 0, NULL, 0,
 			     M->d_logits, &M->d_st->tok, NULL, 0, M->stream))
 		return 0;
 	M->st.pos += (int)n;
@@ -1192,7 +1330,7 @@ int hip_lm_generate(hip_lm *M, const int *prompt, size_t n_prompt, size_t n_gen,
 	size_t first = 0; /* the first step that runs a step graph */
 	if (pf) {
 		if (!enqueue_prefill(M, M->st.size, M->st.pos, n_prompt, 1, M->d_prompt, M->d_kc,
-				     M->d_vc, 0, M->d_logits, &M->d_st->tok,
+				     M->d_vc, 0, NULL, 0, M->d_logits, &M->d_st->tok,
 				     M->d_tokens + (n_prompt - 1), 0, M->stream))
 			return 0;
 		M->st.step = (int)n_prompt;
@@ -1307,6 +1445,7 @@ struct hip_lm_batch {
 	hip_lm *M;
 	size_t S;
 	hipStream_t stream;
+	struct lm_kv4 *kv4; /* instead of the fp32 caches */
 	float *d_kc, *d_vc; /* [S][L][KH][C][HL] */
 	float *d_h0, *d_h1, *d_xn, *d_moe_in, *d_moe_out; /* [S][E] */
 	float *d_qkv;       /* [S][EQ + 2 EKV] */
@@ -1353,6 +1492,7 @@ void hip_lm_batch_free(hip_lm_batch *B)
 	batch_drop_graphs(B);
 	free(B->g_body);
 	free(B->g_head);
+	kv4_free(B->kv4);
 	void *bufs[] = {B->d_kc, B->d_vc, B->d_h0, B->d_h1, B->d_xn, B->d_moe_in, B->d_moe_out,
 			B->d_qkv, B->d_attn, B->d_logits, B->d_part, B->d_cnt, B->d_btok, B->d_st,
 			B->d_prompt, B->d_tokens, B->d_split};
@@ -1372,7 +1512,7 @@ void hip_lm_batch_free(hip_lm_batch *B)
 
 static int batch_io(hip_lm_batch *B, size_t n_prompt, size_t n_tokens);
 
-hip_lm_batch *hip_lm_batch_new(hip_lm *M, size_t nseq)
+static hip_lm_batch *batch_new(hip_lm *M, size_t nseq, int kv4)
 {
 	if (!M || nseq < 1 || nseq > 4096) {
 		lm_err("lm_batch_new: NULL model or %zu sequences (1 .. 4096)", nseq);
@@ -1413,10 +1553,6 @@ hip_lm_batch *hip_lm_batch_new(hip_lm *M, size_t nseq)
 	}
 	HIPCHK(hipEventCreate(&B->ev0), "hipEventCreate");
 	HIPCHK(hipEventCreate(&B->ev1), "hipEventCreate");
-	HIPCHK(hipMalloc((void **)&B->d_kc, cache), "hipMalloc(batch k caches)");
-	HIPCHK(hipMalloc((void **)&B->d_vc, cache), "hipMalloc(batch v caches)");
-	HIPCHK(hipMemset(B->d_kc, 0, cache), "clear k caches");
-	HIPCHK(hipMemset(B->d_vc, 0, cache), "clear v caches");
 	HIPCHK(hipMalloc((void **)&B->d_h0, S * E * 4), "hipMalloc(h0)");
 	HIPCHK(hipMalloc((void **)&B->d_h1, S * E * 4), "hipMalloc(h1)");
 	HIPCHK(hipMalloc((void **)&B->d_xn, S * E * 4), "hipMalloc(xn)");
@@ -1425,10 +1561,20 @@ hip_lm_batch *hip_lm_batch_new(hip_lm *M, size_t nseq)
 	HIPCHK(hipMalloc((void **)&B->d_qkv, S * NQKV * 4), "hipMalloc(qkv)");
 	HIPCHK(hipMalloc((void **)&B->d_attn, S * M->EQ * 4), "hipMalloc(attn)");
 	HIPCHK(hipMalloc((void **)&B->d_logits, S * M->V * 4), "hipMalloc(logits)");
-	HIPCHK(hipMalloc((void **)&B->d_part, part), "hipMalloc(attention partials)");
-	HIPCHK(hipMemset(B->d_part, 0, part), "clear attention partials");
-	HIPCHK(hipMalloc((void **)&B->d_cnt, S * M->H * sizeof(uint32_t)), "hipMalloc(counters)");
-	HIPCHK(hipMemset(B->d_cnt, 0, S * M->H * sizeof(uint32_t)), "clear counters");
+	HIPCHK(hipMalloc((void **)&B->d_st, sizeof(LmState)), "hipMalloc(state)");
+	if (kv4) {
+		if (!(B->kv4 = kv4_new(M, S, (uint32_t *)&B->d_st->err)))
+			goto fail;
+	} else {
+		HIPCHK(hipMalloc((void **)&B->d_kc, cache), "hipMalloc(batch k caches)");
+		HIPCHK(hipMalloc((void **)&B->d_vc, cache), "hipMalloc(batch v caches)");
+		HIPCHK(hipMemset(B->d_kc, 0, cache), "clear k caches");
+		HIPCHK(hipMemset(B->d_vc, 0, cache), "clear v caches");
+		HIPCHK(hipMalloc((void **)&B->d_part, part), "hipMalloc(attention partials)");
+		HIPCHK(hipMemset(B->d_part, 0, part), "clear attention partials");
+		HIPCHK(hipMalloc((void **)&B->d_cnt, S * M->H * sizeof(uint32_t)), "hipMalloc(counters)");
+		HIPCHK(hipMemset(B->d_cnt, 0, S * M->H * sizeof(uint32_t)), "clear counters");
+	}
 	{ /* the largest partial sums: the lm_head's or the q/k/v product's */
 		size_t wb = moe_qmm_work_most((int)S, (int)M->V, (int)E);
 		const size_t w2 = moe_qmm_work_most((int)S, (int)(M->EQ + 2 * M->EKV), (int)E);
@@ -1440,7 +1586,6 @@ hip_lm_batch *hip_lm_batch_new(hip_lm *M, size_t nseq)
 	}
 	HIPCHK(hipMalloc((void **)&B->d_btok, S * sizeof(int)), "hipMalloc(tokens)");
 	HIPCHK(hipMemset(B->d_btok, 0, S * sizeof(int)), "clear tokens");
-	HIPCHK(hipMalloc((void **)&B->d_st, sizeof(LmState)), "hipMalloc(state)");
 	/* epoch 1: tags never match the zeroed partials */
 	B->st.epoch = 1;
 	HIPCHK(hipMemcpy(B->d_st, &B->st, sizeof(LmState), hipMemcpyHostToDevice), "set state");
@@ -1459,12 +1604,34 @@ fail:
 	return NULL;
 }
 
+hip_lm_batch *hip_lm_batch_new(hip_lm *M, size_t nseq)
+{
+	return batch_new(M, nseq, 0);
+}
+
+hip_lm_batch *hip_lm_batch_new_kv4(hip_lm *M, size_t nseq)
+{
+	return batch_new(M, nseq, 1);
+}
+
+/* caches in 4 bits keep every row: steps more of them have to fit */
+static int kv4_fits(const hip_lm_batch *B, size_t steps)
+{
+	if (!B->kv4 || (size_t)B->st.size + steps <= B->M->C)
+		return 1;
+	lm_err("lm_batch: %zu steps from cache row %d do not fit the context of %zu, which 4-bit caches do "
+	       "not rotate", steps, B->st.size, B->M->C);
+	return 0;
+}
+
 /* kvcache_rotate of every sequence's cache (they are all at one size) */
 static int batch_rotate_if_full(hip_lm_batch *B)
 {
 	hip_lm *M = B->M;
 	if ((size_t)B->st.size < M->C)
 		return 1;
+	if (!kv4_fits(B, 1))
+		return 0;
 	const size_t keep = rotate_keep(M, (size_t)B->st.size);
 	if (!keep)
 		return 0;
@@ -1509,7 +1676,11 @@ static int batch_step(hip_lm_batch *B, int head, int nact)
 	const int wt = M->wtype, E = (int)M->E, S = (int)B->S;
 	const int NQKV = (int)(M->EQ + 2 * M->EKV);
 	const size_t cseq = batch_cache_floats(M);
+	/* rows that a step of nact chunks reaches, at most */
+	const size_t reach = (size_t)nact * LM_CHUNK < M->C && !M->window ? (size_t)nact * LM_CHUNK : M->C;
 	hipStream_t s = B->stream;
+	if (B->kv4)
+		LCHK(lm_launch_kv_len(B->kv4->d_len, S, B->d_st, 1, s), "cache lengths");
 	for (size_t l = 0; l < M->L; l++) {
 		struct lm_layer *y = &M->ly[l];
 		const size_t co = l * M->KH * M->C * M->HL;
@@ -1519,11 +1690,15 @@ static int batch_step(hip_lm_batch *B, int head, int nact)
 					 B->d_prompt, B->d_btok, s), "batch norm");
 		if (!batch_product(B, y->wqkv, NQKV, E, B->d_xn, NULL, B->d_qkv))
 			return 0;
-		LCHK(lm_launch_attn(B->d_qkv, y->q_norm, y->k_norm, M->d_freq, B->d_st, B->d_kc + co,
-				    B->d_vc + co, B->d_part, B->d_cnt, B->d_attn, (int)M->H,
-				    (int)M->KH, (int)M->C, (int)M->window, M->scale,
-				    M->arch != HIP_LM_OLMOE, (int)l, nact, S, cseq, s),
-		     "batch attention");
+		if (!B->kv4)
+			LCHK(lm_launch_attn(B->d_qkv, y->q_norm, y->k_norm, M->d_freq, B->d_st,
+					    B->d_kc + co, B->d_vc + co, B->d_part, B->d_cnt, B->d_attn,
+					    (int)M->H, (int)M->KH, (int)M->C, (int)M->window, M->scale,
+					    M->arch != HIP_LM_OLMOE, (int)l, nact, S, cseq, s),
+			     "batch attention");
+		else if (!kv4_attention(M, B->kv4, l, 0, B->S, 1, reach, B->d_qkv, B->d_attn,
+					B->kv4->d_ws, B->kv4->ws, s))
+			return 0;
 		/* h1 = h0 + attn . Wo^T, moe_in = rms_norm(h1): where the matrix-core
 		 * product leaves partial sums, one launch adds them (the reduce's
 		 * order), adds h0 and normalises */
@@ -1707,6 +1882,8 @@ int hip_lm_batch_generate(hip_lm_batch *B, const int *prompts, size_t n_prompt, 
 	/* the prompts as prefills of groups of sequences (~PF_GROUP_ROWS rows:
 	 * every MoE layer's scratch grows with the rows of one launch) where
 	 * they fit the caches; else a step per id */
+	if (!kv4_fits(B, steps))
+		return 0;
 	const int pf = n_prompt >= 2 && (size_t)B->st.size + n_prompt <= M->C;
 	size_t gseq = n_prompt >= PF_GROUP_ROWS ? 1 : PF_GROUP_ROWS / n_prompt;
 	gseq = gseq < B->S ? gseq : B->S;
@@ -1716,11 +1893,19 @@ int hip_lm_batch_generate(hip_lm_batch *B, const int *prompts, size_t n_prompt, 
 	size_t first = 0; /* the first step that runs a step graph */
 	if (pf) {
 		const size_t cseq = batch_cache_floats(M);
+		const int reach = B->st.size + (int)n_prompt;
+		if (B->kv4) {
+			if (!kv4_prefill_ws(M, B->kv4, B->S, gseq, n_prompt, (size_t)reach))
+				return 0;
+			LCHK(lm_launch_kv_len(B->kv4->d_len, (int)B->S, NULL, reach, B->stream),
+			     "cache lengths");
+		}
 		for (size_t z0 = 0; z0 < B->S; z0 += gseq) {
 			const size_t gz = B->S - z0 < gseq ? B->S - z0 : gseq;
+			float *kc = B->kv4 ? NULL : B->d_kc + z0 * cseq, *vc = B->kv4 ? NULL : B->d_vc + z0 * cseq;
 			if (!enqueue_prefill(M, B->st.size, B->st.pos, n_prompt, gz,
-					     B->d_prompt + z0 * n_prompt, B->d_kc + z0 * cseq,
-					     B->d_vc + z0 * cseq, cseq, B->d_logits + z0 * M->V,
+					     B->d_prompt + z0 * n_prompt, kc, vc, cseq, B->kv4, z0,
+					     B->d_logits + z0 * M->V,
 					     B->d_btok + z0,
 					     B->d_tokens + z0 * B->tokens_cap + (n_prompt - 1),
 					     (int)B->tokens_cap, B->stream))
@@ -1801,8 +1986,10 @@ int hip_lm_batch_reset(hip_lm_batch *B)
 	}
 	const size_t cache = B->S * batch_cache_floats(B->M) * sizeof(float);
 	HIPCHK(hipStreamSynchronize(B->stream), "synchronize");
-	HIPCHK(hipMemset(B->d_kc, 0, cache), "clear k caches");
-	HIPCHK(hipMemset(B->d_vc, 0, cache), "clear v caches");
+	if (!B->kv4) { /* 4-bit rows behind the length are not read */
+		HIPCHK(hipMemset(B->d_kc, 0, cache), "clear k caches");
+		HIPCHK(hipMemset(B->d_vc, 0, cache), "clear v caches");
+	}
 	memset(&B->st, 0, sizeof(B->st));
 	HIPCHK(hipMemcpy(B->d_st, &B->st, 5 * sizeof(int), hipMemcpyHostToDevice), "clear state");
 	HIPCHK(hipDeviceSynchronize(), "synchronize");

@@ -76,6 +76,11 @@ int lm_launch_embed(int wtype, const uint8_t *wte, int K, const LmState *st, con
 int lm_launch_pf_qk(const float *qkv, const float *q_norm, const float *k_norm,
                     const float *freq, float *kc, float *vc, float *qo, int H, int KH, int C,
                     int size, int pos0, int T, int nseq, size_t cstride, void *stream);
+/* the same norms of q and k alone, in place: rows of EQ + EKV + EKV floats */
+int lm_launch_qk_norm(float *qkv, const float *q_norm, const float *k_norm, int EQ, int EKV, int rows,
+                      void *stream);
+/* len[s] = st->size + add (st NULL: add), s < n */
+int lm_launch_kv_len(int32_t *len, int n, const LmState *st, int add, void *stream);
 /* causal (and sliding-window) attention of those rows over the cache rows
  * 0 .. size + T - 1 into out [nseq * T][H * 128] */
 int lm_launch_pf_attn(const float *qo, const float *kc, const float *vc, float *out, int H,

@@ -808,6 +808,14 @@ void k_lm_head(const uint8_t *__restrict__ W, size_t rb, int N, int K, const flo
 }
 
 /* the step's counters advance (a step without the lm_head) */
+/* the lengths of caches in 4 bits: the step's rows and `add` more (st NULL: add) */
+__global__ void k_lm_kv_len(int32_t *len, int n, const LmState *st, int add)
+{
+	const int v = (st ? st->size : 0) + add;
+	for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x)
+		len[i] = v;
+}
+
 __global__ void k_lm_step_end(LmState *st)
 {
 	if (threadIdx.x == 0) {
@@ -1209,6 +1217,25 @@ __global__ __launch_bounds__(LM_NT) void k_lm_pf_qk(const float *__restrict__ qk
 	}
 }
 
+/* The norms of k_lm_pf_qk in place (row blockIdx.x; q for y = 0, k for y = 1), for
+ * rows whose rotation and storing the 4-bit cache's append does. */
+__global__ __launch_bounds__(LM_NT) void k_lm_qk_norm(float *__restrict__ qkv, const float *__restrict__ q_norm,
+						      const float *__restrict__ k_norm, int EQ, int EK)
+{
+	__shared__ float red[LM_NT / WAVE];
+	const int n = blockIdx.y ? EK : EQ;
+	float *x = qkv + (size_t)blockIdx.x * (EQ + 2 * EK) + (blockIdx.y ? EQ : 0);
+	const float *w = blockIdx.y ? k_norm : q_norm;
+	float s = 0.0f;
+	for (int i = threadIdx.x; i < n; i += LM_NT) {
+		const float v = x[i] * x[i];
+		s = s + v;
+	}
+	const float r = sqrtf(block_sum(s, red) / (float)n + 1e-5f);
+	for (int i = threadIdx.x; i < n; i += LM_NT)
+		x[i] = (x[i] / r) * w[i];
+}
+
 #define PF_QB 16    /* query rows of a prefill attention workgroup */
 #define PF_KB 32    /* cache rows per step of a wave's key loop */
 #define PF_WAVES 4
@@ -1563,6 +1590,21 @@ extern "C" int lm_launch_pick_rows(const float *logits, int nseq, int V, const L
 extern "C" int lm_launch_step_end(LmState *st, void *stream)
 {
 	hipLaunchKernelGGL(k_lm_step_end, dim3(1), dim3(64), 0, (hipStream_t)stream, st);
+	return (int)hipGetLastError();
+}
+
+extern "C" int lm_launch_kv_len(int32_t *len, int n, const LmState *st, int add, void *stream)
+{
+	hipLaunchKernelGGL(k_lm_kv_len, dim3((n + 255) / 256), dim3(256), 0, (hipStream_t)stream, len, n, st,
+			   add);
+	return (int)hipGetLastError();
+}
+
+extern "C" int lm_launch_qk_norm(float *qkv, const float *q_norm, const float *k_norm, int EQ, int EKV,
+				 int rows, void *stream)
+{
+	hipLaunchKernelGGL(k_lm_qk_norm, dim3(rows, 2), dim3(LM_NT), 0, (hipStream_t)stream, qkv, q_norm,
+			   k_norm, EQ, EKV);
 	return (int)hipGetLastError();
 }
 

@@ -212,6 +212,8 @@ def _bind():
     L.hip_lm_free.argtypes = [_vp]
     L.hip_lm_batch_new.restype = _vp
     L.hip_lm_batch_new.argtypes = [_vp, _sz]
+    L.hip_lm_batch_new_kv4.restype = _vp
+    L.hip_lm_batch_new_kv4.argtypes = [_vp, _sz]
     L.hip_lm_batch_decode.restype = i32
     L.hip_lm_batch_decode.argtypes = [_vp, _vp, _vp, _vp]
     L.hip_lm_batch_generate.restype = i32
@@ -345,11 +347,12 @@ class LmModel:
 
 class LmBatch:
     """nseq sequences decoding in lockstep on an LmModel's weights
-    (hip_lm_batch_*)."""
+    (hip_lm_batch_*), their caches in fp32 or, with kv4, in 4 bits."""
 
-    def __init__(self, model: LmModel, nseq: int):
+    def __init__(self, model: LmModel, nseq: int, kv4: bool = False):
         self.model, self.S, self.V = model, nseq, model.V
-        self.h = _bind().hip_lm_batch_new(model.h, nseq)
+        new = _bind().hip_lm_batch_new_kv4 if kv4 else _bind().hip_lm_batch_new
+        self.h = new(model.h, nseq)
         if not self.h:
             raise HipMoeError("hip_lm_batch_new: " + last_error())
 
