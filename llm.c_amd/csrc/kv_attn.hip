@@ -44,10 +44,17 @@ __device__ static inline half8_t as_half8(u32 a, u32 b, u32 c, u32 d)
 }
 
 /*
- * A word's codes, in their order, as f16 with the mantissa's bits where they lie
- * and nothing else, subnormals: code * 2^-22 for codes 0, 1, 4 and 5, code * 2^-18
- * for the others.  One turn and four masks for eight; the other operand has 16
- * times the value where the code has the smaller step.
+ * A word's codes as f16, in their order: a turn and four masks for eight.
+ *
+ * 16-bit types (kv_word): the bits where they lie and nothing around them,
+ * subnormals: code * 2^-22 for codes 0, 1, 4 and 5, code * 2^-18 for the others; the
+ * other operand has 16 times the value where the code has the smaller step.  The
+ * matrix cores align products by the exponent that an operand has, not by its
+ * leading bit, so that the smaller ones lose four bits of the sum's 24, more than
+ * enough for outputs of 8 or 11 bits (3e-6 of the output's norm).
+ *
+ * fp32 (kv_word8): with exponents that make both steps 1/16, 16 + code / 16 and
+ * 1 + code / 16, of which 16.5 and 1.5 leave (code - 8) / 16, normal and exact (5e-7).
  */
 __device__ static inline half8_t kv_word(u32 w)
 {
@@ -55,24 +62,39 @@ __device__ static inline half8_t kv_word(u32 w)
 	return as_half8(w & 0x003c003cu, w & 0x03c003c0u, r & 0x003c003cu, r & 0x03c003c0u);
 }
 
-#define KV_CODE_STEP (1.0f / (1 << 18))
-
 /* whether code j has the smaller step */
 __device__ static constexpr bool kv_small(int j)
 {
 	return j % 4 < 2;
 }
 
-/* 8 in the steps of a word's codes, and the codes less that */
+/* how a type's operands are made: the codes' step, the exponents of a query row's
+ * largest value and of its largest probability times value scale (kv_soft below) */
+template <int TY> struct kv_form {
+	static constexpr bool EVEN = TY == HIP_KV_F32;
+	static constexpr float STEP = EVEN ? 1.0f / 16.0f : 1.0f / (1 << 18);
+	static constexpr float MORE = EVEN ? 1.0f : 16.0f; /* where the codes have the smaller step */
+	static constexpr int QUERY = EVEN ? 14 : 10;
+	static constexpr float LOG_MORE = EVEN ? 0.0f : 4.0f;
+	static constexpr float REF = EVEN ? 9.0f : 5.0f, TOP = EVEN ? 15.0f : 11.0f;
+};
+
+/* 8 in the steps of kv_word's codes */
 __device__ static inline half8_t kv_surplus8()
 {
-	const _Float16 a = (_Float16)(8.0f * KV_CODE_STEP / 16.0f), b = (_Float16)(8.0f * KV_CODE_STEP);
+	const _Float16 a = (_Float16)(8.0f / (1 << 22)), b = (_Float16)(8.0f / (1 << 18));
 	return half8_t{a, a, b, b, a, a, b, b};
 }
 
-__device__ static inline half8_t kv_word8(u32 w)
+/* the codes less 8 */
+template <int TY> __device__ static inline half8_t kv_word8(u32 w)
 {
-	return kv_word(w) - kv_surplus8();
+	if constexpr (!kv_form<TY>::EVEN)
+		return kv_word(w) - kv_surplus8();
+	const u32 r = kv_rotr(w, 8), m = 0x003c003cu, n = 0x03c003c0u, sixteen = 0x4c004c00u, one = 0x3c003c00u;
+	const _Float16 a = (_Float16)16.5f, b = (_Float16)1.5f;
+	return as_half8((w & m) | sixteen, (w & n) | one, (r & m) | sixteen, (r & n) | one) -
+	       half8_t{a, a, b, b, a, a, b, b};
 }
 
 /* x = hi + lo in f16; the products with the hidden -1 stay fused with the
@@ -234,13 +256,13 @@ struct kv_factor {
 	float query, score;
 };
 
-__device__ static inline kv_factor kv_query_factor(float top, float scale)
+template <int TY> __device__ static inline kv_factor kv_query_factor(float top, float scale)
 {
-	int e = 10 - __builtin_amdgcn_frexp_expf(top);
+	int e = kv_form<TY>::QUERY - __builtin_amdgcn_frexp_expf(top);
 	e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 122) : 0;
 	/* a negative scale turns the query around, 0 makes it 0 */
 	return {scale > 0.0f ? pow2(e) : scale < 0.0f ? -pow2(e) : 0.0f,
-		(scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / KV_CODE_STEP) * pow2(-e)};
+		(scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / kv_form<TY>::STEP) * pow2(-e)};
 }
 
 /* eight channels of a query row in f16 parts, and their sum */
@@ -250,11 +272,11 @@ __device__ static inline float kv_split8(const kv_vec<TY, 8> &w, float factor, h
 	float sum = 0.0f;
 #pragma unroll
 	for (int j = 0; j < 8; j++) {
-		const float y = kv_type<TY>::get(w.v[j]) * (kv_small(j) ? 16.0f * factor : factor);
+		const float y = kv_type<TY>::get(w.v[j]) * (kv_small(j) ? kv_form<TY>::MORE * factor : factor);
 		float z = (float)(f[0][j] = (_Float16)y);
 		if (QP > 1)
 			z += (float)(f[QP - 1][j] = rest(y, f[0][j]));
-		sum += kv_small(j) ? z * (1.0f / 16.0f) : z;
+		sum += kv_small(j) ? z * (1.0f / kv_form<TY>::MORE) : z;
 	}
 	return sum;
 }
@@ -272,24 +294,27 @@ __device__ static inline float kv_put_query(kv_query<D, QP> &q, const kv_vec<TY,
 #pragma unroll
 		for (int j = 0; j < 8; j++)
 			top = fmaxf(top, fabsf(kv_type<TY>::get(w[g].v[j])));
-	const kv_factor f = kv_query_factor(row_max(top), scale);
+	const kv_factor f = kv_query_factor<TY>(row_max(top), scale);
 #pragma unroll
 	for (int g = 0; g < D / 32; g++) {
 		if (g % waves != wave)
 			continue;
 		half8_t z[QP];
-		const float sum = row_sum(kv_split8<QP, TY>(w[g], f.query, z));
+		const float sum = kv_split8<QP, TY>(w[g], f.query, z);
 #pragma unroll
 		for (int p = 0; p < QP; p++)
 			q.f[p][g][lane] = z[p];
-		if (lane < 16)
-			q.start[g][lane] = (floatx4)(-8.0f * KV_CODE_STEP * sum);
+		if constexpr (!kv_form<TY>::EVEN) {
+			const float start = -8.0f * kv_form<TY>::STEP * row_sum(sum);
+			if (lane < 16)
+				q.start[g][lane] = (floatx4)start;
+		}
 	}
 	return f.score;
 }
 
 /* scores of 32 cached rows: 4 part + j of each half */
-template <int D, int QP>
+template <int D, int QP, int TY>
 __device__ static inline floatx8 kv_scores(const kv_keys<D> &k, const kv_query<D, QP> &q, int lane)
 {
 	floatx8 x;
@@ -299,11 +324,13 @@ __device__ static inline floatx8 kv_scores(const kv_keys<D> &k, const kv_query<D
 #pragma unroll
 		for (int p = 0; p < QP; p++)
 			f[p] = q.f[p][g][lane];
-		const floatx4 start = q.start[g][lane % 16];
+		floatx4 start = (floatx4)0.0f;
+		if constexpr (!kv_form<TY>::EVEN)
+			start = q.start[g][lane % 16];
 #pragma unroll
 		for (int h = 0; h < 2; h++) {
 			floatx4 acc = start;
-			const half8_t kf = kv_word(k.w[h][g]);
+			const half8_t kf = kv_form<TY>::EVEN ? kv_word8<TY>(k.w[h][g]) : kv_word(k.w[h][g]);
 #pragma unroll
 			for (int p = 0; p < QP; p++)
 				acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, f[p], acc, 0, 0, 0);
@@ -318,15 +345,12 @@ __device__ static inline floatx8 kv_scores(const kv_keys<D> &k, const kv_query<D
 /*
  * The running softmax of a query row.  ref is its reference in powers of two: a
  * probability is 2^(logit - ref), and ref the largest logit plus the exponent of
- * the value scales that come with it, less KV_REF, so that probability times value
- * scale stays below 2^KV_REF.  It stays as it is until the product would reach
- * 2^KV_TOP (16 times that is below f16's largest): most tiles then leave the output
+ * the value scales that come with it, less REF, so that probability times value
+ * scale stays below 2^REF.  It stays as it is until the product would reach 2^TOP
+ * (2^15 with kv_word's factor, below f16's largest): most tiles then leave the output
  * alone.  Sums and outputs carry the same factor, which the division at the end
  * takes out.
  */
-#define KV_REF 5.0f
-#define KV_TOP 11.0f
-
 struct kv_soft {
 	float ref, sum;
 };
@@ -335,7 +359,7 @@ struct kv_soft {
  * of 2), in f16 parts, 16 times that where the codes have the smaller step: rows
  * 4 i + j are codes 4 (i / (N / 8)) + j of step i % (N / 8).  Returns what the output
  * so far is multiplied by. */
-template <int N, int PP>
+template <int N, int PP, int TY>
 __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half4_t *dv, float rs,
 					  half8_t (&pf)[N / 8][PP])
 {
@@ -357,10 +381,10 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
 	/* (scales of nothing but zeros: exponent 0) */
 	const float most = fmaf(top, rs, (float)__builtin_amdgcn_frexp_expf(big));
 	const float high = N == 8 ? row_max(most) : half_max(most);
-	const float next = high - s.ref > KV_TOP ? high - KV_REF : s.ref;
+	const float next = high - s.ref > kv_form<TY>::TOP ? high - kv_form<TY>::REF : s.ref;
 	const float back = weight(s.ref, next);
 	s.ref = next;
-	const float ref = next == -__builtin_inff() ? 0.0f : next, ref16 = ref - 4.0f;
+	const float ref = next == -__builtin_inff() ? 0.0f : next, ref16 = ref - kv_form<TY>::LOG_MORE;
 	float sum = 0.0f, sum16 = 0.0f;
 #pragma unroll
 	for (int j = 0; j < N; j++) {
@@ -374,7 +398,7 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
 		if (PP > 1)
 			pf[h][PP - 1][at] = rest(w, pf[h][0][at]);
 	}
-	s.sum = s.sum * back + fmaf(sum16, 1.0f / 16.0f, sum);
+	s.sum = s.sum * back + fmaf(sum16, 1.0f / kv_form<TY>::MORE, sum);
 	return back;
 }
 
@@ -478,7 +502,7 @@ void k_kv_attn(
 		const half8_t vd8 = __builtin_bit_cast(half8_t, vd);
 		half4_t dv[2] = {vd8.lo, vd8.hi};
 		half8_t pf[1][PP];
-		floatx8 x = kv_scores<D, QP>(k, s_q, lane);
+		floatx8 x = kv_scores<D, QP, TY>(k, s_q, lane);
 		/* the scales are used up before their registers are loaded again */
 		asm volatile("" : "+v"(x) : : "memory");
 		if constexpr (more.value)
@@ -495,7 +519,7 @@ void k_kv_attn(
 			if (hidden && lane == 0)
 				kv_error(a, HIP_KV_ERR_PAGE);
 		}
-		const float back = kv_softmax<8, PP>(soft, (const float *)&x, dv, rs, pf);
+		const float back = kv_softmax<8, PP, TY>(soft, (const float *)&x, dv, rs, pf);
 		if (__ballot(back != 1.0f)) {
 #pragma unroll
 			for (int c = 0; c < CT; c++)
@@ -503,7 +527,7 @@ void k_kv_attn(
 		}
 #pragma unroll
 		for (int c = 0; c < CT; c++) {
-			const half8_t vf = kv_word8(v.w[c]);
+			const half8_t vf = kv_word8<TY>(v.w[c]);
 #pragma unroll
 			for (int p = 0; p < PP; p++)
 				o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[0][p], o[c], 0, 0, 0);
@@ -519,7 +543,7 @@ void k_kv_attn(
 		step(n - 1, std::false_type());
 
 	/* the waves' results: to one reference, then added in wave order */
-	float sum = KV_CODE_STEP * row_sum(soft.sum); /* the outputs' own factor */
+	float sum = kv_form<TY>::STEP * row_sum(soft.sum); /* the outputs' own factor */
 	if (part == 0)
 		s_ref[wave][lane] = soft.ref;
 	__syncthreads();
@@ -773,7 +797,7 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 #pragma unroll
 			for (int j = 0; j < 8; j++)
 				top = fmaxf(top, fabsf(T::get(w[u].v[j])));
-		const kv_factor f = kv_query_factor(half_max(top), scale);
+		const kv_factor f = kv_query_factor<TY>(half_max(top), scale);
 		rs = f.score;
 #pragma unroll
 		for (int u = 0; u < L::G; u++) {
@@ -788,8 +812,8 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 						sh.q[p][u][h][lane] = z[p];
 			}
 			/* in two f16 parts, of 11 bits and of the rest times 64 */
-			sum = -8.0f * KV_CODE_STEP * half_sum(sum);
-			if (part == 0) {
+			sum = -8.0f * kv_form<TY>::STEP * half_sum(sum);
+			if (!kv_form<TY>::EVEN && part == 0) {
 				surplus[u] = (_Float16)sum;
 				surplus[4 + u] = (_Float16)(64.0f * (sum - (float)surplus[u]));
 			}
@@ -842,13 +866,15 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 		const bool hidden = lost;
 		const uint8_t *next = tile_of(min(i + 1, n - 1));
 		half4_t dv[4];
-		floatx16 x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k.scales8(), surplus, (floatx16)0.0f, 0, 0, 0);
+		floatx16 x = (floatx16)0.0f;
+		if (!kv_form<TY>::EVEN)
+			x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k.scales8(), surplus, x, 0, 0, 0);
 #pragma unroll
 		for (int g = 0; g < L::G; g++) {
 			floatx16 acc = (floatx16)0.0f;
 #pragma unroll
 			for (int h = 0; h < 2; h++) {
-				const half8_t kf = kv_word(k.w[h][g]);
+				const half8_t kf = kv_form<TY>::EVEN ? kv_word8<TY>(k.w[h][g]) : kv_word(k.w[h][g]);
 #pragma unroll
 				for (int p = 0; p < QP; p++)
 					acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, sh.q[p][g][h][lane], acc, 0, 0, 0);
@@ -876,7 +902,7 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 				kv_error(a, HIP_KV_ERR_PAGE);
 		}
 		half8_t pf[2][PP];
-		const float back = kv_softmax<16, PP>(soft, (const float *)&x, dv, rs, pf);
+		const float back = kv_softmax<16, PP, TY>(soft, (const float *)&x, dv, rs, pf);
 		if (__ballot(back != 1.0f)) {
 			late *= back;
 #pragma unroll
@@ -888,7 +914,7 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 #pragma unroll
 			for (int h = 0; h < 2; h++) {
 				const u32 w = v.w[c / 2][h][c % 2];
-				const half8_t vf = LATE ? kv_word(w) : kv_word8(w);
+				const half8_t vf = LATE ? kv_word(w) : kv_word8<TY>(w);
 #pragma unroll
 				for (int p = 0; p < PP; p++)
 					o[c] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[h][p], o[c], 0, 0, 0);
@@ -905,7 +931,7 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 			o[c] -= late;
 
 	/* the waves' results: to one reference, then added in wave order */
-	const float sum = KV_CODE_STEP * half_sum(soft.sum);
+	const float sum = kv_form<TY>::STEP * half_sum(soft.sum);
 	if (part == 0)
 		s_ref[wave][lane] = soft.ref;
 	__syncthreads();
