@@ -53,8 +53,10 @@ __device__ static inline half8_t as_half8(u32 a, u32 b, u32 c, u32 d)
  * leading bit, so that the smaller ones lose four bits of the sum's 24, more than
  * enough for outputs of 8 or 11 bits (3e-6 of the output's norm).
  *
- * fp32 (kv_word8): with exponents that make both steps 1/16, 16 + code / 16 and
- * 1 + code / 16, of which 16.5 and 1.5 leave (code - 8) / 16, normal and exact (5e-7).
+ * fp32: all with the larger step (kv_word_even), for keys whose surplus of 8 is in the
+ * accumulators' start; or with exponents that make both steps 1/16, 16 + code / 16
+ * and 1 + code / 16, of which 16.5 and 1.5 leave (code - 8) / 16, normal and exact
+ * (kv_word8): 4e-7.
  */
 __device__ static inline half8_t kv_word(u32 w)
 {
@@ -72,12 +74,20 @@ __device__ static constexpr bool kv_small(int j)
  * largest value and of its largest probability times value scale (kv_soft below) */
 template <int TY> struct kv_form {
 	static constexpr bool EVEN = TY == HIP_KV_F32;
-	static constexpr float STEP = EVEN ? 1.0f / 16.0f : 1.0f / (1 << 18);
+	static constexpr float KEY_STEP = 1.0f / (1 << 18); /* kv_word, kv_word_even */
+	static constexpr float STEP = EVEN ? 1.0f / 16.0f : KEY_STEP; /* kv_word8 */
 	static constexpr float MORE = EVEN ? 1.0f : 16.0f; /* where the codes have the smaller step */
 	static constexpr int QUERY = EVEN ? 14 : 10;
 	static constexpr float LOG_MORE = EVEN ? 0.0f : 4.0f;
 	static constexpr float REF = EVEN ? 9.0f : 5.0f, TOP = EVEN ? 15.0f : 11.0f;
 };
+
+/* all codes with the larger step */
+__device__ static inline half8_t kv_word_even(u32 w)
+{
+	const u32 m = 0x03c003c0u;
+	return as_half8(w << 4 & m, w & m, w >> 4 & m, kv_rotr(w, 8) & m);
+}
 
 /* 8 in the steps of kv_word's codes */
 __device__ static inline half8_t kv_surplus8()
@@ -256,13 +266,13 @@ struct kv_factor {
 	float query, score;
 };
 
-template <int TY> __device__ static inline kv_factor kv_query_factor(float top, float scale)
+template <int TY> __device__ static inline kv_factor kv_query_factor(float top, float scale, float key_step)
 {
 	int e = kv_form<TY>::QUERY - __builtin_amdgcn_frexp_expf(top);
 	e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 122) : 0;
 	/* a negative scale turns the query around, 0 makes it 0 */
 	return {scale > 0.0f ? pow2(e) : scale < 0.0f ? -pow2(e) : 0.0f,
-		(scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / kv_form<TY>::STEP) * pow2(-e)};
+		(scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / key_step) * pow2(-e)};
 }
 
 /* eight channels of a query row in f16 parts, and their sum */
@@ -294,7 +304,7 @@ __device__ static inline float kv_put_query(kv_query<D, QP> &q, const kv_vec<TY,
 #pragma unroll
 		for (int j = 0; j < 8; j++)
 			top = fmaxf(top, fabsf(kv_type<TY>::get(w[g].v[j])));
-	const kv_factor f = kv_query_factor<TY>(row_max(top), scale);
+	const kv_factor f = kv_query_factor<TY>(row_max(top), scale, kv_form<TY>::KEY_STEP);
 #pragma unroll
 	for (int g = 0; g < D / 32; g++) {
 		if (g % waves != wave)
@@ -304,11 +314,9 @@ __device__ static inline float kv_put_query(kv_query<D, QP> &q, const kv_vec<TY,
 #pragma unroll
 		for (int p = 0; p < QP; p++)
 			q.f[p][g][lane] = z[p];
-		if constexpr (!kv_form<TY>::EVEN) {
-			const float start = -8.0f * kv_form<TY>::STEP * row_sum(sum);
-			if (lane < 16)
-				q.start[g][lane] = (floatx4)start;
-		}
+		const float start = -8.0f * kv_form<TY>::KEY_STEP * row_sum(sum);
+		if (lane < 16)
+			q.start[g][lane] = (floatx4)start;
 	}
 	return f.score;
 }
@@ -324,13 +332,11 @@ __device__ static inline floatx8 kv_scores(const kv_keys<D> &k, const kv_query<D
 #pragma unroll
 		for (int p = 0; p < QP; p++)
 			f[p] = q.f[p][g][lane];
-		floatx4 start = (floatx4)0.0f;
-		if constexpr (!kv_form<TY>::EVEN)
-			start = q.start[g][lane % 16];
+		const floatx4 start = q.start[g][lane % 16];
 #pragma unroll
 		for (int h = 0; h < 2; h++) {
 			floatx4 acc = start;
-			const half8_t kf = kv_form<TY>::EVEN ? kv_word8<TY>(k.w[h][g]) : kv_word(k.w[h][g]);
+			const half8_t kf = kv_form<TY>::EVEN ? kv_word_even(k.w[h][g]) : kv_word(k.w[h][g]);
 #pragma unroll
 			for (int p = 0; p < QP; p++)
 				acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, f[p], acc, 0, 0, 0);
@@ -797,7 +803,7 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 #pragma unroll
 			for (int j = 0; j < 8; j++)
 				top = fmaxf(top, fabsf(T::get(w[u].v[j])));
-		const kv_factor f = kv_query_factor<TY>(half_max(top), scale);
+		const kv_factor f = kv_query_factor<TY>(half_max(top), scale, kv_form<TY>::STEP);
 		rs = f.score;
 #pragma unroll
 		for (int u = 0; u < L::G; u++) {
