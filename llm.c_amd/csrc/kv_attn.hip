@@ -96,6 +96,14 @@ __device__ static inline half8_t kv_surplus8()
 	return half8_t{a, a, b, b, a, a, b, b};
 }
 
+/* (the compiler takes two instructions for want of a second scalar operand) */
+__device__ static inline u32 and_or(u32 x, u32 mask, u32 bits)
+{
+	u32 y;
+	asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(y) : "v"(x), "s"(mask), "v"(bits));
+	return y;
+}
+
 /* the codes less 8 */
 template <int TY> __device__ static inline half8_t kv_word8(u32 w)
 {
@@ -103,7 +111,7 @@ template <int TY> __device__ static inline half8_t kv_word8(u32 w)
 		return kv_word(w) - kv_surplus8();
 	const u32 r = kv_rotr(w, 8), m = 0x003c003cu, n = 0x03c003c0u, sixteen = 0x4c004c00u, one = 0x3c003c00u;
 	const _Float16 a = (_Float16)16.5f, b = (_Float16)1.5f;
-	return as_half8((w & m) | sixteen, (w & n) | one, (r & m) | sixteen, (r & n) | one) -
+	return as_half8(and_or(w, m, sixteen), and_or(w, n, one), and_or(r, m, sixteen), and_or(r, n, one)) -
 	       half8_t{a, a, b, b, a, a, b, b};
 }
 
@@ -177,14 +185,14 @@ struct kv_span {
 	bool valid;
 };
 
-template <int ROWS = KV_ROWS>
+template <int ROWS, int SLOTS = 1>
 __device__ static inline kv_span kv_rows_of(const kv_seq &sq, int tile, int G, int kv_head, int window,
 					    int lane)
 {
 	kv_span r;
 	const int base = sq.len - sq.n, all = sq.n * G;
-	const int mine = tile * ROWS + lane % ROWS, kept = min(mine, all - 1), i = kept / G;
-	const int i0 = __builtin_amdgcn_readlane(i, 0), i1 = __builtin_amdgcn_readlane(i, ROWS - 1);
+	const int mine = tile * ROWS + lane % (ROWS * SLOTS) / SLOTS, kept = min(mine, all - 1), i = kept / G;
+	const int i0 = __builtin_amdgcn_readlane(i, 0), i1 = __builtin_amdgcn_readlane(i, ROWS * SLOTS - 1);
 	r.valid = mine < all;
 	r.hi = base + i + 1;
 	r.lo = window ? max(0, r.hi - window) : 0;
@@ -205,6 +213,12 @@ template <int D> struct kv_keys {
 	__device__ inline float scale(int h, int j, int g) const
 	{
 		return (float)__builtin_bit_cast(half8_t, d[h][(j * L::G + g) / 8])[(j * L::G + g) % 8];
+	}
+	/* the one of two or four from word u on whose bytes pick names */
+	__device__ inline float scale_of(int h, int u, int n, u32 pick) const
+	{
+		const u32 lo = d[h][u / 4][u % 4], hi = n > 2 ? d[h][u / 4][u % 4 + 1] : lo;
+		return (float)__builtin_bit_cast(half2_t, __builtin_amdgcn_perm(hi, lo, pick))[0];
 	}
 	__device__ inline void load(const uint8_t *tile, int lane)
 	{
@@ -242,22 +256,33 @@ template <int D> struct kv_values {
 	}
 };
 
-/* value scales of the lane's eight rows */
-__device__ static inline u32x4 kv_value_scales(const uint8_t *scales, int lane)
-{
-	const u32x2 *p = (const u32x2 *)scales + lane / 16;
-	const u32x2 a = p[0], b = p[4];
-	return u32x4{a.x, a.y, b.x, b.y};
-}
+/* value scales of the lane's rows: two or four of its eight with slots */
+template <int SLOTS> struct kv_dv {
+	u32 w[4 / SLOTS];
+	__device__ inline void load(const uint8_t *scales, int lane)
+	{
+		const int c = lane % SLOTS, part = lane / 16;
+		if constexpr (SLOTS == 4) {
+			w[0] = ((const u32 *)scales)[8 * (c / 2) + 2 * part + c % 2];
+		} else {
+#pragma unroll
+			for (int h = 0; h < 2 / SLOTS; h++) {
+				const u32x2 a = ((const u32x2 *)scales)[4 * (SLOTS == 2 ? c : h) + part];
+				w[2 * h] = a.x;
+				w[2 * h + 1] = a.y;
+			}
+		}
+	}
+};
 
 /*
  * A tile of query rows as the products take it, in LDS for all waves: part p of
  * group g of the lane's row at f[p][g][lane], and what the accumulators start
- * with, -8 steps times the group's sum.
+ * with, -8 steps times the groups' sum.
  */
-template <int D, int QP> struct kv_query {
+template <int D, int QP, int SLOTS> struct kv_query {
 	half8_t f[QP][D / 32][WAVE];
-	floatx4 start[D / 32][16];
+	floatx4 start[D / 32 / SLOTS][16];
 };
 
 /* what a query row whose largest value is top is multiplied by, and its scores
@@ -294,9 +319,9 @@ __device__ static inline float kv_split8(const kv_vec<TY, 8> &w, float factor, h
 /* The groups g % waves == wave of a tile of query rows into LDS, from w, the lane's
  * quarter of each group of its row; returns the scores' factor.  The caller
  * synchronises. */
-template <int D, int QP, int TY>
-__device__ static inline float kv_put_query(kv_query<D, QP> &q, const kv_vec<TY, 8> (&w)[D / 32], float scale,
-					    int lane, int wave, int waves)
+template <int D, int QP, int SLOTS, int TY>
+__device__ static inline float kv_put_query(kv_query<D, QP, SLOTS> &q, const kv_vec<TY, 8> (&w)[D / 32],
+					    float scale, int lane, int wave, int waves)
 {
 	float top = 0.0f;
 #pragma unroll
@@ -309,42 +334,88 @@ __device__ static inline float kv_put_query(kv_query<D, QP> &q, const kv_vec<TY,
 	for (int g = 0; g < D / 32; g++) {
 		if (g % waves != wave)
 			continue;
+		const bool own = lane % SLOTS == g % SLOTS;
 		half8_t z[QP];
-		const float sum = kv_split8<QP, TY>(w[g], f.query, z);
+		const float start = -8.0f * kv_form<TY>::KEY_STEP * row_sum(kv_split8<QP, TY>(w[g], f.query, z));
 #pragma unroll
 		for (int p = 0; p < QP; p++)
-			q.f[p][g][lane] = z[p];
-		const float start = -8.0f * kv_form<TY>::KEY_STEP * row_sum(sum);
-		if (lane < 16)
-			q.start[g][lane] = (floatx4)start;
+			q.f[p][g][lane] = own ? z[p] : (half8_t)(_Float16)0.0f;
+		if (own && lane < 16)
+			q.start[g / SLOTS][lane] = (floatx4)start;
 	}
 	return f.score;
 }
 
-/* scores of 32 cached rows: 4 part + j of each half */
-template <int D, int QP, int TY>
-__device__ static inline floatx8 kv_scores(const kv_keys<D> &k, const kv_query<D, QP> &q, int lane)
+/* v of the lane whose number differs in the bit BY, 1 or 2 */
+template <int BY> __device__ static inline float other(float v)
 {
-	floatx8 x;
+	/* quad_perm 1 0 3 2, 2 3 0 1 */
+	return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), BY == 1 ? 0xb1 : 0x4e,
+								  0xf, 0xf, true));
+}
+
+/* the sums of v[N] over the lane and the one beside it: the lower lane's are the
+ * first half, the upper's the second */
+template <int BY, int N> __device__ static inline void halved(const float (&v)[N], bool upper, float *out)
+{
 #pragma unroll
-	for (int g = 0; g < D / 32; g++) {
-		half8_t f[QP];
+	for (int i = 0; i < N / 2; i++) {
+		const float mine = upper ? v[N / 2 + i] : v[i], theirs = upper ? v[i] : v[N / 2 + i];
+		out[i] = mine + other<BY>(theirs);
+	}
+}
+
+/* Scores of the lane's 8 / SLOTS cached rows: of 4 part + j of each half, j < 4, the
+ * share of the lane's slot. */
+template <int D, int QP, int SLOTS, int TY>
+__device__ static inline auto kv_scores(const kv_keys<D> &k, const kv_query<D, QP, SLOTS> &q, int lane)
+{
+	typedef float floats __attribute__((ext_vector_type(8 / SLOTS)));
+	constexpr int G = D / 32, NA = G / SLOTS; /* groups, and of a slot */
+	const u32 b = 2 * (lane % SLOTS), pick = b | (b + 1) << 8 | 0x0c0c0000u;
+	floats x;
+	float y[8];
 #pragma unroll
-		for (int p = 0; p < QP; p++)
-			f[p] = q.f[p][g][lane];
-		const floatx4 start = q.start[g][lane % 16];
+	for (int a = 0; a < NA; a++) {
+		const floatx4 start = q.start[a][lane % 16];
+		floatx4 acc[2] = {start, start};
 #pragma unroll
-		for (int h = 0; h < 2; h++) {
-			floatx4 acc = start;
-			const half8_t kf = kv_form<TY>::EVEN ? kv_word_even(k.w[h][g]) : kv_word(k.w[h][g]);
+		for (int g = a * SLOTS; g < (a + 1) * SLOTS; g++) {
+			half8_t f[QP];
 #pragma unroll
 			for (int p = 0; p < QP; p++)
-				acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, f[p], acc, 0, 0, 0);
+				f[p] = q.f[p][g][lane];
 #pragma unroll
-			for (int j = 0; j < 4; j++)
-				x[4 * h + j] = fmaf(k.scale(h, j, g), acc[j], g ? x[4 * h + j] : 0.0f);
+			for (int h = 0; h < 2; h++) {
+				const half8_t kf = kv_form<TY>::EVEN ? kv_word_even(k.w[h][g]) : kv_word(k.w[h][g]);
+#pragma unroll
+				for (int p = 0; p < QP; p++)
+					acc[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, f[p], acc[h], 0, 0, 0);
+			}
 		}
+#pragma unroll
+		for (int h = 0; h < 2; h++)
+#pragma unroll
+			for (int j = 0; j < 4; j++) {
+				const int at = 4 * h + j;
+				const float d = SLOTS == 1 ? k.scale(h, j, a) : k.scale_of(h, (j * G + a * SLOTS) / 2, SLOTS, pick);
+				y[at] = fmaf(d, acc[h][j], a ? y[at] : 0.0f);
+			}
 	}
+	if constexpr (SLOTS == 4) {
+		float t[4];
+		halved<2>(y, lane & 2, t);
+		halved<1>(t, lane & 1, y);
+	} else if constexpr (SLOTS == 2) {
+		float t[4];
+		halved<1>(y, lane & 1, t);
+#pragma unroll
+		for (int j = 0; j < 4; j++)
+			y[j] = t[j];
+	}
+#pragma unroll
+	for (int j = 0; j < 8 / SLOTS; j++)
+		x[j] = y[j];
 	return x;
 }
 
@@ -361,14 +432,19 @@ struct kv_soft {
 	float ref, sum;
 };
 
-/* probabilities times value scales of the lane's N cached rows (8 of 4 lanes, 16
- * of 2), in f16 parts, 16 times that where the codes have the smaller step: rows
- * 4 i + j are codes 4 (i / (N / 8)) + j of step i % (N / 8).  Returns what the output
- * so far is multiplied by. */
-template <int N, int PP, int TY>
-__device__ static inline float kv_softmax(kv_soft &s, const float *x, const half4_t *dv, float rs,
-					  half8_t (&pf)[N / 8][PP])
+template <int N> using kv_halves = _Float16 __attribute__((ext_vector_type(N)));
+
+/*
+ * Probabilities times value scales of the lane's N cached rows, in f16 parts;
+ * 16 times that where the codes have the smaller step: two of four rows, or (N = 2)
+ * both of a lane with more = 4.  SPAN lanes 16 apart, or two 32 apart, hold the query
+ * row's others.  Returns what the output so far is multiplied by.
+ */
+template <int N, int SPAN, int PP, int TY>
+__device__ static inline float kv_softmax(kv_soft &s, const float *x, const half2_t *dv, float rs, float more,
+					  kv_halves<N> (&pf)[PP])
 {
+	constexpr float LOG_MORE = kv_form<TY>::LOG_MORE, MORE = kv_form<TY>::MORE;
 	float top = x[0];
 #pragma unroll
 	for (int j = 1; j < N; j++)
@@ -376,35 +452,34 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
 	/* f16 without their sign order as whole numbers do */
 	ushort2_t most2 = {0, 0};
 #pragma unroll
-	for (int i = 0; i < N / 4; i++) {
-		const u32x2 w = __builtin_bit_cast(u32x2, dv[i]);
-		const u32 a = w.x & 0x7fff7fffu, b = w.y & 0x7fff7fffu; /* (bit_cast takes no element) */
+	for (int i = 0; i < N / 2; i++) {
+		const u32 a = __builtin_bit_cast(u32, dv[i]) & 0x7fff7fffu;
 		most2 = __builtin_elementwise_max(most2, __builtin_bit_cast(ushort2_t, a));
-		most2 = __builtin_elementwise_max(most2, __builtin_bit_cast(ushort2_t, b));
 	}
 	const unsigned short most1 = most2.x > most2.y ? most2.x : most2.y;
 	const float big = (float)__builtin_bit_cast(_Float16, most1);
 	/* (scales of nothing but zeros: exponent 0) */
 	const float most = fmaf(top, rs, (float)__builtin_amdgcn_frexp_expf(big));
-	const float high = N == 8 ? row_max(most) : half_max(most);
+	const float high = SPAN == 4 ? row_max(most) : half_max(most);
 	const float next = high - s.ref > kv_form<TY>::TOP ? high - kv_form<TY>::REF : s.ref;
 	const float back = weight(s.ref, next);
 	s.ref = next;
-	const float ref = next == -__builtin_inff() ? 0.0f : next, ref16 = ref - kv_form<TY>::LOG_MORE;
+	const float ref = next == -__builtin_inff() ? 0.0f : next;
+	const float ref16 = N == 2 && LOG_MORE > 0.0f ? ref - more : ref - LOG_MORE;
 	float sum = 0.0f, sum16 = 0.0f;
 #pragma unroll
 	for (int j = 0; j < N; j++) {
 		const float p = __builtin_amdgcn_exp2f(fmaf(x[j], rs, kv_small(j) ? -ref16 : -ref));
 		(kv_small(j) ? sum16 : sum) += p;
-		float w = fmaf((float)dv[j / 4][j % 4], p, 0.0f); /* fma: takes an f16 as it is */
+		float w = fmaf((float)dv[j / 2][j % 2], p, 0.0f); /* fma: takes an f16 as it is */
 		if (PP > 1)
 			asm("" : "+v"(w)); /* once, not once for each part */
-		const int h = j / 4 % (N / 8), at = j / 4 / (N / 8) * 4 + j % 4;
-		pf[h][0][at] = (_Float16)w;
+		pf[0][j] = (_Float16)w;
 		if (PP > 1)
-			pf[h][PP - 1][at] = rest(w, pf[h][0][at]);
+			pf[PP - 1][j] = rest(w, pf[0][j]);
 	}
-	s.sum = s.sum * back + fmaf(sum16, 1.0f / kv_form<TY>::MORE, sum);
+	const float less = N == 2 && more == 0.0f ? 1.0f : 1.0f / MORE;
+	s.sum = s.sum * back + fmaf(sum16, less, sum);
 	return back;
 }
 
@@ -415,11 +490,20 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
  * and unnormalised output in ws for k_kv_merge.  A wave loads a tile's keys
  * while it still works on the values of the tile before, and the values while
  * it works on the keys.
+ *
+ * SLOTS columns of the products belong to one query row where there are few, four
+ * for rows up to 4 (heads of 128 and 256), two for up to 8.  In the first product a
+ * slot has its share of the channel groups and zeros for the others: the partial
+ * scores of a row's groups come out in different lanes, which multiply them by their
+ * own scales, add up and keep 8 / SLOTS of the cached rows each (scale products and
+ * exponentials a row: 8 and 2 instead of 32 and 8 for four slots).  In the second
+ * product a slot has its cached rows and zeros for the others; its statistics and
+ * output are its own, like another wave's.
  */
-/* three waves a SIMD, so that nothing is kept in accumulation registers and moved;
- * heads of 256 do not fit */
-template <int D, int TY, int NW>
-__global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(D < 256 ? 3 : 1)))
+/* by the registers: four waves a SIMD with slots, three without, two for heads of
+ * 256.  Nothing is kept in accumulation registers and moved. */
+template <int D, int TY, int NW, int SLOTS>
+__global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(D == 256 ? 2 : SLOTS > 1 ? 4 : 3)))
 void k_kv_attn(
 	kv_args a, const typename kv_type<TY>::t *q, size_t q_stride, int G,
 	typename kv_type<TY>::t *out, size_t out_stride, float scale, int window, float *ws,
@@ -429,12 +513,16 @@ void k_kv_attn(
 	typedef kv_tile<D> L;
 	constexpr int QP = TY == HIP_KV_F32 ? 2 : 1, PP = TY == HIP_KV_BF16 ? 1 : 2;
 	constexpr int CT = D / 16; /* channel tiles of O^T */
-	__shared__ float s_o[NW][KV_ROWS][D + 4];
+	constexpr int ROWS = KV_ROWS / SLOTS, N = 8 / SLOTS;
+	/* the queries, then the waves' outputs */
+	__shared__ union {
+		kv_query<D, QP, SLOTS> q;
+		float o[NW][KV_ROWS][D + 4];
+	} sh;
 	__shared__ float s_ref[NW][KV_ROWS], s_sum[NW][KV_ROWS];
-	__shared__ int s_row[KV_ROWS], s_head[KV_ROWS];
-	__shared__ kv_query<D, QP> s_q;
+	__shared__ int s_row[ROWS], s_head[ROWS];
 
-	const int lane = threadIdx.x % WAVE, part = lane / 16;
+	const int lane = threadIdx.x % WAVE, part = lane / 16, slot = lane % SLOTS;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
 	const int kv_head = blockIdx.x % a.kv_heads, rt = blockIdx.x / a.kv_heads;
 	const int split = blockIdx.y, splits = gridDim.y, s = blockIdx.z;
@@ -449,9 +537,9 @@ void k_kv_attn(
 		page = at < a.table_stride ? table[at] : -1;
 	}
 	const kv_seq sq = kv_sequence(a, s);
-	if (rt * KV_ROWS >= sq.n * G)
+	if (rt * ROWS >= sq.n * G)
 		return;
-	const kv_span r = kv_rows_of(sq, rt, G, kv_head, window, lane);
+	const kv_span r = kv_rows_of<ROWS, SLOTS>(sq, rt, G, kv_head, window, lane);
 	const int t0 = r.first / KV_TILE + split * chunk;
 	const int t1 = min(t0 + chunk, (max(r.last, 0) + KV_TILE - 1) / KV_TILE);
 	if (split > 0 && t0 >= t1)
@@ -477,19 +565,19 @@ void k_kv_attn(
 	};
 	kv_keys<D> k;
 	kv_values<D> v;
-	u32x4 vd;
+	kv_dv<SLOTS> vd;
 	if (n > 0) {
 		const uint8_t *tile = tile_of(0);
 		k.load(tile, lane);
-		vd = kv_value_scales(tile + L::V_SCALES, lane);
+		vd.load(tile + L::V_SCALES, lane);
 		v.load(tile, lane);
 	} else if (!a.pages && lane == 0) {
 		kv_error(a, HIP_KV_ERR_PAGE);
 	}
-	const float rs = kv_put_query<D, QP, TY>(s_q, qv, scale, lane, wave, NW);
-	if (threadIdx.x < KV_ROWS) {
-		s_row[threadIdx.x] = r.valid ? r.row : -1;
-		s_head[threadIdx.x] = r.hi > r.lo ? r.head : ~r.head;
+	const float rs = kv_put_query<D, QP, SLOTS, TY>(sh.q, qv, scale, lane, wave, NW);
+	if (threadIdx.x < KV_ROWS && slot == 0) {
+		s_row[threadIdx.x / SLOTS] = r.valid ? r.row : -1;
+		s_head[threadIdx.x / SLOTS] = r.hi > r.lo ? r.head : ~r.head;
 	}
 	__syncthreads();
 
@@ -505,10 +593,13 @@ void k_kv_attn(
 		const uint8_t *next = NULL;
 		if constexpr (more.value)
 			next = tile_of(i + 1);
-		const half8_t vd8 = __builtin_bit_cast(half8_t, vd);
-		half4_t dv[2] = {vd8.lo, vd8.hi};
-		half8_t pf[1][PP];
-		floatx8 x = kv_scores<D, QP, TY>(k, s_q, lane);
+		half2_t dv[N / 2];
+		kv_halves<N> pp[PP];
+#pragma unroll
+		for (int j = 0; j < N / 2; j++)
+			dv[j] = __builtin_bit_cast(half2_t, vd.w[j]);
+		typedef float floats __attribute__((ext_vector_type(N)));
+		floats x = kv_scores<D, QP, SLOTS, TY>(k, sh.q, lane);
 		/* the scales are used up before their registers are loaded again */
 		asm volatile("" : "+v"(x) : : "memory");
 		if constexpr (more.value)
@@ -516,16 +607,32 @@ void k_kv_attn(
 		if (hidden || t * KV_TILE < r.inner0 || (t + 1) * KV_TILE > r.inner1) {
 			const int lo = hidden ? 0x7fffffff : r.lo;
 #pragma unroll
-			for (int j = 0; j < 8; j++) {
-				const int at = t * KV_TILE + 16 * (j / 4) + 4 * part + j % 4;
+			for (int j = 0; j < N; j++) {
+				const int u = slot * N + j, at = t * KV_TILE + 16 * (u / 4) + 4 * part + u % 4;
 				const bool hide = at < lo || at >= r.hi;
 				x[j] = hide ? -__builtin_inff() : x[j];
-				dv[j / 4][j % 4] = hide ? (_Float16)0.0f : dv[j / 4][j % 4];
+				dv[j / 2][j % 2] = hide ? (_Float16)0.0f : dv[j / 2][j % 2];
 			}
 			if (hidden && lane == 0)
 				kv_error(a, HIP_KV_ERR_PAGE);
 		}
-		const float back = kv_softmax<8, PP, TY>(soft, (const float *)&x, dv, rs, pf);
+		const float back = kv_softmax<N, 4, PP, TY>(soft, (const float *)&x, dv, rs, slot % 2 ? 0.0f : 4.0f, pp);
+		/* a slot's column has its rows alone */
+		half8_t pf[PP];
+#pragma unroll
+		for (int p = 0; p < PP; p++) {
+			if constexpr (SLOTS == 1) {
+				pf[p] = pp[p];
+			} else {
+				typedef u32 words __attribute__((ext_vector_type(N / 2)));
+				const words z = __builtin_bit_cast(words, pp[p]);
+				u32 w[4];
+#pragma unroll
+				for (int u = 0; u < 4; u++)
+					w[u] = u / (N / 2) == slot ? z[u % (N / 2)] : 0;
+				pf[p] = as_half8(w[0], w[1], w[2], w[3]);
+			}
+		}
 		if (__ballot(back != 1.0f)) {
 #pragma unroll
 			for (int c = 0; c < CT; c++)
@@ -536,10 +643,10 @@ void k_kv_attn(
 			const half8_t vf = kv_word8<TY>(v.w[c]);
 #pragma unroll
 			for (int p = 0; p < PP; p++)
-				o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[0][p], o[c], 0, 0, 0);
+				o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[p], o[c], 0, 0, 0);
 		}
 		if constexpr (more.value) {
-			vd = kv_value_scales(next + L::V_SCALES, lane);
+			vd.load(next + L::V_SCALES, lane);
 			v.load(next, lane);
 		}
 	};
@@ -553,31 +660,33 @@ void k_kv_attn(
 	if (part == 0)
 		s_ref[wave][lane] = soft.ref;
 	__syncthreads();
-	float ref = s_ref[0][lane % 16];
+	float ref = -__builtin_inff(); /* of the row, whichever column */
 #pragma unroll
-	for (int w = 1; w < NW; w++)
-		ref = fmaxf(ref, s_ref[w][lane % 16]);
+	for (int w = 0; w < NW; w++)
+#pragma unroll
+		for (int c = 0; c < SLOTS; c++)
+			ref = fmaxf(ref, s_ref[w][lane % 16 - slot + c]);
 	const float factor = weight(soft.ref, ref);
 	if (r.valid) {
 #pragma unroll
 		for (int c = 0; c < CT; c++)
-			*(floatx4 *)&s_o[wave][lane % 16][16 * c + 4 * part] = o[c] * factor;
+			*(floatx4 *)&sh.o[wave][lane % 16][16 * c + 4 * part] = o[c] * factor;
 		if (part == 0)
 			s_sum[wave][lane] = sum * factor;
 	}
 	__syncthreads();
-	const size_t slot = ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
-	float *to = ws + slot * nrows * (D + 4);
-	for (int at = threadIdx.x; at < KV_ROWS * D / 4; at += NW * WAVE) {
+	const size_t piece = ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
+	float *to = ws + piece * nrows * (D + 4);
+	for (int at = threadIdx.x; at < ROWS * D / 4; at += NW * WAVE) {
 		const int i = at / (D / 4), c = at % (D / 4) * 4, row = s_row[i];
 		if (row < 0)
 			break; /* the rows behind are not there either */
-		float den = s_sum[0][i];
-		floatx4 y = *(const floatx4 *)&s_o[0][i][c];
+		float den = s_sum[0][i * SLOTS];
+		floatx4 y = *(const floatx4 *)&sh.o[0][i * SLOTS][c];
 #pragma unroll
-		for (int w = 1; w < NW; w++) {
-			den += s_sum[w][i];
-			y += *(const floatx4 *)&s_o[w][i][c];
+		for (int w = 1; w < NW * SLOTS; w++) {
+			den += s_sum[w / SLOTS][i * SLOTS + w % SLOTS];
+			y += *(const floatx4 *)&sh.o[w / SLOTS][i * SLOTS + w % SLOTS][c];
 		}
 		if (splits == 1) {
 			kv_vec<TY, 4> z;
@@ -590,10 +699,10 @@ void k_kv_attn(
 		}
 		*(floatx4 *)(to + i * (D + 4) + c) = y;
 		if (c == 0) {
-			float high = s_ref[0][i];
+			float high = s_ref[0][i * SLOTS];
 #pragma unroll
-			for (int w = 1; w < NW; w++)
-				high = fmaxf(high, s_ref[w][i]);
+			for (int w = 1; w < NW * SLOTS; w++)
+				high = fmaxf(high, s_ref[w / SLOTS][i * SLOTS + w % SLOTS]);
 			to[i * (D + 4) + D] = high;
 			to[i * (D + 4) + D + 1] = den;
 		}
@@ -871,7 +980,8 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 		const int t = t0 + wave + i * KV_WAVES;
 		const bool hidden = lost;
 		const uint8_t *next = tile_of(min(i + 1, n - 1));
-		half4_t dv[4];
+		half2_t dv[8];
+		kv_halves<16> pp[PP];
 		floatx16 x = (floatx16)0.0f;
 		if (!kv_form<TY>::EVEN)
 			x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k.scales8(), surplus, x, 0, 0, 0);
@@ -893,8 +1003,12 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 		asm volatile("" : "+v"(x) : : "memory");
 		k.load(next, lane);
 #pragma unroll
-		for (int j = 0; j < 4; j++)
-			dv[j] = __builtin_bit_cast(half4_t, v.d[j]);
+		for (int j = 0; j < 4; j++) {
+			const u32x2 w = v.d[j];
+			const u32 lo = w.x, hi = w.y; /* (bit_cast takes no element) */
+			dv[2 * j] = __builtin_bit_cast(half2_t, lo);
+			dv[2 * j + 1] = __builtin_bit_cast(half2_t, hi);
+		}
 		if (hidden || t * KV_TILE < r.inner0 || (t + 1) * KV_TILE > r.inner1) {
 			const int lo = hidden ? 0x7fffffff : r.lo;
 #pragma unroll
@@ -902,13 +1016,19 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 				const int at = t * KV_TILE + 8 * (j / 4) + 4 * part + j % 4;
 				const bool hide = at < lo || at >= r.hi;
 				x[j] = hide ? -__builtin_inff() : x[j];
-				dv[j / 4][j % 4] = hide ? (_Float16)0.0f : dv[j / 4][j % 4];
+				dv[j / 2][j % 2] = hide ? (_Float16)0.0f : dv[j / 2][j % 2];
 			}
 			if (hidden && lane == 0)
 				kv_error(a, HIP_KV_ERR_PAGE);
 		}
 		half8_t pf[2][PP];
-		const float back = kv_softmax<16, PP, TY>(soft, (const float *)&x, dv, rs, pf);
+		const float back = kv_softmax<16, 2, PP, TY>(soft, (const float *)&x, dv, rs, 0.0f, pp);
+		/* rows 8 i + .. are in step i % 2, codes 4 (i / 2) .. of the words */
+#pragma unroll
+		for (int p = 0; p < PP; p++) {
+			pf[0][p] = __builtin_shufflevector(pp[p], pp[p], 0, 1, 2, 3, 8, 9, 10, 11);
+			pf[1][p] = __builtin_shufflevector(pp[p], pp[p], 4, 5, 6, 7, 12, 13, 14, 15);
+		}
 		if (__ballot(back != 1.0f)) {
 			late *= back;
 #pragma unroll
@@ -1004,6 +1124,7 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	const long rows = (long)a->max_rows * G;
 	p->row_tiles = (int)((rows + KV_ROWS - 1) / KV_ROWS);
 	p->rows = (int)(rows < KV_ROWS ? rows : KV_ROWS);
+	p->slots = rows <= 4 && head_len > 64 ? 4 : rows <= 8 ? 2 : 1;
 	const size_t wgs = (size_t)a->nseq * a->kv_heads * p->row_tiles;
 	p->wide = head_len < 256 && rows >= 2 * KV_WIDE && wgs >= 512;
 	if (p->wide) {
@@ -1052,16 +1173,19 @@ extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const vo
 				p->row_tiles);
 			return (int)hipGetLastError();
 		}
-		/* (heads of 256 have no room for KV_MANY waves) */
-		constexpr int MANY = D < 256 ? KV_MANY : KV_WAVES;
+		/* (heads of 256 have no room for KV_MANY waves, of 64 no four groups) */
+		constexpr int MANY = D < 256 ? KV_MANY : KV_WAVES, FOUR = D > 64 ? 4 : 2;
+		const auto launch = [&](auto kernel) {
+			kernel<<<grid, p->waves * WAVE, 0, (hipStream_t)stream>>>(
+				*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window, (float *)ws,
+				p->row_tiles, p->chunk, p->rows);
+		};
 		if (p->waves == KV_MANY)
-			k_kv_attn<D, TY, MANY><<<grid, MANY * WAVE, 0, (hipStream_t)stream>>>(
-				*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window,
-				(float *)ws, p->row_tiles, p->chunk, p->rows);
+			launch(p->slots == 4 ? k_kv_attn<D, TY, MANY, FOUR> :
+			       p->slots == 2 ? k_kv_attn<D, TY, MANY, 2> : k_kv_attn<D, TY, MANY, 1>);
 		else
-			k_kv_attn<D, TY, KV_WAVES><<<grid, KV_NT, 0, (hipStream_t)stream>>>(
-				*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window,
-				(float *)ws, p->row_tiles, p->chunk, p->rows);
+			launch(p->slots == 4 ? k_kv_attn<D, TY, KV_WAVES, FOUR> :
+			       p->slots == 2 ? k_kv_attn<D, TY, KV_WAVES, 2> : k_kv_attn<D, TY, KV_WAVES, 1>);
 		if (p->splits > 1)
 			k_kv_merge<D, TY><<<rows, KV_NT, 0, (hipStream_t)stream>>>(
 				*a, G, (t *)out, out_stride, window, (const float *)ws, p->row_tiles,

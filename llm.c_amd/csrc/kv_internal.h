@@ -42,6 +42,7 @@ typedef struct kv_plan {
 	int row_tiles; /* tiles of query rows of one (sequence, kv head) */
 	int wide;      /* tiles of 32 query rows */
 	int rows;      /* query rows of a tile, at most */
+	int slots;     /* columns of a query row */
 	int waves;     /* of a workgroup */
 	int chunk;     /* cache tiles of one workgroup */
 	int splits;    /* workgroups along the cache */
