@@ -233,7 +233,7 @@ static int make_args(const char *what, const hip_kv_cache *C, const hip_kv_batch
 	a->rows = (int)B->rows;
 	a->max_rows = (int)B->max_rows;
 	a->max_len = (int)B->max_len;
-	if (grid_of(B->nseq, B->max_rows / KV_TILE + 2, C->kv_heads) >= MAX_GRID)
+	if (grid_of(B->nseq, 4 * (B->max_rows / KV_TILE + 2), C->kv_heads) >= MAX_GRID)
 		return kv_err("%s: %zu sequences of up to %zu rows are too many for one call", what,
 			      B->nseq, B->max_rows);
 	return 1;

@@ -503,7 +503,7 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
 /* by the registers: four waves a SIMD with slots, three without, two for heads of
  * 256.  Nothing is kept in accumulation registers and moved. */
 template <int D, int TY, int NW, int SLOTS>
-__global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(D == 256 ? 2 : SLOTS > 1 ? 4 : 3)))
+__global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(D == 256 ? 2 : SLOTS > 1 && NW == KV_WAVES ? 4 : 3)))
 void k_kv_attn(
 	kv_args a, const typename kv_type<TY>::t *q, size_t q_stride, int G,
 	typename kv_type<TY>::t *out, size_t out_stride, float scale, int window, float *ws,

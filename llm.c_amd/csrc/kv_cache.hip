@@ -279,21 +279,23 @@ template <int LANES, int N> __device__ static inline _Float16 kv_encode(const fl
 }
 
 /*
- * One workgroup: the call's rows in one tile of one sequence, for `per` kv heads
- * and as large a share of the q heads.  The rows' angles go into LDS once; then a
- * wave takes a row and as many heads as it has lanes for (16 bytes of a head row a
- * lane) at a time, keys and values or queries.  Keys meet their group's scale, values
- * their row's, over a few lanes.  The value codes go to LDS, since one word holds
- * eight rows' codes of a channel: the words are put together from there, and a word
- * that has other rows' codes too is read first and keeps them.
+ * One workgroup: the call's rows among the eight of one tile of one sequence that
+ * share value words (4 part + (0 .. 3) of each half), for `per` kv heads and as large
+ * a share of the q heads: few rows and many heads, since each workgroup works out the
+ * angles of its rows, into LDS.  Then a wave takes a row and as many heads as it has
+ * lanes for (16 bytes of a head row a lane) at a time, keys and values or queries.
+ * Keys meet their group's scale, values their row's, over a few lanes.  The value codes
+ * go to LDS: the words are put together from there, and a word that has other rows'
+ * codes too is read first and keeps them.
  */
 #define KV_APPEND_NT 512
+#define KV_PART 8 /* rows of a workgroup, at most */
 
 template <int D, int TY>
 __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 	kv_args a, hip_rope R, const typename kv_type<TY>::t *k, const typename kv_type<TY>::t *v,
 	size_t kv_stride, const int32_t *pos, const typename kv_type<TY>::t *q, size_t q_stride,
-	int heads, typename kv_type<TY>::t *q_out, size_t q_out_stride, int per, int tiles, int most)
+	int heads, typename kv_type<TY>::t *q_out, size_t q_out_stride, int per, int tiles, int parts)
 {
 	typedef kv_type<TY> T;
 	typedef kv_tile<D> L;
@@ -301,19 +303,27 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 	constexpr int HP = WAVE / HL;                 /* heads of a wave's step */
 	constexpr int GL = 32 / N;                    /* lanes of a key group */
 	typedef typename kv_wide<TY>::vec vec;
-	extern __shared__ double2 turns[]; /* [most][kv_slot(rot / 2)], then the codes [per][most][D] */
+	extern __shared__ double2 turns[]; /* [rows][kv_slot(rot / 2)], then the codes [per][rows][D] */
 	const int half = (int)R.rot / 2, slots = kv_slot(half);
+	const int most = parts > 1 ? KV_PART : 1;
 	uint8_t *codes = (uint8_t *)(turns + most * slots);
 
 	const int groups = (a.kv_heads + per - 1) / per;
-	const int hg = blockIdx.x % groups, tb = blockIdx.x / groups % tiles;
-	const int s = blockIdx.x / groups / tiles;
+	const int hg = blockIdx.x % groups, unit = blockIdx.x / groups % (tiles * parts);
+	const int s = blockIdx.x / groups / (tiles * parts);
 	const kv_seq sq = kv_sequence(a, s);
-	const int base = sq.len - sq.n, p0 = max(0, base), t = p0 / KV_TILE + tb;
-	const int lo = max(p0, t * KV_TILE), hi = min(sq.len, (t + 1) * KV_TILE);
-	if (lo >= hi)
+	const int base = sq.len - sq.n, p0 = max(0, base), t = p0 / KV_TILE + unit / parts;
+	/* the part (a single row's own), and its rows i0 .. i0 + n - 1 in their order: row
+	 * 16 (i / 4) + 4 part + i % 4 of the tile */
+	const int part = parts > 1 ? unit % parts : p0 % 16 / 4;
+	const auto row_of = [&](int i) { return i / 4 * 16 + 4 * part + i % 4; };
+	const auto below = [&](int r) { /* rows of the part before row r of the tile */
+		return min(4, max(0, r - 4 * part)) + min(4, max(0, r - 16 - 4 * part));
+	};
+	const int i0 = below(p0 - t * KV_TILE), n = below(min(sq.len - t * KV_TILE, KV_TILE)) - i0;
+	if (n <= 0)
 		return;
-	const int n = hi - lo, r0 = lo % KV_TILE, row0 = sq.row + lo - base;
+	const int row0 = sq.row + t * KV_TILE - base; /* + r: row r of the tile among the call's */
 	const int h0 = hg * per, h1 = min(h0 + per, a.kv_heads);
 	const int q0 = q ? (int)((long)heads * h0 / a.kv_heads) : 0;
 	const int q1 = q ? (int)((long)heads * h1 / a.kv_heads) : 0;
@@ -335,13 +345,13 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 		kv_turn_in<TY> in;
 		vec val;
 		const typename T::t *x;
-		int i, h; /* row of the tile, head; h < 0: query head ~h */
+		int i, h; /* row of the part, head; h < 0: query head ~h */
 	};
 	const auto fetch = [&](int at) {
 		item z;
 		z.i = at / steps;
 		const int step = at % steps;
-		const size_t row = row0 + z.i;
+		const size_t row = row0 + row_of(i0 + z.i);
 		if (step >= ks) {
 			const int h = min(q0 + (step - ks) * HP + sub, q1 - 1); /* (the last head again) */
 			z.h = ~h;
@@ -358,8 +368,8 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 	if (wave < n * steps)
 		next = fetch(wave);
 	for (int at = threadIdx.x; at < n * half; at += KV_APPEND_NT) {
-		const int r = at / half;
-		turns[r * slots + kv_slot(at % half)] = kv_turn(R, pos ? pos[row0 + r] : lo + r, at % half);
+		const int i = at / half, r = row_of(i0 + i);
+		turns[i * slots + kv_slot(at % half)] = kv_turn(R, pos ? pos[row0 + r] : t * KV_TILE + r, at % half);
 	}
 	__syncthreads();
 	for (int at = wave; at < n * steps; at += NW) {
@@ -375,11 +385,11 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 			for (int u = 0; u < N; u++)
 				o.v[u] = T::put(y[u]);
 			__builtin_amdgcn_wave_barrier(); /* in place: the lanes' loads come first */
-			*(vec *)(q_out + (size_t)(row0 + i) * q_out_stride + (size_t)~z.h * D + c0) = o;
+			*(vec *)(q_out + (size_t)(row0 + row_of(i0 + i)) * q_out_stride + (size_t)~z.h * D + c0) = o;
 			continue;
 		}
 		uint8_t *const tile = page + z.h * head_bytes;
-		const int r = r0 + i;
+		const int r = row_of(i0 + i);
 		u32 z4[N], w = 0;
 		_Float16 d = kv_encode<GL, N>(y, z4);
 #pragma unroll
@@ -413,21 +423,20 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 		return;
 
 	/* four words that lie together: channels 64 b + m, + 16, + 32, + 48 */
-	for (int at = threadIdx.x; at < (h1 - h0) * D; at += KV_APPEND_NT) {
-		const int h = at / D, b = at % D / 64, part = at % 64 / 16, c = 64 * b + at % 16;
-		u32 w[4] = {}, mine = 0;
+	u32 mine = 0;
+	for (int j = 0; j < n; j++)
+		mine |= kv_rotr(15, 32 - kv_bit(i0 + j));
+	for (int at = threadIdx.x; at < (h1 - h0) * D / 4; at += KV_APPEND_NT) {
+		const int h = at / (D / 4), b = at % (D / 4) / 16, c = 64 * b + at % 16;
+		u32 w[4] = {};
 #pragma unroll
-		for (int j = 0; j < 8; j++) {
-			const int r = j / 4 * 16 + part * 4 + j % 4 - r0;
-			if (r < 0 || r >= n)
+		for (int j = 0; j < KV_PART; j++) {
+			if (j < i0 || j >= i0 + n)
 				continue;
-			mine |= kv_rotr(15, 32 - kv_bit(j));
 #pragma unroll
 			for (int u = 0; u < 4; u++)
-				w[u] |= kv_rotr(codes[(h * most + r) * D + c + 16 * u], 32 - kv_bit(j));
+				w[u] |= kv_rotr(codes[(h * most + j - i0) * D + c + 16 * u], 32 - kv_bit(j));
 		}
-		if (!mine)
-			continue;
 		u32x4 *to = (u32x4 *)(page + (h0 + h) * head_bytes + L::V_CODES) + L::v_word(part * 4, c) / 4;
 		u32x4 old = {w[0], w[1], w[2], w[3]};
 		if (~mine)
@@ -541,21 +550,23 @@ extern "C" int kv_launch_append(const kv_args *a, int head_len, int type, const 
 				void *q_out, size_t q_out_stride, void *stream)
 {
 	const hip_rope none = {0, HIP_ROPE_PAIRS, NULL, 1.0};
-	const int tiles = kv_tiles_of(a->max_rows), most = a->max_rows < KV_TILE ? a->max_rows : KV_TILE;
-	/* all kv heads a workgroup (32 KB of codes at most) where the tiles alone
-	 * are four a CU; else fewer, down to one */
+	const int tiles = kv_tiles_of(a->max_rows), parts = a->max_rows > 1 ? 4 : 1;
+	/* all kv heads a workgroup (32 KB of codes at most) where the rows alone
+	 * are two workgroups a CU; else fewer, down to one */
+	const int most = parts > 1 ? KV_PART : 1;
 	int per = 1;
-	const int top = 32768 / (KV_TILE * head_len);
-	while (per < top && per < a->kv_heads && (size_t)a->nseq * tiles * a->kv_heads / (2 * per) >= 1024)
+	const int top = 32768 / (KV_PART * head_len);
+	while (per < top && per < a->kv_heads &&
+	       (size_t)a->nseq * tiles * parts * ((a->kv_heads + 2 * per - 1) / (2 * per)) >= 512)
 		per *= 2;
 	per = per < a->kv_heads ? per : a->kv_heads;
-	const size_t grid = (size_t)a->nseq * tiles * ((a->kv_heads + per - 1) / per);
+	const size_t grid = (size_t)a->nseq * tiles * parts * ((a->kv_heads + per - 1) / per);
 	const size_t lds = (size_t)most * ((R ? kv_slot((int)R->rot / 2) * sizeof(double2) : 0) + (size_t)per * head_len);
 	KV_DISPATCH_HEAD(head_len, D, KV_DISPATCH_TYPE(type, TY, {
 		typedef kv_type<TY>::t t;
 		k_kv_append<D, TY><<<dim3((unsigned)grid), KV_APPEND_NT, lds, (hipStream_t)stream>>>(
 			*a, R ? *R : none, (const t *)k, (const t *)v, kv_stride, pos, (const t *)q,
-			q_stride, heads, (t *)q_out, q_out_stride, per, tiles, most);
+			q_stride, heads, (t *)q_out, q_out_stride, per, tiles, parts);
 	}))
 	return (int)hipGetLastError();
 }
