@@ -517,9 +517,9 @@ void k_kv_attn(
 	/* the queries, then the waves' outputs */
 	__shared__ union {
 		kv_query<D, QP, SLOTS> q;
-		float o[NW][KV_ROWS][D + 4];
+		float o[NW][ROWS][D + 4];
 	} sh;
-	__shared__ float s_ref[NW][KV_ROWS], s_sum[NW][KV_ROWS];
+	__shared__ float s_ref[NW][KV_ROWS], s_sum[NW][ROWS], s_high[ROWS];
 	__shared__ int s_row[ROWS], s_head[ROWS];
 
 	const int lane = threadIdx.x % WAVE, part = lane / 16, slot = lane % SLOTS;
@@ -667,12 +667,36 @@ void k_kv_attn(
 		for (int c = 0; c < SLOTS; c++)
 			ref = fmaxf(ref, s_ref[w][lane % 16 - slot + c]);
 	const float factor = weight(soft.ref, ref);
+	const int row = lane % 16 / SLOTS;
+	sum *= factor;
+	float y[4 * CT], z[2 * CT]; /* the row's slots added: each keeps its share of the channels */
+#pragma unroll
+	for (int u = 0; u < 4 * CT; u++)
+		y[u] = o[u / 4][u % 4] * factor;
+	if constexpr (SLOTS == 4) {
+		sum += other<2>(sum);
+		halved<2>(y, lane & 2, z);
+#pragma unroll
+		for (int u = 0; u < 2 * CT; u++)
+			y[u] = z[u];
+	}
+	if constexpr (SLOTS > 1) {
+		float w[8 * CT / SLOTS];
+#pragma unroll
+		for (int u = 0; u < 8 * CT / SLOTS; u++)
+			w[u] = y[u];
+		sum += other<1>(sum);
+		halved<1>(w, lane & 1, y);
+	}
 	if (r.valid) {
 #pragma unroll
-		for (int c = 0; c < CT; c++)
-			*(floatx4 *)&sh.o[wave][lane % 16][16 * c + 4 * part] = o[c] * factor;
-		if (part == 0)
-			s_sum[wave][lane] = sum * factor;
+		for (int u = 0; u < CT / SLOTS; u++)
+			*(floatx4 *)&sh.o[wave][row][16 * (slot * (CT / SLOTS) + u) + 4 * part] =
+				floatx4{y[4 * u], y[4 * u + 1], y[4 * u + 2], y[4 * u + 3]};
+		if (part == 0 && slot == 0) {
+			s_sum[wave][row] = sum;
+			s_high[row] = ref; /* (every wave's the same) */
+		}
 	}
 	__syncthreads();
 	const size_t piece = ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
@@ -681,12 +705,12 @@ void k_kv_attn(
 		const int i = at / (D / 4), c = at % (D / 4) * 4, row = s_row[i];
 		if (row < 0)
 			break; /* the rows behind are not there either */
-		float den = s_sum[0][i * SLOTS];
-		floatx4 y = *(const floatx4 *)&sh.o[0][i * SLOTS][c];
+		float den = s_sum[0][i];
+		floatx4 y = *(const floatx4 *)&sh.o[0][i][c];
 #pragma unroll
-		for (int w = 1; w < NW * SLOTS; w++) {
-			den += s_sum[w / SLOTS][i * SLOTS + w % SLOTS];
-			y += *(const floatx4 *)&sh.o[w / SLOTS][i * SLOTS + w % SLOTS][c];
+		for (int w = 1; w < NW; w++) {
+			den += s_sum[w][i];
+			y += *(const floatx4 *)&sh.o[w][i][c];
 		}
 		if (splits == 1) {
 			kv_vec<TY, 4> z;
@@ -699,11 +723,7 @@ void k_kv_attn(
 		}
 		*(floatx4 *)(to + i * (D + 4) + c) = y;
 		if (c == 0) {
-			float high = s_ref[0][i * SLOTS];
-#pragma unroll
-			for (int w = 1; w < NW * SLOTS; w++)
-				high = fmaxf(high, s_ref[w / SLOTS][i * SLOTS + w % SLOTS]);
-			to[i * (D + 4) + D] = high;
+			to[i * (D + 4) + D] = s_high[i];
 			to[i * (D + 4) + D + 1] = den;
 		}
 	}
@@ -1100,18 +1120,20 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 }
 
 /*
- * Along the cache.  A workgroup of KV_MANY waves (three a SIMD: all that their
- * registers allow) takes a row tile's whole cache while that leaves each wave
- * KV_SHORT tiles or fewer: pieces would need a second launch to add them up
- * (16 sequences x 1100 rows, 32 heads on 8: 9.9 us against 12.0 + 4.1 us; 16 heads
- * x 1024 rows: 8.1 against 5.8 + 4.5).  Longer caches are cut into pieces for
- * workgroups of four waves, as many as the chip holds at once (256 CUs; two or one
- * wave a SIMD by the registers of the head length), and of many sequences into
- * pieces of at most KV_CHUNK tiles, so that different lengths fill the chip evenly.
+ * Along the cache.  A workgroup of KV_MANY waves takes a row tile's whole cache where
+ * that beats pieces, which need a second launch to add them up: up to 32 tiles, 72
+ * where there are 128 workgroups and 128 where there are 512, which fill the chip by
+ * themselves (32 heads on 8 of 128 in fp32: 1 sequence x 1024 rows 10.2 us either way,
+ * x 2048 15.0 whole and 10.0 in pieces; 16 x 2300 rows 15.1 and 15.6; 64 x 2300 rows
+ * 30.7 and 39.8, 64 x 4000 rows 53 and 60).  Other caches are cut into pieces for
+ * workgroups of four waves, as many as the chip holds twice over for heads of 64 and
+ * 128 (131072 rows: 64 pieces a kv head 35.4 us, 128 pieces 36.3), and of many
+ * sequences into pieces of at most KV_CHUNK tiles, so that different lengths fill the
+ * chip evenly (64 sequences of 2000 rows to 16384: pieces of 16 tiles 107 us, 32 tiles
+ * 100, 64 tiles 111, 128 tiles 140).
  */
 #define KV_CHUNK 32
-#define KV_MANY 12
-#define KV_SHORT 6
+#define KV_MANY 8
 
 extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int window, kv_plan *p)
 {
@@ -1135,13 +1157,14 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	}
 	const size_t room = head_len == 64 ? 1024 : head_len == 128 ? 512 : 256;
 	const long by_room = wgs < room ? (long)(room / wgs) : 1;
-	p->waves = head_len < 256 && p->row_tiles == 1 && tiles <= KV_MANY * KV_SHORT ? KV_MANY : KV_WAVES;
+	const long whole = head_len < 256 && p->row_tiles == 1 ? wgs < 128 ? 32 : wgs < 512 ? 72 : 128 : 0;
+	p->waves = tiles <= whole ? KV_MANY : KV_WAVES;
 	long chunk = (tiles + by_room - 1) / by_room;
 	if (wgs >= room / 8 && chunk > KV_CHUNK && p->row_tiles == 1)
 		chunk = KV_CHUNK;
 	if (chunk < (tiles + KV_SPLITS - 1) / KV_SPLITS)
 		chunk = (tiles + KV_SPLITS - 1) / KV_SPLITS;
-	if (p->waves == KV_MANY)
+	if (p->waves > KV_WAVES)
 		chunk = tiles;
 	p->chunk = (int)(chunk < KV_WAVES ? KV_WAVES : chunk);
 	p->splits = (int)((tiles + p->chunk - 1) / p->chunk);
@@ -1152,7 +1175,7 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	long most = p->row_tiles == 1 && by_chunk > by_room ? by_chunk : by_room;
 	most = most < few ? most : few;
 	most = most < KV_SPLITS ? most : KV_SPLITS;
-	if (head_len < 256 && p->row_tiles == 1 && all <= KV_MANY * KV_SHORT)
+	if (all <= whole)
 		most = 1;
 	p->ws = most > 1 ? wgs * most * p->rows * (head_len + 4) * sizeof(float) : 0;
 }
@@ -1180,7 +1203,7 @@ extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const vo
 				*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window, (float *)ws,
 				p->row_tiles, p->chunk, p->rows);
 		};
-		if (p->waves == KV_MANY)
+		if (p->waves > KV_WAVES)
 			launch(p->slots == 4 ? k_kv_attn<D, TY, MANY, FOUR> :
 			       p->slots == 2 ? k_kv_attn<D, TY, MANY, 2> : k_kv_attn<D, TY, MANY, 1>);
 		else
