@@ -854,15 +854,14 @@ template <int D> struct kv_keys32 {
 		for (int u = 0; u < L::G / 2; u++)
 			own[u] = ((const u32 *)(tile + L::K_SCALES))[r * L::G / 2 + u];
 	}
-	/* the row's scales, and again with a 64th of them: the operand that
-	 * kv_attn_wide's surplus is multiplied with */
+	/* the row's scales, twice: the operand that k_kv_attn_wide's surplus is
+	 * multiplied with */
 	__device__ inline half8_t scales8() const
 	{
 		u32 w[4] = {};
 #pragma unroll
 		for (int u = 0; u < L::G / 2; u++) {
-			w[u] = own[u];
-			w[2 + u] = __builtin_bit_cast(u32, __builtin_bit_cast(half2_t, own[u]) * (half2_t)(_Float16)0.015625f);
+			w[u] = w[2 + u] = own[u];
 		}
 		return as_half8(w[0], w[1], w[2], w[3]);
 	}
@@ -946,11 +945,11 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 					if (u % KV_WAVES == wave)
 						sh.q[p][u][h][lane] = z[p];
 			}
-			/* in two f16 parts, of 11 bits and of the rest times 64 */
+			/* in two f16 parts (of at most 1 and 2^-12) */
 			sum = -8.0f * kv_form<TY>::STEP * half_sum(sum);
 			if (!kv_form<TY>::EVEN && part == 0) {
 				surplus[u] = (_Float16)sum;
-				surplus[4 + u] = (_Float16)(64.0f * (sum - (float)surplus[u]));
+				surplus[4 + u] = rest(sum, surplus[u]);
 			}
 		}
 	}

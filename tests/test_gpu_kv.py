@@ -410,6 +410,38 @@ def test_attention_of_many_rows(dev, ty, D, KH, H, rows, lens, page, window):
     check_attention(dev, c, H, ty, window, rng, qscale=2.0, pad=8, check=check)
 
 
+@pytest.mark.parametrize("window", (0, 45))
+@pytest.mark.parametrize("ty,D,KH,G,rows,lens", tuple(
+    # one to eight query rows of a kv head, in columns of two and of four or alone
+    (ty, D, 2, G, rows, lens)
+    for ty, D in ((F32, 128), (F16, 256), (BF16, 64), (BF16, 128), (F32, 256), (F16, 64))
+    for G, rows, lens in ((1, [1] * 3, [1, 33, 300]), (2, [2, 1], [70, 31]), (3, [1], [95]), (4, [1] * 2, [640, 32]),
+                          (5, [1], [200]), (1, [4, 3, 1], [4, 100, 67]), (2, [3, 2], [129, 2]), (8, [1], [257]),
+                          (7, [1], [64]), (1, [9, 5, 0], [40, 77, 0]))) + (
+    # longer than a workgroup's whole cache, in pieces
+    (F32, 128, 1, 4, [1], [1100]), (BF16, 128, 2, 1, [3], [2500]), (F16, 64, 1, 8, [1], [1300]),
+    (F32, 256, 1, 3, [1], [700]), (BF16, 256, 1, 6, [1], [700])))
+def test_attention_of_few_rows(dev, ty, D, KH, G, rows, lens, window):
+    rng = np.random.default_rng(sum(lens) + G)
+    c = Case(dev, rng, rows, lens, 32, KH, D)
+    check_attention(dev, c, KH * G, ty, window, rng, qscale=2.0, pad=8)
+    assert c.errors() == 0
+
+
+@pytest.mark.parametrize("ty", (F16, BF16))
+@pytest.mark.parametrize("many", (False, True))
+@pytest.mark.parametrize("size,qscale", ((1e-5, 1.0), (1e-3, 30.0), (40.0, 1e-3), (1.0, 1.0)))
+def test_attention_sizes_in_16_bits(dev, ty, many, size, qscale):
+    """Scales down to f16's subnormals, for few rows and in tiles of 32."""
+    rng = np.random.default_rng(14)
+    rows, lens, KH, H = ([270] * 4, [270, 300, 333, 400], 16, 32) if many else ([2, 1], [200, 90], 2, 4)
+    c = Case(dev, rng, rows, lens, 32, KH, 128)
+    half = c.pool.bytes[..., 34 * 128 - 256:].view(np.float16)
+    half[..., :128] = half[..., :128] / np.float16(0.25) * np.float16(size)
+    check_attention(dev, c_upload(c), H, ty, 0, rng, qscale=qscale,
+                    check=sorted({0, 1, 100, 269, 270, 700, c.T - 1} & set(range(c.T))) if many else None)
+
+
 @pytest.mark.parametrize("qscale,scale", ((1e-20, 1.0), (1e-38, 1.0), (30.0, None), (1e6, 1e-7), (1.0, 0.0),
                                           (1.0, -0.1)))
 def test_attention_sizes_of_queries(dev, qscale, scale):
