@@ -17,16 +17,19 @@
  *
  * Exactness.  Codes are small integers, exact in f16, and stay unscaled in the
  * operands: a key group's scale multiplies its partial scores in fp32, a value
- * row's scale its probability.  A code enters as a subnormal, its bits
- * where they lie and nothing around them (a mask for two).  The keys'
- * surplus of 8 a channel leaves through the accumulator's start (-8 sum of the
- * query's channels), the values' by a subtraction, exact as well, since over many
- * cached rows a surplus would outweigh the sum.  A query row is scaled by a power of two (its largest value into [2^13, 2^14))
- * and, from fp32, split into two f16 parts of together 22 bits; f16 and bf16
- * queries are exact in one.  The probability times the value scale is scaled
- * by a power of two that keeps the largest below 2^15, and split in two as
- * well (in one part, 11 bits, for bf16 outputs of 8).  Sums, maxima and
- * exponents are fp32.
+ * row's scale its probability.  How a code becomes f16 is at kv_word below.  The keys'
+ * surplus of 8 a channel leaves through the accumulator's start (-8 sum of the query's
+ * channels) or through a product of its own, the values' by a subtraction, exact as
+ * well, since over many cached rows a surplus would outweigh the sum.  A query row is
+ * scaled by a power of two and, from fp32, split into two f16 parts of together 22
+ * bits; f16 and bf16 queries are exact in one.  The probability times the value scale
+ * is scaled by a power of two that keeps it within f16, and split in two as well (in
+ * one part, 11 bits, for bf16 outputs of 8).  Sums, maxima and exponents are fp32.
+ *
+ * Three forms, chosen by kv_attn_plan: few rows in slots of columns and up to 16 rows
+ * (k_kv_attn; HBM bounds long caches, latency short ones), and tiles of 32 rows for
+ * prompts (k_kv_attn_wide; VALU: making f16 of codes, scales and exponentials take
+ * three times the matrix instructions' cycles).
  */
 #include "kv_device.h"
 
@@ -498,7 +501,13 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
  * own scales, add up and keep 8 / SLOTS of the cached rows each (scale products and
  * exponentials a row: 8 and 2 instead of 32 and 8 for four slots).  In the second
  * product a slot has its cached rows and zeros for the others; its statistics and
- * output are its own, like another wave's.
+ * output are its own, like another wave's, until the end.
+ *
+ * 131072 rows, 32 bf16 heads on 8 of 128 (145 MB): 31.8 us and the merge 4.2, 4.1 TB/s
+ * in all; without slots 34.9.  64 sequences of 2000 to 16384 rows in fp32 (341 MB):
+ * 96 and 6.1, 3.5 TB/s; without slots, at three waves a SIMD, 112: pieces of 1024 rows
+ * have 8 tiles a wave between their first loads and their sums, and lengths are uneven
+ * (64 of 8190 rows: 126 us, 4.6 TB/s).
  */
 /* by the registers: four waves a SIMD with slots, three without, two for heads of
  * 256.  Nothing is kept in accumulation registers and moved. */
@@ -732,7 +741,7 @@ void k_kv_attn(
 /*
  * The pieces' results of one query row: first their weights, then D / 4 threads
  * take the row's channels, KV_NT / (D / 4) times over, each its share of the
- * pieces.
+ * pieces.  Two dependent reads: 4.2 us for 64 pieces of 32 rows.
  */
 template <int D, int TY>
 __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename kv_type<TY>::t *out,
@@ -823,6 +832,13 @@ __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename k
  * A workgroup's four waves share 32 query rows and deal the cache's tiles among
  * them, and the row tiles that see most come first: even the last workgroups are
  * short.
+ *
+ * 8192 bf16 rows of 32 heads on 8 of 128: 900 to 920 us, 600 TFLOP/s of the formula's
+ * operations (in tiles of 16 rows 1.5 ms); about 400 VALU and 19 matrix instructions of 32
+ * cycles for 32 x 32 scores.  2048 fp32 rows of 16 heads on as many cached: 54 us (in
+ * two parts, 620 TFLOP/s).  Waves with 32 rows each that share a tile's f16 codes
+ * through LDS took 8 to 12 % longer: the barrier a tile keeps matrix and VALU work of
+ * the two waves of a SIMD from overlapping.
  */
 #define KV_WIDE 32
 
@@ -1145,9 +1161,15 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	const long rows = (long)a->max_rows * G;
 	p->row_tiles = (int)((rows + KV_ROWS - 1) / KV_ROWS);
 	p->rows = (int)(rows < KV_ROWS ? rows : KV_ROWS);
+	/* slots: 64 sequences x 4000 rows, 32 fp32 heads on 8: 52.8 us with four, 61.4 with
+	 * two, 66.3 without; 64 heads on 8 in 16 bits: 46.0 with two, 56.8 without */
 	p->slots = rows <= 4 && head_len > 64 ? 4 : rows <= 8 ? 2 : 1;
 	const size_t wgs = (size_t)a->nseq * a->kv_heads * p->row_tiles;
-	p->wide = head_len < 256 && rows >= 2 * KV_WIDE && wgs >= 512;
+	/* tiles of 32 rows (heads of 256 have no registers for them) where they fill the
+	 * chip: 8 x 64 rows on 2048, 32 heads on 8: 35.5 us, in tiles of 16 41.8; 512
+	 * workgroups only on longer caches: 512 rows of 16 heads alone 13.2 and 12.3, 4 x 64
+	 * rows of 32 heads of 64 on 4096 44.2 and 49.5 */
+	p->wide = head_len < 256 && rows >= 2 * KV_WIDE && (wgs >= 1024 || (wgs >= 512 && all >= 32));
 	if (p->wide) {
 		p->row_tiles = (int)((rows + KV_WIDE - 1) / KV_WIDE);
 		p->splits = 1;
@@ -1165,12 +1187,15 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 		chunk = (tiles + KV_SPLITS - 1) / KV_SPLITS;
 	if (p->waves > KV_WAVES)
 		chunk = tiles;
-	p->chunk = (int)(chunk < KV_WAVES ? KV_WAVES : chunk);
+	/* many rows cost the merge more than short pieces save: 256 rows of 16 heads alone
+	 * 16.8 us in two pieces of 4 tiles, 8.0 in one of 8 */
+	const long least = p->row_tiles > 4 ? 2 * KV_WAVES : KV_WAVES;
+	p->chunk = (int)(chunk < least ? least : chunk);
 	p->splits = (int)((tiles + p->chunk - 1) / p->chunk);
 	p->splits = p->splits < 1 ? 1 : p->splits;
 	/* without regard to the window, so that one workspace serves any: pieces by
 	 * room, or of KV_CHUNK tiles, and none below KV_WAVES */
-	const long by_chunk = (all + KV_CHUNK - 1) / KV_CHUNK, few = (all + KV_WAVES - 1) / KV_WAVES;
+	const long by_chunk = (all + KV_CHUNK - 1) / KV_CHUNK, few = (all + least - 1) / least;
 	long most = p->row_tiles == 1 && by_chunk > by_room ? by_chunk : by_room;
 	most = most < few ? most : few;
 	most = most < KV_SPLITS ? most : KV_SPLITS;
