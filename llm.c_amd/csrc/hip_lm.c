@@ -113,6 +113,7 @@ static void lm_err(const char *fmt, ...)
 		hipError_t e_ = (call);                                           \
 		if (e_ != hipSuccess) {                                           \
 			lm_err("%s: %s", what, hipGetErrorString(e_));             \
+			(void)hipGetLastError(); /* the launches check it */      \
 			goto fail;                                                \
 		}                                                                 \
 	} while (0)

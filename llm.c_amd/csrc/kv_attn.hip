@@ -504,7 +504,7 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
  * output are its own, like another wave's, until the end.
  *
  * 131072 rows, 32 bf16 heads on 8 of 128 (145 MB): 31.8 us and the merge 4.2, 4.1 TB/s
- * in all; without slots 34.9.  64 sequences of 2000 to 16384 rows in fp32 (341 MB):
+ * in all; without slots 34.9.  64 sequences of 340 to 16384 rows in fp32 (341 MB):
  * 96 and 6.1, 3.5 TB/s; without slots, at three waves a SIMD, 112: pieces of 1024 rows
  * have 8 tiles a wave between their first loads and their sums, and lengths are uneven
  * (64 of 8190 rows: 126 us, 4.6 TB/s).

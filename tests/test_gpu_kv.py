@@ -609,6 +609,62 @@ def test_output_may_be_the_queries(dev):
         assert np.array_equal(dev.get(d_q, q.shape, np.float32), dev.get(d_o, q.shape, np.float32))
 
 
+@pytest.mark.parametrize("ty,H,KH,D,rows,lens", (
+    (F32, 3, 1, 128, [1], [90]), (BF16, 8, 1, 64, [1, 1], [70, 64]),          # slots
+    (F16, 4, 4, 256, [9], [300]), (F32, 16, 16, 128, [300] * 2, [300, 1100]),  # tiles of 16
+    (BF16, 32, 16, 128, [270] * 4, [270, 1100, 300, 290]),                    # of 32
+    (F32, 32, 32, 64, [200] * 3, [1030, 200, 450])))
+def test_every_form_in_place_and_without_a_page(dev, ty, H, KH, D, rows, lens):
+    """Outputs over the queries are those beside them, and a page outside the pool is
+    left out of the sum and reported, whatever takes the call."""
+    rng = np.random.default_rng(sum(lens) + D)
+    c = Case(dev, rng, rows, lens, 32, KH, D)
+    q = rng.standard_normal((c.T, H, D)).astype(np.float32)
+    shape, np_ty = q.shape, ref.np_dtype(ty)
+    ws = hipkv.attn_ws(c.cache, c.batch, H)
+    d_ws = dev.h.malloc(max(ws, 16))
+    dev.p.append(d_ws)
+
+    def run(table, in_place):
+        d_q = dev.up(ref.to_type(q, ty))
+        d_o = d_q if in_place else dev.up(np.zeros(shape, np_ty))
+        b = hipkv.Batch(len(rows), c.T, max(rows), max(lens), c.d_start, c.d_len, dev.up(table),
+                        table.shape[1])
+        hipkv.attn(c.cache, b, ty, d_q, H * D, H, d_o, H * D, D ** -0.5, 0, d_ws, ws)
+        return dev.get(d_o, shape, np_ty)
+
+    want = run(c.table, False)
+    assert np.array_equal(run(c.table, True), want) and c.errors() == 0
+    for bad in (-1, c.pages, 1 << 30):
+        table = c.table.copy()
+        table[0, 1] = bad  # rows 32 .. 63 of the first sequence
+        got = ref.from_type(run(table, False), ty)
+        assert c.errors() == hipkv.ERR_PAGE
+        dev.h.copy_in(c.d_err, np.zeros(1, np.uint32))
+        n = rows[0]
+        assert np.array_equal(got[n:], ref.from_type(want, ty)[n:])
+        kk, vv = (np.stack(x) for x in zip(*[c.pool.load(c.table[0], p) for p in range(lens[0])]))
+        x = ref.from_type(ref.to_type(q, ty), ty)
+        for i in sorted({0, n // 2, n - 1}):
+            p = lens[0] - n + i
+            keep = [j for j in range(p + 1) if not 32 <= j < 64]
+            w = ref.attend(x[i], kk[keep], vv[keep], len(keep) - 1, D ** -0.5, 0)[0]
+            assert np.linalg.norm(got[i] - w) <= max(1e-5, 2 * ref.HALF_STEP[ty]) * np.linalg.norm(w), i
+
+
+@pytest.mark.parametrize("ty,D", ((F32, 128), (BF16, 128), (F16, 64), (BF16, 64)))
+@pytest.mark.parametrize("rows", (64, 65, 95, 97))
+def test_rows_beside_the_tiles_of_32(dev, ty, D, rows):
+    """Rows that end beside a tile's end, lengths beside the cache's tiles, one row
+    and none in the same call."""
+    rng = np.random.default_rng(rows + D)
+    all_rows = [rows, 1, rows, 0, rows, 2, rows, rows]
+    c = Case(dev, rng, all_rows, [1024, 1, rows, 0, rows + 31, 33, rows + 32, rows + 1], 32, 32, D)
+    at = c.start[[0, 2, 4, 6, 7]]
+    check = sorted({int(i) for k in (0, 31, 32, 63, rows - 1) for i in at + k} | {rows, int(c.start[5])})
+    check_attention(dev, c, 32, ty, 0, rng, qscale=2.0, check=check)
+
+
 # --------------------------------------------------------------------------
 # the operators together, as a decode loop runs them
 # --------------------------------------------------------------------------

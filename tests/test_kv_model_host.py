@@ -48,3 +48,31 @@ def test_steps_prompts_and_the_context(context):
     B.free()
     M.free()
     """)
+
+
+def test_allocations_that_fail():
+    """Each allocation of a new batch and of its first prompts in turn: refused with
+    a message, and the next try has what it needs."""
+    on_fake(f"""
+    M = hiplm.LmModel({TINY}, 640)
+    ids = np.tile(np.arange(9, dtype=np.int32), (3, 1))
+    def run():
+        B = hiplm.LmBatch(M, 3, kv4=True)
+        B.generate(ids, 2)
+        B.free()
+    hiplm.LmBatch(M, 2).free()
+    F.fake_sizes()
+    run()
+    sizes = sorted({{int(n) for n in F.fake_sizes().split()}})
+    assert len(sizes) > 8, sizes
+    failed = 0
+    for n in sizes:
+        F.fake_fail_size(n)
+        try:
+            run()
+        except hipmoe.HipMoeError as e:
+            failed += 1
+        F.fake_fail_size(0)
+        run()
+    assert failed > 6, (failed, sizes)
+    """)
