@@ -149,7 +149,8 @@ typedef struct hip_kv_batch {
  * the codes are made of), by pos[row] (device) or, with pos NULL, by its
  * cache position.  With q (NULL: none), q_out = q rotated, rows of `heads`
  * heads; in place where q_out == q and the strides are equal.  Without R, q
- * must be NULL.  Two sequences of one call must not store into one page.
+ * must be NULL.  A call must not store into one page from two sequences, or from two
+ * places of one.
  * Rows that are not the call's keep their bytes.  k, v, q and q_out are
  * 16-byte aligned, the strides multiples of 16 bytes.
  */

@@ -69,7 +69,9 @@ def test_steps(arch, window, seeds, made):
 @pytest.mark.parametrize("arch,window,S,n,C", (
     ("olmoe", 0, 2, 100, 128), ("olmoe", 0, 1, 2, 70), ("mixtral", 0, 2, 33, 64),
     ("mixtral", 50, 3, 129, 200), ("mixtral", 0, 4, 512, 520),
-    ("olmoe", 0, 3, 1000, 1024), ("mixtral", 200, 3, 1000, 1001)))
+    ("olmoe", 0, 3, 1000, 1024), ("mixtral", 200, 3, 1000, 1001),
+    ("olmoe", 0, 1, 2200, 2210),    # steps in pieces
+    ("mixtral", 0, 130, 20, 40)))   # prompts in two groups
 def test_prompts(arch, window, S, n, C, made):
     """generate's prompts (a launch for up to 2048 rows) and the step after them."""
     md = small(arch, 1, window)
@@ -151,3 +153,24 @@ def test_a_full_cache_is_refused(made):
     for i in range(1, 40):
         again = B.decode(ids[:, i])[1]
     assert np.array_equal(again, lg)
+
+
+def test_replayed_steps_over_long_caches(made):
+    """Captured steps across the row counts at which the attention cuts a cache into
+    pieces, against decoded ones, and two batches' graphs in turn."""
+    md = small("olmoe", 1)
+    M = made(hiplm.LmModel(md, 1100))
+    A, B = made(hiplm.LmBatch(M, 2, kv4=True)), made(hiplm.LmBatch(M, 2, kv4=True))
+    ids = prompts_of(md, (1, 2), 1000)
+    steps = A.generate(ids, 0)[0][:, 0]
+    want = [steps]
+    for _ in range(60):
+        want.append(A.decode(want[-1])[0])
+    want = np.stack(want, 1)
+    A.reset()
+    for _ in range(2):
+        for X in (A, B):
+            assert np.array_equal(X.generate(ids, 30)[0], want[:, :31])
+        for X in (B, A):
+            assert np.array_equal(X.generate(want[:, 30:31], 29)[0], want[:, 31:])
+            X.reset()
