@@ -177,8 +177,10 @@ int hip_kv_read_dev(const hip_kv_cache *C, const hip_kv_batch *B, int type, void
  * that are multiples of 16 bytes; out == q with equal strides is allowed.
  * Rows outside the batch keep what out holds.  A row on a page outside the
  * pool is left out of the sum; where that leaves nothing the output is NaN.
- * ws: hip_kv_attn_ws bytes, 16-byte aligned, not used by another call at the
- * same time (NULL if 0 bytes); graphs that may run at once need one each.
+ * ws: hip_kv_attn_ws bytes (of the same cache, bounds and heads, whatever the
+ * window), 16-byte aligned, not used by another call at the same time (NULL if 0
+ * bytes); graphs that may run at once need one each.  Where the heads of a kv head
+ * times max_rows are 16 at most, a workspace serves every smaller max_len too.
  */
 size_t hip_kv_attn_ws(const hip_kv_cache *C, const hip_kv_batch *B, size_t heads);
 int hip_kv_attn_dev(const hip_kv_cache *C, const hip_kv_batch *B, int type, const void *q,

@@ -487,6 +487,52 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
 }
 
 /*
+ * The caches of a call with one row tile a sequence as one line of tiles, sequence
+ * after sequence, cut into equal shares: of this workgroup's sequences (a thread
+ * each, KV_SEQS at most) where they start in it, and the whole line's length.  A
+ * sequence with rows has a tile at least.
+ */
+#define KV_SEQS KV_NT
+
+struct kv_line {
+	int start, tiles; /* of sequence threadIdx.x */
+	int all;
+};
+
+__device__ static inline kv_line kv_line_of(const kv_args &a, int window)
+{
+	__shared__ int s_wave[KV_WAVES];
+	const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+	int tiles = 0;
+	if ((int)threadIdx.x < a.nseq) {
+		const kv_seq sq = kv_sequence(a, threadIdx.x, true);
+		const int first = window ? max(0, sq.len - sq.n + 1 - window) : 0;
+		tiles = sq.n ? max(1, (max(sq.len, 0) + KV_TILE - 1) / KV_TILE - first / KV_TILE) : 0;
+	}
+	int end = tiles;
+	for (int o = 1; o < WAVE; o <<= 1) {
+		const int before = __shfl_up(end, o, WAVE);
+		end += lane >= o ? before : 0;
+	}
+	if (lane == WAVE - 1)
+		s_wave[wave] = end;
+	__syncthreads();
+	kv_line r = {end - tiles, tiles, 0};
+#pragma unroll
+	for (int w = 0; w < KV_WAVES; w++) {
+		r.start += w < wave ? s_wave[w] : 0;
+		r.all += s_wave[w];
+	}
+	return r;
+}
+
+/* tiles of each of n shares */
+__device__ static inline int kv_share(int all, int n)
+{
+	return max((all + n - 1) / n, KV_WAVES);
+}
+
+/*
  * Few query rows: one workgroup takes a tile of them over `chunk` tiles of the
  * cache, dealt to its waves one by one; the waves' results meet in LDS.
  * With more than one workgroup along the cache each leaves its reference, sum
@@ -503,15 +549,17 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
  * product a slot has its cached rows and zeros for the others; its statistics and
  * output are its own, like another wave's, until the end.
  *
+ * SHARE: instead of a piece of one cache the workgroup has an equal share of all of
+ * them, one after the other, and takes the sequences in it in turn.
+ *
  * 131072 rows, 32 bf16 heads on 8 of 128 (145 MB): 31.8 us and the merge 4.2, 4.1 TB/s
  * in all; without slots 34.9.  64 sequences of 340 to 16384 rows in fp32 (341 MB):
- * 96 and 6.1, 3.5 TB/s; without slots, at three waves a SIMD, 112: pieces of 1024 rows
- * have 8 tiles a wave between their first loads and their sums, and lengths are uneven
- * (64 of 8190 rows: 126 us, 4.6 TB/s).
+ * 87 us with the merge, 3.9 TB/s; in pieces 97.5, without slots and at three waves a
+ * SIMD 118.  64 of 8190 rows: 125 us, 4.6 TB/s.
  */
 /* by the registers: four waves a SIMD with slots, three without, two for heads of
  * 256.  Nothing is kept in accumulation registers and moved. */
-template <int D, int TY, int NW, int SLOTS>
+template <int D, int TY, int NW, int SLOTS, bool SHARE>
 __global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(D == 256 ? 2 : SLOTS > 1 && NW == KV_WAVES ? 4 : 3)))
 void k_kv_attn(
 	kv_args a, const typename kv_type<TY>::t *q, size_t q_stride, int G,
@@ -529,30 +577,63 @@ void k_kv_attn(
 		float o[NW][ROWS][D + 4];
 	} sh;
 	__shared__ float s_ref[NW][KV_ROWS], s_sum[NW][ROWS], s_high[ROWS];
-	__shared__ int s_row[ROWS], s_head[ROWS];
+	__shared__ int s_row[ROWS], s_head[ROWS], s_seq[2];
+	__shared__ int2 s_line[SHARE ? KV_SEQS : 1]; /* a sequence's start and tiles in the line */
 
-	const int lane = threadIdx.x % WAVE, part = lane / 16, slot = lane % SLOTS;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
 	const int kv_head = blockIdx.x % a.kv_heads, rt = blockIdx.x / a.kv_heads;
-	const int split = blockIdx.y, splits = gridDim.y, s = blockIdx.z;
+	const int split = blockIdx.y, splits = gridDim.y, shift = a.page_shift - 5;
+	int at = 0, end = 1; /* of the workgroup's share of the line */
+	if constexpr (SHARE) {
+		const kv_line line = kv_line_of(a, window);
+		s_line[threadIdx.x] = make_int2(line.start, line.tiles);
+		const int share = kv_share(line.all, splits);
+		at = split * share;
+		end = min(at + share, line.all);
+	}
+	while (at < end) {
+	int lane = threadIdx.x % WAVE;
+	if constexpr (SHARE) { /* nothing of the lane's is kept in registers from turn to turn */
+		asm volatile("" : "+v"(lane));
+		__builtin_assume(lane >= 0 && lane < WAVE);
+	}
+	const int part = lane / 16, slot = lane % SLOTS;
+	int s = blockIdx.z, t0 = 0, t1 = 0, page = -1;
+	if constexpr (SHARE) {
+		const int2 line = s_line[threadIdx.x];
+		if (line.x <= at && at < line.x + line.y) {
+			s_seq[0] = threadIdx.x;
+			s_seq[1] = line.x;
+		}
+		__syncthreads();
+		s = __builtin_amdgcn_readfirstlane(s_seq[0]);
+		t0 = at - __builtin_amdgcn_readfirstlane(s_seq[1]);
+	}
 	/* the wave's tiles t0 + wave, + NW, ..; a lane holds the page of one of the
 	 * next 64.  Without a window the first lot needs no length, only the table's
 	 * bound, and is on its way before the length is known */
-	const int shift = a.page_shift - 5;
 	const int32_t *table = a.table + s * a.table_stride;
-	int page = -1;
-	if (!window) {
+	if (!window && !SHARE) {
 		const int at = (split * chunk + wave + lane * NW) >> shift;
 		page = at < a.table_stride ? table[at] : -1;
 	}
 	const kv_seq sq = kv_sequence(a, s);
-	if (rt * ROWS >= sq.n * G)
+	if (!SHARE && rt * ROWS >= sq.n * G)
 		return;
 	const kv_span r = kv_rows_of<ROWS, SLOTS>(sq, rt, G, kv_head, window, lane);
-	const int t0 = r.first / KV_TILE + split * chunk;
-	const int t1 = min(t0 + chunk, (max(r.last, 0) + KV_TILE - 1) / KV_TILE);
-	if (split > 0 && t0 >= t1)
-		return;
+	t1 = (max(r.last, 0) + KV_TILE - 1) / KV_TILE;
+	if constexpr (SHARE) {
+		const int from = at;
+		t0 += r.first / KV_TILE;
+		at += max(1, min(end - at, t1 - t0));
+		t1 = min(t1, t0 + at - from);
+	} else {
+		t0 = r.first / KV_TILE + split * chunk;
+		t1 = min(t0 + chunk, t1);
+		at = end;
+		if (split > 0 && t0 >= t1)
+			return;
+	}
 	kv_vec<TY, 8> qv[L::G];
 #pragma unroll
 	for (int g = 0; g < L::G; g++)
@@ -563,7 +644,7 @@ void k_kv_attn(
 	bool lost = false;
 	const auto tile_of = [&](int i) -> const uint8_t * {
 		const int t = t0 + wave + i * NW;
-		if (i % WAVE == 0 && (i || window)) {
+		if (i % WAVE == 0 && (i || window || SHARE)) {
 			const int tl = t + lane * NW;
 			page = tl < t1 ? table[tl >> shift] : -1;
 		}
@@ -708,7 +789,8 @@ void k_kv_attn(
 		}
 	}
 	__syncthreads();
-	const size_t piece = ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
+	const size_t piece = SHARE ? (size_t)kv_head * (splits + a.nseq) + split + s
+				   : ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
 	float *to = ws + piece * nrows * (D + 4);
 	for (int at = threadIdx.x; at < ROWS * D / 4; at += NW * WAVE) {
 		const int i = at / (D / 4), c = at % (D / 4) * 4, row = s_row[i];
@@ -721,7 +803,7 @@ void k_kv_attn(
 			den += s_sum[w][i];
 			y += *(const floatx4 *)&sh.o[w][i][c];
 		}
-		if (splits == 1) {
+		if (!SHARE && splits == 1) {
 			kv_vec<TY, 4> z;
 			const int head = s_head[i];
 #pragma unroll
@@ -736,6 +818,9 @@ void k_kv_attn(
 			to[i * (D + 4) + D + 1] = den;
 		}
 	}
+	if constexpr (SHARE)
+		__syncthreads();
+	}
 }
 
 /*
@@ -746,23 +831,34 @@ void k_kv_attn(
 template <int D, int TY>
 __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename kv_type<TY>::t *out,
 						     size_t out_stride, int window, const float *ws,
-						     int row_tiles, int chunk, int splits, int nrows)
+						     int row_tiles, int chunk, int splits, int nrows, int shares)
 {
 	typedef kv_type<TY> T;
 	constexpr int CH = D / 4, PARTS = KV_NT / CH;
 	__shared__ floatx4 s_y[PARTS][CH];
 	__shared__ float s_w[KV_SPLITS], s_ref[KV_WAVES], s_sum[KV_WAVES];
 	const int kv_head = blockIdx.x % a.kv_heads, mine = blockIdx.x / a.kv_heads, s = blockIdx.y;
+	__shared__ int s_from[2];
 	const kv_seq sq = kv_sequence(a, s);
 	if (mine >= sq.n * G)
 		return;
+	if (shares) { /* the first share that the sequence is in, and their count */
+		const kv_line line = kv_line_of(a, window);
+		const int share = kv_share(line.all, shares);
+		if ((int)threadIdx.x == s) {
+			s_from[0] = line.start / share;
+			s_from[1] = (line.start + line.tiles - 1) / share + 1 - s_from[0];
+		}
+		__syncthreads();
+	}
 	const int rt = mine / KV_ROWS, i = mine / G, base = sq.len - sq.n;
 	const int i0 = rt * KV_ROWS / G, i1 = (min(rt * KV_ROWS + KV_ROWS, sq.n * G) - 1) / G;
 	const int first = window ? max(0, base + i0 + 1 - window) : 0, last = max(base + i1 + 1, 0);
 	const int tiles = (last + KV_TILE - 1) / KV_TILE - first / KV_TILE;
-	const int n = min(splits, max(1, (tiles + chunk - 1) / chunk));
-	const float *p = ws + (((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits) * nrows * (D + 4) +
-			 mine % KV_ROWS * (D + 4);
+	const int n = shares ? s_from[1] : min(splits, max(1, (tiles + chunk - 1) / chunk));
+	const size_t piece = shares ? (size_t)kv_head * (shares + a.nseq) + s_from[0] + s
+				    : ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits;
+	const float *p = ws + piece * nrows * (D + 4) + mine % KV_ROWS * (D + 4);
 	const int c = threadIdx.x % CH, part = threadIdx.x / CH;
 	const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
 	const size_t step = nrows * (D + 4);
@@ -1142,10 +1238,17 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
  * x 2048 15.0 whole and 10.0 in pieces; 16 x 2300 rows 15.1 and 15.6; 64 x 2300 rows
  * 30.7 and 39.8, 64 x 4000 rows 53 and 60).  Other caches are cut into pieces for
  * workgroups of four waves, as many as the chip holds twice over for heads of 64 and
- * 128 (131072 rows: 64 pieces a kv head 35.4 us, 128 pieces 36.3), and of many
+ * 128 (131072 rows: 64 pieces a kv head 35.4 us, 128 pieces 36.3), and of several
  * sequences into pieces of at most KV_CHUNK tiles, so that different lengths fill the
- * chip evenly (64 sequences of 2000 rows to 16384: pieces of 16 tiles 107 us, 32 tiles
+ * chip evenly (64 sequences of 340 to 16384 rows: pieces of 16 tiles 107 us, 32 tiles
  * 100, 64 tiles 111, 128 tiles 140).
+ *
+ * Of many sequences, where the longest that may come would be 4096 pieces in all and
+ * more, most of which find nothing to do (launching one costs its XCD 90 cycles), the
+ * caches are one line in equal shares, as many as the chip holds: the same 64 87 us
+ * instead of 97.5, 64 of 8190 rows 125 instead of 133.  Finding a share's sequences
+ * costs 2 us a launch: 16 sequences on 8 kv heads 30.3 instead of 29.1 us, one of 131072
+ * rows 39.5 instead of 35.4.
  */
 #define KV_CHUNK 32
 #define KV_MANY 8
@@ -1165,6 +1268,7 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	 * two, 66.3 without; 64 heads on 8 in 16 bits: 46.0 with two, 56.8 without */
 	p->slots = rows <= 4 && head_len > 64 ? 4 : rows <= 8 ? 2 : 1;
 	const size_t wgs = (size_t)a->nseq * a->kv_heads * p->row_tiles;
+	p->shares = 0;
 	/* tiles of 32 rows (heads of 256 have no registers for them) where they fill the
 	 * chip: 8 x 64 rows on 2048, 32 heads on 8: 35.5 us, in tiles of 16 41.8; 512
 	 * workgroups only on longer caches: 512 rows of 16 heads alone 13.2 and 12.3, 4 x 64
@@ -1180,6 +1284,17 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	const long by_room = wgs < room ? (long)(room / wgs) : 1;
 	const long whole = head_len < 256 && p->row_tiles == 1 ? wgs < 128 ? 32 : wgs < 512 ? 72 : 128 : 0;
 	p->waves = tiles <= whole ? KV_MANY : KV_WAVES;
+	const size_t pieces = (size_t)a->nseq * a->kv_heads * ((all + KV_CHUNK - 1) / KV_CHUNK);
+	if (p->row_tiles == 1 && all > whole && a->nseq <= KV_SEQS && wgs >= 512 && pieces >= 4096) {
+		const int chip = head_len == 256 ? 512 : 1024, shares = a->kv_heads < chip ? chip / a->kv_heads : 1;
+		/* (never less than shorter bounds need) */
+		const size_t slots = (size_t)a->kv_heads * (shares + a->nseq);
+		p->ws = (slots > 4096 ? slots : 4096) * p->rows * (head_len + 4) * sizeof(float);
+		p->shares = tiles > whole ? shares : 0;
+		p->splits = p->shares ? shares : 1;
+		p->chunk = (int)tiles;
+		return;
+	}
 	long chunk = (tiles + by_room - 1) / by_room;
 	if (wgs >= room / 8 && chunk > KV_CHUNK && p->row_tiles == 1)
 		chunk = KV_CHUNK;
@@ -1223,20 +1338,23 @@ extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const vo
 		/* (heads of 256 have no room for KV_MANY waves, of 64 no four groups) */
 		constexpr int MANY = D < 256 ? KV_MANY : KV_WAVES, FOUR = D > 64 ? 4 : 2;
 		const auto launch = [&](auto kernel) {
-			kernel<<<grid, p->waves * WAVE, 0, (hipStream_t)stream>>>(
+			kernel<<<dim3(grid.x, grid.y, p->shares ? 1 : grid.z), p->waves * WAVE, 0, (hipStream_t)stream>>>(
 				*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window, (float *)ws,
 				p->row_tiles, p->chunk, p->rows);
 		};
-		if (p->waves > KV_WAVES)
-			launch(p->slots == 4 ? k_kv_attn<D, TY, MANY, FOUR> :
-			       p->slots == 2 ? k_kv_attn<D, TY, MANY, 2> : k_kv_attn<D, TY, MANY, 1>);
+		if (p->shares)
+			launch(p->slots == 4 ? k_kv_attn<D, TY, KV_WAVES, FOUR, true> :
+			       p->slots == 2 ? k_kv_attn<D, TY, KV_WAVES, 2, true> : k_kv_attn<D, TY, KV_WAVES, 1, true>);
+		else if (p->waves == KV_MANY)
+			launch(p->slots == 4 ? k_kv_attn<D, TY, MANY, FOUR, false> :
+			       p->slots == 2 ? k_kv_attn<D, TY, MANY, 2, false> : k_kv_attn<D, TY, MANY, 1, false>);
 		else
-			launch(p->slots == 4 ? k_kv_attn<D, TY, KV_WAVES, FOUR> :
-			       p->slots == 2 ? k_kv_attn<D, TY, KV_WAVES, 2> : k_kv_attn<D, TY, KV_WAVES, 1>);
-		if (p->splits > 1)
+			launch(p->slots == 4 ? k_kv_attn<D, TY, KV_WAVES, FOUR, false> :
+			       p->slots == 2 ? k_kv_attn<D, TY, KV_WAVES, 2, false> : k_kv_attn<D, TY, KV_WAVES, 1, false>);
+		if (p->splits > 1 || p->shares)
 			k_kv_merge<D, TY><<<rows, KV_NT, 0, (hipStream_t)stream>>>(
 				*a, G, (t *)out, out_stride, window, (const float *)ws, p->row_tiles,
-				p->chunk, p->splits, p->rows);
+				p->chunk, p->splits, p->rows, p->shares);
 	}))
 	return (int)hipGetLastError();
 }

@@ -90,7 +90,7 @@ __device__ static inline void kv_error(const kv_args &a, u32 bit)
 		atomicOr(a.err, bit);
 }
 
-__device__ static inline kv_seq kv_sequence(const kv_args &a, int s)
+__device__ static inline kv_seq kv_sequence(const kv_args &a, int s, bool report)
 {
 	kv_seq q;
 	int end;
@@ -113,10 +113,15 @@ __device__ static inline kv_seq kv_sequence(const kv_args &a, int s)
 		bad = true;
 		q.len = min(max(q.len, 0), a.max_len);
 	}
-	if (bad && threadIdx.x == 0)
+	if (bad && report)
 		kv_error(a, HIP_KV_ERR_BATCH);
 	q.n = end - q.row;
 	return q;
+}
+
+__device__ static inline kv_seq kv_sequence(const kv_args &a, int s)
+{
+	return kv_sequence(a, s, threadIdx.x == 0);
 }
 
 /* tile t (rows 32 t ..) of kv head h of sequence s, NULL where its page is

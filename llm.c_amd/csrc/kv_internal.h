@@ -46,6 +46,7 @@ typedef struct kv_plan {
 	int waves;     /* of a workgroup */
 	int chunk;     /* cache tiles of one workgroup */
 	int splits;    /* workgroups along the cache */
+	int shares;    /* of all caches together, for each kv head, instead (0: no) */
 	size_t ws;     /* bytes of partial results, whatever the window */
 } kv_plan;
 void kv_attn_plan(const kv_args *a, int head_len, int heads, int window, kv_plan *p);

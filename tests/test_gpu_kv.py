@@ -609,6 +609,38 @@ def test_output_may_be_the_queries(dev):
         assert np.array_equal(dev.get(d_q, q.shape, np.float32), dev.get(d_o, q.shape, np.float32))
 
 
+@pytest.mark.parametrize("window", (0, 70))
+@pytest.mark.parametrize("ty,D,KH,G,nseq", ((F32, 128, 8, 4, 64), (BF16, 128, 8, 1, 64), (F16, 64, 16, 8, 40),
+                                            (F32, 64, 16, 1, 130), (BF16, 256, 8, 4, 64), (F32, 256, 4, 6, 128),
+                                            (F32, 128, 8, 8, 64), (BF16, 128, 2, 7, 256)))
+def test_many_caches_in_shares(dev, ty, D, KH, G, nseq, window):
+    """A batch whose bound is far above its lengths: shares of a few tiles that begin
+    and end inside sequences, of every length, without rows, or before their start."""
+    rng = np.random.default_rng(nseq + D + G)
+    lens = [int(n) for n in rng.integers(1, 200, nseq)]
+    rows = [int(n) for n in rng.integers(1, max(1, 16 // G) + 1, nseq)]
+    rows[3], lens[3], rows[nseq - 1], lens[nseq - 1] = 0, 50, 0, 0
+    lens[0], lens[7], lens[20] = 900, 0, 32
+    rows[0], rows[7] = 1, 1
+    c = Case(dev, rng, rows, lens, 32, KH, D, slack=16384 // 32)
+    c.batch.max_len = 16384
+    at = [int(i) for i in c.start[:-1]]
+    check = sorted({i for i in at if i < c.T} & set(at[:10] + at[-6:] + [at[int(k)] for k in rng.integers(0, nseq, 20)]))
+    check_attention(dev, c, KH * G, ty, window, rng, qscale=2.0, pad=8, check=check)
+    assert c.errors() == 0
+    # a bad page and a bad length in one sequence each
+    table, length = c.table.copy(), np.asarray(lens, np.int32)
+    table[0, 1], length[5] = c.pages, 20000
+    b = hipkv.Batch(nseq, c.T, max(rows), 16384, c.d_start, dev.up(length), dev.up(table), table.shape[1])
+    q = rng.standard_normal((c.T, KH * G, D)).astype(np.float32)
+    d_q, d_o = dev.up(ref.to_type(q, ty)), dev.up(np.zeros(q.shape, ref.np_dtype(ty)))
+    ws = hipkv.attn_ws(c.cache, b, KH * G)
+    d_ws = dev.h.malloc(ws)
+    dev.p.append(d_ws)
+    hipkv.attn(c.cache, b, ty, d_q, KH * G * D, KH * G, d_o, KH * G * D, 0.1, 0, d_ws, ws)
+    assert c.errors() == hipkv.ERR_PAGE | hipkv.ERR_BATCH
+
+
 @pytest.mark.parametrize("ty,H,KH,D,rows,lens", (
     (F32, 3, 1, 128, [1], [90]), (BF16, 8, 1, 64, [1, 1], [70, 64]),          # slots
     (F16, 4, 4, 256, [9], [300]), (F32, 16, 16, 128, [300] * 2, [300, 1100]),  # tiles of 16

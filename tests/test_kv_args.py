@@ -199,3 +199,18 @@ def test_calls_without_rows_do_nothing():
         hipkv.attn(cache(), b, 0, None, 0, 4, None, 0, 1.0)
         assert hipkv.attn_ws(cache(), b, 4) == 0
     hipkv.rope(rope(), 0, DEV, 512, 2 * DEV, 512, 0, 4, 128, DEV)
+
+
+@pytest.mark.parametrize("D", (64, 128, 256))
+@pytest.mark.parametrize("nseq,KH,G,rows", ((1, 8, 4, 1), (16, 8, 4, 1), (64, 8, 4, 1), (64, 8, 4, 4), (256, 2, 8, 2),
+                                            (257, 2, 8, 1), (100, 16, 1, 16), (3, 1, 1, 5), (1000, 8, 4, 1)))
+def test_a_workspace_serves_shorter_bounds(D, nseq, KH, G, rows):
+    """What a step's attention needs grows with the bound of the lengths."""
+    before = 0
+    for max_len in list(range(1, 500, 31)) + list(range(500, 40000, 517)):
+        c = cache(kv_heads=KH, head_len=D, page=64)
+        b = batch(nseq=nseq, rows=nseq * rows, max_rows=rows, max_len=max_len, table_stride=700, row_start=None)
+        ws = hipkv.attn_ws(c, b, KH * G)
+        assert ws >= before, max_len
+        before = ws
+    assert before > 0
