@@ -583,243 +583,243 @@ void k_kv_attn(
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
 	const int kv_head = blockIdx.x % a.kv_heads, rt = blockIdx.x / a.kv_heads;
 	const int split = blockIdx.y, splits = gridDim.y, shift = a.page_shift - 5;
-	int at = 0, end = 1; /* of the workgroup's share of the line */
+	int pos = 0, end = 1; /* of the workgroup's share of the line */
 	if constexpr (SHARE) {
 		const kv_line line = kv_line_of(a, window);
 		s_line[threadIdx.x] = make_int2(line.start, line.tiles);
 		const int share = kv_share(line.all, splits);
-		at = split * share;
-		end = min(at + share, line.all);
+		pos = split * share;
+		end = min(pos + share, line.all);
 	}
-	while (at < end) {
-	int lane = threadIdx.x % WAVE;
-	if constexpr (SHARE) { /* nothing of the lane's is kept in registers from turn to turn */
-		asm volatile("" : "+v"(lane));
-		__builtin_assume(lane >= 0 && lane < WAVE);
-	}
-	const int part = lane / 16, slot = lane % SLOTS;
-	int s = blockIdx.z, t0 = 0, t1 = 0, page = -1;
-	if constexpr (SHARE) {
-		const int2 line = s_line[threadIdx.x];
-		if (line.x <= at && at < line.x + line.y) {
-			s_seq[0] = threadIdx.x;
-			s_seq[1] = line.x;
+	while (pos < end) {
+		int lane = threadIdx.x % WAVE;
+		if constexpr (SHARE) { /* nothing of the lane's is kept in registers from turn to turn */
+			asm volatile("" : "+v"(lane));
+			__builtin_assume(lane >= 0 && lane < WAVE);
+		}
+		const int part = lane / 16, slot = lane % SLOTS;
+		int s = blockIdx.z, t0 = 0, t1 = 0, page = -1;
+		if constexpr (SHARE) {
+			const int2 line = s_line[threadIdx.x];
+			if (line.x <= pos && pos < line.x + line.y) {
+				s_seq[0] = threadIdx.x;
+				s_seq[1] = line.x;
+			}
+			__syncthreads();
+			s = __builtin_amdgcn_readfirstlane(s_seq[0]);
+			t0 = pos - __builtin_amdgcn_readfirstlane(s_seq[1]);
+		}
+		/* the wave's tiles t0 + wave, + NW, ..; a lane holds the page of one of the
+		 * next 64.  Without a window the first lot needs no length, only the table's
+		 * bound, and is on its way before the length is known */
+		const int32_t *table = a.table + s * a.table_stride;
+		if (!window && !SHARE) {
+			const int at = (split * chunk + wave + lane * NW) >> shift;
+			page = at < a.table_stride ? table[at] : -1;
+		}
+		const kv_seq sq = kv_sequence(a, s);
+		if (!SHARE && rt * ROWS >= sq.n * G)
+			return;
+		const kv_span r = kv_rows_of<ROWS, SLOTS>(sq, rt, G, kv_head, window, lane);
+		t1 = (max(r.last, 0) + KV_TILE - 1) / KV_TILE;
+		if constexpr (SHARE) {
+			t0 += r.first / KV_TILE;
+			const int take = max(1, min(end - pos, t1 - t0));
+			t1 = min(t1, t0 + take);
+			pos += take;
+		} else {
+			t0 = r.first / KV_TILE + split * chunk;
+			t1 = min(t0 + chunk, t1);
+			pos = end;
+			if (split > 0 && t0 >= t1)
+				return;
+		}
+		kv_vec<TY, 8> qv[L::G];
+#pragma unroll
+		for (int g = 0; g < L::G; g++)
+			qv[g] = *(const kv_vec<TY, 8> *)(q + (size_t)r.row * q_stride + (size_t)r.head * D + 32 * g + 8 * part);
+
+		/* (a page outside the pool: its first tile, with every row hidden) */
+		const int n = a.pages ? (t1 - t0 - wave + NW - 1) / NW : 0;
+		bool lost = false;
+		const auto tile_of = [&](int i) -> const uint8_t * {
+			const int t = t0 + wave + i * NW;
+			if (i % WAVE == 0 && (i || window || SHARE)) {
+				const int tl = t + lane * NW;
+				page = tl < t1 ? table[tl >> shift] : -1;
+			}
+			const int id = __builtin_amdgcn_readlane(page, i % WAVE);
+			lost = (u32)id >= (u32)a.pages;
+			const size_t at = lost ? 0 : ((((size_t)id * a.kv_heads + kv_head) << shift) + (t & ((1 << shift) - 1)));
+			return a.pool + at * L::BYTES;
+		};
+		kv_keys<D> k;
+		kv_values<D> v;
+		kv_dv<SLOTS> vd;
+		if (n > 0) {
+			const uint8_t *tile = tile_of(0);
+			k.load(tile, lane);
+			vd.load(tile + L::V_SCALES, lane);
+			v.load(tile, lane);
+		} else if (!a.pages && lane == 0) {
+			kv_error(a, HIP_KV_ERR_PAGE);
+		}
+		const float rs = kv_put_query<D, QP, SLOTS, TY>(sh.q, qv, scale, lane, wave, NW);
+		if (threadIdx.x < KV_ROWS && slot == 0) {
+			s_row[threadIdx.x / SLOTS] = r.valid ? r.row : -1;
+			s_head[threadIdx.x / SLOTS] = r.hi > r.lo ? r.head : ~r.head;
 		}
 		__syncthreads();
-		s = __builtin_amdgcn_readfirstlane(s_seq[0]);
-		t0 = at - __builtin_amdgcn_readfirstlane(s_seq[1]);
-	}
-	/* the wave's tiles t0 + wave, + NW, ..; a lane holds the page of one of the
-	 * next 64.  Without a window the first lot needs no length, only the table's
-	 * bound, and is on its way before the length is known */
-	const int32_t *table = a.table + s * a.table_stride;
-	if (!window && !SHARE) {
-		const int at = (split * chunk + wave + lane * NW) >> shift;
-		page = at < a.table_stride ? table[at] : -1;
-	}
-	const kv_seq sq = kv_sequence(a, s);
-	if (!SHARE && rt * ROWS >= sq.n * G)
-		return;
-	const kv_span r = kv_rows_of<ROWS, SLOTS>(sq, rt, G, kv_head, window, lane);
-	t1 = (max(r.last, 0) + KV_TILE - 1) / KV_TILE;
-	if constexpr (SHARE) {
-		const int from = at;
-		t0 += r.first / KV_TILE;
-		at += max(1, min(end - at, t1 - t0));
-		t1 = min(t1, t0 + at - from);
-	} else {
-		t0 = r.first / KV_TILE + split * chunk;
-		t1 = min(t0 + chunk, t1);
-		at = end;
-		if (split > 0 && t0 >= t1)
-			return;
-	}
-	kv_vec<TY, 8> qv[L::G];
-#pragma unroll
-	for (int g = 0; g < L::G; g++)
-		qv[g] = *(const kv_vec<TY, 8> *)(q + (size_t)r.row * q_stride + (size_t)r.head * D + 32 * g + 8 * part);
 
-	/* (a page outside the pool: its first tile, with every row hidden) */
-	const int n = a.pages ? (t1 - t0 - wave + NW - 1) / NW : 0;
-	bool lost = false;
-	const auto tile_of = [&](int i) -> const uint8_t * {
-		const int t = t0 + wave + i * NW;
-		if (i % WAVE == 0 && (i || window || SHARE)) {
-			const int tl = t + lane * NW;
-			page = tl < t1 ? table[tl >> shift] : -1;
-		}
-		const int id = __builtin_amdgcn_readlane(page, i % WAVE);
-		lost = (u32)id >= (u32)a.pages;
-		const size_t at = lost ? 0 : ((((size_t)id * a.kv_heads + kv_head) << shift) + (t & ((1 << shift) - 1)));
-		return a.pool + at * L::BYTES;
-	};
-	kv_keys<D> k;
-	kv_values<D> v;
-	kv_dv<SLOTS> vd;
-	if (n > 0) {
-		const uint8_t *tile = tile_of(0);
-		k.load(tile, lane);
-		vd.load(tile + L::V_SCALES, lane);
-		v.load(tile, lane);
-	} else if (!a.pages && lane == 0) {
-		kv_error(a, HIP_KV_ERR_PAGE);
-	}
-	const float rs = kv_put_query<D, QP, SLOTS, TY>(sh.q, qv, scale, lane, wave, NW);
-	if (threadIdx.x < KV_ROWS && slot == 0) {
-		s_row[threadIdx.x / SLOTS] = r.valid ? r.row : -1;
-		s_head[threadIdx.x / SLOTS] = r.hi > r.lo ? r.head : ~r.head;
-	}
-	__syncthreads();
+		floatx4 o[CT];
+#pragma unroll
+		for (int c = 0; c < CT; c++)
+			o[c] = (floatx4)0.0f;
+		kv_soft soft = {-__builtin_inff(), 0.0f};
 
-	floatx4 o[CT];
+		const auto step = [&](int i, auto more) {
+			const int t = t0 + wave + i * NW;
+			const bool hidden = lost;
+			const uint8_t *next = NULL;
+			if constexpr (more.value)
+				next = tile_of(i + 1);
+			half2_t dv[N / 2];
+			kv_halves<N> pp[PP];
 #pragma unroll
-	for (int c = 0; c < CT; c++)
-		o[c] = (floatx4)0.0f;
-	kv_soft soft = {-__builtin_inff(), 0.0f};
-
-	const auto step = [&](int i, auto more) {
-		const int t = t0 + wave + i * NW;
-		const bool hidden = lost;
-		const uint8_t *next = NULL;
-		if constexpr (more.value)
-			next = tile_of(i + 1);
-		half2_t dv[N / 2];
-		kv_halves<N> pp[PP];
+			for (int j = 0; j < N / 2; j++)
+				dv[j] = __builtin_bit_cast(half2_t, vd.w[j]);
+			typedef float floats __attribute__((ext_vector_type(N)));
+			floats x = kv_scores<D, QP, SLOTS, TY>(k, sh.q, lane);
+			/* the scales are used up before their registers are loaded again */
+			asm volatile("" : "+v"(x) : : "memory");
+			if constexpr (more.value)
+				k.load(next, lane);
+			if (hidden || t * KV_TILE < r.inner0 || (t + 1) * KV_TILE > r.inner1) {
+				const int lo = hidden ? 0x7fffffff : r.lo;
 #pragma unroll
-		for (int j = 0; j < N / 2; j++)
-			dv[j] = __builtin_bit_cast(half2_t, vd.w[j]);
-		typedef float floats __attribute__((ext_vector_type(N)));
-		floats x = kv_scores<D, QP, SLOTS, TY>(k, sh.q, lane);
-		/* the scales are used up before their registers are loaded again */
-		asm volatile("" : "+v"(x) : : "memory");
-		if constexpr (more.value)
-			k.load(next, lane);
-		if (hidden || t * KV_TILE < r.inner0 || (t + 1) * KV_TILE > r.inner1) {
-			const int lo = hidden ? 0x7fffffff : r.lo;
-#pragma unroll
-			for (int j = 0; j < N; j++) {
-				const int u = slot * N + j, at = t * KV_TILE + 16 * (u / 4) + 4 * part + u % 4;
-				const bool hide = at < lo || at >= r.hi;
-				x[j] = hide ? -__builtin_inff() : x[j];
-				dv[j / 2][j % 2] = hide ? (_Float16)0.0f : dv[j / 2][j % 2];
+				for (int j = 0; j < N; j++) {
+					const int u = slot * N + j, at = t * KV_TILE + 16 * (u / 4) + 4 * part + u % 4;
+					const bool hide = at < lo || at >= r.hi;
+					x[j] = hide ? -__builtin_inff() : x[j];
+					dv[j / 2][j % 2] = hide ? (_Float16)0.0f : dv[j / 2][j % 2];
+				}
+				if (hidden && lane == 0)
+					kv_error(a, HIP_KV_ERR_PAGE);
 			}
-			if (hidden && lane == 0)
-				kv_error(a, HIP_KV_ERR_PAGE);
-		}
-		const float back = kv_softmax<N, 4, PP, TY>(soft, (const float *)&x, dv, rs, slot % 2 ? 0.0f : 4.0f, pp);
-		/* a slot's column has its rows alone */
-		half8_t pf[PP];
+			const float back = kv_softmax<N, 4, PP, TY>(soft, (const float *)&x, dv, rs, slot % 2 ? 0.0f : 4.0f, pp);
+			/* a slot's column has its rows alone */
+			half8_t pf[PP];
 #pragma unroll
-		for (int p = 0; p < PP; p++) {
-			if constexpr (SLOTS == 1) {
-				pf[p] = pp[p];
-			} else {
-				typedef u32 words __attribute__((ext_vector_type(N / 2)));
-				const words z = __builtin_bit_cast(words, pp[p]);
-				u32 w[4];
+			for (int p = 0; p < PP; p++) {
+				if constexpr (SLOTS == 1) {
+					pf[p] = pp[p];
+				} else {
+					typedef u32 words __attribute__((ext_vector_type(N / 2)));
+					const words z = __builtin_bit_cast(words, pp[p]);
+					u32 w[4];
+#pragma unroll
+					for (int u = 0; u < 4; u++)
+						w[u] = u / (N / 2) == slot ? z[u % (N / 2)] : 0;
+					pf[p] = as_half8(w[0], w[1], w[2], w[3]);
+				}
+			}
+			if (__ballot(back != 1.0f)) {
+#pragma unroll
+				for (int c = 0; c < CT; c++)
+					o[c] *= back;
+			}
+#pragma unroll
+			for (int c = 0; c < CT; c++) {
+				const half8_t vf = kv_word8<TY>(v.w[c]);
+#pragma unroll
+				for (int p = 0; p < PP; p++)
+					o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[p], o[c], 0, 0, 0);
+			}
+			if constexpr (more.value) {
+				vd.load(next + L::V_SCALES, lane);
+				v.load(next, lane);
+			}
+		};
+		for (int i = 0; i < n - 1; i++)
+			step(i, std::true_type());
+		if (n > 0)
+			step(n - 1, std::false_type());
+
+		/* the waves' results: to one reference, then added in wave order */
+		float sum = kv_form<TY>::STEP * row_sum(soft.sum); /* the outputs' own factor */
+		if (part == 0)
+			s_ref[wave][lane] = soft.ref;
+		__syncthreads();
+		float ref = -__builtin_inff(); /* of the row, whichever column */
+#pragma unroll
+		for (int w = 0; w < NW; w++)
+#pragma unroll
+			for (int c = 0; c < SLOTS; c++)
+				ref = fmaxf(ref, s_ref[w][lane % 16 - slot + c]);
+		const float factor = weight(soft.ref, ref);
+		const int row = lane % 16 / SLOTS;
+		sum *= factor;
+		float y[4 * CT], z[2 * CT]; /* the row's slots added: each keeps its share of the channels */
+#pragma unroll
+		for (int u = 0; u < 4 * CT; u++)
+			y[u] = o[u / 4][u % 4] * factor;
+		if constexpr (SLOTS == 4) {
+			sum += other<2>(sum);
+			halved<2>(y, lane & 2, z);
+#pragma unroll
+			for (int u = 0; u < 2 * CT; u++)
+				y[u] = z[u];
+		}
+		if constexpr (SLOTS > 1) {
+			float w[8 * CT / SLOTS];
+#pragma unroll
+			for (int u = 0; u < 8 * CT / SLOTS; u++)
+				w[u] = y[u];
+			sum += other<1>(sum);
+			halved<1>(w, lane & 1, y);
+		}
+		if (r.valid) {
+#pragma unroll
+			for (int u = 0; u < CT / SLOTS; u++)
+				*(floatx4 *)&sh.o[wave][row][16 * (slot * (CT / SLOTS) + u) + 4 * part] =
+					floatx4{y[4 * u], y[4 * u + 1], y[4 * u + 2], y[4 * u + 3]};
+			if (part == 0 && slot == 0) {
+				s_sum[wave][row] = sum;
+				s_high[row] = ref; /* (every wave's the same) */
+			}
+		}
+		__syncthreads();
+		const size_t piece = SHARE ? (size_t)kv_head * (splits + a.nseq) + split + s
+					   : ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
+		float *to = ws + piece * nrows * (D + 4);
+		for (int at = threadIdx.x; at < ROWS * D / 4; at += NW * WAVE) {
+			const int i = at / (D / 4), c = at % (D / 4) * 4, row = s_row[i];
+			if (row < 0)
+				break; /* the rows behind are not there either */
+			float den = s_sum[0][i];
+			floatx4 y = *(const floatx4 *)&sh.o[0][i][c];
+#pragma unroll
+			for (int w = 1; w < NW; w++) {
+				den += s_sum[w][i];
+				y += *(const floatx4 *)&sh.o[w][i][c];
+			}
+			if (!SHARE && splits == 1) {
+				kv_vec<TY, 4> z;
+				const int head = s_head[i];
 #pragma unroll
 				for (int u = 0; u < 4; u++)
-					w[u] = u / (N / 2) == slot ? z[u % (N / 2)] : 0;
-				pf[p] = as_half8(w[0], w[1], w[2], w[3]);
+					z.v[u] = T::put(head >= 0 ? y[u] / den : 0.0f);
+				*(kv_vec<TY, 4> *)(out + row * out_stride + (size_t)(head < 0 ? ~head : head) * D + c) = z;
+				continue;
+			}
+			*(floatx4 *)(to + i * (D + 4) + c) = y;
+			if (c == 0) {
+				to[i * (D + 4) + D] = s_high[i];
+				to[i * (D + 4) + D + 1] = den;
 			}
 		}
-		if (__ballot(back != 1.0f)) {
-#pragma unroll
-			for (int c = 0; c < CT; c++)
-				o[c] *= back;
-		}
-#pragma unroll
-		for (int c = 0; c < CT; c++) {
-			const half8_t vf = kv_word8<TY>(v.w[c]);
-#pragma unroll
-			for (int p = 0; p < PP; p++)
-				o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[p], o[c], 0, 0, 0);
-		}
-		if constexpr (more.value) {
-			vd.load(next + L::V_SCALES, lane);
-			v.load(next, lane);
-		}
-	};
-	for (int i = 0; i < n - 1; i++)
-		step(i, std::true_type());
-	if (n > 0)
-		step(n - 1, std::false_type());
-
-	/* the waves' results: to one reference, then added in wave order */
-	float sum = kv_form<TY>::STEP * row_sum(soft.sum); /* the outputs' own factor */
-	if (part == 0)
-		s_ref[wave][lane] = soft.ref;
-	__syncthreads();
-	float ref = -__builtin_inff(); /* of the row, whichever column */
-#pragma unroll
-	for (int w = 0; w < NW; w++)
-#pragma unroll
-		for (int c = 0; c < SLOTS; c++)
-			ref = fmaxf(ref, s_ref[w][lane % 16 - slot + c]);
-	const float factor = weight(soft.ref, ref);
-	const int row = lane % 16 / SLOTS;
-	sum *= factor;
-	float y[4 * CT], z[2 * CT]; /* the row's slots added: each keeps its share of the channels */
-#pragma unroll
-	for (int u = 0; u < 4 * CT; u++)
-		y[u] = o[u / 4][u % 4] * factor;
-	if constexpr (SLOTS == 4) {
-		sum += other<2>(sum);
-		halved<2>(y, lane & 2, z);
-#pragma unroll
-		for (int u = 0; u < 2 * CT; u++)
-			y[u] = z[u];
-	}
-	if constexpr (SLOTS > 1) {
-		float w[8 * CT / SLOTS];
-#pragma unroll
-		for (int u = 0; u < 8 * CT / SLOTS; u++)
-			w[u] = y[u];
-		sum += other<1>(sum);
-		halved<1>(w, lane & 1, y);
-	}
-	if (r.valid) {
-#pragma unroll
-		for (int u = 0; u < CT / SLOTS; u++)
-			*(floatx4 *)&sh.o[wave][row][16 * (slot * (CT / SLOTS) + u) + 4 * part] =
-				floatx4{y[4 * u], y[4 * u + 1], y[4 * u + 2], y[4 * u + 3]};
-		if (part == 0 && slot == 0) {
-			s_sum[wave][row] = sum;
-			s_high[row] = ref; /* (every wave's the same) */
-		}
-	}
-	__syncthreads();
-	const size_t piece = SHARE ? (size_t)kv_head * (splits + a.nseq) + split + s
-				   : ((size_t)(s * row_tiles + rt) * a.kv_heads + kv_head) * splits + split;
-	float *to = ws + piece * nrows * (D + 4);
-	for (int at = threadIdx.x; at < ROWS * D / 4; at += NW * WAVE) {
-		const int i = at / (D / 4), c = at % (D / 4) * 4, row = s_row[i];
-		if (row < 0)
-			break; /* the rows behind are not there either */
-		float den = s_sum[0][i];
-		floatx4 y = *(const floatx4 *)&sh.o[0][i][c];
-#pragma unroll
-		for (int w = 1; w < NW; w++) {
-			den += s_sum[w][i];
-			y += *(const floatx4 *)&sh.o[w][i][c];
-		}
-		if (!SHARE && splits == 1) {
-			kv_vec<TY, 4> z;
-			const int head = s_head[i];
-#pragma unroll
-			for (int u = 0; u < 4; u++)
-				z.v[u] = T::put(head >= 0 ? y[u] / den : 0.0f);
-			*(kv_vec<TY, 4> *)(out + row * out_stride + (size_t)(head < 0 ? ~head : head) * D + c) = z;
-			continue;
-		}
-		*(floatx4 *)(to + i * (D + 4) + c) = y;
-		if (c == 0) {
-			to[i * (D + 4) + D] = s_high[i];
-			to[i * (D + 4) + D + 1] = den;
-		}
-	}
-	if constexpr (SHARE)
-		__syncthreads();
+		if constexpr (SHARE)
+			__syncthreads();
 	}
 }
 
@@ -1285,7 +1285,8 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	const long whole = head_len < 256 && p->row_tiles == 1 ? wgs < 128 ? 32 : wgs < 512 ? 72 : 128 : 0;
 	p->waves = tiles <= whole ? KV_MANY : KV_WAVES;
 	const size_t pieces = (size_t)a->nseq * a->kv_heads * ((all + KV_CHUNK - 1) / KV_CHUNK);
-	if (p->row_tiles == 1 && all > whole && a->nseq <= KV_SEQS && wgs >= 512 && pieces >= 4096) {
+	if (p->row_tiles == 1 && all > whole && a->nseq <= KV_SEQS && wgs >= 512 && pieces >= 4096 &&
+	    (size_t)a->nseq * all < (size_t)1 << 30) {
 		const int chip = head_len == 256 ? 512 : 1024, shares = a->kv_heads < chip ? chip / a->kv_heads : 1;
 		/* (never less than shorter bounds need) */
 		const size_t slots = (size_t)a->kv_heads * (shares + a->nseq);
