@@ -424,15 +424,24 @@ __device__ static inline auto kv_scores(const kv_keys<D> &k, const kv_query<D, Q
 
 /*
  * The running softmax of a query row.  ref is its reference in powers of two: a
- * probability is 2^(logit - ref), and ref the largest logit plus the exponent of
- * the value scales that come with it, less REF, so that probability times value
- * scale stays below 2^REF.  It stays as it is until the product would reach 2^TOP
- * (2^15 with kv_word's factor, below f16's largest): most tiles then leave the output
- * alone.  Sums and outputs carry the same factor, which the division at the end
- * takes out.
+ * probability is 2^(logit - ref), and ref the largest sum of a logit and its value
+ * scale's exponent, less REF, so that probability times value scale stays below
+ * 2^REF and the largest is at least 2^(REF - 1 - SPREAD): the f16 parts hold the others
+ * relative to it.  ref stays as it is until a product would reach 2^TOP (2^15 with
+ * kv_word's factor, below f16's largest): most tiles then leave the output alone.
+ * Sums and outputs carry the same factor, which the division at the end takes out.
+ *
+ * That sum's bound is the lane's largest logit plus its largest exponent.  They may be
+ * different rows': where the bound would move ref and the lane's scales are 2^SPREAD
+ * apart, subnormal or 0, it is taken row by row.  (Row by row always: 900 -> 950 us for the prompt
+ * at k_kv_attn_wide.)  A row without a value (scale 0) then counts with the exponent
+ * NO_VALUE: it moves ref only where its logit is far above all that has a value, and
+ * its probability stays below 2^(TOP - NO_VALUE), of which fp32 holds the sum of 2^31.
  */
 struct kv_soft {
 	float ref, sum;
+	static constexpr int SPREAD = 8;
+	static constexpr float NO_VALUE = -80.0f;
 };
 
 template <int N> using kv_halves = _Float16 __attribute__((ext_vector_type(N)));
@@ -441,11 +450,11 @@ template <int N> using kv_halves = _Float16 __attribute__((ext_vector_type(N)));
  * Probabilities times value scales of the lane's N cached rows, in f16 parts;
  * 16 times that where the codes have the smaller step: two of four rows, or (N = 2)
  * both of a lane with more = 4.  SPAN lanes 16 apart, or two 32 apart, hold the query
- * row's others.  Returns what the output so far is multiplied by.
+ * row's others.  rescale(f) multiplies the output so far, where the reference moves.
  */
-template <int N, int SPAN, int PP, int TY>
-__device__ static inline float kv_softmax(kv_soft &s, const float *x, const half2_t *dv, float rs, float more,
-					  kv_halves<N> (&pf)[PP])
+template <int N, int SPAN, int PP, int TY, class Fn>
+__device__ static inline void kv_softmax(kv_soft &s, const float *x, const half2_t *dv, float rs, float more,
+					 kv_halves<N> (&pf)[PP], Fn rescale)
 {
 	constexpr float LOG_MORE = kv_form<TY>::LOG_MORE, MORE = kv_form<TY>::MORE;
 	float top = x[0];
@@ -461,11 +470,34 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
 	}
 	const unsigned short most1 = most2.x > most2.y ? most2.x : most2.y;
 	const float big = (float)__builtin_bit_cast(_Float16, most1);
-	/* (scales of nothing but zeros: exponent 0) */
+	/* (scales of nothing but zeros: exponent 0, and row by row below) */
 	const float most = fmaf(top, rs, (float)__builtin_amdgcn_frexp_expf(big));
-	const float high = SPAN == 4 ? row_max(most) : half_max(most);
-	const float next = high - s.ref > kv_form<TY>::TOP ? high - kv_form<TY>::REF : s.ref;
-	const float back = weight(s.ref, next);
+	float high = SPAN == 4 ? row_max(most) : half_max(most);
+	float next = high - s.ref > kv_form<TY>::TOP ? high - kv_form<TY>::REF : s.ref;
+	float back = weight(s.ref, next);
+	if (__ballot(back != 1.0f)) {
+		ushort2_t least2 = {0xffff, 0xffff};
+#pragma unroll
+		for (int i = 0; i < N / 2; i++) {
+			const u32 a = __builtin_bit_cast(u32, dv[i]) & 0x7fff7fffu;
+			least2 = __builtin_elementwise_min(least2, __builtin_bit_cast(ushort2_t, a));
+		}
+		const unsigned short least1 = least2.x < least2.y ? least2.x : least2.y;
+		if (__ballot(least1 < 1 << 10 || most1 - least1 > kv_soft::SPREAD << 10)) {
+			float own = -__builtin_inff();
+#pragma unroll
+			for (int j = 0; j < N; j++) {
+				const float d = (float)dv[j / 2][j % 2];
+				own = fmaxf(own, fmaf(x[j], rs, d == 0.0f ? kv_soft::NO_VALUE
+									  : (float)__builtin_amdgcn_frexp_expf(d)));
+				asm("" : "+v"(own)); /* (few registers) */
+			}
+			high = SPAN == 4 ? row_max(own) : half_max(own);
+			next = high - s.ref > kv_form<TY>::TOP ? high - kv_form<TY>::REF : s.ref;
+			back = weight(s.ref, next);
+		}
+		rescale(back);
+	}
 	s.ref = next;
 	const float ref = next == -__builtin_inff() ? 0.0f : next;
 	const float ref16 = N == 2 && LOG_MORE > 0.0f ? ref - more : ref - LOG_MORE;
@@ -483,7 +515,6 @@ __device__ static inline float kv_softmax(kv_soft &s, const float *x, const half
 	}
 	const float less = N == 2 && more == 0.0f ? 1.0f : 1.0f / MORE;
 	s.sum = s.sum * back + fmaf(sum16, less, sum);
-	return back;
 }
 
 /*
@@ -706,7 +737,11 @@ void k_kv_attn(
 				if (hidden && lane == 0)
 					kv_error(a, HIP_KV_ERR_PAGE);
 			}
-			const float back = kv_softmax<N, 4, PP, TY>(soft, (const float *)&x, dv, rs, slot % 2 ? 0.0f : 4.0f, pp);
+			kv_softmax<N, 4, PP, TY>(soft, (const float *)&x, dv, rs, slot % 2 ? 0.0f : 4.0f, pp, [&](float back) {
+#pragma unroll
+				for (int c = 0; c < CT; c++)
+					o[c] *= back;
+			});
 			/* a slot's column has its rows alone */
 			half8_t pf[PP];
 #pragma unroll
@@ -722,11 +757,6 @@ void k_kv_attn(
 						w[u] = u / (N / 2) == slot ? z[u % (N / 2)] : 0;
 					pf[p] = as_half8(w[0], w[1], w[2], w[3]);
 				}
-			}
-			if (__ballot(back != 1.0f)) {
-#pragma unroll
-				for (int c = 0; c < CT; c++)
-					o[c] *= back;
 			}
 #pragma unroll
 			for (int c = 0; c < CT; c++) {
@@ -1153,18 +1183,17 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 				kv_error(a, HIP_KV_ERR_PAGE);
 		}
 		half8_t pf[2][PP];
-		const float back = kv_softmax<16, 2, PP, TY>(soft, (const float *)&x, dv, rs, 0.0f, pp);
+		kv_softmax<16, 2, PP, TY>(soft, (const float *)&x, dv, rs, 0.0f, pp, [&](float back) {
+			late *= back;
+#pragma unroll
+			for (int c = 0; c < CT; c++)
+				o[c] *= back;
+		});
 		/* rows 8 i + .. are in step i % 2, codes 4 (i / 2) .. of the words */
 #pragma unroll
 		for (int p = 0; p < PP; p++) {
 			pf[0][p] = __builtin_shufflevector(pp[p], pp[p], 0, 1, 2, 3, 8, 9, 10, 11);
 			pf[1][p] = __builtin_shufflevector(pp[p], pp[p], 4, 5, 6, 7, 12, 13, 14, 15);
-		}
-		if (__ballot(back != 1.0f)) {
-			late *= back;
-#pragma unroll
-			for (int c = 0; c < CT; c++)
-				o[c] *= back;
 		}
 #pragma unroll
 		for (int c = 0; c < CT; c++)

@@ -1,0 +1,181 @@
+"""The calls of hip_kv.h at the ends of their ranges: value scales that differ by
+the whole range of f16, long caches of one sign, workgroups of several rows and
+heads, lengths of nothing and near the largest, workspaces' ends.
+
+Tolerances.  As in test_gpu_kv.py where values are compared one by one.  Whole
+outputs are compared by their relative L2 error, to which a 16-bit type's own
+rounding adds at most HALF_STEP (and 0.4 of it, 1 / sqrt(3) at a value's lower end and
+half of that at its upper, where values are spread evenly): a kernel that is within
+HALF_STEP altogether has erred by less than its rounding.  For fp32, see FP32.
+"""
+import numpy as np
+import pytest
+
+import hipkv
+import kv_ref as ref
+from kv_ref import BF16, F16, F32
+from test_gpu_kv import TYPES, Case, c_upload, dev, up_typed  # noqa: F401  (dev: a fixture)
+
+pytestmark = pytest.mark.gpu
+
+# fp32, logits in powers of two within 16 of the reference 2^9 below the largest: a
+# logit's last sum is rounded by up to 2^-21, rms 2^-21 / sqrt(3), times ln 2: 1.9e-7 of a
+# probability; a probability in 22 bits, 2^-23 / sqrt(3) = 0.7e-7; a query's 22 bits, as
+# much of a logit of 1 or 2; exponentials, the sums of 16 or 32 tiles a wave and the
+# quotient about 1e-7 together: 2.5e-7, all of them independent from row to row.  Four
+# times that; codes as subnormals would be 3e-6.
+FP32 = 1e-6
+WHOLE = {F32: FP32, F16: ref.HALF_STEP[F16], BF16: ref.HALF_STEP[BF16]}
+
+
+def rows_of(c, s, n):
+    """(k, v) [n][KH][D] float64, the first n cached rows of sequence s."""
+    P, D, KH = c.pool, c.D, c.KH
+    t = np.arange(-(-n // 32))
+    tiles = P.bytes[c.table[s][t * 32 // c.page], :, t % (c.page // 32)]  # [tiles][KH][bytes]
+    words = np.ascontiguousarray(tiles).view(np.uint32)
+    half = np.ascontiguousarray(tiles[..., 32 * D:]).view(np.float16).astype(np.float64)
+    k, v = np.empty((2, len(t), 32, KH, D))
+    for r in range(32):
+        w, b = P._key_words(r)
+        k[:, r] = (P._get(words.transpose(2, 0, 1), w, b[:, None, None]) - 8).transpose(1, 2, 0)
+        k[:, r] *= np.repeat(half[..., r * (D // 32):(r + 1) * (D // 32)], 32, -1)
+        w, b = P._value_words(r)
+        v[:, r] = (P._get(words.transpose(2, 0, 1), w, b[:, None, None]) - 8).transpose(1, 2, 0)
+        v[:, r] *= half[..., D + r, None]
+    return k.reshape(-1, KH, D)[:n], v.reshape(-1, KH, D)[:n]
+
+
+def attention(dev, c, H, ty, q, scale, window=0, batch=None, in_place=False):
+    """hip_kv_attn_dev of q [T][H][D] (its type's values), with a pattern behind the
+    workspace that has to stay."""
+    b = batch or c.batch
+    d_q = dev.up(ref.to_type(q, ty))
+    d_o = d_q if in_place else dev.up(np.zeros(q.shape, ref.np_dtype(ty)))
+    ws = hipkv.attn_ws(c.cache, b, H)
+    d_ws = dev.up(np.full(ws + 4096, 0xa5, np.uint8))
+    hipkv.attn(c.cache, b, ty, d_q, H * c.D, H, d_o, H * c.D, scale, window, d_ws, ws)
+    got = ref.from_type(dev.get(d_o, q.shape, ref.np_dtype(ty)), ty)
+    assert np.all(dev.get(d_ws, (ws + 4096,), np.uint8)[ws:] == 0xa5)
+    return got
+
+
+def typed(x, ty):
+    return ref.from_type(ref.to_type(x, ty), ty)
+
+
+def off(got, want):
+    return np.linalg.norm(got - want) / np.linalg.norm(want)
+
+
+# how a call is taken: (rows, lengths, KH, H)
+FORMS = {"slots of 4": ([1], [200], 2, 6), "slots of 2": ([2, 1], [150, 77], 2, 6),
+         "16 rows": ([9], [170], 1, 3), "pieces": ([1], [2200], 1, 4),
+         "32 rows": ([270] * 4, [270, 300, 400, 290], 16, 32),
+         "shares": ([1] * 64, [100] * 64, 8, 16)}
+
+
+def form_case(dev, rng, form, D):
+    rows, lens, KH, H = FORMS[form]
+    c = Case(dev, rng, rows, lens, 32, KH, D, slack=512 if form == "shares" else 0)
+    if form == "shares":
+        c.batch.max_len = 16384
+    return c, H
+
+
+def check_rows(c, most=6):
+    """Some rows of the call, the first and the last of sequences among them."""
+    at = sorted({int(i) for s in range(len(c.rows)) for i in (c.start[s], c.start[s + 1] - 1) if c.rows[s]})
+    return at if len(at) <= most else at[:most // 2] + at[-(most // 2):]
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("form", FORMS)
+def test_whole_outputs(dev, ty, form):
+    rng = np.random.default_rng(31)
+    c, H = form_case(dev, rng, form, 128)
+    q = typed(rng.standard_normal((c.T, H, 128)), ty)
+    got = attention(dev, c, H, ty, q, 128 ** -0.5)
+    pos, seq = c.positions(), c.sequences()
+    for i in check_rows(c):
+        k, v = rows_of(c, seq[i], pos[i] + 1)
+        want = ref.attend(q[i], k, v, pos[i], 128 ** -0.5, 0)[0]
+        assert off(got[i], want) <= WHOLE[ty], i
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("what", ("large", "larger than subnormal", "zeros", "zero sink"))
+def test_value_scales_of_any_range(dev, ty, form, what):
+    """Rows that carry nothing of the sum but have a large value scale (2^24 times the
+    others', or 2^17 times f16's smallest, at a logit of -60), that have no value at all among rows of the smallest
+    scales, or that take the probability (e^40 times the others') without a value.
+    Logits are up to 2^7 from the reference: in fp32 they are rounded by 2^-18, rms
+    2^-18 / sqrt(3) * ln 2 = 1.5e-6 of a probability, within 4 FP32 with the rest."""
+    rng = np.random.default_rng(32)
+    D = 128
+    c, H = form_case(dev, rng, form, D)
+    scale = D ** -0.5
+    u = rng.standard_normal(D)
+    u /= np.linalg.norm(u)
+    # every query leans on u by 20; every key is without it, but for the odd rows
+    q = rng.standard_normal((c.T, H, D))
+    q += (20 - q @ u)[..., None] * u
+    q = typed(q, ty)
+    half = c.pool.bytes[..., 34 * D:].view(np.float16)  # value scales, by the row of a tile
+    small, odd = {"large": (2.0 ** -10, 2.0 ** 14), "larger than subnormal": (2.0 ** -24, 2.0 ** -7),
+                  "zeros": (2.0 ** -22, 0), "zero sink": (0.25, 0)}[what]
+    half[...] = np.where(rng.random(half.shape) < 0.5, small, -small)
+    if what == "zeros":
+        half[..., np.arange(32) % 3 > 0] = 0
+    else:
+        half[..., 5] = odd
+        codes, d = ref.quantize((u * (-60 if odd else 40) / 20 / scale).reshape(-1, 32))
+        for s, n in enumerate(c.lens):
+            for p in range(5, n, 32):
+                tile = c.pool.bytes[c.table[s, p // 32], :, 0]
+                for h in range(c.KH):
+                    c.pool._put(tile[h].view(np.uint32), *c.pool._key_words(5), codes.ravel())
+                    tile[h, 32 * D:].view(np.float16)[5 * D // 32:6 * D // 32] = d
+    c_upload(c)
+    got = attention(dev, c, H, ty, q, scale)
+    assert np.all(np.isfinite(got))
+    pos, seq = c.positions(), c.sequences()
+    for i in check_rows(c):
+        k, v = rows_of(c, seq[i], pos[i] + 1)
+        want, _, size = ref.attend(q[i], k, v, pos[i], scale, 0)
+        tol = 4 * WHOLE[ty]
+        if ty == F16:  # results below its smallest normal
+            tol += 2.0 ** -25 * np.sqrt(want.size) / np.linalg.norm(want)
+        if what == "zero sink":
+            # these rows are the whole sum, with one logit, which fp32 holds to 2^-24 of the
+            # sum of its terms' sizes twice (its sum, its distance to the reference)
+            tol += 2.0 ** -23 * size.max()
+        e = off(got[i], want)
+        assert e <= tol, (i, e, tol)
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("D", (64, 128))
+def test_long_caches_of_one_sign(dev, ty, D):
+    """Tiles of 32 rows over 131072 cached rows whose value scales all have one sign and
+    whose values cancel: a surplus of 8 a code, where it is carried along, does not, and
+    outweighs the output 600 times."""
+    rng = np.random.default_rng(33)
+    n, rows, H = 131072, 512, 16
+    c = Case(dev, rng, [rows], [n], 1024, 1, D)
+    half = c.pool.bytes[..., 34 * D:].view(np.float16)
+    half[...] = np.abs(half)
+    nibbles = rng.integers(1, 16, (*c.pool.bytes.shape[:3], 32 * D), np.uint8)
+    words = (nibbles[..., ::2] | nibbles[..., 1::2] << 4).view(np.uint32)
+    c.pool.bytes[..., 16 * D:32 * D] = (words << 2 | words >> 30).view(np.uint8)
+    c_upload(c)
+    q = typed(rng.standard_normal((rows, H, D)), ty)
+    got = attention(dev, c, H, ty, q, D ** -0.5)
+    k, v = rows_of(c, 0, n)
+    for i in (0, 300, 511):
+        p = n - rows + i
+        want = ref.attend(q[i], k[:p + 1], v[:p + 1], p, D ** -0.5, 0)[0]
+        e = off(got[i], want)
+        # (fp32: a wave adds n / 128 tiles, rounding each sum by up to 2^-24)
+        assert e <= 2 * WHOLE[ty] + np.sqrt(n / 128) * 2.0 ** -24, i
