@@ -1312,7 +1312,7 @@ extern "C" void kv_attn_plan(const kv_args *a, int head_len, int heads, int wind
 	const size_t room = head_len == 64 ? 1024 : head_len == 128 ? 512 : 256;
 	const long by_room = wgs < room ? (long)(room / wgs) : 1;
 	const long whole = head_len < 256 && p->row_tiles == 1 ? wgs < 128 ? 32 : wgs < 512 ? 72 : 128 : 0;
-	p->waves = tiles <= whole ? KV_MANY : KV_WAVES;
+	p->waves = whole && tiles <= whole ? KV_MANY : KV_WAVES; /* (no tiles at all: max_len 0) */
 	const size_t pieces = (size_t)a->nseq * a->kv_heads * ((all + KV_CHUNK - 1) / KV_CHUNK);
 	if (p->row_tiles == 1 && all > whole && a->nseq <= KV_SEQS && wgs >= 512 && pieces >= 4096 &&
 	    (size_t)a->nseq * all < (size_t)1 << 30) {
@@ -1367,20 +1367,20 @@ extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const vo
 		}
 		/* (heads of 256 have no room for KV_MANY waves, of 64 no four groups) */
 		constexpr int MANY = D < 256 ? KV_MANY : KV_WAVES, FOUR = D > 64 ? 4 : 2;
-		const auto launch = [&](auto kernel) {
-			kernel<<<dim3(grid.x, grid.y, p->shares ? 1 : grid.z), p->waves * WAVE, 0, (hipStream_t)stream>>>(
+		const auto launch = [&](auto kernel, int waves) { /* as many as it is made for */
+			kernel<<<dim3(grid.x, grid.y, p->shares ? 1 : grid.z), waves * WAVE, 0, (hipStream_t)stream>>>(
 				*a, (const t *)q, q_stride, G, (t *)out, out_stride, scale, window, (float *)ws,
 				p->row_tiles, p->chunk, p->rows);
 		};
 		if (p->shares)
 			launch(p->slots == 4 ? k_kv_attn<D, TY, KV_WAVES, FOUR, true> :
-			       p->slots == 2 ? k_kv_attn<D, TY, KV_WAVES, 2, true> : k_kv_attn<D, TY, KV_WAVES, 1, true>);
+			       p->slots == 2 ? k_kv_attn<D, TY, KV_WAVES, 2, true> : k_kv_attn<D, TY, KV_WAVES, 1, true>, KV_WAVES);
 		else if (p->waves == KV_MANY)
 			launch(p->slots == 4 ? k_kv_attn<D, TY, MANY, FOUR, false> :
-			       p->slots == 2 ? k_kv_attn<D, TY, MANY, 2, false> : k_kv_attn<D, TY, MANY, 1, false>);
+			       p->slots == 2 ? k_kv_attn<D, TY, MANY, 2, false> : k_kv_attn<D, TY, MANY, 1, false>, MANY);
 		else
 			launch(p->slots == 4 ? k_kv_attn<D, TY, KV_WAVES, FOUR, false> :
-			       p->slots == 2 ? k_kv_attn<D, TY, KV_WAVES, 2, false> : k_kv_attn<D, TY, KV_WAVES, 1, false>);
+			       p->slots == 2 ? k_kv_attn<D, TY, KV_WAVES, 2, false> : k_kv_attn<D, TY, KV_WAVES, 1, false>, KV_WAVES);
 		if (p->splits > 1 || p->shares)
 			k_kv_merge<D, TY><<<rows, KV_NT, 0, (hipStream_t)stream>>>(
 				*a, G, (t *)out, out_stride, window, (const float *)ws, p->row_tiles,

@@ -179,3 +179,16 @@ def test_long_caches_of_one_sign(dev, ty, D):
         e = off(got[i], want)
         # (fp32: a wave adds n / 128 tiles, rounding each sum by up to 2^-24)
         assert e <= 2 * WHOLE[ty] + np.sqrt(n / 128) * 2.0 ** -24, i
+
+
+@pytest.mark.parametrize("ty", TYPES)
+@pytest.mark.parametrize("D", (64, 128, 256))
+@pytest.mark.parametrize("rows,KH,H", (([1], 1, 4), ([1, 2], 2, 2), ([40], 1, 2)))
+def test_a_bound_of_no_rows_at_all(dev, ty, D, rows, KH, H):
+    """max_len 0: every row is before its sequence's start, and its output 0."""
+    rng = np.random.default_rng(35)
+    c = Case(dev, rng, rows, [0] * len(rows), 32, KH, D)
+    c.batch.max_len = 0
+    q = typed(rng.standard_normal((c.T, H, D)), ty)
+    assert np.all(attention(dev, c, H, ty, q, 0.1, in_place=True) == 0)
+    assert c.errors() == 0
