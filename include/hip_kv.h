@@ -173,8 +173,10 @@ int hip_kv_read_dev(const hip_kv_cache *C, const hip_kv_batch *B, int type, void
  * head h reads kv head h / (heads / kv_heads)) heads of head_len: a row at
  * position p sees the cache positions p - window + 1 .. p (window 0: 0 .. p),
  *   out = sum_j softmax_j(scale q . k_j) v_j,
- * 0 for a row that is not there.  q and out are 16-byte aligned with strides
- * that are multiples of 16 bytes; out == q with equal strides is allowed.
+ * 0 for a row that is not there.  The scale is any finite number, the logits (scale
+ * q . k_j) up to 2^21 in size, past which fp32 has no two of them nearer than 1/4.
+ * q and out are 16-byte aligned with strides that are multiples of 16 bytes;
+ * out == q with equal strides is allowed.
  * Rows outside the batch keep what out holds.  A row on a page outside the
  * pool is left out of the sum; where that leaves nothing the output is NaN.
  * ws: hip_kv_attn_ws bytes (of the same cache, bounds and heads, whatever the

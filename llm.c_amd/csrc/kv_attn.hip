@@ -289,7 +289,8 @@ template <int D, int QP, int SLOTS> struct kv_query {
 };
 
 /* what a query row whose largest value is top is multiplied by, and its scores
- * then, to be logits in powers of two (the latter above 0) */
+ * then, to be logits in powers of two (the latter a normal number whatever the scale:
+ * a score of 0 or minus infinity stays what it is) */
 struct kv_factor {
 	float query, score;
 };
@@ -299,8 +300,8 @@ template <int TY> __device__ static inline kv_factor kv_query_factor(float top, 
 	int e = kv_form<TY>::QUERY - __builtin_amdgcn_frexp_expf(top);
 	e = top > 0.0f && top < __builtin_inff() ? min(max(e, -126), 122) : 0;
 	/* a negative scale turns the query around, 0 makes it 0 */
-	return {scale > 0.0f ? pow2(e) : scale < 0.0f ? -pow2(e) : 0.0f,
-		(scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / key_step) * pow2(-e)};
+	const float score = (scale == 0.0f ? 1.0f : fabsf(scale)) * (1.44269504088896341f / key_step) * pow2(-e);
+	return {scale > 0.0f ? pow2(e) : scale < 0.0f ? -pow2(e) : 0.0f, fminf(fmaxf(score, 0x1p-126f), 0x1.fffffep127f)};
 }
 
 /* eight channels of a query row in f16 parts, and their sum */

@@ -192,3 +192,24 @@ def test_a_bound_of_no_rows_at_all(dev, ty, D, rows, KH, H):
     q = typed(rng.standard_normal((c.T, H, D)), ty)
     assert np.all(attention(dev, c, H, ty, q, 0.1, in_place=True) == 0)
     assert c.errors() == 0
+
+
+@pytest.mark.parametrize("ty", (F32, BF16))
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("size,scale", ((1e-37, 1e-20), (0.0, 3e37), (1.0, 1e6)))
+def test_scales_of_any_size(dev, ty, form, size, scale):
+    """Logits that do not differ from 0: every row is the mean of the rows it sees, and
+    of none that it does not see.  Logits that differ by thousands: it is one row."""
+    rng = np.random.default_rng(34)
+    D = 128
+    c, H = form_case(dev, rng, form, D)
+    half = c.pool.bytes[..., 32 * D:34 * D].view(np.float16)
+    half[...] = half * np.float16(0.01)  # key scales: logits below 2^21
+    c_upload(c)
+    q = typed(rng.standard_normal((c.T, H, D)) * size, ty)
+    got = attention(dev, c, H, ty, q, scale)
+    pos, seq = c.positions(), c.sequences()
+    for i in check_rows(c):
+        k, v = rows_of(c, seq[i], pos[i] + 1)
+        want = ref.attend(q[i], k, v, pos[i], scale, 0)[0]
+        assert off(got[i], want) <= WHOLE[ty], i
