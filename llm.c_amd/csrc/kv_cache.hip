@@ -322,6 +322,8 @@ __global__ __launch_bounds__(KV_APPEND_NT) void k_kv_append(
 	const int s = blockIdx.x / groups / (tiles * parts);
 	const kv_seq sq = kv_sequence(a, s);
 	const int base = sq.len - sq.n, p0 = max(0, base), t = p0 / KV_TILE + unit / parts;
+	if (t >= (sq.len + KV_TILE - 1) / KV_TILE) /* (t * KV_TILE may pass 31 bits) */
+		return;
 	/* the part (a single row's own), and its rows i0 .. i0 + n - 1 in their order: row
 	 * 16 (i / 4) + 4 part + i % 4 of the tile */
 	const int part = parts > 1 ? unit % parts : p0 % 16 / 4;
@@ -474,6 +476,8 @@ __global__ __launch_bounds__(KV_NT) void k_kv_read(kv_args a, typename kv_type<T
 	const int s = blockIdx.x / a.kv_heads / tiles;
 	const kv_seq sq = kv_sequence(a, s);
 	const int base = sq.len - sq.n, p0 = max(0, base), t = p0 / KV_TILE + tb;
+	if (t >= (sq.len + KV_TILE - 1) / KV_TILE)
+		return;
 	const int lo = max(p0, t * KV_TILE), hi = min(sq.len, (t + 1) * KV_TILE);
 	if (lo >= hi)
 		return;
@@ -521,7 +525,7 @@ __global__ __launch_bounds__(KV_NT) void k_kv_read(kv_args a, typename kv_type<T
 /* tiles that n consecutive rows of a sequence can touch, at most */
 static int kv_tiles_of(int n)
 {
-	return (n + 2 * KV_TILE - 2) / KV_TILE;
+	return (int)(((long)n + 2 * KV_TILE - 2) / KV_TILE);
 }
 
 extern "C" int kv_launch_rope(int type, const void *x, size_t x_stride, void *out,

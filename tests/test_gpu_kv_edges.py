@@ -213,3 +213,62 @@ def test_scales_of_any_size(dev, ty, form, size, scale):
         k, v = rows_of(c, seq[i], pos[i] + 1)
         want = ref.attend(q[i], k, v, pos[i], scale, 0)[0]
         assert off(got[i], want) <= WHOLE[ty], i
+
+
+@pytest.mark.parametrize("ty,D,max_rows", ((F32, 128, 2), (F16, 64, 70000), (BF16, 256, 70000)))
+def test_positions_near_the_largest(dev, ty, D, max_rows):
+    """Rows at positions up to 2^31 - 2^16 - 2, with a bound of rows that reaches past
+    2^31, beside a short sequence: stored, read back and attended to in a window."""
+    rng = np.random.default_rng(36)
+    KH, H, page, window = 2, 4, 1024, 40
+    longest = (1 << 31) - (1 << 16) - 1
+    rows, lens = [2, 1], [longest, 7]
+    c = Case(dev, rng, [2, 1], [2, 7], page, KH, D)  # pages 0, 1 of each in turn
+    stride = -(-longest // page)
+    d_table = dev.h.malloc(2 * stride * 4)
+    dev.p.append(d_table)
+    # the last page of the long sequence, the first of the short one
+    dev.h.copy_in(d_table + (stride - 1) * 4, c.table[0, :1])
+    dev.h.copy_in(d_table + stride * 4, c.table[1, :1])
+    b = hipkv.Batch(2, max(3, max_rows), max_rows, longest, c.d_start, dev.up(np.asarray(lens, np.int32)),
+                    d_table, stride)
+    x = rng.standard_normal((3, H + 2 * KH, D)).astype(np.float32)
+    d_x, n, e = dev.up(ref.to_type(x, ty)), (H + 2 * KH) * D, ref.BYTES[ty]
+    x = typed(x, ty)
+    pos = np.array([longest - 2, longest - 1, 6])
+    f, mag = hipkv.rope_freqs(D, 1e4)
+    hipkv.append(c.cache, b, ty, d_x + H * D * e, d_x + (H + KH) * D * e, n, q=d_x, q_stride=n, heads=H, q_out=d_x,
+                 q_out_stride=n, rope=hipkv.Rope(D, hipkv.HALVES, dev.up(f), mag))
+    # angles to 2^31 have their own last bit: 2^-22 of a pair; keys are those that were stored
+    for i, s in ((0, 0), (1, 0), (2, 1)):
+        c.pool.store(np.repeat(c.table[s], 2), pos[i] % page, np.zeros((KH, D)), x[i, H + KH:].astype(np.float32))
+    got, want = c.pool_bytes(), c.pool.bytes
+    keys = np.zeros(want.shape[-1], bool)
+    keys[:16 * D] = keys[32 * D:34 * D] = True
+    assert np.array_equal(got[..., ~keys], want[..., ~keys]) and c.errors() == 0
+    untouched = np.ones(c.pages, bool)
+    untouched[c.table[:, 0]] = False
+    assert np.array_equal(got[untouched], want[untouched])
+    c.pool.bytes = got
+    stored = [c.pool.load(np.repeat(c.table[s], 2), pos[i] % page) for i, s in ((0, 0), (1, 0), (2, 1))]
+    q = ref.rotate(x, pos, f, mag, hipkv.HALVES)
+    for i in range(3):
+        top = np.abs(q[i, H:H + KH]).reshape(KH, -1, 32).max(-1).repeat(32, -1)
+        assert np.all(np.abs(stored[i][0] - q[i, H:H + KH]) <= top / 8 * 1.01)
+    back = [dev.up(np.zeros((3, KH * D), ref.np_dtype(ty))) for _ in "kv"]
+    hipkv.read(c.cache, b, ty, *back, KH * D)
+    for d, which in zip(back, (0, 1)):
+        want = np.stack([stored[i][which].ravel() for i in range(3)])
+        assert np.array_equal(dev.get(d, (3, KH * D), ref.np_dtype(ty)), ref.to_type(want, ty))
+    ws = hipkv.attn_ws(c.cache, b, H)
+    d_ws, d_o = dev.h.malloc(max(ws, 16)), dev.up(np.zeros((3, H * D), ref.np_dtype(ty)))
+    dev.p.append(d_ws)
+    hipkv.attn(c.cache, b, ty, d_x, n, H, d_o, H * D, D ** -0.5, window, d_ws, ws)
+    got = ref.from_type(dev.get(d_o, (3, H, D), ref.np_dtype(ty)), ty)
+    q = ref.from_type(dev.get(d_x, (3, H + 2 * KH, D), ref.np_dtype(ty)), ty)[:, :H]
+    for i, s in ((0, 0), (1, 0), (2, 1)):
+        rows = range(max(0, pos[i] % page + 1 - window), pos[i] % page + 1)
+        k, v = (np.stack(y) for y in zip(*[c.pool.load(np.repeat(c.table[s], 2), p) for p in rows]))
+        want = ref.attend(q[i], k, v, len(rows) - 1, D ** -0.5, 0)[0]
+        assert off(got[i], want) <= 2 * WHOLE[ty], i
+    assert c.errors() == 0
