@@ -272,3 +272,137 @@ def test_positions_near_the_largest(dev, ty, D, max_rows):
         want = ref.attend(q[i], k, v, len(rows) - 1, D ** -0.5, 0)[0]
         assert off(got[i], want) <= 2 * WHOLE[ty], i
     assert c.errors() == 0
+
+
+# --------------------------------------------------------------------------
+# workgroups of several rows and heads
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("layout", (hipkv.PAIRS, hipkv.HALVES))
+@pytest.mark.parametrize("ty,rows,heads,D,rot,pad", (
+    (F32, 1025, 3, 128, 128, 0), (BF16, 4099, 2, 128, 96, 8), (F16, 4099, 5, 64, 64, 0),
+    (F32, 4099, 1, 90, 50, 3), (BF16, 1030, 3, 77, 70, 1),  # value by value
+    (F32, 4099, 1, 1024, 1024, 0), (F16, 4101, 2, 1024, 912, 0), (F32, 4098, 1, 1023, 1022, 0)))
+def test_rotations_of_many_rows(dev, ty, layout, rows, heads, D, rot, pad):
+    """Up to eight rows a workgroup and a last one of fewer, whose angles take up to
+    72 KB of LDS."""
+    rng = np.random.default_rng(rows + D)
+    x = rng.standard_normal((rows, heads, D)).astype(np.float32)
+    pos = rng.integers(0, 1 << 17, rows).astype(np.int32)
+    f, mag = hipkv.rope_freqs(rot, 1e6)
+    stride = heads * D + pad
+    d_x = up_typed(dev, x.reshape(rows, -1), ty, stride)
+    d_o = up_typed(dev, np.zeros((rows + 1, heads * D), np.float32), ty, stride, fill=-3.0)
+    R = hipkv.Rope(rot, layout, dev.up(f), mag)
+    d_pos = dev.up(pos)
+    hipkv.rope(R, ty, d_x, stride, d_o, stride, rows, heads, D, d_pos)
+    got = ref.from_type(dev.get(d_o, (rows + 1, stride), ref.np_dtype(ty)), ty)
+    assert np.all(got[:, heads * D:] == -3.0) and np.all(got[rows, :heads * D] == 0)
+    want = ref.rotate(typed(x, ty), pos, f, mag, layout)
+    err = np.abs(got[:rows, :heads * D].reshape(want.shape) - want)
+    # angles to 2^17 have their last bit at 2^-36, times pairs of up to 8; f16's subnormals
+    tol = np.abs(want) * (ref.HALF_STEP[ty] + 2.0 ** -24) + 2.0 ** -33 + (2.0 ** -25 if ty == F16 else 0)
+    assert np.all(err <= tol), (err / tol).max()
+    hipkv.rope(R, ty, d_x, stride, d_x, stride, rows, heads, D, d_pos)
+    again = ref.from_type(dev.get(d_x, (rows, stride), ref.np_dtype(ty)), ty)
+    assert np.array_equal(again[:, :heads * D], got[:rows, :heads * D]) and np.all(again[:, heads * D:] == 7.0)
+
+
+def store_row(P, table, p, k, v):
+    """Pool.store of one row, all heads at once."""
+    D, KH = P.D, P.KH
+    pg, t, r = int(table[p // P.page]), p % P.page // 32, p % 32
+    tile = P.bytes[pg, :, t]
+    words, half = tile.view(np.uint32), tile[:, 32 * D:].view(np.float16)
+
+    def turned(codes, bit):
+        z = codes.astype(np.uint64) << bit.astype(np.uint64)
+        return ((z | z >> np.uint64(32)) & np.uint64(0xffffffff)).astype(np.uint32)
+
+    q, d = ref.quantize(k.reshape(KH, -1, 32))
+    w, b = P._key_words(r)
+    words[:, w[::8]] = np.bitwise_or.reduce(turned(q.reshape(KH, D), b).reshape(KH, -1, 8), -1)
+    half[:, r * (D // 32):(r + 1) * (D // 32)] = d
+    q, d = ref.quantize(v)
+    w, b = P._value_words(r)
+    words[:, w] = words[:, w] & ~turned(np.full(D, 15), b) | turned(q, b)
+    half[:, D + r] = d
+
+
+@pytest.mark.parametrize("ty,D", ((F32, 64), (F16, 64), (BF16, 128), (F32, 128), (F16, 256), (F32, 256)))
+@pytest.mark.parametrize("nseq,n,KH,H", ((22, 33, 5, 7),    # two heads a workgroup, the last one alone
+                                         (64, 20, 5, 10),   # all five
+                                         (300, 1, 5, 13),   # single rows, four heads and one
+                                         (1, 2100, 7, 3)))  # fewer query heads than kv heads
+def test_appends_of_many_rows_and_heads(dev, ty, D, nseq, n, KH, H):
+    rng = np.random.default_rng(nseq + D + ty)
+    rows = [int(i) for i in rng.integers(max(1, n // 2), n + 1, nseq)]
+    rows[0] = n
+    lens = [r + int(b) for r, b in zip(rows, rng.integers(0, 90, nseq))]
+    if nseq > 1:
+        lens[1] = rows[1] // 2  # some of its rows are not there
+    c = Case(dev, rng, rows, lens, 64, KH, D)
+    x = rng.standard_normal((c.T, H + 2 * KH, D)).astype(np.float32)
+    x[:, H:H + KH, ::11] *= 7
+    stride, e = (H + 2 * KH) * D, ref.BYTES[ty]
+    d_x = dev.up(ref.to_type(x, ty))
+    x = typed(x, ty)
+    f, mag = hipkv.rope_freqs(D // 2, 1e4)
+    hipkv.append(c.cache, c.batch, ty, d_x + H * D * e, d_x + (H + KH) * D * e, stride,
+                 rope=hipkv.Rope(D // 2, hipkv.PAIRS, dev.up(f), mag), q=d_x, q_stride=stride, heads=H,
+                 q_out=d_x, q_out_stride=stride)
+    pos, seq = c.positions(), c.sequences()
+    there = pos >= 0
+    turned = ref.rotate(x[:, :H + KH], pos, f, mag, hipkv.PAIRS)
+    got = ref.from_type(dev.get(d_x, x.shape, ref.np_dtype(ty)), ty)
+    # rows that are not there keep their queries, as k and v do
+    want = np.where(there[:, None, None], turned[:, :H], x[:, :H])
+    tol = np.abs(want) * (ref.HALF_STEP[ty] + 2.0 ** -24) + 2.0 ** -25
+    assert np.all(np.abs(got[:, :H] - want) <= tol)
+    assert np.array_equal(got[:, H:], x[:, H:])
+    for i in np.flatnonzero(there):
+        store_row(c.pool, c.table[seq[i]], pos[i], turned[i, H:].astype(np.float32), x[i, H + KH:].astype(np.float32))
+    got = c.pool_bytes()
+    assert np.array_equal(got, c.pool.bytes), np.argwhere(got != c.pool.bytes)[:5]
+    assert c.errors() == 0
+
+
+# --------------------------------------------------------------------------
+# shares of many caches
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("ty,D,KH,G,nseq,window", ((F32, 128, 8, 4, 64, 0), (BF16, 64, 16, 2, 70, 0), (F16, 256, 8, 3, 64, 70),
+                                                   (BF16, 128, 4, 16, 129, 0)))
+def test_shares_in_place_and_beside_bad_sequences(dev, ty, D, KH, G, nseq, window):
+    """Outputs over the queries; a page outside the pool, which changes its own sequence
+    alone; a length past the bound, which moves where every other sequence is cut."""
+    rng = np.random.default_rng(37)
+    H, scale = KH * G, D ** -0.5
+    lens = [int(i) for i in rng.integers(1, 200, nseq)]
+    lens[0], lens[5] = 333, 64
+    c = Case(dev, rng, [1] * nseq, lens, 32, KH, D, slack=16384 // 32)
+    c.batch.max_len = 16384
+    q = typed(rng.standard_normal((nseq, H, D)), ty)
+    want = attention(dev, c, H, ty, q, scale, window)
+    assert np.array_equal(attention(dev, c, H, ty, q, scale, window, in_place=True), want) and c.errors() == 0
+
+    def batch(table, length):
+        return hipkv.Batch(nseq, nseq, 1, 16384, c.d_start, dev.up(np.asarray(length, np.int32)), dev.up(table),
+                           table.shape[1])
+
+    table = c.table.copy()
+    table[0, 9] = c.pages  # rows 288 .. 319 of the first sequence
+    got = attention(dev, c, H, ty, q, scale, window, batch=batch(table, lens))
+    assert c.errors() == hipkv.ERR_PAGE
+    assert np.array_equal(got[1:], want[1:])
+    k, v = rows_of(c, 0, 333)
+    keep = [j for j in range(max(0, 333 - window) if window else 0, 333) if not 288 <= j < 320]
+    assert off(got[0], ref.attend(q[0], k[keep], v[keep], len(keep) - 1, scale, 0)[0]) <= 2 * WHOLE[ty]
+
+    dev.h.copy_in(c.d_err, np.zeros(1, np.uint32))
+    length = list(lens)
+    length[5] = 20000
+    got = attention(dev, c, H, ty, q, scale, window, batch=batch(c.table, length))
+    assert c.errors() == hipkv.ERR_PAGE | hipkv.ERR_BATCH  # (nor has it pages to its bound)
+    for i in (0, 1, 4, 6, 7, nseq - 2, nseq - 1):
+        assert off(got[i], want[i]) <= 2 * WHOLE[ty], i
