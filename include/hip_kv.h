@@ -128,9 +128,11 @@ size_t hip_kv_page_bytes(size_t page, size_t kv_heads, size_t head_len);
  * The rows of a call.  Sequence s has the rows row_start[s] .. row_start[s + 1]
  * - 1 of q, k, v and out, at the cache positions len[s] - n .. len[s] - 1 (n
  * its rows, len[s] its length with them).  Position p is row p % page of page
- * table[s * table_stride + p / page]; entries past the length are not read,
- * nor, in a windowed call, those before the window.  A row at a position below 0
- * is not there: nothing is stored or read for it, and its output is 0.
+ * table[s * table_stride + p / page]; entries past the length, and in a windowed
+ * call those before the window, may hold anything: they are not used, though an
+ * attention without a window reads entries up to table_stride before it knows the
+ * length.  A row at a position below 0 is not there: nothing is stored or read for
+ * it, its place in a call's k, v and q_out is left as it was, and its attention is 0.
  */
 typedef struct hip_kv_batch {
 	size_t nseq;              /* 0 .. 65535; 0: nothing to do */
