@@ -1792,7 +1792,8 @@ static int batch_errors(hip_lm_batch *B, const char *what)
 		const int zero = 0;
 		HIPCHK(hipMemcpy(&B->d_st->err, &zero, sizeof(int), hipMemcpyHostToDevice),
 		       "clear error");
-		lm_err("%s: a gather of the step kernels ran out of polls (%d)", what, err);
+		lm_err(err & LM_ERR_GATHER ? "%s: a gather of the step kernels ran out of polls (%d)"
+					   : "%s: a page or length outside the 4-bit caches (%d)", what, err);
 		return 0;
 	}
 	for (size_t l = 0; l < B->M->L; l++) {

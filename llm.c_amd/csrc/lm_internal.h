@@ -24,7 +24,7 @@ extern "C" {
 #define LM_REPORT_LAYERS 64 /* MoE layers lm_launch_report looks at */
 #define LM_REPORT_WORDS 4   /* words before the sequences' picks */
 
-#define LM_ERR_GATHER 1    /* a gather's poll ran out */
+#define LM_ERR_GATHER 4    /* a gather's poll ran out (the bits below: HIP_KV_ERR_*) */
 
 /* The step's counters in device memory, read by every step kernel so that
  * one captured graph serves every step.  The host writes the first four
@@ -36,7 +36,7 @@ typedef struct LmState {
 	int size;     /* KV cache rows in use (kvcache.h:14) */
 	int tok;      /* the last greedy pick */
 	int epoch;    /* steps since upload, never reset: the gathers' tags */
-	int err;      /* LM_ERR_* set by a kernel, 0 if none */
+	int err;      /* LM_ERR_* or HIP_KV_ERR_* set by a kernel, 0 if none */
 	int pad;
 } LmState;
 

@@ -21,6 +21,11 @@ static size_t fail_host;    /* and the next ones of host memory, if not 0 */
 static size_t host_allocs;
 static char log_buf[1 << 20], sizes_buf[1 << 20];
 static struct {
+	size_t n;
+	void *p;
+} taken[1 << 16]; /* the last device allocations */
+static size_t ntaken;
+static struct {
 	const void *host;
 	const char *name;
 } fns[4096];
@@ -46,6 +51,16 @@ const char *fake_sizes(void)
 size_t fake_host_allocs(void)
 {
 	return host_allocs;
+}
+
+/* the last device allocation of n bytes, if it is among the last */
+void *fake_last_of(size_t n)
+{
+	const size_t cap = sizeof(taken) / sizeof(taken[0]);
+	for (size_t i = 0; i < cap && i < ntaken; i++)
+		if (taken[(ntaken - 1 - i) % cap].n == n)
+			return taken[(ntaken - 1 - i) % cap].p;
+	return NULL;
 }
 
 void fake_fail_size(size_t n)
@@ -90,6 +105,8 @@ int hipMalloc(void **p, size_t n)
 	snprintf(s, sizeof(s), "%zu", n);
 	note(sizes_buf, sizeof(sizes_buf), s);
 	*p = take(n);
+	taken[ntaken % (sizeof(taken) / sizeof(taken[0]))].n = n;
+	taken[ntaken++ % (sizeof(taken) / sizeof(taken[0]))].p = *p;
 	return *p ? 0 : (last_error = OOM);
 }
 
