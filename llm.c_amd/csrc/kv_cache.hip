@@ -8,8 +8,8 @@
 
 /*
  * cos and sin, times mag, of the angle pos * freq in 64 bits.  The quarter turns n
- * nearest to the angle go off it in three steps, pi / 2 as a sum of three doubles,
- * each step one rounding; what is left, up to pi / 4 in size, goes through the Taylor
+ * nearest to the angle go off it in three steps, pi / 2 as a sum of three doubles
+ * (Cody and Waite's reduction), each step one rounding; what is left, up to pi / 4 in size, goes through the Taylor
  * series of both functions, whose first terms left out are below 2^-54 of 1; n mod 4
  * says which is which.  Within 2^-52 of the functions' values, at a fifth of the
  * instructions of a function for any argument (which takes the angles past 2^31).

@@ -807,7 +807,6 @@ void k_lm_head(const uint8_t *__restrict__ W, size_t rb, int N, int K, const flo
 	}
 }
 
-/* the step's counters advance (a step without the lm_head) */
 /* the lengths of caches in 4 bits: the step's rows and `add` more (st NULL: add) */
 __global__ void k_lm_kv_len(int32_t *len, int n, const LmState *st, int add)
 {
@@ -816,6 +815,7 @@ __global__ void k_lm_kv_len(int32_t *len, int n, const LmState *st, int add)
 		len[i] = v;
 }
 
+/* the step's counters advance (a step without the lm_head) */
 __global__ void k_lm_step_end(LmState *st)
 {
 	if (threadIdx.x == 0) {
