@@ -589,10 +589,12 @@ __device__ static inline int kv_share(int all, int n)
  * 87 us with the merge, 3.9 TB/s; in pieces 97.5, without slots and at three waves a
  * SIMD 118.  64 of 8190 rows: 125 us, 4.6 TB/s.
  */
-/* by the registers: four waves a SIMD with slots, three without, two for heads of
- * 256.  Nothing is kept in accumulation registers and moved. */
+/* by the registers: four waves a SIMD with slots, which is two workgroups of KV_MANY a
+ * CU (64 sequences x 2300 rows, 32 fp32 heads on 8: 37.9 us; with two registers too many
+ * for that 41.9), three without, two for heads of 256.  Nothing is kept in accumulation
+ * registers and moved. */
 template <int D, int TY, int NW, int SLOTS, bool SHARE>
-__global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(D == 256 ? 2 : SLOTS > 1 && NW == KV_WAVES ? 4 : 3)))
+__global__ __launch_bounds__(NW * WAVE) __attribute__((amdgpu_waves_per_eu(D == 256 ? 2 : SLOTS > 1 ? 4 : 3)))
 void k_kv_attn(
 	kv_args a, const typename kv_type<TY>::t *q, size_t q_stride, int G,
 	typename kv_type<TY>::t *out, size_t out_stride, float scale, int window, float *ws,
@@ -1032,8 +1034,10 @@ template <int D> struct kv_values32 {
 	}
 };
 
+/* (heads of 64 in fp32 fit four waves a SIMD: 4096 rows of 32 heads on 8 201 us; with
+ * one register too many for that 209) */
 template <int D, int TY>
-__global__ __launch_bounds__(KV_NT) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(KV_NT) __attribute__((amdgpu_waves_per_eu(D == 64 && TY == HIP_KV_F32 ? 4 : 2)))
 void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride, int G,
 		    typename kv_type<TY>::t *out, size_t out_stride, float scale, int window, int row_tiles)
 {
