@@ -32,8 +32,14 @@
 extern "C" {
 #endif
 
-/* Types of q, k, v and outputs.  Sums, softmax statistics and products are
- * at fp32 accuracy for HIP_KV_F32. */
+/*
+ * Types of q, k, v and outputs.  Sums and softmax statistics are fp32 for all of them.
+ * What the attention multiplies is held in f16 parts: a query's value to 2^-22 of itself
+ * (exactly in the 16-bit types) and 2^-38 (2^-34) of its head's largest, a probability
+ * times its row's value scale to 2^-22 of itself (HIP_KV_BF16: 2^-11) and 2^-25 (16-bit
+ * types: 2^-21) of the largest.  Whole outputs are 3e-7 to 5e-7 off in fp32, as far as
+ * fp32 products and sums are, and by their own rounding in 16 bits.
+ */
 #define HIP_KV_F32 0
 #define HIP_KV_F16 1
 #define HIP_KV_BF16 2

@@ -23,8 +23,10 @@
  * well, since over many cached rows a surplus would outweigh the sum.  A query row is
  * scaled by a power of two and, from fp32, split into two f16 parts of together 22
  * bits; f16 and bf16 queries are exact in one.  The probability times the value scale
- * is scaled by a power of two that keeps it within f16, and split in two as well (in
- * one part, 11 bits, for bf16 outputs of 8).  Sums, maxima and exponents are fp32.
+ * is scaled by a power of two that keeps it within f16, and split in two as well.  For
+ * bf16 outputs one part is enough: it is rounded by 2^-11 at most, with no bias (the
+ * denominator sums what was not rounded), where the output is rounded by up to 2^-8.
+ * Sums, maxima and exponents are fp32.
  *
  * Three forms, chosen by kv_attn_plan: few rows in slots of columns and up to 16 rows
  * (k_kv_attn; HBM bounds long caches, latency short ones), and tiles of 32 rows for
@@ -586,8 +588,8 @@ __device__ static inline int kv_share(int all, int n)
  *
  * 131072 rows, 32 bf16 heads on 8 of 128 (145 MB): 31.8 us and the merge 4.2, 4.1 TB/s
  * in all; without slots 34.9.  64 sequences of 340 to 16384 rows in fp32 (341 MB):
- * 87 us with the merge, 3.9 TB/s; in pieces 97.5, without slots and at three waves a
- * SIMD 118.  64 of 8190 rows: 125 us, 4.6 TB/s.
+ * 88 us with the merge, 3.9 TB/s; in pieces 97.5, without slots and at three waves a
+ * SIMD 118.
  */
 /* by the registers: four waves a SIMD with slots, which is two workgroups of KV_MANY a
  * CU (64 sequences x 2300 rows, 32 fp32 heads on 8: 37.9 us; with two registers too many
@@ -962,10 +964,10 @@ __global__ __launch_bounds__(KV_NT) void k_kv_merge(kv_args a, int G, typename k
  * them, and the row tiles that see most come first: even the last workgroups are
  * short.
  *
- * 8192 bf16 rows of 32 heads on 8 of 128: 900 to 920 us, 600 TFLOP/s of the formula's
- * operations (in tiles of 16 rows 1.5 ms); about 400 VALU and 19 matrix instructions of 32
- * cycles for 32 x 32 scores.  2048 fp32 rows of 16 heads on as many cached: 54 us (in
- * two parts, 620 TFLOP/s).  Waves with 32 rows each that share a tile's f16 codes
+ * 8192 bf16 rows of 32 heads on 8 of 128: 905 to 945 us, 600 TFLOP/s of the formula's
+ * operations (in tiles of 16 rows 1.5 ms); 347 instructions on the vector unit's side for
+ * 32 x 32 scores, 19 of them matrix instructions of 32 cycles.  2048 fp32 rows of 16 heads
+ * on as many cached: 54.6 us (in two parts, 620 TFLOP/s).  Waves with 32 rows each that share a tile's f16 codes
  * through LDS took 8 to 12 % longer: the barrier a tile keeps matrix and VALU work of
  * the two waves of a SIMD from overlapping.
  */
@@ -1133,7 +1135,8 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 	/* For bf16 outputs the values' surplus of 8 leaves at the end, as 8 times the
 	 * sum of the (rounded) probabilities times scales: it outweighs the output by
 	 * up to 3 times the root of the rows that matter, which fp32 sums have to
-	 * spare over bf16's 8 bits. */
+	 * spare over bf16's 8 bits: over 131072 rows whose scales have one sign and
+	 * whose values cancel, outputs are 1.7e-3 off, by their rounding. */
 	constexpr bool LATE = TY == HIP_KV_BF16;
 	floatx16 o[CT], late = (floatx16)0.0f;
 #pragma unroll
@@ -1268,9 +1271,10 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
  * Along the cache.  A workgroup of KV_MANY waves takes a row tile's whole cache where
  * that beats pieces, which need a second launch to add them up: up to 32 tiles, 72
  * where there are 128 workgroups and 128 where there are 512, which fill the chip by
- * themselves (32 heads on 8 of 128 in fp32: 1 sequence x 1024 rows 10.2 us either way,
- * x 2048 15.0 whole and 10.0 in pieces; 16 x 2300 rows 15.1 and 15.6; 64 x 2300 rows
- * 30.7 and 39.8, 64 x 4000 rows 53 and 60).  Other caches are cut into pieces for
+ * themselves.  32 heads on 8 of 128 in fp32, whole and in pieces: 1 sequence x 2048 rows
+ * 15.1 and 11.2 us; 8 x 1100 rows 11.0 and 11.4, 16 x 11.3 and 13.8, 32 x 11.9 and 17.7;
+ * 8 x 2300 rows 17.8 and 13.8, 16 x 17.9 and 17.4, 32 x 18.6 and 24.5, 64 x 37.9 and 48;
+ * 32 x 4000 rows 33.5 and 36.6, 48 x 60.6 and 54.7, 64 x 58.5 and 66.8.  Other caches are cut into pieces for
  * workgroups of four waves, as many as the chip holds twice over for heads of 64 and
  * 128 (131072 rows: 64 pieces a kv head 35.4 us, 128 pieces 36.3), and of several
  * sequences into pieces of at most KV_CHUNK tiles, so that different lengths fill the
@@ -1279,10 +1283,13 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
  *
  * Of many sequences, where the longest that may come would be 4096 pieces in all and
  * more, most of which find nothing to do (launching one costs its XCD 90 cycles), the
- * caches are one line in equal shares, as many as the chip holds: the same 64 87 us
- * instead of 97.5, 64 of 8190 rows 125 instead of 133.  Finding a share's sequences
- * costs 2 us a launch: 16 sequences on 8 kv heads 30.3 instead of 29.1 us, one of 131072
- * rows 39.5 instead of 35.4.
+ * caches are one line in equal shares, as many as the chip holds: the same 64 88 us
+ * instead of 97.5, 96 110 instead of 130, 64 of 8190 rows each (bf16) 115.5 instead of
+ * 118.6.  Finding a share's sequences costs 2 us a launch, so that fewer lose where their
+ * lengths are equal (8190 rows: 48 93 instead of 91, 32 64.5 instead of 62.7, 16 38.8
+ * instead of 34.6; one of 131072 rows 39.5 instead of 35.4), though 32 and 48 of 340 to
+ * 16384 rows would gain (50 instead of 55, 67 instead of 76): they begin at 512 workgroups,
+ * where both gain.
  */
 #define KV_CHUNK 32
 #define KV_MANY 8

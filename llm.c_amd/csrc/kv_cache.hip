@@ -292,10 +292,12 @@ template <int LANES, int N> __device__ static inline _Float16 kv_encode(const fl
  * go to LDS: the words are put together from there, and a word that has other rows'
  * codes too is read first and keeps them.
  *
- * 8192 fp32 rows of 8 kv and 32 q heads of 128 (344 MB) take 86 us, 4.0 TB/s: HBM.
- * 7500 bf16 rows of 16 and 16 heads (154 MB) take 59: half of the issue slots hold VALU
- * work (about 40 instructions for a key or value, 16 for a query's), the rest waits for
- * loads.  With 32 rows and two heads a workgroup: 88 and 62.5 us.
+ * 8192 fp32 rows of 8 kv and 32 q heads of 128 (345 MB) take 86 us, 4.0 TB/s: HBM.
+ * 7971 bf16 rows of 16 and 16 heads in five sequences (148 MB, 29 us of a large copy)
+ * take 59: VALU work, about 40 instructions for a key or value and 16 for a query's, of
+ * which full issue would take 35 us, beside waits for loads, of which a workgroup's first
+ * are behind its sequence's length and page.  With 32 rows and two heads a workgroup: 88
+ * and 62.5 us.
  */
 #define KV_APPEND_NT 512
 #define KV_PART 8 /* rows of a workgroup, at most */

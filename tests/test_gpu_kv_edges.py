@@ -20,9 +20,9 @@ pytestmark = pytest.mark.gpu
 
 # fp32, logits in powers of two within 16 of the reference 2^9 below the largest: a
 # logit's last sum is rounded by up to 2^-21, rms 2^-21 / sqrt(3), times ln 2: 1.9e-7 of a
-# probability; a probability in 22 bits, 2^-23 / sqrt(3) = 0.7e-7; a query's 22 bits, as
-# much of a logit of 1 or 2; exponentials, the sums of 16 or 32 tiles a wave and the
-# quotient about 1e-7 together: 2.5e-7, all of them independent from row to row.  Four
+# probability; a probability in two f16 parts by up to 2^-22, rms 1.4e-7; a query's values
+# by as much, of a logit of 1 or 2; exponentials, the sums of 16 or 32 tiles a wave and
+# the quotient about 1e-7 together: 3.2e-7, all of them independent from row to row.  Three
 # times that; codes as subnormals would be 3e-6.
 FP32 = 1e-6
 WHOLE = {F32: FP32, F16: ref.HALF_STEP[F16], BF16: ref.HALF_STEP[BF16]}
