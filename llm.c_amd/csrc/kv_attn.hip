@@ -1366,8 +1366,12 @@ extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const vo
 			      int window, void *ws, const kv_plan *p, void *stream)
 {
 	const int G = heads / a->kv_heads;
-	const dim3 grid((unsigned)(a->kv_heads * p->row_tiles), (unsigned)p->splits, (unsigned)a->nseq);
-	const dim3 rows((unsigned)(a->kv_heads * a->max_rows * G), (unsigned)a->nseq);
+	const size_t tiles = (size_t)a->kv_heads * p->row_tiles, all = (size_t)heads * a->max_rows;
+	const bool merge = !p->wide && (p->splits > 1 || p->shares);
+	if (!kv_launchable(tiles, KV_MANY * WAVE) || (merge && !kv_launchable(all, KV_NT)))
+		return (int)hipErrorInvalidConfiguration;
+	const dim3 grid((unsigned)tiles, (unsigned)p->splits, (unsigned)a->nseq);
+	const dim3 rows((unsigned)all, (unsigned)a->nseq);
 	KV_DISPATCH_HEAD(head_len, D, KV_DISPATCH_TYPE(type, TY, {
 		typedef kv_type<TY>::t t;
 		constexpr int WIDE = D < 256 ? D : 128; /* heads of 256 have no registers for it */
@@ -1393,7 +1397,7 @@ extern "C" int kv_launch_attn(const kv_args *a, int head_len, int type, const vo
 		else
 			launch(p->slots == 4 ? k_kv_attn<D, TY, KV_WAVES, FOUR, false> :
 			       p->slots == 2 ? k_kv_attn<D, TY, KV_WAVES, 2, false> : k_kv_attn<D, TY, KV_WAVES, 1, false>, KV_WAVES);
-		if (p->splits > 1 || p->shares)
+		if (merge)
 			k_kv_merge<D, TY><<<rows, KV_NT, 0, (hipStream_t)stream>>>(
 				*a, G, (t *)out, out_stride, window, (const float *)ws, p->row_tiles,
 				p->chunk, p->splits, p->rows, p->shares);

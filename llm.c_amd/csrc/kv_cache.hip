@@ -541,6 +541,8 @@ extern "C" int kv_launch_rope(int type, const void *x, size_t x_stride, void *ou
 		per /= 2;
 	while (heads_per > 4 && rows * ((heads + heads_per - 1) / heads_per) < 512)
 		heads_per = (heads_per + 1) / 2;
+	if (!kv_launchable((rows + per - 1) / per, KV_NT))
+		return (int)hipErrorInvalidConfiguration;
 	const dim3 grid((unsigned)((rows + per - 1) / per), (unsigned)((heads + heads_per - 1) / heads_per));
 	const size_t lds = per * kv_slot((int)R->rot / 2) * sizeof(double2);
 	KV_DISPATCH_TYPE(type, TY, {
@@ -577,6 +579,8 @@ extern "C" int kv_launch_append(const kv_args *a, int head_len, int type, const 
 		per *= 2;
 	per = per < a->kv_heads ? per : a->kv_heads;
 	const size_t grid = (size_t)a->nseq * tiles * parts * ((a->kv_heads + per - 1) / per);
+	if (!kv_launchable(grid, KV_APPEND_NT))
+		return (int)hipErrorInvalidConfiguration;
 	const size_t lds = (size_t)most * ((R ? kv_slot((int)R->rot / 2) * sizeof(double2) : 0) + (size_t)per * head_len);
 	KV_DISPATCH_HEAD(head_len, D, KV_DISPATCH_TYPE(type, TY, {
 		typedef kv_type<TY>::t t;
@@ -592,6 +596,8 @@ extern "C" int kv_launch_read(const kv_args *a, int head_len, int type, void *k,
 {
 	const int tiles = kv_tiles_of(a->max_rows);
 	const size_t grid = (size_t)a->nseq * tiles * a->kv_heads;
+	if (!kv_launchable(grid, KV_NT))
+		return (int)hipErrorInvalidConfiguration;
 	KV_DISPATCH_HEAD(head_len, D, KV_DISPATCH_TYPE(type, TY, {
 		typedef kv_type<TY>::t t;
 		k_kv_read<D, TY><<<dim3((unsigned)grid), KV_NT, 0, (hipStream_t)stream>>>(

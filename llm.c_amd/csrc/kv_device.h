@@ -137,6 +137,12 @@ __device__ static inline uint8_t *kv_tile_at(const kv_args &a, int s, int h, int
 	return a.pool + tile * kv_tile<D>::BYTES;
 }
 
+/* whether a launch has as many workgroups along x: below 2^32 threads */
+static inline bool kv_launchable(size_t workgroups, int threads)
+{
+	return workgroups <= 0xffffffffu / (unsigned)threads;
+}
+
 #define KV_DISPATCH_TYPE(ty, TY, ...)                                             \
 	switch (ty) {                                                             \
 	case HIP_KV_F32: { constexpr int TY = HIP_KV_F32; __VA_ARGS__; break; }   \
