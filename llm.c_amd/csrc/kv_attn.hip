@@ -697,7 +697,7 @@ void k_kv_attn(
 			k.load(tile, lane);
 			vd.load(tile + L::V_SCALES, lane);
 			v.load(tile, lane);
-		} else if (!a.pages && lane == 0) {
+		} else if (!a.pages && t1 > t0 && lane == 0) {
 			kv_error(a, HIP_KV_ERR_PAGE);
 		}
 		const float rs = kv_put_query<D, QP, SLOTS, TY>(sh.q, qv, scale, lane, wave, NW);
@@ -1129,7 +1129,7 @@ void k_kv_attn_wide(kv_args a, const typename kv_type<TY>::t *q, size_t q_stride
 		const uint8_t *tile = tile_of(0);
 		k.load(tile, lane);
 		v.load(tile, lane);
-	} else if (!a.pages && lane == 0) {
+	} else if (!a.pages && t1 > t0 && lane == 0) {
 		kv_error(a, HIP_KV_ERR_PAGE);
 	}
 	/* For bf16 outputs the values' surplus of 8 leaves at the end, as 8 times the

@@ -406,3 +406,21 @@ def test_shares_in_place_and_beside_bad_sequences(dev, ty, D, KH, G, nseq, windo
     assert c.errors() == hipkv.ERR_PAGE | hipkv.ERR_BATCH  # (nor has it pages to its bound)
     for i in (0, 1, 4, 6, 7, nseq - 2, nseq - 1):
         assert off(got[i], want[i]) <= 2 * WHOLE[ty], i
+
+
+@pytest.mark.parametrize("H,n", ((2, 1), (16, 300)))
+def test_a_pool_without_pages(dev, H, n):
+    """Rows that see nothing report nothing; those that would are NaN and reported."""
+    rng = np.random.default_rng(38)
+    D, KH = 64, 2
+    c = Case(dev, rng, [n] * 9, [0] * 9, 32, KH, D)
+    c.cache.pages = 0
+    q = typed(rng.standard_normal((c.T, H, D)), F32)
+    c.batch.max_len = 2000
+    c.batch.table, c.batch.table_stride = dev.up(np.zeros((9, 63), np.int32)), 63
+    assert np.all(attention(dev, c, H, F32, q, 0.1) == 0) and c.errors() == 0
+    c.batch.len = dev.up(np.full(9, 40, np.int32))
+    got = attention(dev, c, H, F32, q, 0.1).reshape(9, n, -1)
+    there = np.arange(n) >= n - 40
+    assert np.all(np.isnan(got[:, there])) and np.all(got[:, ~there] == 0)
+    assert c.errors() == hipkv.ERR_PAGE
