@@ -35,13 +35,14 @@ typedef struct f8_mul_args {
 
 /* how a product is cut up, from the host's bounds alone */
 typedef struct f8_plan {
-	int bt, bn;      /* rows of X and of W of one workgroup's tile */
+	int type, big;
+	int bt, bn;      /* rows of X and outputs of a row of one workgroup's tile */
 	size_t row_tiles; /* tiles of rows, at most, over all experts */
 	size_t n_tiles;
 	int threads;
 } f8_plan;
 void f8_mul_plan(const f8_mul_args *a, f8_plan *p);
-int f8_launch_mul(const f8_mul_args *a, const f8_plan *p, int type, void *stream);
+int f8_launch_mul(const f8_mul_args *a, const f8_plan *p, void *stream);
 
 size_t f8_quantize_grid(size_t rows, size_t k);
 int f8_launch_quantize(int type, const void *x, size_t x_stride, const hip_f8_rows *X, void *stream);

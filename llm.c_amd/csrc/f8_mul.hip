@@ -126,150 +126,259 @@ __device__ static inline float f8_gate(float a, float b)
 	return a / (1.0f + expf(-a)) * b;
 }
 
-/* Four neighbouring outputs of a row, from n on */
-template <int TY>
-__device__ static inline void f8_store(const f8_mul_args &A, int row, int n, floatx4 y)
+/* N neighbouring outputs of a row, from n on */
+template <int TY, int N>
+__device__ static inline void f8_store(const f8_mul_args &A, int row, int n, float *y)
 {
 	typedef kv_type<TY> T;
-	typedef kv_vec<TY, 4> vec;
+	constexpr int PER = 16 / sizeof(typename T::t) < N ? 16 / sizeof(typename T::t) : N;
+	typedef kv_vec<TY, PER> vec;
 	typename T::t *o = (typename T::t *)A.out + row * A.out_stride + n;
-	if (A.add) {
-		const typename T::t *p = (const typename T::t *)A.add + row * A.add_stride + n;
+	const typename T::t *p = (const typename T::t *)A.add + row * A.add_stride + n;
 #pragma unroll
-		for (int u = 0; u < 4; u++)
-			if (n + u < A.n)
-				y[u] += T::get(p[u]);
-	}
-	if (n + 4 <= A.n) {
-		vec v;
+	for (int v0 = 0; v0 < N; v0 += PER) {
+		if (n + v0 + PER <= A.n) {
+			if (A.add) {
+				const vec v = *(const vec *)(p + v0);
 #pragma unroll
-		for (int u = 0; u < 4; u++)
-			v.v[u] = T::put(y[u]);
-		*(vec *)o = v;
-	} else {
+				for (int u = 0; u < PER; u++)
+					y[v0 + u] += T::get(v.v[u]);
+			}
+			vec v;
 #pragma unroll
-		for (int u = 0; u < 4; u++)
-			if (n + u < A.n)
-				o[u] = T::put(y[u]);
+			for (int u = 0; u < PER; u++)
+				v.v[u] = T::put(y[v0 + u]);
+			*(vec *)(o + v0) = v;
+		} else {
+#pragma unroll
+			for (int u = 0; u < PER; u++)
+				if (n + v0 + u < A.n)
+					o[v0 + u] = T::put(A.add ? y[v0 + u] + T::get(p[v0 + u]) : y[v0 + u]);
+		}
 	}
 }
 
-/* Tiles of 64 rows of X and 64 of W, a wave 16 of these. */
-#define BT 64
-#define BN 64
-#define MUL_THREADS 256
-
-template <int TY, bool GATED>
-__global__ __launch_bounds__(MUL_THREADS) void k_f8_mul(f8_mul_args A, int n_tiles)
+/* 16 bytes a lane from its address to lds + 16 * lane, in flight until a wait that
+ * the caller makes (moe_device.h's dma_dwordx4 with whole addresses) */
+__device__ static inline void f8_dma16(const uint8_t *p, u32 lds)
 {
-	constexpr int M = GATED ? 2 : 1;
+	asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+		     :
+		     : "v"(p), "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+		     : "memory");
+}
+
+/* the same, 4 bytes a lane */
+__device__ static inline void f8_dma4(const float *p, u32 lds)
+{
+	asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off"
+		     :
+		     : "v"(p), "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+		     : "memory");
+}
+
+/* All waves have come here, their LDS reads are done, and of each one's loads
+ * all but the last N have arrived */
+template <int N>
+__device__ static inline void f8_meet()
+{
+	static_assert(N >= 0 && N < 64, "vmcnt is six bits");
+	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+/*
+ * Tiles of 16 NB WT rows of X and 16 NA WN rows of W (gated: half of them W's, half
+ * up's), a wave 16 NB by 16 NA of them.  A step is a block of 128 channels, all rows'
+ * 128 bytes and X's scales in one of STAGES buffers, filled by loads that go past the
+ * registers, STAGES - 1 steps ahead.
+ *
+ * A row's 128 bytes are eight pieces of 16; piece p lies at place p ^ (row % 8), so
+ * that the 16 rows whose same piece an operand's read takes meet no bank twice.  Row
+ * i of an operand's 16 is the output that gives a lane its 4 NA neighbouring ones.
+ */
+template <int TY, bool GATED, int NA, int NB, int WN, int WT, int STAGES>
+__global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_tiles, int row_tiles)
+{
+	constexpr int M = GATED ? 2 : 1, FA = NA / M; /* operands of one matrix */
+	constexpr int BN = 16 * NA * WN, BT = 16 * NB * WT, NO = BN / M;
+	constexpr int NW = WN * WT, SLOTS = (BN + BT) / 8 / NW, SCALES = BT < 64 ? 64 : BT;
+	constexpr int BYTES = (BN + BT) * HIP_F8_BLOCK + SCALES * 4;
+	static_assert((BN + BT) / 8 % NW == 0 && HIP_F8_BLOCK % (16 * FA) == 0, "whole loads, one scale");
 	typedef f8_operand<TY == HIP_F8_F32> operand;
-	const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-	const int tile = blockIdx.x / n_tiles, n0 = blockIdx.x % n_tiles * BN + wave * 16;
-	const f8_rows_of R = f8_find<BT>(A, tile);
-	if (R.a >= R.b || n0 >= A.n)
+	__shared__ __attribute__((aligned(16))) uint8_t lds[STAGES * BYTES];
+
+	const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+	const int wn = wave % WN, wt = wave / WN;
+	/* Workgroups go to the eight XCDs in turn: each takes a stretch of the tiles, in
+	 * groups of 8 row tiles that share what the L2 holds of W. */
+	const int grid = n_tiles * row_tiles, xcd = blockIdx.x % 8;
+	const int id = xcd * (grid / 8) + (xcd < grid % 8 ? xcd : grid % 8) + blockIdx.x / 8;
+	const int group = id / (8 * n_tiles), g0 = group * 8;
+	const int many = row_tiles - g0 < 8 ? row_tiles - g0 : 8;
+	const int in = id - group * 8 * n_tiles;
+	const int tile = g0 + in % many, n0 = in / many * NO;
+
+	f8_rows_of R = f8_find<BT>(A, tile);
+	R.e = __builtin_amdgcn_readfirstlane(R.e);
+	R.a = __builtin_amdgcn_readfirstlane(R.a);
+	R.b = __builtin_amdgcn_readfirstlane(R.b);
+	if (R.a >= R.b)
 		return;
-	const int at = lane / 16 * 16; /* of a block's halves of 64 channels */
-	long src[BT / 16];
-	bool bad[BT / 16];
+
+	/* what this wave loads: slots of eight rows */
+	const int piece = ((lane % 8) ^ (lane / 8)) * 16, last = (A.k - 1) & ~15;
+	const uint8_t *p[SLOTS];
 #pragma unroll
-	for (int f = 0; f < BT / 16; f++) {
-		const int r = R.a + f * 16 + lane % 16;
-		int x = r < R.b ? r : R.b - 1;
-		x = A.from ? A.from[x] : x;
-		bad[f] = (unsigned)x >= (unsigned)A.x_rows;
-		src[f] = bad[f] ? 0 : x;
-	}
-	const int wr = n0 + lane % 16 < A.n ? n0 + lane % 16 : A.n - 1;
-	floatx4 acc[M][BT / 16] = {};
-	const int blocks = (A.k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
-	for (int kb = 0; kb < blocks; kb++) {
-		const int c = kb * HIP_F8_BLOCK + at;
-		const bool part = (kb + 1) * HIP_F8_BLOCK > A.k;
-		/* channels past the last 16 of a row that hold any are not read */
-		const int last = (A.k - 1) & ~15;
-		const int c0 = c < last ? c : last, c1 = c + 64 < last ? c + 64 : last;
-		operand w[M];
-		float sw[M];
-#pragma unroll
-		for (int m = 0; m < M; m++) {
-			const uint8_t *p = A.w[m] + R.e * A.w_step[m] + wr * A.w_stride[m];
-			i32x4 lo = *(const i32x4 *)(p + c0), hi = *(const i32x4 *)(p + c1);
-			if (part) {
-				lo = f8_masked(lo, c, A.k);
-				hi = f8_masked(hi, c + 64, A.k);
-			}
-			w[m].set(lo, hi);
-			sw[m] = A.ws[m][R.e * A.ws_step[m] + n0 / HIP_F8_BLOCK * A.ws_stride[m] + kb];
+	for (int i = 0; i < SLOTS; i++) {
+		const int s = wave + i * NW, row = s * 8 + lane / 8;
+		if (row < BN) {
+			const int j = row % (16 * NA), m = j / (16 * FA), f = j / 16 % FA, r = j % 16;
+			int n = n0 + row / (16 * NA) * (16 * FA) + r / 4 * (4 * FA) + f * 4 + r % 4;
+			n = n < A.n ? n : A.n - 1;
+			p[i] = (m ? A.w[M - 1] + R.e * A.w_step[M - 1] + n * A.w_stride[M - 1]
+				  : A.w[0] + R.e * A.w_step[0] + n * A.w_stride[0]);
+		} else {
+			int x = R.a + row - BN;
+			x = x < R.b ? x : R.b - 1;
+			x = A.from ? A.from[x] : x;
+			x = (unsigned)x < (unsigned)A.x_rows ? x : 0;
+			p[i] = A.x + x * A.x_stride;
 		}
+	}
+	const float *ps;
+	const int sslot = wave % (SCALES / 64);
+	{
+		int x = R.a + sslot * 64 + lane;
+		x = x < R.b ? x : R.b - 1;
+		x = A.from ? A.from[x] : x;
+		ps = A.xs + ((unsigned)x < (unsigned)A.x_rows ? x : 0);
+	}
+	const int blocks = (A.k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
+	const u32 base = lds_addr(lds);
+	auto load = [&](int kb, int stage) {
+		int c = kb * HIP_F8_BLOCK + piece;
+		c = c < last ? c : last; /* nothing past the row's last 16 that hold any is read */
+		const u32 to = base + stage * BYTES;
 #pragma unroll
-		for (int f = 0; f < BT / 16; f++) {
-			const uint8_t *p = A.x + src[f] * A.x_stride;
-			i32x4 lo = *(const i32x4 *)(p + c0), hi = *(const i32x4 *)(p + c1);
-			if (part) {
-				lo = f8_masked(lo, c, A.k);
-				hi = f8_masked(hi, c + 64, A.k);
+		for (int i = 0; i < SLOTS; i++)
+			f8_dma16(p[i] + c, to + (wave + i * NW) * 1024);
+		f8_dma4(ps + kb * A.xs_stride, to + (BN + BT) * HIP_F8_BLOCK + sslot * 256);
+	};
+	const float *sw[M];
+#pragma unroll
+	for (int m = 0; m < M; m++) {
+		const int n = n0 + wn * 16 * FA < A.n ? n0 + wn * 16 * FA : A.n - 1;
+		sw[m] = A.ws[m] + R.e * A.ws_step[m] + n / HIP_F8_BLOCK * A.ws_stride[m];
+	}
+
+	floatx4 acc[NA][NB] = {};
+#pragma unroll
+	for (int s = 0; s < STAGES - 1; s++)
+		load(s < blocks ? s : blocks - 1, s);
+	int stage = 0;
+	const int place = ((lane / 16) ^ (lane % 8)) * 16;
+	for (int kb = 0; kb < blocks; kb++) {
+		f8_meet<(STAGES - 2) * (SLOTS + 1)>();
+		const int ahead = kb + STAGES - 1;
+		load(ahead < blocks ? ahead : blocks - 1, stage == 0 ? STAGES - 1 : stage - 1);
+		uint8_t *buf = lds + stage * BYTES;
+		if ((kb + 1) * HIP_F8_BLOCK > A.k) { /* the last block's rest: zeros */
+			for (int i = threadIdx.x; i < (BN + BT) * 8; i += 64 * NW) {
+				const int c = kb * HIP_F8_BLOCK + ((i % 8) ^ (i / 8 % 8)) * 16;
+				i32x4 *q = (i32x4 *)(buf + i * 16);
+				if (c + 16 > A.k)
+					*q = f8_masked(*q, c, A.k);
 			}
-			operand x;
-			x.set(lo, hi);
-			const float sx = A.xs[kb * A.xs_stride + src[f]];
+			f8_meet<63>();
+		}
+		const float *sx = (const float *)(buf + (BN + BT) * HIP_F8_BLOCK) + wt * 16 * NB + lane % 16;
+		float s[M][NB];
 #pragma unroll
-			for (int m = 0; m < M; m++) {
-				const floatx4 y = operand::mul(w[m], x);
-				const float s = sx * sw[m];
+		for (int b = 0; b < NB; b++)
+#pragma unroll
+			for (int m = 0; m < M; m++)
+				s[m][b] = sx[b * 16] * sw[m][kb];
+		operand x[NB];
+		const uint8_t *xb = buf + (BN + wt * 16 * NB + lane % 16) * HIP_F8_BLOCK;
+#pragma unroll
+		for (int b = 0; b < NB; b++)
+			x[b].set(*(const i32x4 *)(xb + b * 2048 + place), *(const i32x4 *)(xb + b * 2048 + (place ^ 64)));
+		const uint8_t *wb = buf + (wn * 16 * NA + lane % 16) * HIP_F8_BLOCK;
+#pragma unroll
+		for (int a = 0; a < NA; a++) {
+			operand w;
+			w.set(*(const i32x4 *)(wb + a * 2048 + place), *(const i32x4 *)(wb + a * 2048 + (place ^ 64)));
+#pragma unroll
+			for (int b = 0; b < NB; b++) {
+				const floatx4 y = operand::mul(w, x[b]);
 #pragma unroll
 				for (int u = 0; u < 4; u++)
-					acc[m][f][u] = __builtin_fmaf(y[u], s, acc[m][f][u]);
+					acc[a][b][u] = __builtin_fmaf(y[u], s[a / FA][b], acc[a][b][u]);
 			}
 		}
+		stage = stage + 1 == STAGES ? 0 : stage + 1;
 	}
+	f8_meet<0>(); /* no load outlives the workgroup's LDS */
+	const int n = n0 + wn * 16 * FA + lane / 16 * (4 * FA);
 #pragma unroll
-	for (int f = 0; f < BT / 16; f++) {
-		const int r = R.a + f * 16 + lane % 16;
-		if (r >= R.b)
+	for (int b = 0; b < NB; b++) {
+		const int r = R.a + (wt * NB + b) * 16 + lane % 16;
+		if (r >= R.b || n >= A.n)
 			continue;
-		floatx4 y = acc[0][f];
+		const bool bad = A.from && (unsigned)A.from[r] >= (unsigned)A.x_rows;
+		float y[4 * FA];
 #pragma unroll
-		for (int u = 0; u < 4; u++) {
-			if (GATED)
-				y[u] = f8_gate(y[u], acc[M - 1][f][u]);
-			if (bad[f])
-				y[u] = __builtin_nanf("");
-		}
-		f8_store<TY>(A, r, n0 + lane / 16 * 4, y);
+		for (int f = 0; f < FA; f++)
+#pragma unroll
+			for (int u = 0; u < 4; u++) {
+				y[4 * f + u] = GATED ? f8_gate(acc[f][b][u], acc[NA - FA + f][b][u]) : acc[f][b][u];
+				if (bad)
+					y[4 * f + u] = __builtin_nanf("");
+			}
+		f8_store<TY, 4 * FA>(A, r, n, y);
 	}
 }
+
+/* the tiles of a type and form: NA, NB, WN, WT, STAGES */
+#define F8_BIG 8, 4, 2, 4, 2     /* 256 x 256 */
+#define F8_BIG_F32 4, 4, 2, 4, 2 /* 128 x 256 */
+#define F8_SMALL 2, 4, 4, 1, 3   /* 128 x 64 */
+#define F8_SMALL_F32 2, 2, 4, 2, 3 /* 128 x 64 */
 
 void f8_mul_plan(const f8_mul_args *a, f8_plan *p)
 {
 	const size_t rows = (size_t)a->rows, n = (size_t)a->n;
-	p->bt = BT;
-	p->bn = BN;
-	p->threads = MUL_THREADS;
-	p->n_tiles = (n + BN - 1) / BN;
-	p->row_tiles = (rows + BT - 1) / BT;
+	const size_t per = a->start ? (rows + (size_t)a->count - 1) / (size_t)a->count : rows;
+	p->big = per > 128;
+	p->bt = p->big ? 256 : 64;
+	p->bn = p->big && p->type != HIP_F8_F32 ? 256 : 128;
+	if (a->w[1])
+		p->bn /= 2;
+	p->threads = p->big || p->type == HIP_F8_F32 ? 512 : 256;
+	p->n_tiles = (n + (size_t)p->bn - 1) / (size_t)p->bn;
+	p->row_tiles = (rows + (size_t)p->bt - 1) / (size_t)p->bt;
 	if (a->start) /* every expert may end with a tile that is not full */
-		p->row_tiles = rows / BT + (rows < (size_t)a->count ? rows : (size_t)a->count);
+		p->row_tiles = rows / (size_t)p->bt + (rows < (size_t)a->count ? rows : (size_t)a->count);
 }
 
-template <int TY>
-static void mul_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)
+template <int TY, int... FORM>
+static void tile_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)
 {
 	const size_t grid = p->row_tiles * p->n_tiles;
 	if (a->w[1])
-		k_f8_mul<TY, true><<<grid, MUL_THREADS, 0, s>>>(*a, (int)p->n_tiles);
+		k_f8_tile<TY, true, FORM...><<<grid, p->threads, 0, s>>>(*a, (int)p->n_tiles, (int)p->row_tiles);
 	else
-		k_f8_mul<TY, false><<<grid, MUL_THREADS, 0, s>>>(*a, (int)p->n_tiles);
+		k_f8_tile<TY, false, FORM...><<<grid, p->threads, 0, s>>>(*a, (int)p->n_tiles, (int)p->row_tiles);
 }
 
-int f8_launch_mul(const f8_mul_args *a, const f8_plan *p, int type, void *stream)
+int f8_launch_mul(const f8_mul_args *a, const f8_plan *p, void *stream)
 {
 	hipStream_t s = (hipStream_t)stream;
-	if (type == HIP_F8_F32)
-		mul_typed<HIP_F8_F32>(a, p, s);
-	else if (type == HIP_F8_F16)
-		mul_typed<HIP_F8_F16>(a, p, s);
+	if (p->type == HIP_F8_F32)
+		p->big ? tile_typed<HIP_F8_F32, F8_BIG_F32>(a, p, s) : tile_typed<HIP_F8_F32, F8_SMALL_F32>(a, p, s);
+	else if (p->type == HIP_F8_F16)
+		p->big ? tile_typed<HIP_F8_F16, F8_BIG>(a, p, s) : tile_typed<HIP_F8_F16, F8_SMALL>(a, p, s);
 	else
-		mul_typed<HIP_F8_BF16>(a, p, s);
+		p->big ? tile_typed<HIP_F8_BF16, F8_BIG>(a, p, s) : tile_typed<HIP_F8_BF16, F8_SMALL>(a, p, s);
 	return hipGetLastError();
 }

@@ -202,11 +202,12 @@ static int launch_mul(const char *what, f8_mul_args *a, int type, void *out, siz
 		return 0;
 	a->out = out;
 	a->out_stride = (long)out_stride;
+	p.type = type;
 	f8_mul_plan(a, &p);
 	if (!check_grid(what, p.row_tiles, p.n_tiles, (size_t)p.threads) ||
 	    !call_stream(what, out, stream, &s))
 		return 0;
-	return launched(what, f8_launch_mul(a, &p, type, s));
+	return launched(what, f8_launch_mul(a, &p, s));
 }
 
 int hip_f8_mul_dev(const hip_f8_rows *X, const hip_f8_mat *W, const hip_f8_mat *up, int type,
