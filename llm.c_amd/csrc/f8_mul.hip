@@ -186,6 +186,9 @@ __device__ static inline void f8_meet()
 	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+#ifndef F8_SCHEDULE
+#define F8_SCHEDULE
+#endif
 /*
  * Tiles of 16 NB WT rows of X and 16 NA WN rows of W (gated: half of them W's, half
  * up's), a wave 16 NB by 16 NA of them.  A step is a block of 128 channels, all rows'
@@ -202,8 +205,9 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 	constexpr int M = GATED ? 2 : 1, FA = NA / M; /* operands of one matrix */
 	constexpr int BN = 16 * NA * WN, BT = 16 * NB * WT, NO = BN / M;
 	constexpr int NW = WN * WT, SLOTS = (BN + BT) / 8 / NW, SCALES = BT < 64 ? 64 : BT;
-	constexpr int BYTES = (BN + BT) * HIP_F8_BLOCK + SCALES * 4;
+	constexpr int BYTES = (BN + BT) * HIP_F8_BLOCK + SCALES * 4 + 256;
 	static_assert((BN + BT) / 8 % NW == 0 && HIP_F8_BLOCK % (16 * FA) == 0, "whole loads, one scale");
+	static_assert(SCALES / 64 < NW && WN * M <= 64, "a wave is left for W's scales");
 	typedef f8_operand<TY == HIP_F8_F32> operand;
 	__shared__ __attribute__((aligned(16))) uint8_t lds[STAGES * BYTES];
 
@@ -245,13 +249,22 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 			p[i] = A.x + x * A.x_stride;
 		}
 	}
+	/* and of the scales: X's 64 at a time, then W's, one for each wn and matrix */
 	const float *ps;
-	const int sslot = wave % (SCALES / 64);
-	{
+	long ps_step;
+	const int sslot = wave < SCALES / 64 ? wave : SCALES / 64;
+	if (sslot < SCALES / 64) {
 		int x = R.a + sslot * 64 + lane;
 		x = x < R.b ? x : R.b - 1;
 		x = A.from ? A.from[x] : x;
 		ps = A.xs + ((unsigned)x < (unsigned)A.x_rows ? x : 0);
+		ps_step = A.xs_stride;
+	} else {
+		const int m = lane % M;
+		int n = n0 + lane / M % WN * 16 * FA;
+		n = n < A.n ? n : A.n - 1;
+		ps = A.ws[m] + R.e * A.ws_step[m] + n / HIP_F8_BLOCK * A.ws_stride[m];
+		ps_step = 1;
 	}
 	const int blocks = (A.k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
 	const u32 base = lds_addr(lds);
@@ -262,15 +275,8 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 #pragma unroll
 		for (int i = 0; i < SLOTS; i++)
 			f8_dma16(p[i] + c, to + (wave + i * NW) * 1024);
-		f8_dma4(ps + kb * A.xs_stride, to + (BN + BT) * HIP_F8_BLOCK + sslot * 256);
+		f8_dma4(ps + kb * ps_step, to + (BN + BT) * HIP_F8_BLOCK + sslot * 256);
 	};
-	const float *sw[M];
-#pragma unroll
-	for (int m = 0; m < M; m++) {
-		const int n = n0 + wn * 16 * FA < A.n ? n0 + wn * 16 * FA : A.n - 1;
-		sw[m] = A.ws[m] + R.e * A.ws_step[m] + n / HIP_F8_BLOCK * A.ws_stride[m];
-	}
-
 	floatx4 acc[NA][NB] = {};
 #pragma unroll
 	for (int s = 0; s < STAGES - 1; s++)
@@ -291,31 +297,39 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 			}
 			f8_meet<63>();
 		}
-		const float *sx = (const float *)(buf + (BN + BT) * HIP_F8_BLOCK) + wt * 16 * NB + lane % 16;
+		const float *sx = (const float *)(buf + (BN + BT) * HIP_F8_BLOCK);
 		float s[M][NB];
 #pragma unroll
 		for (int b = 0; b < NB; b++)
 #pragma unroll
 			for (int m = 0; m < M; m++)
-				s[m][b] = sx[b * 16] * sw[m][kb];
-		operand x[NB];
+				s[m][b] = sx[(wt * NB + b) * 16 + lane % 16] * sx[SCALES + wn * M + m];
+		operand x[NB], w[2];
 		const uint8_t *xb = buf + (BN + wt * 16 * NB + lane % 16) * HIP_F8_BLOCK;
+		const uint8_t *wb = buf + (wn * 16 * NA + lane % 16) * HIP_F8_BLOCK;
+		w[0].set(*(const i32x4 *)(wb + place), *(const i32x4 *)(wb + (place ^ 64)));
 #pragma unroll
 		for (int b = 0; b < NB; b++)
 			x[b].set(*(const i32x4 *)(xb + b * 2048 + place), *(const i32x4 *)(xb + b * 2048 + (place ^ 64)));
-		const uint8_t *wb = buf + (wn * 16 * NA + lane % 16) * HIP_F8_BLOCK;
+		/* the sums of operand a are made while those of a - 1 join the accumulators */
+		floatx4 y[2][NB];
 #pragma unroll
-		for (int a = 0; a < NA; a++) {
-			operand w;
-			w.set(*(const i32x4 *)(wb + a * 2048 + place), *(const i32x4 *)(wb + a * 2048 + (place ^ 64)));
+		for (int a = 0; a <= NA; a++) {
+			if (a + 1 < NA)
+				w[(a + 1) % 2].set(*(const i32x4 *)(wb + (a + 1) * 2048 + place),
+						   *(const i32x4 *)(wb + (a + 1) * 2048 + (place ^ 64)));
 #pragma unroll
 			for (int b = 0; b < NB; b++) {
-				const floatx4 y = operand::mul(w, x[b]);
+				if (a < NA)
+					y[a % 2][b] = operand::mul(w[a % 2], x[b]);
+				if (a > 0)
 #pragma unroll
-				for (int u = 0; u < 4; u++)
-					acc[a][b][u] = __builtin_fmaf(y[u], s[a / FA][b], acc[a][b][u]);
+					for (int u = 0; u < 4; u++)
+						acc[a - 1][b][u] = __builtin_fmaf(y[(a - 1) % 2][b][u], s[(a - 1) / FA][b],
+										  acc[a - 1][b][u]);
 			}
 		}
+		F8_SCHEDULE
 		stage = stage + 1 == STAGES ? 0 : stage + 1;
 	}
 	f8_meet<0>(); /* no load outlives the workgroup's LDS */
