@@ -52,7 +52,7 @@ extern "C" {
  * Quantized rows.  Channel c of row r stands for
  *   e4m3(codes[r * stride + c]) * scale[c / 128 * scale_stride + r],
  * so that the scales of neighbouring rows lie next to each other.  The codes are
- * 16-byte aligned, the stride a multiple of 16 and at least k; bytes between k and
+ * 16-byte aligned, the stride a multiple of 16, at least k and at most 2^24; bytes between k and
  * the stride may hold anything.
  */
 typedef struct hip_f8_rows {
@@ -67,8 +67,8 @@ typedef struct hip_f8_rows {
  * `count` matrices of n rows of k columns.  Column c of row r of matrix e stands for
  *   e4m3(codes[e * step + r * stride + c]) *
  *   scale[e * scale_step + r / 128 * scale_stride + c / 128].
- * The codes are 16-byte aligned, stride and step multiples of 16; bytes between k
- * and the stride may hold anything.
+ * The codes are 16-byte aligned, stride and step multiples of 16, the stride at most
+ * 2^24; bytes between k and the stride may hold anything.
  */
 typedef struct hip_f8_mat {
 	const uint8_t *codes; /* device */

@@ -22,14 +22,25 @@
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
+/* An operand's codes as they lie in LDS, at p and at the place of the piece that is
+ * four further */
+struct f8_raw {
+	i32x8 v;
+	__device__ inline void get(const uint8_t *p, int place)
+	{
+		const i32x4 lo = *(const i32x4 *)p, hi = *(const i32x4 *)(p + (place & 64 ? -64 : 64));
+		v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+	}
+};
+
 /* 16 rows (columns) of an operand, 128 deep: lane l has row l % 16, and of the 128 any
  * 32 as long as both operands have the same */
 template <bool EXACT> struct f8_operand;
 template <> struct f8_operand<false> {
 	i32x8 v;
-	__device__ inline void set(i32x4 lo, i32x4 hi)
+	__device__ inline void set(const f8_raw &r)
 	{
-		v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+		v = r.v;
 	}
 	/* the block's sum */
 	__device__ static inline floatx4 mul(const f8_operand &a, const f8_operand &b)
@@ -40,13 +51,13 @@ template <> struct f8_operand<false> {
 };
 template <> struct f8_operand<true> {
 	half8_t v[4];
-	__device__ inline void set(i32x4 lo, i32x4 hi)
+	__device__ inline void set(const f8_raw &r)
 	{
 #pragma unroll
 		for (int i = 0; i < 4; i++)
 #pragma unroll
 			for (int j = 0; j < 2; j++) {
-				const u32 w = i < 2 ? lo[2 * i + j] : hi[2 * i - 4 + j];
+				const u32 w = r.v[2 * i + j];
 				const auto a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
 				const auto b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
 				v[i][4 * j] = a[0];
@@ -131,35 +142,31 @@ template <int TY, int N>
 __device__ static inline void f8_store(const f8_mul_args &A, int row, int n, float *y)
 {
 	typedef kv_type<TY> T;
-	constexpr int PER = 16 / sizeof(typename T::t) < N ? 16 / sizeof(typename T::t) : N;
-	typedef kv_vec<TY, PER> vec;
+	typedef kv_vec<TY, N> vec;
 	typename T::t *o = (typename T::t *)A.out + row * A.out_stride + n;
 	const typename T::t *p = (const typename T::t *)A.add + row * A.add_stride + n;
+	if (n + N <= A.n) {
+		vec v;
+		if (A.add) {
+			v = *(const vec *)p;
 #pragma unroll
-	for (int v0 = 0; v0 < N; v0 += PER) {
-		if (n + v0 + PER <= A.n) {
-			if (A.add) {
-				const vec v = *(const vec *)(p + v0);
-#pragma unroll
-				for (int u = 0; u < PER; u++)
-					y[v0 + u] += T::get(v.v[u]);
-			}
-			vec v;
-#pragma unroll
-			for (int u = 0; u < PER; u++)
-				v.v[u] = T::put(y[v0 + u]);
-			*(vec *)(o + v0) = v;
-		} else {
-#pragma unroll
-			for (int u = 0; u < PER; u++)
-				if (n + v0 + u < A.n)
-					o[v0 + u] = T::put(A.add ? y[v0 + u] + T::get(p[v0 + u]) : y[v0 + u]);
+			for (int u = 0; u < N; u++)
+				y[u] += T::get(v.v[u]);
 		}
+#pragma unroll
+		for (int u = 0; u < N; u++)
+			v.v[u] = T::put(y[u]);
+		*(vec *)o = v;
+	} else {
+#pragma unroll
+		for (int u = 0; u < N; u++)
+			if (n + u < A.n)
+				o[u] = T::put(A.add ? y[u] + T::get(p[u]) : y[u]);
 	}
 }
 
-/* 16 bytes a lane from its address to lds + 16 * lane, in flight until a wait that
- * the caller makes (moe_device.h's dma_dwordx4 with whole addresses) */
+/* 16 bytes a lane from its address to lds + 16 * lane, in flight until a wait that the
+ * caller makes (moe_device.h's dma_dwordx4 with whole addresses) */
 __device__ static inline void f8_dma16(const uint8_t *p, u32 lds)
 {
 	asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
@@ -168,7 +175,26 @@ __device__ static inline void f8_dma16(const uint8_t *p, u32 lds)
 		     : "memory");
 }
 
-/* the same, 4 bytes a lane */
+/* An address that all lanes share, for scalar registers */
+__device__ static inline uint64_t f8_shared(const uint8_t *p)
+{
+	const uint64_t b = (uint64_t)(uintptr_t)p;
+	return (uint64_t)(u32)__builtin_amdgcn_readfirstlane((int)(u32)b) |
+	       ((uint64_t)(u32)__builtin_amdgcn_readfirstlane((int)(u32)(b >> 32)) << 32);
+}
+
+/* The first form from such a base.  The compiler may bring it to its scalar registers
+ * right before, by vector instructions, and does not know that these five wait states
+ * are needed then. */
+__device__ static inline void f8_dma16(uint64_t base, u32 off, u32 lds)
+{
+	asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"
+		     :
+		     : "v"(off), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+		     : "memory");
+}
+
+/* The first form, 4 bytes a lane */
 __device__ static inline void f8_dma4(const float *p, u32 lds)
 {
 	asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off"
@@ -186,30 +212,43 @@ __device__ static inline void f8_meet()
 	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-#ifndef F8_SCHEDULE
-#define F8_SCHEDULE
-#endif
 /*
  * Tiles of 16 NB WT rows of X and 16 NA WN rows of W (gated: half of them W's, half
- * up's), a wave 16 NB by 16 NA of them.  A step is a block of 128 channels, all rows'
- * 128 bytes and X's scales in one of STAGES buffers, filled by loads that go past the
- * registers, STAGES - 1 steps ahead.
+ * up's), a wave 16 NB by 16 NA of them.  A step is a block of 128 channels, in two
+ * parts: X's rows with their scales and half of W's operands, then the other half.
+ * Each part has STAGES buffers, filled by loads that go past the registers.  A part's
+ * buffer is free, and is filled for STAGES steps later, once all waves have read it,
+ * which they do an operand ahead of its products: a load has STAGES - 1/2 steps to
+ * arrive, and the reads after a meeting have an operand's products to hide behind.
+ *
+ * The order of the instructions is this source's (sched_barrier): a product, then the
+ * scaling of the one LAG before it, four instructions that the matrix cores' 32 cycles
+ * cover.  Left to itself the compiler kept fewer sums and waited for each (989 us
+ * instead of 925, 8192 x 28672 x 4096).
  *
  * A row's 128 bytes are eight pieces of 16; piece p lies at place p ^ (row % 8), so
  * that the 16 rows whose same piece an operand's read takes meet no bank twice.  Row
- * i of an operand's 16 is the output that gives a lane its 4 NA neighbouring ones.
+ * i of an operand's 16 is the output that gives a lane 16 bytes of neighbouring ones
+ * from as many operands as that takes, and four lanes 64 bytes.
  */
-template <int TY, bool GATED, int NA, int NB, int WN, int WT, int STAGES>
+template <int TY, bool GATED, int NA, int NB, int WN, int WT, int STAGES, bool FAR>
 __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_tiles, int row_tiles)
 {
 	constexpr int M = GATED ? 2 : 1, FA = NA / M; /* operands of one matrix */
-	constexpr int BN = 16 * NA * WN, BT = 16 * NB * WT, NO = BN / M;
-	constexpr int NW = WN * WT, SLOTS = (BN + BT) / 8 / NW, SCALES = BT < 64 ? 64 : BT;
-	constexpr int BYTES = (BN + BT) * HIP_F8_BLOCK + SCALES * 4 + 256;
-	static_assert((BN + BT) / 8 % NW == 0 && HIP_F8_BLOCK % (16 * FA) == 0, "whole loads, one scale");
+	constexpr int BN = 16 * NA * WN, BT = 16 * NB * WT, NO = BN / M, HALF = NA / 2;
+	constexpr int NW = WN * WT, SCALES = BT < 64 ? 64 : BT;
+	constexpr int ROWS1 = BT + BN / 2, ROWS2 = BN / 2;
+	constexpr int XSLOTS = BT / 8 / NW, SLOTS1 = ROWS1 / 8 / NW, SLOTS2 = ROWS2 / 8 / NW;
+	constexpr int BYTES1 = ROWS1 * HIP_F8_BLOCK + SCALES * 4 + 256, BYTES2 = ROWS2 * HIP_F8_BLOCK;
+	constexpr int AHEAD = (STAGES - 1) * (SLOTS1 + 1 + SLOTS2); /* loads that a wait leaves in flight */
+	constexpr int LAG = NB < 3 ? NB : 3; /* sums that are not scaled yet */
+	constexpr int EACH = TY == HIP_F8_F32 || FA == 1 ? 1 : 2; /* operands whose outputs neighbour */
+	static_assert(BT / 8 % NW == 0 && ROWS2 / 8 % NW == 0, "whole loads");
+	static_assert(NA % 2 == 0 && HIP_F8_BLOCK % (16 * FA) == 0 && FA % EACH == 0, "two parts, one scale");
+	static_assert(NA * NB % 4 == 0, "the sums' places go round with the steps");
 	static_assert(SCALES / 64 < NW && WN * M <= 64, "a wave is left for W's scales");
 	typedef f8_operand<TY == HIP_F8_F32> operand;
-	__shared__ __attribute__((aligned(16))) uint8_t lds[STAGES * BYTES];
+	__shared__ __attribute__((aligned(16))) uint8_t lds[STAGES * (BYTES1 + BYTES2)];
 
 	const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 	const int wn = wave % WN, wt = wave / WN;
@@ -229,24 +268,36 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 	if (R.a >= R.b)
 		return;
 
-	/* what this wave loads: slots of eight rows */
+	/* what this wave loads: slots of eight rows, X's, W's first half, W's second; a row
+	 * by its distance from the tile's first, or where X is gathered from X's first */
 	const int piece = ((lane % 8) ^ (lane / 8)) * 16, last = (A.k - 1) & ~15;
-	const uint8_t *p[SLOTS];
+	const uint8_t *const first = A.from ? A.x : A.x + R.a * A.x_stride;
+	const uint64_t from_x = f8_shared(first);
+	const uint64_t from_w = f8_shared(A.w[0] + R.e * A.w_step[0] + n0 * A.w_stride[0]);
+	const uint64_t from_u = f8_shared(A.w[M - 1] + R.e * A.w_step[M - 1] + n0 * A.w_stride[M - 1]);
+	u32 off[SLOTS1 + SLOTS2];
+	const uint8_t *far[FAR ? XSLOTS : 1];
 #pragma unroll
-	for (int i = 0; i < SLOTS; i++) {
-		const int s = wave + i * NW, row = s * 8 + lane / 8;
-		if (row < BN) {
-			const int j = row % (16 * NA), m = j / (16 * FA), f = j / 16 % FA, r = j % 16;
-			int n = n0 + row / (16 * NA) * (16 * FA) + r / 4 * (4 * FA) + f * 4 + r % 4;
-			n = n < A.n ? n : A.n - 1;
-			p[i] = (m ? A.w[M - 1] + R.e * A.w_step[M - 1] + n * A.w_stride[M - 1]
-				  : A.w[0] + R.e * A.w_step[0] + n * A.w_stride[0]);
+	for (int i = 0; i < SLOTS1 + SLOTS2; i++) {
+		const int row = (wave + i * NW) * 8 + lane / 8;
+		if (i < XSLOTS) {
+			int x = R.a + row < R.b ? R.a + row : R.b - 1;
+			if (A.from) {
+				x = A.from[x];
+				x = (unsigned)x < (unsigned)A.x_rows ? x : 0;
+			} else {
+				x -= R.a;
+			}
+			off[i] = FAR ? 0 : (u32)x * (u32)A.x_stride;
+			if constexpr (FAR)
+				far[i] = first + x * A.x_stride;
 		} else {
-			int x = R.a + row - BN;
-			x = x < R.b ? x : R.b - 1;
-			x = A.from ? A.from[x] : x;
-			x = (unsigned)x < (unsigned)A.x_rows ? x : 0;
-			p[i] = A.x + x * A.x_stride;
+			/* half (gated: matrix), wn, operand of the half, row of it */
+			const int j = row - BT, r = j % 16;
+			const int f = (j / (BN / 2) * HALF + j / 16 % HALF) % FA;
+			const int n = j / (16 * HALF) % WN * (16 * FA) + f / EACH * (16 * EACH) +
+				      r / 4 * (4 * EACH) + f % EACH * 4 + r % 4;
+			off[i] = (u32)(n0 + n < A.n ? n : A.n - 1 - n0) * (u32)A.w_stride[i < SLOTS1 ? 0 : M - 1];
 		}
 	}
 	/* and of the scales: X's 64 at a time, then W's, one for each wn and matrix */
@@ -267,103 +318,167 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 		ps_step = 1;
 	}
 	const int blocks = (A.k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
-	const u32 base = lds_addr(lds);
-	auto load = [&](int kb, int stage) {
+	const bool rest = A.k % HIP_F8_BLOCK;
+	uint8_t *const lds2 = lds + STAGES * BYTES1;
+	const u32 base1 = lds_addr(lds), base2 = lds_addr(lds2);
+	/* a block's part into a buffer; past the last block the last again, which nothing reads */
+	auto load1 = [&](int kb, int stage) {
+		kb = kb < blocks ? kb : blocks - 1;
 		int c = kb * HIP_F8_BLOCK + piece;
 		c = c < last ? c : last; /* nothing past the row's last 16 that hold any is read */
-		const u32 to = base + stage * BYTES;
 #pragma unroll
-		for (int i = 0; i < SLOTS; i++)
-			f8_dma16(p[i] + c, to + (wave + i * NW) * 1024);
-		f8_dma4(ps + kb * ps_step, to + (BN + BT) * HIP_F8_BLOCK + sslot * 256);
-	};
-	floatx4 acc[NA][NB] = {};
-#pragma unroll
-	for (int s = 0; s < STAGES - 1; s++)
-		load(s < blocks ? s : blocks - 1, s);
-	int stage = 0;
-	const int place = ((lane / 16) ^ (lane % 8)) * 16;
-	for (int kb = 0; kb < blocks; kb++) {
-		f8_meet<(STAGES - 2) * (SLOTS + 1)>();
-		const int ahead = kb + STAGES - 1;
-		load(ahead < blocks ? ahead : blocks - 1, stage == 0 ? STAGES - 1 : stage - 1);
-		uint8_t *buf = lds + stage * BYTES;
-		if ((kb + 1) * HIP_F8_BLOCK > A.k) { /* the last block's rest: zeros */
-			for (int i = threadIdx.x; i < (BN + BT) * 8; i += 64 * NW) {
-				const int c = kb * HIP_F8_BLOCK + ((i % 8) ^ (i / 8 % 8)) * 16;
-				i32x4 *q = (i32x4 *)(buf + i * 16);
-				if (c + 16 > A.k)
-					*q = f8_masked(*q, c, A.k);
-			}
-			f8_meet<63>();
+		for (int i = 0; i < SLOTS1; i++) {
+			const u32 to = base1 + stage * BYTES1 + (wave + i * NW) * 1024;
+			if (FAR && i < XSLOTS)
+				f8_dma16(far[i < XSLOTS ? i : 0] + c, to);
+			else
+				f8_dma16(i < XSLOTS ? from_x : from_w, off[i] + c, to);
 		}
-		const float *sx = (const float *)(buf + (BN + BT) * HIP_F8_BLOCK);
-		float s[M][NB];
+		f8_dma4(ps + kb * ps_step, base1 + stage * BYTES1 + ROWS1 * HIP_F8_BLOCK + sslot * 256);
+	};
+	auto load2 = [&](int kb, int stage) {
+		kb = kb < blocks ? kb : blocks - 1;
+		int c = kb * HIP_F8_BLOCK + piece;
+		c = c < last ? c : last;
+#pragma unroll
+		for (int i = 0; i < SLOTS2; i++)
+			f8_dma16(from_u, off[SLOTS1 + i] + c, base2 + stage * BYTES2 + (wave + i * NW) * 1024);
+	};
+	/* zeros behind the last block's channels; rows is a multiple of eight */
+	auto cut = [&](uint8_t *buf, int rows) {
+		for (int i = threadIdx.x; i < rows * 8; i += 64 * NW) {
+			const int c = (blocks - 1) * HIP_F8_BLOCK + ((i % 8) ^ (i / 8 % 8)) * 16;
+			i32x4 *q = (i32x4 *)(buf + i * 16);
+			if (c + 16 > A.k)
+				*q = f8_masked(*q, c, A.k);
+		}
+		f8_meet<63>();
+	};
+
+	const int place = ((lane / 16) ^ (lane % 8)) * 16;
+	const int xo = (wt * 16 * NB + lane % 16) * HIP_F8_BLOCK + place;
+	const int wo = (wn * 16 * HALF + lane % 16) * HIP_F8_BLOCK + place;
+	f8_raw xr[NB], wr[2];
+	float s[M][NB], s_last[LAG] = {};
+	auto read_x = [&](int stage, int b) { xr[b].get(lds + stage * BYTES1 + xo + b * 2048, place); };
+	auto read_w = [&](int stage, int a) {
+		const uint8_t *w = a < HALF ? lds + stage * BYTES1 + BT * HIP_F8_BLOCK : lds2 + stage * BYTES2;
+		wr[a % 2].get(w + wo + a % HALF * 2048, place);
+	};
+	auto read_s = [&](int stage) {
+		const float *sx = (const float *)(lds + stage * BYTES1 + ROWS1 * HIP_F8_BLOCK);
 #pragma unroll
 		for (int b = 0; b < NB; b++)
 #pragma unroll
 			for (int m = 0; m < M; m++)
 				s[m][b] = sx[(wt * NB + b) * 16 + lane % 16] * sx[SCALES + wn * M + m];
-		operand x[NB], w[2];
-		const uint8_t *xb = buf + (BN + wt * 16 * NB + lane % 16) * HIP_F8_BLOCK;
-		const uint8_t *wb = buf + (wn * 16 * NA + lane % 16) * HIP_F8_BLOCK;
-		w[0].set(*(const i32x4 *)(wb + place), *(const i32x4 *)(wb + (place ^ 64)));
+	};
+
+#pragma unroll
+	for (int i = 0; i < STAGES; i++) {
+		load1(i, i);
+		if (i + 1 < STAGES)
+			load2(i, i);
+	}
+	f8_meet<AHEAD>();
+	load2(STAGES - 1, STAGES - 1);
+	if (blocks == 1 && rest)
+		cut(lds, ROWS1);
+	read_w(0, 0);
+#pragma unroll
+	for (int b = 0; b < NB; b++)
+		read_x(0, b);
+	read_s(0);
+
+	float acc[NA][NB][4] = {};
+	floatx4 y[4] = {};
+	int stage = 0;
+	for (int kb = 0; kb < blocks; kb++) {
+		const int next = stage + 1 == STAGES ? 0 : stage + 1;
+		operand x[NB], w;
 #pragma unroll
 		for (int b = 0; b < NB; b++)
-			x[b].set(*(const i32x4 *)(xb + b * 2048 + place), *(const i32x4 *)(xb + b * 2048 + (place ^ 64)));
-		/* the sums of operand a are made while those of a - 1 join the accumulators */
-		floatx4 y[2][NB];
+			x[b].set(xr[b]);
 #pragma unroll
-		for (int a = 0; a <= NA; a++) {
-			if (a + 1 < NA)
-				w[(a + 1) % 2].set(*(const i32x4 *)(wb + (a + 1) * 2048 + place),
-						   *(const i32x4 *)(wb + (a + 1) * 2048 + (place ^ 64)));
+		for (int a = 0; a < NA; a++) {
+			if (a == HALF - 1) { /* all have read the first part */
+				f8_meet<AHEAD>();
+				load1(kb + STAGES, stage);
+				if (kb == blocks - 1 && rest)
+					cut(lds2 + stage * BYTES2, ROWS2);
+			}
+			if (a == NA - 1) { /* all have read the second */
+				f8_meet<AHEAD>();
+				load2(kb + STAGES, stage);
+				if (kb == blocks - 2 && rest)
+					cut(lds + next * BYTES1, ROWS1);
+			}
+			w.set(wr[a % 2]);
+			if (a < NA - 1)
+				read_w(stage, a + 1);
+			else
+				read_w(next, 0);
+			__builtin_amdgcn_sched_barrier(0);
 #pragma unroll
 			for (int b = 0; b < NB; b++) {
-				if (a < NA)
-					y[a % 2][b] = operand::mul(w[a % 2], x[b]);
-				if (a > 0)
+				const int i = a * NB + b, j = (i + NA * NB - LAG) % (NA * NB);
+				y[i % 4] = operand::mul(w, x[b]);
+				if (a == NA - 1)
+					read_x(next, b);
+				const float f = i < LAG ? s_last[i] : s[j / NB / FA][j % NB];
 #pragma unroll
-					for (int u = 0; u < 4; u++)
-						acc[a - 1][b][u] = __builtin_fmaf(y[(a - 1) % 2][b][u], s[(a - 1) / FA][b],
-										  acc[a - 1][b][u]);
+				for (int u = 0; u < 4; u++) {
+					acc[j / NB][j % NB][u] = __builtin_fmaf(y[j % 4][u], f, acc[j / NB][j % NB][u]);
+					asm volatile("" : "+v"(acc[j / NB][j % NB][u])); /* here, not behind a branch */
+				}
+				__builtin_amdgcn_sched_barrier(0);
 			}
 		}
-		F8_SCHEDULE
-		stage = stage + 1 == STAGES ? 0 : stage + 1;
+#pragma unroll
+		for (int i = 0; i < LAG; i++)
+			s_last[i] = s[M - 1][NB - LAG + i];
+		read_s(next);
+		stage = next;
 	}
+#pragma unroll
+	for (int i = 0; i < LAG; i++)
+#pragma unroll
+		for (int u = 0; u < 4; u++)
+			acc[NA - 1][NB - LAG + i][u] =
+				__builtin_fmaf(y[(NA * NB - LAG + i) % 4][u], s_last[i], acc[NA - 1][NB - LAG + i][u]);
 	f8_meet<0>(); /* no load outlives the workgroup's LDS */
-	const int n = n0 + wn * 16 * FA + lane / 16 * (4 * FA);
 #pragma unroll
 	for (int b = 0; b < NB; b++) {
 		const int r = R.a + (wt * NB + b) * 16 + lane % 16;
-		if (r >= R.b || n >= A.n)
+		if (r >= R.b)
 			continue;
 		const bool bad = A.from && (unsigned)A.from[r] >= (unsigned)A.x_rows;
-		float y[4 * FA];
 #pragma unroll
-		for (int f = 0; f < FA; f++)
+		for (int f = 0; f < FA; f += EACH) {
+			float out[4 * EACH];
 #pragma unroll
-			for (int u = 0; u < 4; u++) {
-				y[4 * f + u] = GATED ? f8_gate(acc[f][b][u], acc[NA - FA + f][b][u]) : acc[f][b][u];
+			for (int i = 0; i < 4 * EACH; i++) {
+				const float v = acc[f + i / 4][b][i % 4];
+				out[i] = GATED ? f8_gate(v, acc[NA - FA + f + i / 4][b][i % 4]) : v;
 				if (bad)
-					y[4 * f + u] = __builtin_nanf("");
+					out[i] = __builtin_nanf("");
 			}
-		f8_store<TY, 4 * FA>(A, r, n, y);
+			f8_store<TY, 4 * EACH>(A, r, n0 + wn * 16 * FA + f * 16 + lane / 16 * (4 * EACH), out);
+		}
 	}
 }
 
 /* the tiles of a type and form: NA, NB, WN, WT, STAGES */
-#define F8_BIG 8, 4, 2, 4, 2     /* 256 x 256 */
-#define F8_BIG_F32 4, 4, 2, 4, 2 /* 128 x 256 */
-#define F8_SMALL 2, 4, 4, 1, 3   /* 128 x 64 */
-#define F8_SMALL_F32 2, 2, 4, 2, 3 /* 128 x 64 */
+#define F8_BIG 8, 4, 2, 4, 2, false     /* 256 x 256 */
+#define F8_BIG_F32 4, 4, 2, 4, 2, false /* 128 x 256 */
+#define F8_SMALL 2, 4, 4, 1, 3, true    /* 128 x 64 */
+#define F8_SMALL_F32 2, 2, 4, 2, 3, true /* 128 x 64 */
 
 void f8_mul_plan(const f8_mul_args *a, f8_plan *p)
 {
 	const size_t rows = (size_t)a->rows, n = (size_t)a->n;
 	const size_t per = a->start ? (rows + (size_t)a->count - 1) / (size_t)a->count : rows;
-	p->big = per > 128;
+	p->big = per > 128 && (!a->from || (size_t)a->x_rows * (size_t)a->x_stride < ((size_t)1 << 32) - F8_MAX_K);
 	p->bt = p->big ? 256 : 64;
 	p->bn = p->big && p->type != HIP_F8_F32 ? 256 : 128;
 	if (a->w[1])
@@ -375,7 +490,7 @@ void f8_mul_plan(const f8_mul_args *a, f8_plan *p)
 		p->row_tiles = rows / (size_t)p->bt + (rows < (size_t)a->count ? rows : (size_t)a->count);
 }
 
-template <int TY, int... FORM>
+template <int TY, auto... FORM>
 static void tile_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)
 {
 	const size_t grid = p->row_tiles * p->n_tiles;

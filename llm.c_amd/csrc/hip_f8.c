@@ -25,6 +25,8 @@ static int f8_err(const char *fmt, ...)
 #define MAX_SIZE ((size_t)1 << 31)    /* strides: up to this; pairs: below it */
 #define MAX_ROWS (MAX_SIZE - 65536)   /* rows and values of a row: below this, so that tiles that
 					 end behind them are counted in 32 bits */
+#define MAX_CODES ((size_t)1 << 24)   /* from row to row of codes: up to this, so that 256 rows'
+					 distances fit 32 bits */
 #define MAX_STRIDE ((size_t)1 << 40)  /* from matrix to matrix, of scales: up to this */
 #define MAX_THREADS ((size_t)1 << 32) /* of one launch: below this */
 
@@ -82,9 +84,9 @@ static int check_rows(const char *what, const hip_f8_rows *X)
 		return 1;
 	if (!X->codes || !X->scale)
 		return f8_err("%s: NULL codes or scales of rows", what);
-	if (X->stride < X->k || X->stride > MAX_SIZE || X->stride % 16 || (uintptr_t)X->codes % 16)
+	if (X->stride < X->k || X->stride > MAX_CODES || X->stride % 16 || (uintptr_t)X->codes % 16)
 		return f8_err("%s: rows of %zu codes are %zu apart (16-byte aligned, a multiple of 16 "
-			      "apart)", what, X->k, X->stride);
+			      "up to 2^24)", what, X->k, X->stride);
 	if (X->scale_stride < X->rows || X->scale_stride > MAX_SIZE || (uintptr_t)X->scale % 4)
 		return f8_err("%s: scales of %zu rows are %zu apart (4-byte aligned)", what, X->rows,
 			      X->scale_stride);
@@ -100,9 +102,9 @@ static int check_mat(const char *what, const char *name, const hip_f8_mat *W)
 		return f8_err("%s: %zu matrices (1 .. 1024)", what, W->count);
 	if (!W->codes || !W->scale)
 		return f8_err("%s: NULL codes or scales of %s", what, name);
-	if (W->stride < W->k || W->stride > MAX_SIZE || W->stride % 16 || (uintptr_t)W->codes % 16)
+	if (W->stride < W->k || W->stride > MAX_CODES || W->stride % 16 || (uintptr_t)W->codes % 16)
 		return f8_err("%s: %s rows of %zu codes are %zu apart (16-byte aligned, a multiple of 16 "
-			      "apart)", what, name, W->k, W->stride);
+			      "up to 2^24)", what, name, W->k, W->stride);
 	if (W->scale_stride < (W->k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK || W->scale_stride > MAX_SIZE ||
 	    (uintptr_t)W->scale % 4)
 		return f8_err("%s: %s scales of %zu columns are %zu apart (4-byte aligned)", what, name,

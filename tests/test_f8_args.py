@@ -40,7 +40,7 @@ BAD_ROWS = (
     (rows(k=0), "channels"), (rows(k=(1 << 20) + 1, stride=1 << 21), "channels"),
     (rows(rows=(1 << 31) - 65536, scale_stride=1 << 31), "rows"),
     (rows(codes=None), "NULL"), (rows(scale=None), "NULL"), (rows(stride=255), "apart"), (rows(stride=264), "apart"),
-    (rows(stride=(1 << 31) + 16), "apart"), (rows(codes=DEV + 8), "16-byte"), (rows(scale=DEV + 2), "4-byte"),
+    (rows(stride=(1 << 24) + 16), "apart"), (rows(codes=DEV + 8), "16-byte"), (rows(scale=DEV + 2), "4-byte"),
     (rows(scale_stride=7), "scales of"), (rows(scale_stride=(1 << 31) + 1), "scales of"))
 
 BAD_MATS = (
@@ -48,7 +48,7 @@ BAD_MATS = (
     (dict(k=(1 << 20) + 1), "columns"), (dict(count=0), "matrices"), (dict(count=1025), "matrices"),
     (dict(codes=None), "NULL"), (dict(scale=None), "NULL"), (dict(stride=255), "apart"), (dict(stride=264), "apart"),
     (dict(codes=DEV + 4), "16-byte"), (dict(scale=DEV + 1), "4-byte"), (dict(scale_stride=1), "scales"),
-    (dict(scale_stride=(1 << 31) + 1), "scales"), (dict(stride=(1 << 31) + 16), "apart"))
+    (dict(scale_stride=(1 << 31) + 1), "scales"), (dict(stride=(1 << 24) + 16), "apart"))
 
 
 @pytest.mark.parametrize("X,msg", BAD_ROWS)
