@@ -22,6 +22,17 @@
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
+/* The channels c .. c + 15 of a row's codes, zeros from k on */
+__device__ static inline i32x4 f8_masked(i32x4 v, int c, int k)
+{
+#pragma unroll
+	for (int i = 0; i < 4; i++) {
+		const int left = k - c - 4 * i;
+		v[i] = left >= 4 ? v[i] : left <= 0 ? 0 : v[i] & (int)(0xffffffffu >> (32 - 8 * left));
+	}
+	return v;
+}
+
 /* An operand's codes as they lie in LDS, at p and at the place of the piece that is
  * four further */
 struct f8_raw {
@@ -29,6 +40,19 @@ struct f8_raw {
 	__device__ inline void get(const uint8_t *p, int place)
 	{
 		const i32x4 lo = *(const i32x4 *)p, hi = *(const i32x4 *)(p + (place & 64 ? -64 : 64));
+		v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+	}
+	/* the same from two places */
+	__device__ inline void get2(const uint8_t *p, const uint8_t *q)
+	{
+		const i32x4 lo = *(const i32x4 *)p, hi = *(const i32x4 *)q;
+		v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+	}
+	/* zeros from channel k on, of c .. c + 15 and c + 64 .. c + 79 */
+	__device__ inline void cut(int c, int k)
+	{
+		const i32x4 lo = f8_masked(__builtin_shufflevector(v, v, 0, 1, 2, 3), c, k);
+		const i32x4 hi = f8_masked(__builtin_shufflevector(v, v, 4, 5, 6, 7), c + 64, k);
 		v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 	}
 };
@@ -75,17 +99,6 @@ template <> struct f8_operand<true> {
 		return y;
 	}
 };
-
-/* The channels c .. c + 15 of a row's codes, zeros from k on */
-__device__ static inline i32x4 f8_masked(i32x4 v, int c, int k)
-{
-#pragma unroll
-	for (int i = 0; i < 4; i++) {
-		const int left = k - c - 4 * i;
-		v[i] = left >= 4 ? v[i] : left <= 0 ? 0 : v[i] & (int)(0xffffffffu >> (32 - 8 * left));
-	}
-	return v;
-}
 
 /* A tile's expert and rows of out */
 struct f8_rows_of {
@@ -212,6 +225,70 @@ __device__ static inline void f8_meet()
 	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+/* The tile of a workgroup.  Workgroups go to the eight XCDs in turn: each takes a
+ * stretch of the tiles, in groups of 8 row tiles that share what the L2 holds of W. */
+__device__ static inline void f8_tile_of(int n_tiles, int row_tiles, int &row_tile, int &n_tile)
+{
+	const int grid = n_tiles * row_tiles, xcd = blockIdx.x % 8;
+	const int id = xcd * (grid / 8) + (xcd < grid % 8 ? xcd : grid % 8) + blockIdx.x / 8;
+	const int group = id / (8 * n_tiles), g0 = group * 8;
+	const int many = row_tiles - g0 < 8 ? row_tiles - g0 : 8;
+	const int in = id - group * 8 * n_tiles;
+	row_tile = g0 + in % many;
+	n_tile = in / many;
+}
+
+/* Where a lane's scale of slot `slot` of a tile starts, and how far the next block's is:
+ * X's rows 64 a slot, then W's, one for each of WN x NR outputs and M matrices */
+template <int M, int NR, int WN>
+__device__ static inline void f8_scale_from(const f8_mul_args &A, const f8_rows_of &R, int n0, int slot,
+					    int x_slots, const float *&p, long &step)
+{
+	const int lane = threadIdx.x % 64;
+	if (slot < x_slots) {
+		int x = R.a + slot * 64 + lane;
+		x = x < R.b ? x : R.b - 1;
+		x = A.from ? A.from[x] : x;
+		p = A.xs + ((unsigned)x < (unsigned)A.x_rows ? x : 0);
+		step = A.xs_stride;
+	} else {
+		const int m = lane % M;
+		int n = n0 + lane / M % WN * NR;
+		n = n < A.n ? n : A.n - 1;
+		p = A.ws[m] + R.e * A.ws_step[m] + n / HIP_F8_BLOCK * A.ws_stride[m];
+		step = 1;
+	}
+}
+
+/* A wave's sums, of rows r0 .. and outputs n0 .., gated and stored: EACH operands give
+ * a lane neighbouring outputs */
+template <int TY, bool GATED, int NA, int NB, int EACH>
+__device__ static inline void f8_finish(const f8_mul_args &A, const f8_rows_of &R, int r0, int n0,
+					const float (&acc)[NA][NB][4])
+{
+	constexpr int FA = GATED ? NA / 2 : NA;
+	const int lane = threadIdx.x % 64;
+#pragma unroll
+	for (int b = 0; b < NB; b++) {
+		const int r = r0 + b * 16 + lane % 16;
+		if (r >= R.b)
+			continue;
+		const bool bad = A.from && (unsigned)A.from[r] >= (unsigned)A.x_rows;
+#pragma unroll
+		for (int f = 0; f < FA; f += EACH) {
+			float out[4 * EACH];
+#pragma unroll
+			for (int i = 0; i < 4 * EACH; i++) {
+				const float v = acc[f + i / 4][b][i % 4];
+				out[i] = GATED ? f8_gate(v, acc[NA - FA + f + i / 4][b][i % 4]) : v;
+				if (bad)
+					out[i] = __builtin_nanf("");
+			}
+			f8_store<TY, 4 * EACH>(A, r, n0 + f * 16 + lane / 16 * (4 * EACH), out);
+		}
+	}
+}
+
 /*
  * Tiles of 16 NB WT rows of X and 16 NA WN rows of W (gated: half of them W's, half
  * up's), a wave 16 NB by 16 NA of them.  A step is a block of 128 channels, in two
@@ -252,15 +329,9 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 
 	const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 	const int wn = wave % WN, wt = wave / WN;
-	/* Workgroups go to the eight XCDs in turn: each takes a stretch of the tiles, in
-	 * groups of 8 row tiles that share what the L2 holds of W. */
-	const int grid = n_tiles * row_tiles, xcd = blockIdx.x % 8;
-	const int id = xcd * (grid / 8) + (xcd < grid % 8 ? xcd : grid % 8) + blockIdx.x / 8;
-	const int group = id / (8 * n_tiles), g0 = group * 8;
-	const int many = row_tiles - g0 < 8 ? row_tiles - g0 : 8;
-	const int in = id - group * 8 * n_tiles;
-	const int tile = g0 + in % many, n0 = in / many * NO;
-
+	int tile, n0;
+	f8_tile_of(n_tiles, row_tiles, tile, n0);
+	n0 *= NO;
 	f8_rows_of R = f8_find<BT>(A, tile);
 	R.e = __builtin_amdgcn_readfirstlane(R.e);
 	R.a = __builtin_amdgcn_readfirstlane(R.a);
@@ -300,23 +371,11 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 			off[i] = (u32)(n0 + n < A.n ? n : A.n - 1 - n0) * (u32)A.w_stride[i < SLOTS1 ? 0 : M - 1];
 		}
 	}
-	/* and of the scales: X's 64 at a time, then W's, one for each wn and matrix */
+	/* and of the scales: X's 64 at a time, then W's */
 	const float *ps;
 	long ps_step;
 	const int sslot = wave < SCALES / 64 ? wave : SCALES / 64;
-	if (sslot < SCALES / 64) {
-		int x = R.a + sslot * 64 + lane;
-		x = x < R.b ? x : R.b - 1;
-		x = A.from ? A.from[x] : x;
-		ps = A.xs + ((unsigned)x < (unsigned)A.x_rows ? x : 0);
-		ps_step = A.xs_stride;
-	} else {
-		const int m = lane % M;
-		int n = n0 + lane / M % WN * 16 * FA;
-		n = n < A.n ? n : A.n - 1;
-		ps = A.ws[m] + R.e * A.ws_step[m] + n / HIP_F8_BLOCK * A.ws_stride[m];
-		ps_step = 1;
-	}
+	f8_scale_from<M, 16 * FA, WN>(A, R, n0, sslot, SCALES / 64, ps, ps_step);
 	const int blocks = (A.k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
 	const bool rest = A.k % HIP_F8_BLOCK;
 	uint8_t *const lds2 = lds + STAGES * BYTES1;
@@ -447,43 +506,338 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 			acc[NA - 1][NB - LAG + i][u] =
 				__builtin_fmaf(y[(NA * NB - LAG + i) % 4][u], s_last[i], acc[NA - 1][NB - LAG + i][u]);
 	f8_meet<0>(); /* no load outlives the workgroup's LDS */
+	f8_finish<TY, GATED, NA, NB, EACH>(A, R, R.a + wt * NB * 16, n0 + wn * 16 * FA, acc);
+}
+
+/*
+ * Tiles of 16 NB WT rows of X and 16 NA WN rows of W (gated: half of them W's, half
+ * up's) where there are few of them: KS groups of WN WT waves take the blocks of
+ * channels in turn, each into LDS of its own, and add their sums up at the end.  All
+ * groups meet once a step, so that a step's waits are paid once for KS blocks.  Rows
+ * lie in LDS and outputs in the lanes as in k_f8_tile.
+ */
+template <int TY, bool GATED, int NA, int NB, int WN, int WT, int KS, int STAGES>
+__global__ __launch_bounds__(64 * WN * WT * KS) void k_f8_mid(f8_mul_args A, int n_tiles, int row_tiles)
+{
+	constexpr int M = GATED ? 2 : 1, FA = NA / M;
+	constexpr int BN = 16 * NA * WN, BT = 16 * NB * WT, NO = BN / M, NW = WN * WT;
+	constexpr int XSLOTS = BT / 8 / NW, SLOTS = (BN + BT) / 8 / NW, SCALES = BT < 64 ? 64 : BT;
+	constexpr int BYTES = (BN + BT) * HIP_F8_BLOCK + SCALES * 4 + 256; /* of a block */
+	constexpr int EACH = TY == HIP_F8_F32 || FA == 1 ? 1 : 2;
+	static_assert(BT / 8 % NW == 0 && BN / 8 % NW == 0, "whole loads");
+	static_assert(NA % M == 0 && HIP_F8_BLOCK % (16 * FA) == 0 && FA % EACH == 0, "one scale");
+	static_assert(SCALES / 64 < NW && WN * M <= 64, "a wave is left for W's scales");
+	static_assert((KS - 1) * BN * BT * 4 <= STAGES * KS * BYTES, "the groups' sums");
+	typedef f8_operand<TY == HIP_F8_F32> operand;
+	__shared__ __attribute__((aligned(16))) uint8_t lds[STAGES * KS * BYTES];
+
+	const int lane = threadIdx.x % 64;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 % NW);
+	const int ks = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 / NW);
+	const int wn = wave % WN, wt = wave / WN;
+	int tile, n0;
+	f8_tile_of(n_tiles, row_tiles, tile, n0);
+	n0 *= NO;
+	f8_rows_of R = f8_find<BT>(A, tile);
+	R.e = __builtin_amdgcn_readfirstlane(R.e);
+	R.a = __builtin_amdgcn_readfirstlane(R.a);
+	R.b = __builtin_amdgcn_readfirstlane(R.b);
+	if (R.a >= R.b)
+		return;
+
+	const int piece = ((lane % 8) ^ (lane / 8)) * 16, last = (A.k - 1) & ~15;
+	const uint8_t *p[SLOTS];
 #pragma unroll
-	for (int b = 0; b < NB; b++) {
-		const int r = R.a + (wt * NB + b) * 16 + lane % 16;
+	for (int i = 0; i < SLOTS; i++) {
+		const int row = (wave + i * NW) * 8 + lane / 8;
+		if (i < XSLOTS) {
+			int x = R.a + row < R.b ? R.a + row : R.b - 1;
+			x = A.from ? A.from[x] : x;
+			x = (unsigned)x < (unsigned)A.x_rows ? x : 0;
+			p[i] = A.x + x * A.x_stride;
+		} else {
+			/* wn, operand of its NA, row of it */
+			const int j = row - BT, r = j % 16, a = j / 16 % NA, m = a / FA, f = a % FA;
+			int n = n0 + j / (16 * NA) * (16 * FA) + f / EACH * (16 * EACH) + r / 4 * (4 * EACH) +
+				f % EACH * 4 + r % 4;
+			n = n < A.n ? n : A.n - 1;
+			p[i] = m ? A.w[M - 1] + R.e * A.w_step[M - 1] + n * A.w_stride[M - 1]
+				 : A.w[0] + R.e * A.w_step[0] + n * A.w_stride[0];
+		}
+	}
+	const float *ps;
+	long ps_step;
+	const int sslot = wave < SCALES / 64 ? wave : SCALES / 64;
+	f8_scale_from<M, 16 * FA, WN>(A, R, n0, sslot, SCALES / 64, ps, ps_step);
+
+	const int blocks = (A.k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK, steps = (blocks + KS - 1) / KS;
+	const u32 base = lds_addr(lds);
+	auto load = [&](int step, int stage) {
+		int kb = step * KS + ks;
+		kb = kb < blocks ? kb : blocks - 1;
+		int c = kb * HIP_F8_BLOCK + piece;
+		c = c < last ? c : last;
+		const u32 to = base + (stage * KS + ks) * BYTES;
+#pragma unroll
+		for (int i = 0; i < SLOTS; i++)
+			f8_dma16(p[i] + c, to + (wave + i * NW) * 1024);
+		f8_dma4(ps + kb * ps_step, to + (BN + BT) * HIP_F8_BLOCK + sslot * 256);
+	};
+	const int place = ((lane / 16) ^ (lane % 8)) * 16;
+	const int xo = (wt * 16 * NB + lane % 16) * HIP_F8_BLOCK + place;
+	const int wo = (BT + wn * 16 * NA + lane % 16) * HIP_F8_BLOCK + place;
+	float acc[NA][NB][4] = {};
+#pragma unroll
+	for (int i = 0; i < STAGES - 1; i++)
+		load(i, i);
+	int stage = 0;
+	for (int step = 0; step < steps; step++) {
+		f8_meet<(STAGES - 2) * (SLOTS + 1)>();
+		load(step + STAGES - 1, stage == 0 ? STAGES - 1 : stage - 1);
+		uint8_t *buf = lds + (stage * KS + ks) * BYTES;
+		const int kb = step * KS + ks;
+		if (step == steps - 1 && A.k % HIP_F8_BLOCK) {
+			if (kb == blocks - 1)
+				for (int i = wave * 64 + lane; i < (BN + BT) * 8; i += 64 * NW) {
+					const int c = kb * HIP_F8_BLOCK + ((i % 8) ^ (i / 8 % 8)) * 16;
+					i32x4 *q = (i32x4 *)(buf + i * 16);
+					if (c + 16 > A.k)
+						*q = f8_masked(*q, c, A.k);
+				}
+			f8_meet<63>();
+		}
+		if (kb < blocks) {
+			const float *sx = (const float *)(buf + (BN + BT) * HIP_F8_BLOCK);
+			f8_raw xr[NB], wr[2];
+			float s[M][NB];
+			wr[0].get(buf + wo, place);
+#pragma unroll
+			for (int b = 0; b < NB; b++)
+				xr[b].get(buf + xo + b * 2048, place);
+#pragma unroll
+			for (int b = 0; b < NB; b++)
+#pragma unroll
+				for (int m = 0; m < M; m++)
+					s[m][b] = sx[(wt * NB + b) * 16 + lane % 16] * sx[SCALES + wn * M + m];
+			operand x[NB];
+#pragma unroll
+			for (int b = 0; b < NB; b++)
+				x[b].set(xr[b]);
+			floatx4 y[2][NB];
+#pragma unroll
+			for (int a = 0; a <= NA; a++) {
+				operand w;
+				if (a < NA)
+					w.set(wr[a % 2]);
+				if (a + 1 < NA)
+					wr[(a + 1) % 2].get(buf + wo + (a + 1) * 2048, place);
+#pragma unroll
+				for (int b = 0; b < NB; b++) {
+					if (a < NA)
+						y[a % 2][b] = operand::mul(w, x[b]);
+					if (a > 0)
+#pragma unroll
+						for (int u = 0; u < 4; u++)
+							acc[a - 1][b][u] = __builtin_fmaf(y[(a - 1) % 2][b][u],
+											  s[(a - 1) / FA][b], acc[a - 1][b][u]);
+				}
+			}
+		}
+		stage = stage + 1 == STAGES ? 0 : stage + 1;
+	}
+	f8_meet<0>(); /* no load outlives the workgroup's LDS */
+	floatx4 *sums = (floatx4 *)lds; /* [ks - 1][wave][a][b][lane] */
+	if (KS > 1) {
+		if (ks > 0)
+#pragma unroll
+			for (int a = 0; a < NA; a++)
+#pragma unroll
+				for (int b = 0; b < NB; b++)
+					sums[((((ks - 1) * NW + wave) * NA + a) * NB + b) * 64 + lane] =
+						floatx4{acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
+		__syncthreads();
+		if (ks > 0)
+			return;
+#pragma unroll
+		for (int g = 0; g < KS - 1; g++)
+#pragma unroll
+			for (int a = 0; a < NA; a++)
+#pragma unroll
+				for (int b = 0; b < NB; b++) {
+					const floatx4 v = sums[(((g * NW + wave) * NA + a) * NB + b) * 64 + lane];
+#pragma unroll
+					for (int u = 0; u < 4; u++)
+						acc[a][b][u] += v[u];
+				}
+	}
+	f8_finish<TY, GATED, NA, NB, EACH>(A, R, R.a + wt * NB * 16, n0 + wn * 16 * FA, acc);
+}
+
+/*
+ * Few rows: 16 NT rows of X and 16 NF outputs a workgroup, whose NW waves take the
+ * blocks of channels in turn, each with loads of its own from W and X, DEPTH blocks
+ * ahead, and no LDS but for the waves' sums at the end.  W is read as its rows lie,
+ * 64 bytes of each a load; what bounds it is how much of W is in flight.
+ */
+template <int TY, bool GATED, int NF, int NT, int NW, int DEPTH>
+__global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles)
+{
+	constexpr int M = GATED ? 2 : 1, FN = NF * M;
+	typedef f8_operand<TY == HIP_F8_F32> operand;
+	__shared__ floatx4 sums[NW][FN][NT][64];
+	const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+	const int tile = blockIdx.x / n_tiles, n0 = blockIdx.x % n_tiles * (16 * NF);
+	f8_rows_of R = f8_find<16 * NT>(A, tile);
+	R.e = __builtin_amdgcn_readfirstlane(R.e);
+	R.a = __builtin_amdgcn_readfirstlane(R.a);
+	R.b = __builtin_amdgcn_readfirstlane(R.b);
+	if (R.a >= R.b)
+		return;
+	const int piece = lane / 16 * 16, last = (A.k - 1) & ~15; /* of each 64 channels */
+	const uint8_t *px[NT], *pw[FN];
+	const float *sx[NT], *sw[M];
+#pragma unroll
+	for (int t = 0; t < NT; t++) {
+		int x = R.a + t * 16 + lane % 16;
+		x = x < R.b ? x : R.b - 1;
+		x = A.from ? A.from[x] : x;
+		x = (unsigned)x < (unsigned)A.x_rows ? x : 0;
+		px[t] = A.x + x * A.x_stride;
+		sx[t] = A.xs + x;
+	}
+#pragma unroll
+	for (int f = 0; f < FN; f++) {
+		const int m = f / NF, n = n0 + f % NF * 16 + lane % 16;
+		pw[f] = A.w[m] + R.e * A.w_step[m] + (n < A.n ? n : A.n - 1) * A.w_stride[m];
+	}
+#pragma unroll
+	for (int m = 0; m < M; m++)
+		sw[m] = A.ws[m] + R.e * A.ws_step[m] + n0 / HIP_F8_BLOCK * A.ws_stride[m];
+	const int blocks = (A.k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
+
+	struct {
+		f8_raw x[NT], w[FN];
+		float sx[NT], sw[M];
+	} in[DEPTH + 1];
+	auto load = [&](int kb, int i) {
+		const int c = kb * HIP_F8_BLOCK + piece;
+		const int lo = c < last ? c : last, hi = c + 64 < last ? c + 64 : last;
+#pragma unroll
+		for (int f = 0; f < FN; f++)
+			in[i].w[f].get2(pw[f] + lo, pw[f] + hi);
+#pragma unroll
+		for (int t = 0; t < NT; t++) {
+			in[i].x[t].get2(px[t] + lo, px[t] + hi);
+			in[i].sx[t] = sx[t][kb * A.xs_stride];
+		}
+#pragma unroll
+		for (int m = 0; m < M; m++)
+			in[i].sw[m] = sw[m][kb];
+	};
+	floatx4 acc[FN][NT] = {};
+	auto use = [&](int kb, int i) {
+		if ((kb + 1) * HIP_F8_BLOCK > A.k) {
+			const int c = kb * HIP_F8_BLOCK + piece;
+#pragma unroll
+			for (int f = 0; f < FN; f++)
+				in[i].w[f].cut(c, A.k);
+#pragma unroll
+			for (int t = 0; t < NT; t++)
+				in[i].x[t].cut(c, A.k);
+		}
+		operand w[FN];
+#pragma unroll
+		for (int f = 0; f < FN; f++)
+			w[f].set(in[i].w[f]);
+#pragma unroll
+		for (int t = 0; t < NT; t++) {
+			operand x;
+			x.set(in[i].x[t]);
+#pragma unroll
+			for (int f = 0; f < FN; f++) {
+				const floatx4 y = operand::mul(w[f], x);
+				const float s = in[i].sx[t] * in[i].sw[f / NF];
+#pragma unroll
+				for (int u = 0; u < 4; u++)
+					acc[f][t][u] = __builtin_fmaf(y[u], s, acc[f][t][u]);
+			}
+		}
+	};
+#pragma unroll
+	for (int i = 0; i < DEPTH; i++)
+		if (wave + i * NW < blocks)
+			load(wave + i * NW, i);
+	for (int kb = wave; kb < blocks; kb += (DEPTH + 1) * NW) {
+#pragma unroll
+		for (int i = 0; i <= DEPTH; i++) {
+			const int at = kb + i * NW, ahead = at + DEPTH * NW;
+			if (ahead < blocks)
+				load(ahead, (i + DEPTH) % (DEPTH + 1));
+			if (at < blocks)
+				use(at, i);
+		}
+	}
+#pragma unroll
+	for (int f = 0; f < FN; f++)
+#pragma unroll
+		for (int t = 0; t < NT; t++)
+			sums[wave][f][t][lane] = acc[f][t];
+	__syncthreads();
+	for (int i = wave; i < NF * NT; i += NW) {
+		const int f = i % NF, t = i / NF, r = R.a + t * 16 + lane % 16, n = n0 + f * 16 + lane / 16 * 4;
+		floatx4 y[M] = {};
+#pragma unroll
+		for (int m = 0; m < M; m++)
+#pragma unroll
+			for (int w = 0; w < NW; w++)
+				y[m] += sums[w][m * NF + f][t][lane];
 		if (r >= R.b)
 			continue;
 		const bool bad = A.from && (unsigned)A.from[r] >= (unsigned)A.x_rows;
+		float out[4];
 #pragma unroll
-		for (int f = 0; f < FA; f += EACH) {
-			float out[4 * EACH];
-#pragma unroll
-			for (int i = 0; i < 4 * EACH; i++) {
-				const float v = acc[f + i / 4][b][i % 4];
-				out[i] = GATED ? f8_gate(v, acc[NA - FA + f + i / 4][b][i % 4]) : v;
-				if (bad)
-					out[i] = __builtin_nanf("");
-			}
-			f8_store<TY, 4 * EACH>(A, r, n0 + wn * 16 * FA + f * 16 + lane / 16 * (4 * EACH), out);
+		for (int u = 0; u < 4; u++) {
+			out[u] = GATED ? f8_gate(y[0][u], y[M - 1][u]) : y[0][u];
+			if (bad)
+				out[u] = __builtin_nanf("");
 		}
+		f8_store<TY, 4>(A, r, n, out);
 	}
 }
 
-/* the tiles of a type and form: NA, NB, WN, WT, STAGES */
+/* the forms: few rows by 16 NT, NF, NW and DEPTH; tiles by NA, NB, WN, WT, STAGES, FAR */
 #define F8_BIG 8, 4, 2, 4, 2, false     /* 256 x 256 */
 #define F8_BIG_F32 4, 4, 2, 4, 2, false /* 128 x 256 */
 #define F8_SMALL 2, 4, 4, 1, 3, true    /* 128 x 64 */
 #define F8_SMALL_F32 2, 2, 4, 2, 3, true /* 128 x 64 */
+#ifndef FEW1
+#define FEW1 1, 1, 8, 2
+#define FEW2 1, 2, 8, 1
+#define FEW4 1, 4, 8, 1
+#endif
 
 void f8_mul_plan(const f8_mul_args *a, f8_plan *p)
 {
 	const size_t rows = (size_t)a->rows, n = (size_t)a->n;
 	const size_t per = a->start ? (rows + (size_t)a->count - 1) / (size_t)a->count : rows;
-	p->big = per > 128 && (!a->from || (size_t)a->x_rows * (size_t)a->x_stride < ((size_t)1 << 32) - F8_MAX_K);
-	p->bt = p->big ? 256 : 64;
-	p->bn = p->big && p->type != HIP_F8_F32 ? 256 : 128;
-	if (a->w[1])
-		p->bn /= 2;
-	p->threads = p->big || p->type == HIP_F8_F32 ? 512 : 256;
+	p->form = per <= 16 ? 1 : per <= 32 ? 2 : per <= 64 ? 4 : 5;
+#ifdef F8_FORCE
+	if (getenv("F8_FORM"))
+		p->form = atoi(getenv("F8_FORM"));
+#endif
+	if (p->form == 5 && per > 128 && (!a->from || (size_t)a->x_rows * (size_t)a->x_stride < ((size_t)1 << 32) - F8_MAX_K))
+		p->form = 6;
+	static const int few[] = {FEW1, FEW2, FEW4};
+	const int *f = few + (p->form == 1 ? 0 : p->form == 2 ? 4 : 8);
+	if (p->form < 5) {
+		p->bt = 16 * f[1];
+		p->bn = 16 * f[0];
+		p->threads = 64 * f[2];
+	} else {
+		p->bt = p->form == 6 ? 256 : 64;
+		p->bn = (p->form == 6 && p->type != HIP_F8_F32 ? 256 : 128) / (a->w[1] ? 2 : 1);
+		p->threads = p->form == 6 || p->type == HIP_F8_F32 ? 512 : 256;
+	}
 	p->n_tiles = (n + (size_t)p->bn - 1) / (size_t)p->bn;
 	p->row_tiles = (rows + (size_t)p->bt - 1) / (size_t)p->bt;
 	if (a->start) /* every expert may end with a tile that is not full */
@@ -500,14 +854,39 @@ static void tile_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)
 		k_f8_tile<TY, false, FORM...><<<grid, p->threads, 0, s>>>(*a, (int)p->n_tiles, (int)p->row_tiles);
 }
 
+template <int TY, int... FORM>
+static void few_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)
+{
+	const size_t grid = p->row_tiles * p->n_tiles;
+	if (a->w[1])
+		k_f8_few<TY, true, FORM...><<<grid, p->threads, 0, s>>>(*a, (int)p->n_tiles);
+	else
+		k_f8_few<TY, false, FORM...><<<grid, p->threads, 0, s>>>(*a, (int)p->n_tiles);
+}
+
+template <int TY>
+static void mul_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)
+{
+	if (p->form == 1)
+		few_typed<TY, FEW1>(a, p, s);
+	else if (p->form == 2)
+		few_typed<TY, FEW2>(a, p, s);
+	else if (p->form == 4)
+		few_typed<TY, FEW4>(a, p, s);
+	else if constexpr (TY == HIP_F8_F32)
+		p->form == 6 ? tile_typed<TY, F8_BIG_F32>(a, p, s) : tile_typed<TY, F8_SMALL_F32>(a, p, s);
+	else
+		p->form == 6 ? tile_typed<TY, F8_BIG>(a, p, s) : tile_typed<TY, F8_SMALL>(a, p, s);
+}
+
 int f8_launch_mul(const f8_mul_args *a, const f8_plan *p, void *stream)
 {
 	hipStream_t s = (hipStream_t)stream;
 	if (p->type == HIP_F8_F32)
-		p->big ? tile_typed<HIP_F8_F32, F8_BIG_F32>(a, p, s) : tile_typed<HIP_F8_F32, F8_SMALL_F32>(a, p, s);
+		mul_typed<HIP_F8_F32>(a, p, s);
 	else if (p->type == HIP_F8_F16)
-		p->big ? tile_typed<HIP_F8_F16, F8_BIG>(a, p, s) : tile_typed<HIP_F8_F16, F8_SMALL>(a, p, s);
+		mul_typed<HIP_F8_F16>(a, p, s);
 	else
-		p->big ? tile_typed<HIP_F8_BF16, F8_BIG>(a, p, s) : tile_typed<HIP_F8_BF16, F8_SMALL>(a, p, s);
+		mul_typed<HIP_F8_BF16>(a, p, s);
 	return hipGetLastError();
 }
