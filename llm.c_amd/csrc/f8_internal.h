@@ -35,8 +35,8 @@ typedef struct f8_mul_args {
 
 /* how a product is cut up, from the host's bounds alone */
 typedef struct f8_plan {
-	int type, form;
-	int bt, bn;      /* rows of X and outputs of a row of one workgroup's tile */
+	int type;         /* set by the caller */
+	int form;         /* of f8_mul.hip's */
 	size_t row_tiles; /* tiles of rows, at most, over all experts */
 	size_t n_tiles;
 	int threads;

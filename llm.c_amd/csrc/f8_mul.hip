@@ -680,7 +680,7 @@ __global__ __launch_bounds__(64 * WN * WT * KS) void k_f8_mid(f8_mul_args A, int
  * 64 bytes of each a load; what bounds it is how much of W is in flight.
  */
 template <int TY, bool GATED, int NF, int NT, int NW, int DEPTH>
-__global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles)
+__global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles, int)
 {
 	constexpr int M = GATED ? 2 : 1, FN = NF * M;
 	typedef f8_operand<TY == HIP_F8_F32> operand;
@@ -805,88 +805,165 @@ __global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles)
 	}
 }
 
-/* the forms: few rows by 16 NT, NF, NW and DEPTH; tiles by NA, NB, WN, WT, STAGES, FAR */
-#define F8_BIG 8, 4, 2, 4, 2, false     /* 256 x 256 */
-#define F8_BIG_F32 4, 4, 2, 4, 2, false /* 128 x 256 */
-#define F8_SMALL 2, 4, 4, 1, 3, true    /* 128 x 64 */
-#define F8_SMALL_F32 2, 2, 4, 2, 3, true /* 128 x 64 */
-#ifndef FEW1
-#define FEW1 1, 1, 8, 2
-#define FEW2 1, 2, 8, 1
-#define FEW4 1, 4, 8, 1
-#endif
+/*
+ * The forms, and what a call costs in each.  A form's workgroups run in rounds of
+ * `slots` that the chip holds at a time; a round takes `fixed` + `block` microseconds for
+ * each 128 channels, or where not even half of the slots are taken the same without the
+ * neighbours (`alone`).  Measured with 128 to 1024 workgroups, 1024 and 4096 channels (bf16
+ * and fp32 outputs); of the forms that apply the one with the smallest sum is taken, and
+ * where the loads into LDS take longer (10 TB/s of the chip's L2s), those.  Calls of
+ * many rounds cost the same as larger tiles' calls of few, so that sizes alone would not do.
+ *
+ *   4096 channels, us by workgroups     256   512  1024     (fp32  256   512  1024)
+ *   MID   32 x 128, 2 groups           12.9  22.9  43.8           18.1  33.2  63.4
+ *   MID   64 x 64, 4 groups            12.3  22.0  41.5           15.8  29.1  54.0
+ *   MID   64 x 128, 2 groups           17.7  32.8  60.3           25.8  47.2  92.3
+ *   MID  128 x 128, 2 groups              -     -     -           39.4  71.8   143
+ *   TILE  64 x 128                     19.7  30.9  55.7           32.7  47.4  85.8
+ *   TILE 128 x 128                     26.9  46.1  82.9           52.1  74.0   144
+ *   TILE 256 x 256                     70.4   149   296              -     -     -
+ *
+ * One to a few rows are bound by W's way from HBM: FEW.  4096 x 4096 for one row takes
+ * 7.4 us where a tile takes 21, 50304 x 2048 18 where it takes 26.  Waves of 16 outputs
+ * and eight to a workgroup where the outputs alone do not fill the chip (15.5 us
+ * instead of 21.5, 16 rows of 14336 to 4096), else four (18.1 instead of 23.7, the 50304),
+ * and 32 outputs where the product is gated (169 instead of 176, 16 tokens in 8 experts of 14336 x 4096).
+ */
+#define F8_FORMS(X)                                                                    \
+	/*  form        kernel   16-bit fp32  NA NB WN WT KS  STAGES FAR */                \
+	X(FEW_LONG, few, 1, 1, 1, 1, 8, 2)                                             \
+	X(FEW_WIDE, few, 1, 1, 1, 1, 4, 3)                                             \
+	X(FEW_GATED, few, 1, 1, 2, 1, 4, 2)                                            \
+	X(FEW_32, few, 1, 1, 2, 2, 4, 1)                                               \
+	X(MID_32, mid, 1, 1, 2, 2, 4, 1, 2, 3)                                         \
+	X(MID_64, mid, 1, 1, 2, 4, 2, 1, 4, 2)                                         \
+	X(MID_128, mid, 1, 1, 2, 4, 4, 1, 2, 3)                                        \
+	X(MID_SQUARE, mid, 0, 1, 4, 4, 2, 2, 2, 2)                                     \
+	X(TILE_64, tile, 1, 1, 2, 2, 4, 2, 3, true)                                    \
+	X(TILE_128, tile, 1, 0, 4, 2, 2, 4, 2, true)                                   \
+	X(TILE_128F, tile, 0, 1, 4, 4, 2, 2, 2, true)                                  \
+	X(TILE_256, tile, 1, 0, 8, 4, 2, 4, 2, false)
+
+enum {
+#define X(FORM, ...) FORM,
+	F8_FORMS(X)
+#undef X
+	FORMS
+};
+
+/* tiles and costs, by type (16 bits, fp32) */
+static const struct {
+	int bt, bn, threads, slots;
+	struct {
+		float fixed, block, alone_fixed, alone_block;
+	} us[2];
+} forms[FORMS] = {
+	/* in F8_FORMS' order */
+	{16, 16, 512, 0, {}},
+	{16, 16, 256, 0, {}},
+	{16, 32, 256, 0, {}},
+	{32, 32, 256, 0, {}},
+	{32, 128, 512, 256, {{2.5f, .25f, 2.5f, .25f}, {2.8f, .385f, 2.8f, .385f}}},
+	{64, 64, 512, 256, {{3.4f, .2f, 3.4f, .2f}, {3.6f, .277f, 3.6f, .277f}}},
+	{64, 128, 512, 256, {{3.4f, .32f, 3.4f, .32f}, {3.6f, .59f, 3.6f, .59f}}},
+	{128, 128, 512, 256, {{}, {4.7f, .97f, 4.7f, .97f}}},
+	{64, 128, 512, 512, {{4.7f, .63f, 2.5f, .46f}, {4.4f, 1.06f, 3.7f, .83f}}},
+	{128, 128, 512, 512, {{7.5f, .95f, 4.5f, .62f}, {}}},
+	{128, 128, 256, 512, {{}, {5.5f, 2.f, 7.2f, 1.32f}}},
+	{256, 256, 512, 256, {{16.f, 1.67f, 16.f, 1.57f}, {}}},
+};
+
+/* tiles of rows and of outputs; a grouped call's rows may end in a tile that is not
+ * full for every expert */
+static size_t row_tiles_of(const f8_mul_args *a, size_t bt)
+{
+	const size_t rows = (size_t)a->rows, count = (size_t)a->count;
+	return a->start ? rows / bt + (rows < count ? rows : count) : (rows + bt - 1) / bt;
+}
+
+static size_t n_tiles_of(const f8_mul_args *a, int form)
+{
+	/* the tiles' outputs are half of their rows of W where two matrices share them */
+	const size_t bn = (size_t)forms[form].bn / (form >= MID_32 && a->w[1] ? 2 : 1);
+	return ((size_t)a->n + bn - 1) / bn;
+}
+
+static float cost_of(const f8_mul_args *a, int form, int fp32)
+{
+	const size_t bt = (size_t)forms[form].bt, rows = (size_t)a->rows;
+	const size_t blocks = ((size_t)a->k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
+	/* an expert's last tile is half full, on average */
+	const size_t busy = rows < (size_t)a->count ? rows : (size_t)a->count;
+	const float tiles = a->start ? (float)rows / bt + .5f * busy : (float)((rows + bt - 1) / bt);
+	const float wgs = (a->start && tiles < busy ? busy : tiles) * n_tiles_of(a, form);
+	const float slots = forms[form].slots, r = wgs / slots;
+	const float rounds = r < 4 ? ceilf(r) : r;
+	const bool alone = r <= .5f;
+	const float less = a->w[1] ? .7f : 1; /* half the outputs to store */
+	const float us = alone ? less * forms[form].us[fp32].alone_fixed + blocks * forms[form].us[fp32].alone_block
+			       : rounds * (less * forms[form].us[fp32].fixed + blocks * forms[form].us[fp32].block);
+	const float loads = wgs * (bt + forms[form].bn) * blocks * HIP_F8_BLOCK / 10e6f;
+	return us > loads ? us : loads;
+}
 
 void f8_mul_plan(const f8_mul_args *a, f8_plan *p)
 {
-	const size_t rows = (size_t)a->rows, n = (size_t)a->n;
+	const size_t rows = (size_t)a->rows;
 	const size_t per = a->start ? (rows + (size_t)a->count - 1) / (size_t)a->count : rows;
-	p->form = per <= 16 ? 1 : per <= 32 ? 2 : per <= 64 ? 4 : 5;
-#ifdef F8_FORCE
-	if (getenv("F8_FORM"))
-		p->form = atoi(getenv("F8_FORM"));
-#endif
-	if (p->form == 5 && per > 128 && (!a->from || (size_t)a->x_rows * (size_t)a->x_stride < ((size_t)1 << 32) - F8_MAX_K))
-		p->form = 6;
-	static const int few[] = {FEW1, FEW2, FEW4};
-	const int *f = few + (p->form == 1 ? 0 : p->form == 2 ? 4 : 8);
-	if (p->form < 5) {
-		p->bt = 16 * f[1];
-		p->bn = 16 * f[0];
-		p->threads = 64 * f[2];
+	const int fp32 = p->type == HIP_F8_F32;
+	/* the rows of experts differ: those of 8 on average hardly ever are more than 16 */
+	if (per <= (a->start ? 8 : 16)) {
+		const size_t wide = row_tiles_of(a, 16) * (((size_t)a->n + 31) / 32);
+		p->form = wide < 512 ? FEW_LONG : a->w[1] ? FEW_GATED : FEW_WIDE;
+	} else if (a->start && per <= 24) {
+		p->form = FEW_32;
 	} else {
-		p->bt = p->form == 6 ? 256 : 64;
-		p->bn = (p->form == 6 && p->type != HIP_F8_F32 ? 256 : 128) / (a->w[1] ? 2 : 1);
-		p->threads = p->form == 6 || p->type == HIP_F8_F32 ? 512 : 256;
+		float best = 0;
+		for (int f = MID_32; f < FORMS; f++) {
+			if (forms[f].us[fp32].block == 0)
+				continue;
+			/* its rows' distances from X's first are 32 bits */
+			if (f == TILE_256 && a->from &&
+			    (size_t)a->x_rows * (size_t)a->x_stride >= ((size_t)1 << 32) - F8_MAX_K)
+				continue;
+			const float us = cost_of(a, f, fp32);
+			if (best == 0 || us < best) {
+				best = us;
+				p->form = f;
+			}
+		}
 	}
-	p->n_tiles = (n + (size_t)p->bn - 1) / (size_t)p->bn;
-	p->row_tiles = (rows + (size_t)p->bt - 1) / (size_t)p->bt;
-	if (a->start) /* every expert may end with a tile that is not full */
-		p->row_tiles = rows / (size_t)p->bt + (rows < (size_t)a->count ? rows : (size_t)a->count);
+	p->threads = forms[p->form].threads;
+	p->n_tiles = n_tiles_of(a, p->form);
+	p->row_tiles = row_tiles_of(a, (size_t)forms[p->form].bt);
 }
 
-template <int TY, auto... FORM>
-static void tile_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)
-{
-	const size_t grid = p->row_tiles * p->n_tiles;
-	if (a->w[1])
-		k_f8_tile<TY, true, FORM...><<<grid, p->threads, 0, s>>>(*a, (int)p->n_tiles, (int)p->row_tiles);
-	else
-		k_f8_tile<TY, false, FORM...><<<grid, p->threads, 0, s>>>(*a, (int)p->n_tiles, (int)p->row_tiles);
-}
-
-template <int TY, int... FORM>
-static void few_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)
-{
-	const size_t grid = p->row_tiles * p->n_tiles;
-	if (a->w[1])
-		k_f8_few<TY, true, FORM...><<<grid, p->threads, 0, s>>>(*a, (int)p->n_tiles);
-	else
-		k_f8_few<TY, false, FORM...><<<grid, p->threads, 0, s>>>(*a, (int)p->n_tiles);
-}
-
-template <int TY>
+template <int TY, bool GATED>
 static void mul_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)
 {
-	if (p->form == 1)
-		few_typed<TY, FEW1>(a, p, s);
-	else if (p->form == 2)
-		few_typed<TY, FEW2>(a, p, s);
-	else if (p->form == 4)
-		few_typed<TY, FEW4>(a, p, s);
-	else if constexpr (TY == HIP_F8_F32)
-		p->form == 6 ? tile_typed<TY, F8_BIG_F32>(a, p, s) : tile_typed<TY, F8_SMALL_F32>(a, p, s);
-	else
-		p->form == 6 ? tile_typed<TY, F8_BIG>(a, p, s) : tile_typed<TY, F8_SMALL>(a, p, s);
+	const size_t grid = p->row_tiles * p->n_tiles;
+	const int n_tiles = (int)p->n_tiles, row_tiles = (int)p->row_tiles;
+	switch (p->form) {
+#define X(FORM, KERNEL, HALF, FP32, ...)                                                           \
+	case FORM:                                                                                 \
+		if constexpr (TY == HIP_F8_F32 ? FP32 : HALF)                                      \
+			k_f8_##KERNEL<TY, GATED, __VA_ARGS__>                                      \
+				<<<grid, p->threads, 0, s>>>(*a, n_tiles, row_tiles);              \
+		break;
+		F8_FORMS(X)
+#undef X
+	}
 }
 
 int f8_launch_mul(const f8_mul_args *a, const f8_plan *p, void *stream)
 {
 	hipStream_t s = (hipStream_t)stream;
+	const bool gated = a->w[1] != NULL;
 	if (p->type == HIP_F8_F32)
-		mul_typed<HIP_F8_F32>(a, p, s);
+		gated ? mul_typed<HIP_F8_F32, true>(a, p, s) : mul_typed<HIP_F8_F32, false>(a, p, s);
 	else if (p->type == HIP_F8_F16)
-		mul_typed<HIP_F8_F16>(a, p, s);
+		gated ? mul_typed<HIP_F8_F16, true>(a, p, s) : mul_typed<HIP_F8_F16, false>(a, p, s);
 	else
-		mul_typed<HIP_F8_BF16>(a, p, s);
+		gated ? mul_typed<HIP_F8_BF16, true>(a, p, s) : mul_typed<HIP_F8_BF16, false>(a, p, s);
 	return hipGetLastError();
 }

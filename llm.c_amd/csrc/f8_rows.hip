@@ -132,74 +132,146 @@ int f8_launch_quantize(int type, const void *x, size_t x_stride, const hip_f8_ro
 
 /*
  * A workgroup an expert, and one more for the pairs without: each reads all ids, a
- * wave a stretch of them.  The counts of smaller ids and of its own give the
- * expert's first row and each wave's, ballots the rows inside a wave, so that the
- * order is the pairs' and nothing is shared between workgroups.
+ * wave a stretch of up to 4096 of each 65536.  The counts of smaller ids and of its own
+ * give the expert's first row and each wave's, ballots the rows inside a wave, so that
+ * the order is the pairs' and nothing is shared between workgroups.  Up to 65536 pairs
+ * are read once and stay in registers.  It is bound by its own chain: 8192 tokens of 8
+ * slots take 17 us, ten for the launch and 256 KB of ids in every workgroup, three each for
+ * counting, ranking and the scattered stores.  (Waves' loads next to each other, or
+ * starting at another place in each workgroup, took as long.)
  */
 #define SORT_WAVES 16
+#define SORT_LOADS 16 /* of 4 ids a lane */
 
+/* `loads` times 256 ids from a on; what is past the pairs is no expert's.  There is a
+ * pair at least. */
+__device__ static inline void sort_get(dw4 (&v)[SORT_LOADS], const u32 *__restrict__ ids, u32 a,
+				       int loads, u32 pairs)
+{
+	const u32 i0 = a + threadIdx.x % 64 * 4;
+	if (a + loads * 256 <= pairs) {
+#pragma unroll
+		for (int j = 0; j < SORT_LOADS; j++)
+			if (j < loads)
+				v[j] = *(const dw4 *)(ids + (i0 + j * 256));
+		return;
+	}
+#pragma unroll
+	for (int j = 0; j < SORT_LOADS; j++)
+		if (j < loads)
+#pragma unroll
+			for (u32 u = 0; u < 4; u++) {
+				const u32 i = i0 + j * 256 + u;
+				const u32 id = ids[i < pairs ? i : pairs - 1];
+				v[j].v[u] = i < pairs ? id : 0xffffffffu;
+			}
+}
+
+/* A pair's token is pair * magic >> (32 + shift), magic = 2^(32 + shift) / topk rounded up
+ * and 2^shift < topk <= 2^(shift + 1): magic is less than a whole too large, which moves
+ * the quotient by less than 2^31 / 2^(32 + shift) < 1 / topk (topk 1: magic 0). */
 __global__ __launch_bounds__(SORT_WAVES * 64) void k_f8_sort(
-	const u32 *__restrict__ ids, int pairs, int topk, int experts, int *__restrict__ start,
-	int *__restrict__ from, int *__restrict__ pos)
+	const u32 *__restrict__ ids, u32 pairs, int loads, u32 magic, int shift, int experts,
+	int *__restrict__ start, int *__restrict__ from, int *__restrict__ pos)
 {
 	__shared__ int n_own[SORT_WAVES], n_less[SORT_WAVES];
-	const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
+	const int lane = threadIdx.x % 64;
+	const u32 stretch = loads * 256, chunk = waves * stretch, chunks = (pairs + chunk - 1) / chunk;
 	const u32 e = blockIdx.x;
-	const bool none = (int)e == experts;
-	const int per = (int)(((long)pairs + SORT_WAVES * 64 - 1) / (SORT_WAVES * 64)) * 64;
-	const long a = (long)wave * per, b = a + per < pairs ? a + per : pairs;
-	if (none) {
-		for (long i = a + lane; i < b; i += 64)
+	if ((int)e == experts) {
+		for (u32 i = threadIdx.x; i < pairs; i += blockDim.x)
 			if (ids[i] >= e)
 				pos[i] = -1;
 		return;
 	}
-	int own = 0, less = 0;
-	for (long i = a + lane; i < b; i += 64) {
-		const u32 id = ids[i];
-		own += id == e;
-		less += id < e;
-	}
+	dw4 v[SORT_LOADS];
+	int less = 0;
+	/* the chunks from the last to the first, which stays in the registers */
+	for (u32 c = chunks; c-- > 0;) {
+		const u32 a = c * chunk + wave * stretch;
+		sort_get(v, ids, a, loads, pairs);
 #pragma unroll
-	for (int d = 1; d < 64; d *= 2) {
-		own += __shfl_xor(own, d);
-		less += __shfl_xor(less, d);
+		for (int j = 0; j < SORT_LOADS; j++)
+			if (j < loads) {
+#pragma unroll
+				for (int u = 0; u < 4; u++)
+					less += __popcll(__ballot(v[j].v[u] < e));
+			}
 	}
-	if (lane == 0) {
-		n_own[wave] = own;
-		n_less[wave] = less;
+	const unsigned long lower = (1ul << lane) - 1;
+	int first = 0, rows = 0; /* the expert's first, and its rows of the chunks before */
+	for (u32 c = 0; c < chunks; c++) {
+		const u32 a = c * chunk + wave * stretch;
+		if (c > 0)
+			sort_get(v, ids, a, loads, pairs);
+		int own = 0;
+#pragma unroll
+		for (int j = 0; j < SORT_LOADS; j++)
+			if (j < loads) {
+#pragma unroll
+				for (int u = 0; u < 4; u++)
+					own += __popcll(__ballot(v[j].v[u] == e));
+			}
+		if (lane == 0) {
+			n_own[wave] = own;
+			n_less[wave] = less;
+		}
+		__syncthreads();
+		int before = 0, all = 0;
+		for (int w = 0; w < waves; w++) {
+			first += c == 0 ? n_less[w] : 0;
+			before += w < wave ? n_own[w] : 0;
+			all += n_own[w];
+		}
+		int row = first + rows + before;
+		rows += all;
+#pragma unroll
+		for (int j = 0; j < SORT_LOADS; j++)
+			if (j < loads) {
+				int at = row;
+				bool mine[4];
+#pragma unroll
+				for (int u = 0; u < 4; u++) {
+					/* compared again: the masks of all loads have no room */
+					asm volatile("" : "+v"(v[j].v[u]));
+					mine[u] = v[j].v[u] == e;
+					const unsigned long m = __ballot(mine[u]);
+					at += __popcll(m & lower);
+					row += __popcll(m);
+				}
+#pragma unroll
+				for (int u = 0; u < 4; u++)
+					if (mine[u]) {
+						const u32 i = a + j * 256 + lane * 4 + u;
+						from[at] = magic ? (int)(__umulhi(i, magic) >> shift) : (int)i;
+						pos[i] = at++;
+					}
+			}
+		__syncthreads(); /* before the next chunk's counts */
 	}
-	__syncthreads();
-	int first = 0, row = 0, all = 0;
-	for (int w = 0; w < SORT_WAVES; w++) {
-		first += n_less[w];
-		row += w < wave ? n_own[w] : 0;
-		all += n_own[w];
-	}
-	row += first;
 	if (threadIdx.x == 0) {
 		start[e] = first;
 		if ((int)e == experts - 1)
-			start[experts] = first + all;
-	}
-	for (long i0 = a; i0 < b; i0 += 64) {
-		const long i = i0 + lane;
-		const bool mine = i < b && ids[i] == e;
-		const unsigned long m = __ballot(mine);
-		if (mine) {
-			const int r = row + __popcll(m & ((1ul << lane) - 1));
-			from[r] = (int)((u32)i / (u32)topk);
-			pos[i] = r;
-		}
-		row += __popcll(m);
+			start[experts] = first + rows;
 	}
 }
 
 int f8_launch_sort(const uint32_t *ids, int tokens, int topk, int experts, int32_t *start,
 		   int32_t *from, int32_t *pos, void *stream)
 {
-	k_f8_sort<<<experts + 1, SORT_WAVES * 64, 0, (hipStream_t)stream>>>(ids, tokens * topk, topk, experts,
-									      start, from, pos);
+	const long pairs = (long)tokens * topk;
+	/* as few loads a wave as sixteen waves allow */
+	long loads = (pairs + SORT_WAVES * 256 - 1) / (SORT_WAVES * 256);
+	loads = loads < 1 ? 1 : loads > SORT_LOADS ? SORT_LOADS : loads;
+	long waves = (pairs + loads * 256 - 1) / (loads * 256);
+	waves = waves < 1 ? 1 : waves > SORT_WAVES ? SORT_WAVES : waves;
+	int shift = 0;
+	while ((2 << shift) < topk)
+		shift++;
+	const u32 magic = topk == 1 ? 0 : (u32)((((uint64_t)1 << (32 + shift)) + topk - 1) / topk);
+	k_f8_sort<<<experts + 1, 64 * waves, 0, (hipStream_t)stream>>>(ids, (u32)pairs, (int)loads, magic, shift,
+									experts, start, from, pos);
 	return hipGetLastError();
 }
 

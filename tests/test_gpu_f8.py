@@ -288,7 +288,7 @@ def test_nan_codes_and_scales_stay_in_their_rows(dev, rows):
 
 @pytest.mark.parametrize("tokens,topk,experts", (
     (1, 1, 1), (1, 8, 64), (16, 2, 8), (5, 3, 130), (1000, 7, 12), (333, 8, 256), (4000, 6, 1024), (8192, 8, 64),
-    (70000, 1, 3)))
+    (70000, 1, 3), (65537, 1, 5), (30001, 9, 700)))
 @pytest.mark.parametrize("away", (0.0, 0.4, 1.0))
 def test_sort(dev, tokens, topk, experts, away):
     rng = np.random.default_rng(tokens + topk)
