@@ -97,7 +97,7 @@ __global__ __launch_bounds__(F8_ROW_THREADS) void k_f8_quantize(
 		}
 }
 
-#define QUANT_ROWS 4
+#define QUANT_ROWS 2
 
 size_t f8_quantize_grid(size_t rows, size_t k)
 {
