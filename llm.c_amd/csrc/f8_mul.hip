@@ -114,13 +114,13 @@ __device__ static inline int f8_clamp(int v, int lo, int hi)
  * of the lanes up to it */
 template <int BT> struct f8_scan {
 	int a, b, own, upto;
-	__device__ inline void get(const f8_mul_args &A, int e0)
+	__device__ inline void get(const f8_mul_args &A, const int *start, int e0)
 	{
 		const int lane = threadIdx.x % 64, e = e0 + lane;
 		a = b = 0;
 		if (e < A.count) {
-			a = f8_clamp(A.start[e], 0, A.rows);
-			b = f8_clamp(A.start[e + 1], a, A.rows);
+			a = f8_clamp(start[e], 0, A.rows);
+			b = f8_clamp(start[e + 1], a, A.rows);
 		}
 		own = upto = (b - a + BT - 1) / BT;
 #pragma unroll
@@ -129,8 +129,9 @@ template <int BT> struct f8_scan {
 			upto += lane >= d ? o : 0;
 		}
 	}
+	__device__ inline int all() const { return __builtin_amdgcn_readlane(upto, 63); }
 	/* tile `tile` of these, the first of which is tile `before` */
-	__device__ inline bool find(int tile, int before, int e0, f8_rows_of &R)
+	__device__ inline bool find(int tile, int before, int e0, f8_rows_of &R) const
 	{
 		const int first = before + upto - own;
 		const unsigned long m = __ballot(tile >= first && tile < first + own);
@@ -143,59 +144,58 @@ template <int BT> struct f8_scan {
 	}
 };
 
-__device__ static inline f8_rows_of f8_dense(const f8_mul_args &A, int tile, int bt)
-{
-	return f8_rows_of{0, tile * bt, tile * bt + bt < A.rows ? tile * bt + bt : A.rows};
-}
-
-/* Tile `tile` of BT rows over all experts, whose tiles follow each other */
+/* Tiles of BT rows over all experts, whose tiles follow each other; without experts the
+ * host's count */
 template <int BT>
-__device__ static inline f8_rows_of f8_find(const f8_mul_args &A, int tile)
+__device__ static inline int f8_row_tiles(const f8_mul_args &A, const int *start, int row_tiles)
 {
 	if (!A.start)
-		return f8_dense(A, tile, BT);
+		return row_tiles;
+	f8_scan<BT> s;
+	int n = 0;
+	for (int e0 = 0; e0 < A.count; e0 += 64) {
+		s.get(A, start, e0);
+		n += s.all();
+	}
+	return n;
+}
+
+/* Rows of such a tile, none past the last */
+template <int BT>
+__device__ static inline f8_rows_of f8_find(const f8_mul_args &A, const int *start, int tile)
+{
 	f8_rows_of R = {0, 0, 0};
+	if (!A.start) {
+		R.a = tile * BT;
+		R.b = R.a + BT < A.rows ? R.a + BT : A.rows;
+		return R;
+	}
 	f8_scan<BT> s;
 	int before = 0;
 	for (int e0 = 0; e0 < A.count; e0 += 64) {
-		s.get(A, e0);
+		s.get(A, start, e0);
 		if (s.find(tile, before, e0, R))
 			break;
-		before += __builtin_amdgcn_readlane(s.upto, 63);
+		before += s.all();
 	}
-	return R;
+	return f8_rows_of{__builtin_amdgcn_readfirstlane(R.e), __builtin_amdgcn_readfirstlane(R.a),
+			  __builtin_amdgcn_readfirstlane(R.b)};
 }
 
-/* The tile of a workgroup.  Workgroups go to the eight XCDs in turn: each takes a
- * stretch of the tiles, in groups of 8 row tiles that share what the L2 holds of W.  The
- * host knows the experts' tiles only at most: the stretches are of those that there are
- * (else the last XCDs have none, 1190 us instead of 1060 for 8 experts of 1000 rows). */
-template <int BT>
-__device__ static inline f8_rows_of f8_take(const f8_mul_args &A, int n_tiles, int row_tiles, int &n_tile)
+/* The tile that workgroup `turn` of n_tiles * row_tiles takes.  Workgroups go to the eight
+ * XCDs in turn: each XCD has a stretch of the tiles, in groups of 8 row tiles that share
+ * what its L2 holds of W.  The host knows the experts' tiles only at most: row_tiles are
+ * those that there are (else the last XCDs have none, 1190 us instead of 1110 for 8
+ * experts of 1000 rows). */
+__device__ static inline void f8_turn(int turn, int n_tiles, int row_tiles, int &row_tile, int &n_tile)
 {
-	f8_scan<BT> s;
-	if (A.start) {
-		row_tiles = 0;
-		for (int e0 = 0; e0 < A.count; e0 += 64) {
-			s.get(A, e0);
-			row_tiles += __builtin_amdgcn_readlane(s.upto, 63);
-		}
-	}
-	const int grid = n_tiles * row_tiles, xcd = blockIdx.x % 8;
-	f8_rows_of R = {0, 0, 0};
-	if ((int)blockIdx.x >= grid)
-		return R;
-	const int id = xcd * (grid / 8) + (xcd < grid % 8 ? xcd : grid % 8) + blockIdx.x / 8;
+	const int all = n_tiles * row_tiles, xcd = turn % 8;
+	const int id = xcd * (all / 8) + (xcd < all % 8 ? xcd : all % 8) + turn / 8;
 	const int group = id / (8 * n_tiles), g0 = group * 8;
 	const int many = row_tiles - g0 < 8 ? row_tiles - g0 : 8;
-	const int in = id - group * 8 * n_tiles, tile = g0 + in % many;
+	const int in = id - group * 8 * n_tiles;
+	row_tile = g0 + in % many;
 	n_tile = in / many;
-	if (!A.start)
-		return f8_dense(A, tile, BT);
-	if (A.count > 64)
-		return f8_find<BT>(A, tile);
-	s.find(tile, 0, 0, R);
-	return R;
 }
 
 __device__ static inline float f8_gate(float a, float b)
@@ -278,18 +278,24 @@ __device__ static inline void f8_meet()
 	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+/* The row of X that row i of a tile comes from (a tile's last row past its rows; from[r]
+ * is row r's); what is outside X reads its first row, and its outputs become NaN */
+__device__ static inline int f8_source(const f8_mul_args &A, const f8_rows_of &R, const int *from, int i)
+{
+	const int r = R.a + i < R.b ? R.a + i : R.b - 1;
+	const int x = A.from ? from[r] : r;
+	return (unsigned)x < (unsigned)A.x_rows ? x : 0;
+}
+
 /* Where a lane's scale of slot `slot` of a tile starts, and how far the next block's is:
  * X's rows 64 a slot, then W's, one for each of WN x NR outputs and M matrices */
 template <int M, int NR, int WN>
-__device__ static inline void f8_scale_from(const f8_mul_args &A, const f8_rows_of &R, int n0, int slot,
-					    int x_slots, const float *&p, long &step)
+__device__ static inline void f8_scale_from(const f8_mul_args &A, const f8_rows_of &R, const int *from,
+					    int n0, int slot, int x_slots, const float *&p, long &step)
 {
 	const int lane = threadIdx.x % 64;
 	if (slot < x_slots) {
-		int x = R.a + slot * 64 + lane;
-		x = x < R.b ? x : R.b - 1;
-		x = A.from ? A.from[x] : x;
-		p = A.xs + ((unsigned)x < (unsigned)A.x_rows ? x : 0);
+		p = A.xs + f8_source(A, R, from, slot * 64 + lane);
 		step = A.xs_stride;
 	} else {
 		const int m = lane % M;
@@ -301,10 +307,10 @@ __device__ static inline void f8_scale_from(const f8_mul_args &A, const f8_rows_
 }
 
 /* A wave's sums, of rows r0 .. and outputs n0 .., gated and stored: EACH operands give
- * a lane neighbouring outputs */
+ * a lane neighbouring outputs; from[r] is row r's of X */
 template <int TY, bool GATED, int NA, int NB, int EACH>
-__device__ static inline void f8_finish(const f8_mul_args &A, const f8_rows_of &R, int r0, int n0,
-					const float (&acc)[NA][NB][4])
+__device__ static inline void f8_finish(const f8_mul_args &A, const f8_rows_of &R, const int *from, int r0,
+					int n0, const float (&acc)[NA][NB][4])
 {
 	constexpr int FA = GATED ? NA / 2 : NA;
 	const int lane = threadIdx.x % 64;
@@ -313,7 +319,7 @@ __device__ static inline void f8_finish(const f8_mul_args &A, const f8_rows_of &
 		const int r = r0 + b * 16 + lane % 16;
 		if (r >= R.b)
 			continue;
-		const bool bad = A.from && (unsigned)A.from[r] >= (unsigned)A.x_rows;
+		const bool bad = A.from && (unsigned)from[r] >= (unsigned)A.x_rows;
 #pragma unroll
 		for (int f = 0; f < FA; f += EACH) {
 			float out[4 * EACH];
@@ -348,7 +354,7 @@ __device__ static inline void f8_finish(const f8_mul_args &A, const f8_rows_of &
  * i of an operand's 16 is the output that gives a lane 16 bytes of neighbouring ones
  * from as many operands as that takes, and four lanes 64 bytes.
  */
-template <int TY, bool GATED, int NA, int NB, int WN, int WT, int STAGES, bool FAR>
+template <int TY, bool GATED, int NA, int NB, int WN, int WT, int STAGES, bool STREAM>
 __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_tiles, int row_tiles)
 {
 	constexpr int M = GATED ? 2 : 1, FA = NA / M; /* operands of one matrix */
@@ -366,76 +372,114 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 	static_assert(SCALES / 64 < NW && WN * M <= 64, "a wave is left for W's scales");
 	typedef f8_operand<TY == HIP_F8_F32> operand;
 	__shared__ __attribute__((aligned(16))) uint8_t lds[STAGES * (BYTES1 + BYTES2)];
+	__shared__ int starts[STREAM ? F8_MAX_COUNT + 1 : 1], froms[STREAM ? 2 : 1][STREAM ? BT : 1];
 
 	const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 	const int wn = wave % WN, wt = wave / WN;
-	int n0 = 0;
-	f8_rows_of R = f8_take<BT>(A, n_tiles, row_tiles, n0);
-	n0 = __builtin_amdgcn_readfirstlane(n0 * NO);
-	R.e = __builtin_amdgcn_readfirstlane(R.e);
-	R.a = __builtin_amdgcn_readfirstlane(R.a);
-	R.b = __builtin_amdgcn_readfirstlane(R.b);
-	if (R.a >= R.b)
-		return;
-
-	/* what this wave loads: slots of eight rows, X's, W's first half, W's second; a row
-	 * by its distance from the tile's first, or where X is gathered from X's first */
-	const int piece = ((lane % 8) ^ (lane / 8)) * 16, last = (A.k - 1) & ~15;
-	const uint8_t *const first = A.from ? A.x : A.x + R.a * A.x_stride;
-	const uint64_t from_x = f8_shared(first);
-	const uint64_t from_w = f8_shared(A.w[0] + R.e * A.w_step[0] + n0 * A.w_stride[0]);
-	const uint64_t from_u = f8_shared(A.w[M - 1] + R.e * A.w_step[M - 1] + n0 * A.w_stride[M - 1]);
-	u32 off[SLOTS1 + SLOTS2];
-	const uint8_t *far[FAR ? XSLOTS : 1];
-#pragma unroll
-	for (int i = 0; i < SLOTS1 + SLOTS2; i++) {
-		const int row = (wave + i * NW) * 8 + lane / 8;
-		if (i < XSLOTS) {
-			int x = R.a + row < R.b ? R.a + row : R.b - 1;
-			if (A.from) {
-				x = A.from[x];
-				x = (unsigned)x < (unsigned)A.x_rows ? x : 0;
-			} else {
-				x -= R.a;
-			}
-			off[i] = FAR ? 0 : (u32)x * (u32)A.x_stride;
-			if constexpr (FAR)
-				far[i] = first + x * A.x_stride;
-		} else {
-			/* half (gated: matrix), wn, operand of the half, row of it */
-			const int j = row - BT, r = j % 16;
-			const int f = (j / (BN / 2) * HALF + j / 16 % HALF) % FA;
-			const int n = j / (16 * HALF) % WN * (16 * FA) + f / EACH * (16 * EACH) +
-				      r / 4 * (4 * EACH) + f % EACH * 4 + r % 4;
-			off[i] = (u32)(n0 + n < A.n ? n : A.n - 1 - n0) * (u32)A.w_stride[i < SLOTS1 ? 0 : M - 1];
+	/* what a stream asks about experts and rows for its next tiles comes from LDS: a load
+	 * into registers would wait for all that are in flight */
+	if constexpr (STREAM) {
+		if (A.start) {
+			for (int i = threadIdx.x; i <= A.count; i += 64 * NW)
+				starts[i] = A.start[i];
+			__syncthreads();
 		}
 	}
+	const int *const start = STREAM ? starts : A.start;
+	row_tiles = f8_row_tiles<BT>(A, start, row_tiles);
+	const int turns = n_tiles * row_tiles;
+	int turn = blockIdx.x;
+	if (turn >= turns)
+		return;
+	auto take = [&](int at, f8_rows_of &T, int &tn) {
+		int tile;
+		f8_turn(at, n_tiles, row_tiles, tile, tn);
+		tn *= NO;
+		T = f8_find<BT>(A, start, tile);
+	};
+	f8_rows_of R, next_R = {0, 0, 0};
+	int n0, next_n0 = 0, ring = 0;
+	bool more = false;
+	take(turn, R, n0);
+	if constexpr (STREAM) {
+		if (A.from) {
+			for (int i = threadIdx.x; i < BT; i += 64 * NW)
+				froms[0][i] = A.from[R.a + i < R.b ? R.a + i : R.b - 1];
+			__syncthreads();
+		}
+	}
+	/* its rows' sources, from[r] for row r */
+	auto from_of = [&](const f8_rows_of &T, int which) -> const int * {
+		return STREAM ? froms[which] - T.a : A.from;
+	};
+
+	/* what this wave loads of a tile: slots of eight rows, X's, W's first half, W's second; a
+	 * row by its distance from the tile's first, or where X is gathered from X's first (32
+	 * bits; not in a stream X's whole addresses) */
+	const int piece = ((lane % 8) ^ (lane / 8)) * 16, last = (A.k - 1) & ~15;
+	uint64_t from_x = 0, from_w, from_u;
+	u32 off[SLOTS1 + SLOTS2];
+	const uint8_t *far[STREAM ? 1 : XSLOTS];
 	/* and of the scales: X's 64 at a time, then W's */
 	const float *ps;
 	long ps_step;
 	const int sslot = wave < SCALES / 64 ? wave : SCALES / 64;
-	f8_scale_from<M, 16 * FA, WN>(A, R, n0, sslot, SCALES / 64, ps, ps_step);
+	auto w_row = [&](int i, int tn) {
+		/* half (gated: matrix), wn, operand of the half, row of it */
+		const int j = (wave + i * NW) * 8 + lane / 8 - BT, r = j % 16;
+		const int f = (j / (BN / 2) * HALF + j / 16 % HALF) % FA;
+		const int n = j / (16 * HALF) % WN * (16 * FA) + f / EACH * (16 * EACH) +
+			      r / 4 * (4 * EACH) + f % EACH * 4 + r % 4;
+		return (u32)(tn + n < A.n ? n : A.n - 1 - tn);
+	};
+	auto set1 = [&](const f8_rows_of &T, int tn, const int *from) {
+		if constexpr (STREAM)
+			from_x = f8_shared(A.from ? A.x : A.x + T.a * A.x_stride);
+		from_w = f8_shared(A.w[0] + T.e * A.w_step[0] + tn * A.w_stride[0]);
+#pragma unroll
+		for (int i = 0; i < SLOTS1; i++) {
+			if (i >= XSLOTS) {
+				off[i] = w_row(i, tn) * (u32)A.w_stride[0];
+				continue;
+			}
+			const int x = f8_source(A, T, from, (wave + i * NW) * 8 + lane / 8);
+			if constexpr (STREAM)
+				off[i] = (u32)(A.from ? x : x - T.a) * (u32)A.x_stride;
+			else
+				far[i] = A.x + x * A.x_stride;
+		}
+		f8_scale_from<M, 16 * FA, WN>(A, T, from, tn, sslot, SCALES / 64, ps, ps_step);
+	};
+	auto set2 = [&](const f8_rows_of &T, int tn) {
+		from_u = f8_shared(A.w[M - 1] + T.e * A.w_step[M - 1] + tn * A.w_stride[M - 1]);
+#pragma unroll
+		for (int i = SLOTS1; i < SLOTS1 + SLOTS2; i++)
+			off[i] = w_row(i, tn) * (u32)A.w_stride[M - 1];
+	};
+	set1(R, n0, from_of(R, 0));
+	set2(R, n0);
 	const int blocks = (A.k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
 	const bool rest = A.k % HIP_F8_BLOCK;
 	uint8_t *const lds2 = lds + STAGES * BYTES1;
 	const u32 base1 = lds_addr(lds), base2 = lds_addr(lds2);
-	/* a block's part into a buffer; past the last block the last again, which nothing reads */
+	/* a block's part into a buffer; past the last block the next tile's, or without one the
+	 * last again, which nothing reads */
 	auto load1 = [&](int kb, int stage) {
-		kb = kb < blocks ? kb : blocks - 1;
+		kb = kb < blocks ? kb : STREAM && more ? kb - blocks : blocks - 1;
 		int c = kb * HIP_F8_BLOCK + piece;
 		c = c < last ? c : last; /* nothing past the row's last 16 that hold any is read */
 #pragma unroll
 		for (int i = 0; i < SLOTS1; i++) {
 			const u32 to = base1 + stage * BYTES1 + (wave + i * NW) * 1024;
-			if (FAR && i < XSLOTS)
-				f8_dma16(far[i < XSLOTS ? i : 0] + c, to);
+			if (!STREAM && i < XSLOTS)
+				f8_dma16(far[STREAM ? 0 : i < XSLOTS ? i : 0] + c, to);
 			else
 				f8_dma16(i < XSLOTS ? from_x : from_w, off[i] + c, to);
 		}
 		f8_dma4(ps + kb * ps_step, base1 + stage * BYTES1 + ROWS1 * HIP_F8_BLOCK + sslot * 256);
 	};
 	auto load2 = [&](int kb, int stage) {
-		kb = kb < blocks ? kb : blocks - 1;
+		kb = kb < blocks ? kb : STREAM && more ? kb - blocks : blocks - 1;
 		int c = kb * HIP_F8_BLOCK + piece;
 		c = c < last ? c : last;
 #pragma unroll
@@ -491,7 +535,7 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 	float acc[NA][NB][4] = {};
 	floatx4 y[4] = {};
 	int stage = 0;
-	for (int kb = 0; kb < blocks; kb++) {
+	for (int kb = 0;;) {
 		const int next = stage + 1 == STAGES ? 0 : stage + 1;
 		operand x[NB], w;
 #pragma unroll
@@ -501,12 +545,28 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 		for (int a = 0; a < NA; a++) {
 			if (a == HALF - 1) { /* all have read the first part */
 				f8_meet<AHEAD>();
+				if (STREAM && kb == 0) {
+					more = turn + (int)gridDim.x < turns;
+					if (more) {
+						take(turn + gridDim.x, next_R, next_n0);
+						if (A.from) { /* read two meetings on */
+							const int i = wave % (BT / 64) * 64 + lane;
+							const int r = next_R.a + i < next_R.b ? next_R.a + i : next_R.b - 1;
+							f8_dma4((const float *)(A.from + r),
+								lds_addr(&froms[STREAM ? ring ^ 1 : 0][wave % (BT / 64) * 64]));
+						}
+					}
+				}
+				if (STREAM && kb == blocks - STAGES && more)
+					set1(next_R, next_n0, from_of(next_R, ring ^ 1));
 				load1(kb + STAGES, stage);
 				if (kb == blocks - 1 && rest)
 					cut(lds2 + stage * BYTES2, ROWS2);
 			}
 			if (a == NA - 1) { /* all have read the second */
 				f8_meet<AHEAD>();
+				if (STREAM && kb == blocks - STAGES && more)
+					set2(next_R, next_n0);
 				load2(kb + STAGES, stage);
 				if (kb == blocks - 2 && rest)
 					cut(lds + next * BYTES1, ROWS1);
@@ -537,15 +597,37 @@ __global__ __launch_bounds__(64 * WN * WT) void k_f8_tile(f8_mul_args A, int n_t
 			s_last[i] = s[M - 1][NB - LAG + i];
 		read_s(next);
 		stage = next;
+		if (++kb < blocks)
+			continue;
+#pragma unroll
+		for (int i = 0; i < LAG; i++)
+#pragma unroll
+			for (int u = 0; u < 4; u++)
+				acc[NA - 1][NB - LAG + i][u] = __builtin_fmaf(y[(NA * NB - LAG + i) % 4][u], s_last[i],
+									      acc[NA - 1][NB - LAG + i][u]);
+		if (!more)
+			f8_meet<0>(); /* no load outlives the workgroup's LDS */
+		f8_finish<TY, GATED, NA, NB, EACH>(A, R, from_of(R, ring), R.a + wt * NB * 16, n0 + wn * 16 * FA, acc);
+		if (!more)
+			break;
+		turn += gridDim.x;
+		R = next_R;
+		n0 = next_n0;
+		ring ^= 1;
+		kb = 0;
+#pragma unroll
+		for (int a = 0; a < NA; a++)
+#pragma unroll
+			for (int b = 0; b < NB; b++)
+#pragma unroll
+				for (int u = 0; u < 4; u++)
+					acc[a][b][u] = 0.0f;
+#pragma unroll
+		for (int i = 0; i < LAG; i++) {
+			s_last[i] = 0.0f;
+			y[(NA * NB - LAG + i) % 4] = floatx4{0, 0, 0, 0};
+		}
 	}
-#pragma unroll
-	for (int i = 0; i < LAG; i++)
-#pragma unroll
-		for (int u = 0; u < 4; u++)
-			acc[NA - 1][NB - LAG + i][u] =
-				__builtin_fmaf(y[(NA * NB - LAG + i) % 4][u], s_last[i], acc[NA - 1][NB - LAG + i][u]);
-	f8_meet<0>(); /* no load outlives the workgroup's LDS */
-	f8_finish<TY, GATED, NA, NB, EACH>(A, R, R.a + wt * NB * 16, n0 + wn * 16 * FA, acc);
 }
 
 /*
@@ -574,14 +656,13 @@ __global__ __launch_bounds__(64 * WN * WT * KS) void k_f8_mid(f8_mul_args A, int
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 % NW);
 	const int ks = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 / NW);
 	const int wn = wave % WN, wt = wave / WN;
-	int n0 = 0;
-	f8_rows_of R = f8_take<BT>(A, n_tiles, row_tiles, n0);
-	n0 = __builtin_amdgcn_readfirstlane(n0 * NO);
-	R.e = __builtin_amdgcn_readfirstlane(R.e);
-	R.a = __builtin_amdgcn_readfirstlane(R.a);
-	R.b = __builtin_amdgcn_readfirstlane(R.b);
-	if (R.a >= R.b)
+	row_tiles = f8_row_tiles<BT>(A, A.start, row_tiles);
+	if ((int)blockIdx.x >= n_tiles * row_tiles)
 		return;
+	int tile, n0;
+	f8_turn(blockIdx.x, n_tiles, row_tiles, tile, n0);
+	n0 *= NO;
+	const f8_rows_of R = f8_find<BT>(A, A.start, tile);
 
 	const int piece = ((lane % 8) ^ (lane / 8)) * 16, last = (A.k - 1) & ~15;
 	const uint8_t *p[SLOTS];
@@ -589,10 +670,7 @@ __global__ __launch_bounds__(64 * WN * WT * KS) void k_f8_mid(f8_mul_args A, int
 	for (int i = 0; i < SLOTS; i++) {
 		const int row = (wave + i * NW) * 8 + lane / 8;
 		if (i < XSLOTS) {
-			int x = R.a + row < R.b ? R.a + row : R.b - 1;
-			x = A.from ? A.from[x] : x;
-			x = (unsigned)x < (unsigned)A.x_rows ? x : 0;
-			p[i] = A.x + x * A.x_stride;
+			p[i] = A.x + f8_source(A, R, A.from, row) * A.x_stride;
 		} else {
 			/* wn, operand of its NA, row of it */
 			const int j = row - BT, r = j % 16, a = j / 16 % NA, m = a / FA, f = a % FA;
@@ -606,7 +684,7 @@ __global__ __launch_bounds__(64 * WN * WT * KS) void k_f8_mid(f8_mul_args A, int
 	const float *ps;
 	long ps_step;
 	const int sslot = wave < SCALES / 64 ? wave : SCALES / 64;
-	f8_scale_from<M, 16 * FA, WN>(A, R, n0, sslot, SCALES / 64, ps, ps_step);
+	f8_scale_from<M, 16 * FA, WN>(A, R, A.from, n0, sslot, SCALES / 64, ps, ps_step);
 
 	const int blocks = (A.k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK, steps = (blocks + KS - 1) / KS;
 	const u32 base = lds_addr(lds);
@@ -708,7 +786,7 @@ __global__ __launch_bounds__(64 * WN * WT * KS) void k_f8_mid(f8_mul_args A, int
 						acc[a][b][u] += v[u];
 				}
 	}
-	f8_finish<TY, GATED, NA, NB, EACH>(A, R, R.a + wt * NB * 16, n0 + wn * 16 * FA, acc);
+	f8_finish<TY, GATED, NA, NB, EACH>(A, R, A.from, R.a + wt * NB * 16, n0 + wn * 16 * FA, acc);
 }
 
 /*
@@ -725,10 +803,7 @@ __global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles, 
 	__shared__ floatx4 sums[NW][FN][NT][64];
 	const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 	const int tile = blockIdx.x / n_tiles, n0 = blockIdx.x % n_tiles * (16 * NF);
-	f8_rows_of R = f8_find<16 * NT>(A, tile);
-	R.e = __builtin_amdgcn_readfirstlane(R.e);
-	R.a = __builtin_amdgcn_readfirstlane(R.a);
-	R.b = __builtin_amdgcn_readfirstlane(R.b);
+	const f8_rows_of R = f8_find<16 * NT>(A, A.start, tile);
 	if (R.a >= R.b)
 		return;
 	const int piece = lane / 16 * 16, last = (A.k - 1) & ~15; /* of each 64 channels */
@@ -868,7 +943,7 @@ __global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles, 
  * and 32 outputs where the product is gated (169 instead of 176, 16 tokens in 8 experts of 14336 x 4096).
  */
 #define F8_FORMS(X)                                                                    \
-	/*  form        kernel   16-bit fp32  NA NB WN WT KS  STAGES FAR */                \
+	/*  form        kernel   16-bit fp32  NA NB WN WT KS STAGES STREAM */               \
 	X(FEW_LONG, few, 1, 1, 1, 1, 8, 2)                                             \
 	X(FEW_WIDE, few, 1, 1, 1, 1, 4, 3)                                             \
 	X(FEW_GATED, few, 1, 1, 2, 1, 4, 2)                                            \
@@ -877,10 +952,10 @@ __global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles, 
 	X(MID_64, mid, 1, 1, 2, 4, 2, 1, 4, 2)                                         \
 	X(MID_128, mid, 1, 1, 2, 4, 4, 1, 2, 3)                                        \
 	X(MID_SQUARE, mid, 0, 1, 4, 4, 2, 2, 2, 2)                                     \
-	X(TILE_64, tile, 1, 1, 2, 2, 4, 2, 3, true)                                    \
-	X(TILE_128, tile, 1, 0, 4, 2, 2, 4, 2, true)                                   \
-	X(TILE_128F, tile, 0, 1, 4, 4, 2, 2, 2, true)                                  \
-	X(TILE_256, tile, 1, 0, 8, 4, 2, 4, 2, false)
+	X(TILE_64, tile, 1, 1, 2, 2, 4, 2, 3, false)                                   \
+	X(TILE_128, tile, 1, 0, 4, 2, 2, 4, 2, false)                                  \
+	X(TILE_128F, tile, 0, 1, 4, 4, 2, 2, 2, false)                                 \
+	X(TILE_256, tile, 1, 0, 8, 4, 2, 4, 2, true)
 
 enum {
 #define X(FORM, ...) FORM,
@@ -960,9 +1035,11 @@ void f8_mul_plan(const f8_mul_args *a, f8_plan *p)
 		for (int f = MID_32; f < FORMS; f++) {
 			if (forms[f].us[fp32].block == 0)
 				continue;
-			/* its rows' distances from X's first are 32 bits */
-			if (f == TILE_256 && a->from &&
-			    (size_t)a->x_rows * (size_t)a->x_stride >= ((size_t)1 << 32) - F8_MAX_K)
+			/* its rows' distances from X's first are 32 bits; it asks for the next tile two
+			 * steps ahead */
+			if (f == TILE_256 &&
+			    (a->k <= 2 * HIP_F8_BLOCK ||
+			     (a->from && (size_t)a->x_rows * (size_t)a->x_stride >= ((size_t)1 << 32) - F8_MAX_K)))
 				continue;
 			const float us = cost_of(a, f, fp32);
 			if (best == 0 || us < best) {
@@ -976,10 +1053,13 @@ void f8_mul_plan(const f8_mul_args *a, f8_plan *p)
 	p->row_tiles = row_tiles_of(a, (size_t)forms[p->form].bt);
 }
 
+#define F8_CUS 256
+
 template <int TY, bool GATED>
 static void mul_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)
 {
-	const size_t grid = p->row_tiles * p->n_tiles;
+	/* a stream's workgroups take tile after tile */
+	const size_t all = p->row_tiles * p->n_tiles, grid = p->form == TILE_256 && all > F8_CUS ? F8_CUS : all;
 	const int n_tiles = (int)p->n_tiles, row_tiles = (int)p->row_tiles;
 	switch (p->form) {
 #define X(FORM, KERNEL, HALF, FP32, ...)                                                           \
