@@ -954,22 +954,28 @@ __global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles, 
 }
 
 /*
- * The forms, and what a call costs in each.  A form's workgroups run in rounds of
- * `slots` that the chip holds at a time; a round takes `fixed` + `block` microseconds for
- * each 128 channels, or where not even half of the slots are taken the same without the
- * neighbours (`alone`).  Measured with 128 to 1024 workgroups, 1024 and 4096 channels (bf16
- * and fp32 outputs); of the forms that apply the one with the smallest sum is taken, and
- * where the loads into LDS take longer (10 TB/s of the chip's L2s), those.  Calls of
- * many rounds cost the same as larger tiles' calls of few, so that sizes alone would not do.
+ * The forms, and what a call costs in each.  With `n` of a form's workgroups to each of
+ * the 256 compute units, rounded up where they are few, a call takes
+ *   fixed + block * blocks + (n - 1) (more_fixed + more_block * blocks)
+ * microseconds, blocks of 128 channels; the first of them alone on its unit, later ones
+ * next to others.  The four were fitted to 420 calls, dense and grouped (16 to 8192 rows, 1024 to
+ * 14336 outputs, 400 to 5120 channels, up to 64 experts), timed in every form.  The form with the
+ * smallest sum took 2 % longer than the fastest on average for 16 bits and 1 % for fp32, and 2 and
+ * 0.2 % in 160 other calls; in nine of ten at most 8 %.  Sizes alone would not do:
+ * calls of many rounds cost the same as larger tiles' calls of few.
  *
- *   4096 channels, us by workgroups     256   512  1024     (fp32  256   512  1024)
- *   MID   32 x 128, 2 groups           12.9  22.9  43.8           18.1  33.2  63.4
- *   MID   64 x 64, 4 groups            12.3  22.0  41.5           15.8  29.1  54.0
- *   MID   64 x 128, 2 groups           17.7  32.8  60.3           25.8  47.2  92.3
- *   MID  128 x 128, 2 groups              -     -     -           39.4  71.8   143
- *   TILE  64 x 128                     19.7  30.9  55.7           32.7  47.4  85.8
- *   TILE 128 x 128                     26.9  46.1  82.9           52.1  74.0   144
- *   TILE 256 x 256                     70.4   149   296              -     -     -
+ *   4096 channels, us by workgroups     256   512   768  1536     (fp32  256   512   768  1536)
+ *   MID   32 x 128, 2 groups           12.7  22.6  33.2  62.8           18.3  32.9  48.2  94.0
+ *   MID   64 x 64, 4 groups            12.6  22.5  32.3  62.3           16.7  29.3  44.5  86.1
+ *   MID   64 x 128, 2 groups           17.0  32.0  47.0  90.9           25.6  47.9  70.7   138
+ *   MID  128 x 128, 2 groups              -     -     -     -           39.4  71.8     -     -
+ *   TILE  64 x 128                     24.3  31.3  42.1  80.2           35.2  47.6  63.9   122
+ *   TILE 128 x 128                     28.4  45.9  67.7   131           53.4  76.2   115   225
+ *   TILE 256 x 256                     78.7   147   222   431              -     -     -     -
+ *
+ * TILE's 64 x 128 by four waves with two stages, three workgroups a compute unit: eight
+ * waves with three stages, two workgroups, took 46.3 and 86.7 us for 768 and 1536 (fp32
+ * 70.7 and 138: four operands to convert for 4 products instead of six for 8).
  *
  * One to a few rows are bound by W's way from HBM: FEW.  4096 x 4096 for one row takes
  * 7.4 us where a tile takes 21, 50304 x 2048 18 where it takes 26.  Waves of 16 outputs
@@ -987,10 +993,12 @@ __global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles, 
 	X(MID_64, mid, 1, 1, 2, 4, 2, 1, 4, 2)                                         \
 	X(MID_128, mid, 1, 1, 2, 4, 4, 1, 2, 3)                                        \
 	X(MID_SQUARE, mid, 0, 1, 4, 4, 2, 2, 2, 2)                                     \
-	X(TILE_64, tile, 1, 1, 2, 2, 4, 2, 3, false)                                   \
+	X(TILE_64, tile, 1, 1, 4, 2, 2, 2, 2, false)                                   \
 	X(TILE_128, tile, 1, 0, 4, 2, 2, 4, 2, false)                                  \
 	X(TILE_128F, tile, 0, 1, 4, 4, 2, 2, 2, false)                                 \
 	X(TILE_256, tile, 1, 0, 8, 4, 2, 4, 2, true)
+
+#define F8_CUS 256
 
 enum {
 #define X(FORM, ...) FORM,
@@ -1001,24 +1009,24 @@ enum {
 
 /* tiles and costs, by type (16 bits, fp32) */
 static const struct {
-	int bt, bn, threads, slots;
+	int bt, bn, threads;
 	struct {
-		float fixed, block, alone_fixed, alone_block;
+		float fixed, block, more_fixed, more_block;
 	} us[2];
 } forms[FORMS] = {
 	/* in F8_FORMS' order */
-	{16, 16, 512, 0, {}},
-	{16, 16, 256, 0, {}},
-	{16, 32, 256, 0, {}},
-	{32, 32, 256, 0, {}},
-	{32, 128, 512, 256, {{2.5f, .25f, 2.5f, .25f}, {2.8f, .385f, 2.8f, .385f}}},
-	{64, 64, 512, 256, {{3.4f, .2f, 3.4f, .2f}, {3.6f, .277f, 3.6f, .277f}}},
-	{64, 128, 512, 256, {{3.4f, .32f, 3.4f, .32f}, {3.6f, .59f, 3.6f, .59f}}},
-	{128, 128, 512, 256, {{}, {4.7f, .97f, 4.7f, .97f}}},
-	{64, 128, 512, 512, {{4.7f, .63f, 2.5f, .46f}, {4.4f, 1.06f, 3.7f, .83f}}},
-	{128, 128, 512, 512, {{7.5f, .95f, 4.5f, .62f}, {}}},
-	{128, 128, 256, 512, {{}, {5.5f, 2.f, 7.2f, 1.32f}}},
-	{256, 256, 512, 256, {{16.f, 1.67f, 16.f, 1.57f}, {}}},
+	{16, 16, 512, {}},
+	{16, 16, 256, {}},
+	{16, 32, 256, {}},
+	{32, 32, 256, {}},
+	{32, 128, 512, {{3.2f, .17f, 3.3f, .42f}, {2.5f, .36f, 4.4f, .52f}}},
+	{64, 64, 512, {{4.6f, .13f, 5.f, .27f}, {2.9f, .29f, 5.f, .39f}}},
+	{64, 128, 512, {{2.8f, .27f, 5.4f, .56f}, {2.2f, .56f, 6.7f, .68f}}},
+	{128, 128, 512, {{}, {5.7f, .84f, 8.8f, 1.05f}}},
+	{64, 128, 256, {{2.2f, .49f, 2.3f, .38f}, {2.6f, .67f, 2.9f, .59f}}},
+	{128, 128, 512, {{1.9f, .55f, 4.3f, .62f}, {}}},
+	{128, 128, 256, {{}, {6.6f, 1.08f, 4.6f, 1.f}}},
+	{256, 256, 512, {{10.8f, 1.55f, 10.1f, 1.42f}, {}}},
 };
 
 /* tiles of rows and of outputs; a grouped call's rows may end in a tile that is not
@@ -1038,20 +1046,19 @@ static size_t n_tiles_of(const f8_mul_args *a, int form)
 
 static float cost_of(const f8_mul_args *a, int form, int fp32)
 {
-	const size_t bt = (size_t)forms[form].bt, rows = (size_t)a->rows;
-	const size_t blocks = ((size_t)a->k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
-	/* an expert's last tile is half full, on average */
-	const size_t busy = rows < (size_t)a->count ? rows : (size_t)a->count;
-	const float tiles = a->start ? (float)rows / bt + .5f * busy : (float)((rows + bt - 1) / bt);
-	const float wgs = (a->start && tiles < busy ? busy : tiles) * n_tiles_of(a, form);
-	const float slots = forms[form].slots, r = wgs / slots;
-	const float rounds = r < 4 ? ceilf(r) : r;
-	const bool alone = r <= .5f;
+	const float bt = forms[form].bt, rows = a->rows, busy = rows < a->count ? rows : a->count;
+	const float blocks = (a->k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
+	float tiles = ceilf(rows / bt);
+	if (a->start) {
+		/* between experts that have the same rows and some whose last tile is half full */
+		const float even = busy * ceilf(rows / busy / bt), uneven = rows / bt + .5f * busy;
+		tiles = .5f * (even + (uneven > busy ? uneven : busy));
+	}
+	float n = tiles * n_tiles_of(a, form) / F8_CUS;
+	n = n < 6 ? ceilf(n) : n;
 	const float less = a->w[1] ? .7f : 1; /* half the outputs to store */
-	const float us = alone ? less * forms[form].us[fp32].alone_fixed + blocks * forms[form].us[fp32].alone_block
-			       : rounds * (less * forms[form].us[fp32].fixed + blocks * forms[form].us[fp32].block);
-	const float loads = wgs * (bt + forms[form].bn) * blocks * HIP_F8_BLOCK / 10e6f;
-	return us > loads ? us : loads;
+	const auto &c = forms[form].us[fp32];
+	return less * c.fixed + c.block * blocks + (n - 1) * (less * c.more_fixed + c.more_block * blocks);
 }
 
 void f8_mul_plan(const f8_mul_args *a, f8_plan *p)
@@ -1087,8 +1094,6 @@ void f8_mul_plan(const f8_mul_args *a, f8_plan *p)
 	p->n_tiles = n_tiles_of(a, p->form);
 	p->row_tiles = row_tiles_of(a, (size_t)forms[p->form].bt);
 }
-
-#define F8_CUS 256
 
 template <int TY, bool GATED>
 static void mul_typed(const f8_mul_args *a, const f8_plan *p, hipStream_t s)

@@ -30,7 +30,7 @@ def sort(n, topk=1, experts=8):
 @pytest.mark.parametrize("call,kernel", (
     ("quantize(5)", "k_f8_quantize"), ("sort(5)", "k_f8_sort"), ("sort(0)", "k_f8_sort"),
     ("combine(5)", "k_f8_combine"), ("mul(1)", "k_f8_few"), ("mul(16, F32)", "k_f8_few"),
-    ("mul(100)", "k_f8_mid"), ("mul(9000, F16, 4096, 1024)", "k_f8_tile"),
+    ("mul(100, BF16, 4096, 1024)", "k_f8_mid"), ("mul(9000, F16, 4096, 1024)", "k_f8_tile"),
     ("mul(9000, F16, 4096, 1024, True)", "k_f8_tile"), ("mul(9000, F32, 4096, 1024)", "k_f8_tile"),
     ("group(4)", "k_f8_few"), ("group(70)", "k_f8_few"), ("group(9000, BF16, 4096, 1024)", "k_f8_tile"),
     ("group(9000, F32, 4096, 1024, 64, True)", "k_f8_")))

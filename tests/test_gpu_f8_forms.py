@@ -39,10 +39,11 @@ def some(rng, n):
 DENSE = (  # form, type, gated, rows, n, k
     ("FEW_LONG", BF16, False, 7, 500, 1100), ("FEW_LONG", F32, True, 16, 300, 2000), ("FEW_WIDE", F16, False, 3, 20000, 400),
     ("FEW_WIDE", F32, False, 1, 17001, 1030), ("FEW_GATED", BF16, True, 16, 17000, 390), ("MID_32", F16, False, 40, 4000, 650),
-    ("MID_64", BF16, False, 64, 1000, 3000), ("MID_64", F32, True, 64, 4100, 2000), ("MID_128", BF16, False, 1500, 6000, 400),
-    ("MID_128", F32, False, 1300, 1500, 391), ("MID_SQUARE", F32, False, 3000, 3000, 640), ("MID_SQUARE", F32, True, 2100, 2200, 520),
-    ("TILE_64", F16, False, 1300, 1500, 391), ("TILE_64", BF16, True, 1500, 6000, 400), ("TILE_64", F32, True, 1300, 1500, 391),
-    ("TILE_128", BF16, False, 2100, 2200, 520), ("TILE_128", F16, True, 4100, 4352, 400), ("TILE_128F", F32, False, 2100, 2200, 520),
+    ("MID_64", BF16, False, 2725, 285, 2293), ("MID_64", F32, True, 64, 4100, 2000), ("MID_128", BF16, False, 1300, 1500, 391),
+    ("MID_128", F32, False, 1300, 1500, 391), ("MID_SQUARE", F32, False, 1000, 3000, 650), ("MID_SQUARE", F32, True, 450, 3000, 650),
+    ("TILE_64", F16, False, 1300, 6000, 520), ("TILE_64", BF16, True, 1300, 6000, 400), ("TILE_64", F32, True, 1500, 4352, 400),
+    ("TILE_64", F32, False, 3000, 3000, 640),
+    ("TILE_128", BF16, False, 2100, 2200, 520), ("TILE_128", F16, True, 1000, 3000, 520), ("TILE_128F", F32, False, 4100, 4352, 400),
     ("TILE_128F", F32, True, 4100, 4352, 400), ("TILE_256", F16, False, 4100, 6200, 520), ("TILE_256", BF16, True, 4500, 3000, 391),
     ("TILE_256", F16, True, 2100, 6200, 391))
 
@@ -73,10 +74,10 @@ RAGGED = (700, 3, 0, 1300, 257, 900)
 GROUPED = (  # form, type, gated, experts' rows, n, k
     ("FEW_LONG", BF16, False, (3, 0, 17, 1, 5, 40) + (0,) * 94, 100, 300), ("FEW_GATED", F16, True, (9, 0, 30, 1) + (7,) * 90, 200, 520),
     ("FEW_32", F32, False, (20, 0, 45, 31, 1, 33), 300, 391), ("FEW_32", F16, True, (23,) * 70, 96, 200),
-    ("MID_32", BF16, True, (300, 2, 500), 384, 272), ("TILE_64", BF16, True, RAGGED, 1500, 520),
+    ("MID_32", BF16, True, (300, 2, 500), 384, 272), ("TILE_64", BF16, True, (300, 3, 0, 500, 67, 200), 1500, 520),
     ("TILE_64", F32, True, RAGGED, 3000, 520), ("TILE_128", F16, False, (2000, 1, 1500, 0, 40), 2000, 400),
     ("TILE_128F", F32, True, (2000, 1, 1500, 0, 40), 2000, 400), ("TILE_64", BF16, False, (60, 0, 90) * 40, 700, 300),
-    ("TILE_256", BF16, True, RAGGED, 1500, 1000), ("TILE_256", F16, False, RAGGED, 8200, 520))
+    ("TILE_256", BF16, True, RAGGED, 1500, 1000), ("TILE_256", F16, False, RAGGED, 6200, 520))
 
 
 @pytest.mark.parametrize("gather", (False, True))
