@@ -32,6 +32,8 @@ __device__ static inline float f8_quotient(float x, float s, float r)
  * channels of a scale are 32 (fp32) or 16 lanes.  Two rows a wave, whose loads are in
  * flight together, where that leaves 2048 workgroups (28 -> 24 us for 8192 x 4096 bf16, 4.2 TB/s;
  * fp32 33 us, 5.1 TB/s); 16 rows of 4096 take 3.2 us, the launch and one load's latency.
+ * Stores that pass the caches took 22 us, and the product after them 3 us longer (8192 rows by
+ * 4096 x 1024).
  */
 template <int TY, int R>
 __global__ __launch_bounds__(F8_ROW_THREADS) void k_f8_quantize(
