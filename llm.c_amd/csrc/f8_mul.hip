@@ -393,7 +393,7 @@ __device__ static inline void f8_finish(const f8_mul_args &A, const f8_rows_of &
  * found in LDS, a step after the tile's start (98 -> 95 us, 8192 rows by 8192 x 1024
  * gated; two small workgroups a unit cover each other's borders by themselves).
  *
- * 8192 rows by 28672 x 4096 gated, bf16: 875 to 895 us, 2150 to 2200 TFLOP/s, of the
+ * 8192 rows by 28672 x 4096 gated, bf16: 868 to 905 us, 2120 to 2220 TFLOP/s, of the
  * 2600 that a library's product of codes alone reaches; the matrix cores work in 51 % of
  * the cycles, at 1.9 to 2 GHz, which is what the power allows: without any loads
  * 2500 to 2900, products and scalings of registers alone 3600 (4400 with all data the same).
