@@ -1,0 +1,68 @@
+"""How exact the 8-bit floating-point products (hip_f8.h) are: what the header states,
+where other tests' inputs do not reach it.
+
+Sums.  A block's 128 products are exact in fp32, their sum is off by 127 roundings of
+2^-24 of the block's size, size = sum |x w|: below 2^-17 of it.  The product of two scales
+is one rounding, joining the accumulator one more of at most size 2^-24 for each of the
+(k + 127) / 128 blocks (partial sums of blocks that are added up at the end take no more).
+With one more for what is of second order, E = 2^-17 + (k / 128 + 3) 2^-24.  16-bit outputs
+have 2^-10 on top, from the matrix cores' cutting of each of eight products at 2^-13 of the
+largest one's power of two.
+"""
+import numpy as np
+import pytest
+
+import f8_ref as ref
+import hipf8
+from f8_ref import BF16, BLOCK, F16, F32, Dev, wide
+from test_f8_plan import form
+from test_gpu_f8 import dev  # noqa: F401  (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def E(ty, k):
+    return 2.0 ** -17 + (k / BLOCK + 3) * 2.0 ** -24 + (0 if ty == F32 else 2.0 ** -10)
+
+
+def rows_on(dev, codes, scale):  # noqa: F811
+    n, k = codes.shape
+    room = np.full((n, -(-k // 16) * 16), 0x7f, np.uint8)
+    room[:, :k] = codes
+    return hipf8.Rows(dev.up(room), room.shape[1], dev.up(scale.astype(np.float32)), n, n, k)
+
+
+def mat_on(dev, codes, scale, count=1):  # noqa: F811
+    """Matrices that are all the same."""
+    n, k = codes.shape
+    room = np.full((n, -(-k // 16) * 16), 0x7f, np.uint8)
+    room[:, :k] = codes
+    return hipf8.Mat(dev.up(room), room.shape[1], dev.up(scale.astype(np.float32)), ref.blocks(k), n, k, count, 0, 0)
+
+
+@pytest.mark.parametrize("ty", (F32, F16, BF16))
+@pytest.mark.parametrize("rows,n,experts,name", ((3, 40, 0, "FEW_LONG"), (40, 64, 0, "MID_64"), (40, 64, 2, "FEW_32")))
+def test_a_million_channels_of_one_sign(dev, ty, rows, n, experts, name):  # noqa: F811
+    """Blocks that are all the same: an accumulator's roundings go the same way over a whole
+    power of two, which is the most that they can be."""
+    k = 1 << 20
+    assert form(ty, rows, n, k, experts=experts) == name
+    rng = np.random.default_rng(rows + experts)
+    xc, wc = (ref.codes_of(np.abs(rng.standard_normal((m, BLOCK))) * 112 + 16) for m in (rows, n))
+    sx = (1 + rng.random(rows)).astype(np.float32) * np.float32(2.0 ** -16)
+    sw = (1 + rng.random(ref.blocks(n))).astype(np.float32) * np.float32(2.0 ** -19)
+    X = rows_on(dev, np.tile(xc, k // BLOCK), np.tile(sx, (k // BLOCK, 1)))
+    W = mat_on(dev, np.tile(wc, k // BLOCK), np.repeat(sw[:, None], k // BLOCK, 1), max(1, experts))
+    stride = wide(n, ty)
+    d_o = dev.up(np.zeros((rows, stride), ref.np_dtype(ty)))
+    if experts:
+        start = np.linspace(0, rows, experts + 1).astype(np.int32)
+        hipf8.group_mul(X, None, dev.up(start), rows, W, None, ty, d_o, stride)
+    else:
+        hipf8.mul(X, W, None, ty, d_o, stride)
+    got = ref.from_type(dev.get(d_o, (rows, stride), ref.np_dtype(ty)), ty)[:, :n]
+    scale = sx.astype(np.float64)[:, None] * np.repeat(sw.astype(np.float64), BLOCK)[:n]
+    want = ref.VALUES[xc] @ ref.VALUES[wc].T * scale * (k // BLOCK)
+    off = np.abs(got - want) / want
+    print(f"off by 2^{np.log2(off.max()):.2f}")
+    assert np.all(off <= E(ty, k) + ref.HALF_STEP[ty] * (1 + E(ty, k)))
