@@ -66,3 +66,24 @@ def test_a_million_channels_of_one_sign(dev, ty, rows, n, experts, name):  # noq
     off = np.abs(got - want) / want
     print(f"off by 2^{np.log2(off.max()):.2f}")
     assert np.all(off <= E(ty, k) + ref.HALF_STEP[ty] * (1 + E(ty, k)))
+
+
+@pytest.mark.parametrize("ty", (F32, BF16))
+@pytest.mark.parametrize("rows,n,k", ((3, 40, 300), (40, 200, 300), (700, 1500, 300)))
+def test_products_of_scales_below_the_normal_numbers(dev, ty, rows, n, k):  # noqa: F811
+    """They are rounded to multiples of 2^-149: off by half of one times the codes' size more,
+    and so is an output."""
+    rng = np.random.default_rng(rows)
+    xc, wc = (ref.random_codes(rng, (m, k)) for m in (rows, n))
+    sx = ((1 + rng.random((ref.blocks(k), rows))) * 2.0 ** -90).astype(np.float32)
+    sw = ((1 + rng.random((ref.blocks(n), ref.blocks(k)))) * 2.0 ** -50).astype(np.float32)
+    stride = wide(n, ty)
+    d_o = dev.up(np.zeros((rows, stride), ref.np_dtype(ty)))
+    hipf8.mul(rows_on(dev, xc, sx), mat_on(dev, wc, sw), None, ty, d_o, stride)
+    got = ref.from_type(dev.get(d_o, (rows, stride), ref.np_dtype(ty)), ty)[:, :n]
+    x, w = ref.rows_of(xc, sx), ref.mat_of(wc, sw)
+    want, size = x @ w.T, np.abs(x) @ np.abs(w).T
+    codes = np.abs(ref.VALUES[xc]) @ np.abs(ref.VALUES[wc]).T
+    tol = size * E(ty, k) + codes * 2.0 ** -150 + 2.0 ** -149
+    assert np.all(np.abs(got - want) <= tol * (1 + ref.HALF_STEP[ty]) + np.abs(want) * ref.HALF_STEP[ty])
+    assert np.abs(want).max() > 2.0 ** -122  # most of them are normal numbers
