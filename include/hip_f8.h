@@ -95,11 +95,11 @@ int hip_f8_quantize_dev(int type, const void *x, size_t x_stride, const hip_f8_r
 
 /*
  * out = X W^T (+ add), or with `up` (of W's n, k and count; else NULL)
- * out = silu(X W^T) * (X up^T), silu(a) = a / (1 + exp(-a)): X->rows rows of W->n
- * values, out_stride values apart; W->count is 1.  add: rows of the same type,
- * add_stride values apart, or one row for all (add_stride 0), or NULL; with `up` it
- * is NULL.  add == out is allowed with equal strides.  out and add are 16-byte
- * aligned, rows a multiple of 16 bytes apart.
+ * out = silu(X W^T) * (X up^T), silu(a) = a / (1 + exp(-a)), for which 0 may stand where
+ * it is smaller than 2^-119: X->rows rows of W->n values, out_stride values apart; W->count
+ * is 1.  add: rows of the same type, add_stride values apart, or one row for all
+ * (add_stride 0), or NULL; with `up` it is NULL.  add == out is allowed with equal strides.
+ * out and add are 16-byte aligned, rows a multiple of 16 bytes apart.
  * A block's products are summed up and join the others' sum times the product of both
  * scales, in fp32; one rounding to the type at the end.  For fp32 outputs the products
  * are exact and the sums fp32's: off by (2^-17 + (k / 128 + 3) 2^-24) sum |x w| at most,

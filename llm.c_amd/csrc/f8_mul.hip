@@ -208,9 +208,9 @@ __device__ static inline void f8_turn(int turn, int n_tiles, int row_tiles, int 
 }
 
 /* silu(a) * b.  16-bit outputs take the exponential and the reciprocal as the hardware
- * has them, 2^-22 and |a| 2^-24 off in relation, far inside their rounding, and 0 where
- * silu(a) is below 2^-119 (the others' instructions for 64 outputs a lane took 4 us of each
- * tile's 60). */
+ * has them, 2^-22 and |a| 2^-24 off in relation, far inside their rounding (the others'
+ * instructions for 64 outputs a lane took 4 us of each tile's 60).  0 where silu(a) is below
+ * 2^-119: the reciprocal of more than 2^126 is, and in fp32 the exponential's infinity's. */
 template <int TY> __device__ static inline float f8_gate(float a, float b)
 {
 	if constexpr (TY == HIP_F8_F32)

@@ -87,3 +87,32 @@ def test_products_of_scales_below_the_normal_numbers(dev, ty, rows, n, k):  # no
     tol = size * E(ty, k) + codes * 2.0 ** -150 + 2.0 ** -149
     assert np.all(np.abs(got - want) <= tol * (1 + ref.HALF_STEP[ty]) + np.abs(want) * ref.HALF_STEP[ty])
     assert np.abs(want).max() > 2.0 ** -122  # most of them are normal numbers
+
+
+@pytest.mark.parametrize("ty", (F32, F16, BF16))
+@pytest.mark.parametrize("rows", (9, 400))
+def test_gates_of_any_size(dev, ty, rows):  # noqa: F811
+    """silu(a) of exact a from -130 to 130, times a b large enough that no gate's own size
+    hides what it is off by.  The exponential of a rounded a / ln 2 is |a| 2^-23 off in relation
+    and its own, the sum's and the quotient's roundings 2^-20; a silu(a) below 2^-119 may be 0."""
+    rng = np.random.default_rng(rows)
+    a = np.concatenate([[-130, -104, -89, -88.5, -87.6, -87.2, -86, 0.01, 88], rng.uniform(0, 130, rows - 9)])
+    a = a.astype(np.float32)
+    one = np.full((rows, 1), 0x38, np.uint8)
+    sign = np.where(np.arange(20) % 2, 0x38, 0xb8).astype(np.uint8)[:, None]
+    big = np.float32(2.0 ** (90 if ty != F16 else 3))
+    # row r's scale is |a[r]|, the outputs' matrix rows are -1 and 1: both signs of it
+    X = rows_on(dev, one, np.abs(a)[None])
+    W, U = mat_on(dev, sign, np.ones((1, 1))), mat_on(dev, np.full((20, 1), 0x38, np.uint8), np.full((1, 1), big))
+    d_o = dev.up(np.zeros((rows, 24), ref.np_dtype(ty)))
+    hipf8.mul(X, W, U, ty, d_o, 24)
+    got = ref.from_type(dev.get(d_o, (rows, 24), ref.np_dtype(ty)), ty)[:, :20]
+    a = np.abs(a).astype(np.float64)[:, None] * ref.VALUES[sign[:, 0]]
+    b = np.abs(a) * np.float64(big)
+    want = ref.gate(a, b)
+    tol = np.abs(want) * (ref.HALF_STEP[ty] + 2.0 ** -20 + np.abs(a) * 2.0 ** -23) + b * 2.0 ** -119
+    tol += 2.0 ** -25 if ty == F16 else 2.0 ** -140
+    fine = np.abs(got - want) <= tol
+    if ty == F16:  # 65520 and more are rounded to infinity
+        fine |= (got == np.inf) & (want + tol >= 65520)
+    assert np.all(fine)
