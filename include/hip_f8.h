@@ -22,9 +22,11 @@
  * clears nothing: every call can be captured into a HIP graph, needs no
  * workspace, and calls may overlap where none writes what another reads or
  * writes.  Memory is the caller's, on the current device.  Inputs and outputs
- * do not overlap unless a call says so.  A call whose launch would have 2^32 threads
- * or more is refused.  Results do not depend on timing: the same call gives the same
- * bits.
+ * do not overlap unless a call says so.  Of a row of inputs that ends inside 16
+ * bytes, counted from its start, the rest of them may be read too (they are aligned
+ * and in the same page); what is there does not matter.  A call whose launch would have
+ * 2^32 threads or more is refused.  Results do not depend on timing: the same call
+ * gives the same bits.
  */
 #ifndef HIP_F8_H
 #define HIP_F8_H

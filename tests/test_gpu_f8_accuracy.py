@@ -164,3 +164,39 @@ def test_sums_of_16_bit_outputs(dev, name, ty, rows, n, k, outliers):  # noqa: F
     print(f"off by {rms(got - rest) / rms(want):.2e} of the outputs, cutting at most {cut / rms(want):.2e}")
     assert rms(got - rest) <= cut + ref.HALF_STEP[ty] * rms(rest) + (2.0 ** -25 if ty == F16 else 0)
     assert cut <= 1e-4 * rms(want)
+
+
+@pytest.mark.parametrize("ty", (F32, F16, BF16))
+def test_what_follows_a_row_in_its_16_bytes_does_not_matter(dev, ty):  # noqa: F811
+    """Rows of x, y and add end inside 16 bytes, the rest of which is NaN; one row of add for all."""
+    rng = np.random.default_rng(3)
+    n = 101
+    stride = wide(n, ty)
+
+    def up(rows):
+        v = np.full((rows, stride), np.nan, np.float32)
+        v[:, :n] = rng.standard_normal((rows, n))
+        return dev.up(ref.to_type(v, ty)), ref.from_type(ref.to_type(v, ty), ty)[:, :n]
+
+    (d_x, x), (d_add, add) = up(7), up(1)
+    d_c, d_s = dev.up(np.zeros((7, 112), np.uint8)), dev.up(np.zeros((1, 7), np.float32))
+    X = hipf8.Rows(d_c, 112, d_s, 7, 7, n)
+    hipf8.quantize(ty, d_x, stride, X)
+    codes, scale = ref.quantize(x)
+    assert np.array_equal(dev.get(d_c, (7, 112), np.uint8)[:, :n], codes)
+    assert np.array_equal(dev.get(d_s, (1, 7), np.float32), scale)
+    pos, w = rng.integers(0, 7, (5, 2)).astype(np.int32), rng.random((5, 2)).astype(np.float32)
+    d_o = dev.up(np.zeros((7, stride), ref.np_dtype(ty)))
+    for d_a, a in ((d_add, add), (None, 0 * add)):
+        hipf8.combine(ty, d_x, stride, 7, dev.up(pos), dev.up(w), 5, 2, n, d_a, 0, d_o, stride)
+        got = ref.from_type(dev.get(d_o, (7, stride), ref.np_dtype(ty)), ty)[:5, :n]
+        terms = w[..., None].astype(np.float64) * x[pos]
+        want, size = a + terms.sum(1), np.abs(a) + np.abs(terms).sum(1)
+        assert np.all(np.abs(got - want) <= np.abs(want) * ref.HALF_STEP[ty] + size * 3 * 2.0 ** -23 + 2.0 ** -25)
+    wc = ref.random_codes(rng, (n, n))
+    W = mat_on(dev, wc, np.full((1, 1), 2e-4, np.float32))
+    hipf8.mul(X, W, None, ty, d_o, stride, d_add, 0)
+    got = ref.from_type(dev.get(d_o, (7, stride), ref.np_dtype(ty)), ty)[:, :n]
+    xd, wd = ref.rows_of(codes, scale), ref.mat_of(wc, np.full((1, 1), 2e-4, np.float32))
+    want, size = xd @ wd.T + add, np.abs(xd) @ np.abs(wd).T + np.abs(add)
+    assert np.all(np.abs(got - want) <= np.abs(want) * ref.HALF_STEP[ty] + size * E(ty, n) + 2.0 ** -25)
