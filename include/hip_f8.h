@@ -134,7 +134,7 @@ int hip_f8_sort_dev(const uint32_t *ids, size_t tokens, size_t topk, size_t expe
  * start[e + 1] (device, [W->count + 1], not decreasing) is row from[r] of X, or with
  * from NULL row r of X, times matrix e; with `up` gated as above.  `rows`: the rows
  * of out, at least start[W->count]; others keep what out holds.  A row whose from is
- * outside X's rows, or that has none, is NaN.
+ * outside X's rows is NaN.
  */
 int hip_f8_group_mul_dev(const hip_f8_rows *X, const int32_t *from, const int32_t *start,
                          size_t rows, const hip_f8_mat *W, const hip_f8_mat *up, int type,
