@@ -996,6 +996,16 @@ __global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles, 
  * and eight to a workgroup where the outputs alone do not fill the chip (15.5 us
  * instead of 21.5, 16 rows of 14336 to 4096), else four (18.1 instead of 23.7, the 50304),
  * and 32 outputs where the product is gated (169 instead of 176, 16 tokens in 8 experts of 14336 x 4096).
+ * Their costs were fitted to 420 calls of up to 128 rows or 40 for an expert, W from HBM; a gated
+ * call's blocks count twice.  Up to 16 rows (8 for an expert, and few workgroups) they
+ * are taken unasked, 4 % behind the fastest of all forms on average.  Where experts have 8
+ * rows on average some have many more, and with many experts workgroups of 16 rows are tens
+ * of thousands: from there on TILE is taken where its cost is 10 % below (512 rows in 64 experts
+ * of 2048 x 1024: 34 us instead of 50, 33 instead of 51 with a skewed router; 10240 fp32 rows in 1024 of
+ * 512 x 512 gated: 296 instead of 637, 282 instead of 636).  FEW_LONG up to 128 rows where it costs no more than
+ * 15 % below others (24 rows of 4096 x 4096: 10.6 instead of 15.2 us, 48 of 1024 x 4096: 8.7 instead of
+ * 11.7).  In 843 calls of more than those 16 and 8 rows, even and skewed, 5 % behind the
+ * fastest on average, in nine of ten at most 17 %.
  */
 #define F8_FORMS(X)                                                                    \
 	/*  form        kernel   16-bit fp32  NA NB WN WT KS STAGES STREAM */               \
@@ -1029,10 +1039,10 @@ static const struct {
 	} us[2];
 } forms[FORMS] = {
 	/* in F8_FORMS' order */
-	{16, 16, 512, {}},
-	{16, 16, 256, {}},
-	{16, 32, 256, {}},
-	{32, 32, 256, {}},
+	{16, 16, 512, {{2.9f, .035f, .65f, .077f}, {2.9f, .041f, .82f, .062f}}},
+	{16, 16, 256, {{0, .081f, .66f, .03f}, {0, .126f, .61f, .075f}}},
+	{16, 32, 256, {{0, .114f, 1.11f, .084f}, {.46f, .113f, 1.49f, .102f}}},
+	{32, 32, 256, {{0, .2f, 1.11f, .165f}, {.66f, .158f, 1.13f, .18f}}},
 	{32, 128, 512, {{3.2f, .17f, 3.3f, .42f}, {2.5f, .36f, 4.4f, .52f}}},
 	{64, 64, 512, {{4.6f, .13f, 5.f, .27f}, {2.9f, .29f, 5.f, .39f}}},
 	{64, 128, 512, {{2.8f, .27f, 5.4f, .56f}, {2.2f, .56f, 6.7f, .68f}}},
@@ -1061,7 +1071,9 @@ static size_t n_tiles_of(const f8_mul_args *a, int form)
 static float cost_of(const f8_mul_args *a, int form, int fp32)
 {
 	const float bt = forms[form].bt, rows = a->rows, busy = rows < a->count ? rows : a->count;
-	const float blocks = (a->k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK;
+	const bool few = form < MID_32;
+	/* a workgroup's outputs are of one matrix (FEW: of both, which is twice the loads) */
+	const float blocks = (a->k + HIP_F8_BLOCK - 1) / HIP_F8_BLOCK * (few && a->w[1] ? 2 : 1);
 	float tiles = ceilf(rows / bt);
 	if (a->start) {
 		/* between experts that have the same rows and some whose last tile is half full */
@@ -1070,7 +1082,7 @@ static float cost_of(const f8_mul_args *a, int form, int fp32)
 	}
 	float n = tiles * n_tiles_of(a, form) / F8_CUS;
 	n = n < 6 ? ceilf(n) : n;
-	const float less = a->w[1] ? .7f : 1; /* half the outputs to store */
+	const float less = a->w[1] && !few ? .7f : 1; /* half the outputs to store */
 	const auto &c = forms[form].us[fp32];
 	return less * c.fixed + c.block * blocks + (n - 1) * (less * c.more_fixed + c.more_block * blocks);
 }
@@ -1080,28 +1092,37 @@ void f8_mul_plan(const f8_mul_args *a, f8_plan *p)
 	const size_t rows = (size_t)a->rows;
 	const size_t per = a->start ? (rows + (size_t)a->count - 1) / (size_t)a->count : rows;
 	const int fp32 = p->type == HIP_F8_F32;
-	/* the rows of experts differ: those of 8 on average hardly ever are more than 16 */
+	/* of few rows' forms the one that was measured there, or none; against others where there
+	 * are enough workgroups that one of them may be much faster */
+	int few = FORMS, first = MID_32;
 	if (per <= (a->start ? 8 : 16)) {
 		const size_t wide = row_tiles_of(a, 16) * (((size_t)a->n + 31) / 32);
-		p->form = wide < 512 ? FEW_LONG : a->w[1] ? FEW_GATED : FEW_WIDE;
+		few = wide < 512 ? FEW_LONG : a->w[1] ? FEW_GATED : FEW_WIDE;
+		first = a->start && wide >= 2048 ? TILE_64 : FORMS;
 	} else if (a->start && per <= 24) {
-		p->form = FEW_32;
-	} else {
-		float best = 0;
-		for (int f = MID_32; f < FORMS; f++) {
-			if (forms[f].us[fp32].block == 0)
-				continue;
-			/* its rows' distances from X's first are 32 bits; it asks for the next tile two
-			 * steps ahead */
-			if (f == TILE_256 &&
-			    (a->k <= 2 * HIP_F8_BLOCK ||
-			     (a->from && (size_t)a->x_rows * (size_t)a->x_stride >= ((size_t)1 << 32) - F8_MAX_K)))
-				continue;
-			const float us = cost_of(a, f, fp32);
-			if (best == 0 || us < best) {
-				best = us;
-				p->form = f;
-			}
+		few = FEW_32;
+		first = TILE_64;
+	} else if (!a->start && per <= 128) {
+		few = FEW_LONG;
+	}
+	float best = 0;
+	if (few < FORMS) {
+		p->form = few;
+		best = cost_of(a, few, fp32) * (a->start ? .9f : 1.15f);
+	}
+	for (int f = first; f < FORMS; f++) {
+		if (forms[f].us[fp32].block == 0)
+			continue;
+		/* its rows' distances from X's first are 32 bits; it asks for the next tile two
+		 * steps ahead */
+		if (f == TILE_256 &&
+		    (a->k <= 2 * HIP_F8_BLOCK ||
+		     (a->from && (size_t)a->x_rows * (size_t)a->x_stride >= ((size_t)1 << 32) - F8_MAX_K)))
+			continue;
+		const float us = cost_of(a, f, fp32);
+		if (best == 0 || us < best) {
+			best = us;
+			p->form = f;
 		}
 	}
 	p->threads = forms[p->form].threads;

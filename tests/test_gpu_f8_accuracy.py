@@ -41,7 +41,7 @@ def mat_on(dev, codes, scale, count=1):  # noqa: F811
 
 
 @pytest.mark.parametrize("ty", (F32, F16, BF16))
-@pytest.mark.parametrize("rows,n,experts,name", ((3, 40, 0, "FEW_LONG"), (40, 64, 0, "MID_64"), (40, 64, 2, "FEW_32")))
+@pytest.mark.parametrize("rows,n,experts,name", ((3, 40, 0, "FEW_LONG"), (150, 64, 0, "MID_64"), (40, 64, 2, "FEW_32")))
 def test_a_million_channels_of_one_sign(dev, ty, rows, n, experts, name):  # noqa: F811
     """Blocks that are all the same: an accumulator's roundings go the same way over a whole
     power of two, which is the most that they can be."""
