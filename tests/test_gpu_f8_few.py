@@ -19,8 +19,8 @@ def test_dense_few(dev, ty, gated, rows, n, k):  # noqa: F811
 
 @pytest.mark.parametrize("gather", (False, True))
 @pytest.mark.parametrize("ty,gated,counts,n,k", (
-    (F32, False, (7, 0, 12, 1, 3) * 60, 1500, 300), (BF16, True, (7, 0, 12, 1, 3) * 60, 1500, 300),
-    (F32, True, (3, 0, 0, 40, 1) * 60, 2000, 520), (F16, False, (10, 0, 33, 9) * 40, 700, 391),
-    (BF16, False, (0,) * 200 + (1, 300, 0, 70) + (2,) * 100, 2000, 257)))
+    (F32, False, (7, 0, 12, 1, 3) * 30, 700, 257), (BF16, True, (7, 0, 12, 1, 3) * 30, 1000, 257),
+    (F32, True, (3, 0, 0, 40, 1) * 20, 1000, 257), (F16, False, (10, 0, 33, 9) * 20, 700, 391),
+    (BF16, False, (0,) * 60 + (1, 300, 0, 70) + (2,) * 30, 1000, 257)))
 def test_grouped_tiles(dev, ty, gated, counts, n, k, gather):  # noqa: F811
     forms.test_grouped(dev, "TILE_64", ty, gated, counts, n, k, gather)
