@@ -971,21 +971,34 @@ __global__ __launch_bounds__(64 * NW) void k_f8_few(f8_mul_args A, int n_tiles, 
  * The forms, and what a call costs in each.  With `n` of a form's workgroups to each of
  * the 256 compute units, rounded up where they are few, a call takes
  *   fixed + block * blocks + (n - 1) (more_fixed + more_block * blocks)
- * microseconds, blocks of 128 channels; the first of them alone on its unit, later ones
- * next to others.  The four were fitted to 420 calls, dense and grouped (16 to 8192 rows, 1024 to
- * 14336 outputs, 400 to 5120 channels, up to 64 experts), timed in every form.  The form with the
- * smallest sum took 2 % longer than the fastest on average for 16 bits and 1 % for fp32, and 2 and
- * 0.2 % in 160 other calls; in nine of ten at most 8 %.  Sizes alone would not do:
- * calls of many rounds cost the same as larger tiles' calls of few.
+ * microseconds and 5 that all forms share, blocks of 128 channels; the first of them alone on
+ * its unit, later ones next to others.  The four are there to choose by: they were fitted
+ * to 420 calls, dense and grouped (16 to 8192 rows, 1024 to 14336 outputs, 400 to 5120 channels,
+ * up to 64 experts), timed in every form, of which those within twice the fastest counted.
+ * The form with the smallest sum took 2 % longer than the fastest on average, 16 bits and fp32, and in
+ * nine of ten calls at most 8 %, in these and in 240 others.  What a form takes far
+ * from where it is chosen they do not say: dense calls of whole rounds, measured and (by the
+ * formula, with the 5),
  *
- *   4096 channels, us by workgroups     256   512   768  1536     (fp32  256   512   768  1536)
- *   MID   32 x 128, 2 groups           12.7  22.6  33.2  62.8           18.3  32.9  48.2  94.0
- *   MID   64 x 64, 4 groups            12.6  22.5  32.3  62.3           16.7  29.3  44.5  86.1
- *   MID   64 x 128, 2 groups           17.0  32.0  47.0  90.9           25.6  47.9  70.7   138
- *   MID  128 x 128, 2 groups              -     -     -     -           39.4  71.8     -     -
- *   TILE  64 x 128                     24.3  31.3  42.1  80.2           35.2  47.6  63.9   122
- *   TILE 128 x 128                     28.4  45.9  67.7   131           53.4  76.2   115   225
- *   TILE 256 x 256                     78.7   147   222   431              -     -     -     -
+ *   4096 channels, us by workgroups      256          512           1024          2048
+ *   16 bits  MID   32 x 128, 2 groups   13.1 (13.6)   23.3 (30.4)   43.5 (63.9)   84.2 (131)
+ *            MID   64 x 64, 4 groups    12.5 (13.8)   22.9 (27.4)   42.4 (54.7)   82.2 (109)
+ *            MID   64 x 128, 2 groups   17.6 (16.4)   31.5 (39.8)   59.8 (86.4)    118 (180)
+ *            TILE  64 x 128             24.4 (22.9)   31.4 (37.3)   56.4 (66.3)    105 (124)
+ *            TILE 128 x 128             28.2 (24.5)   46.1 (48.6)   87.6 (96.9)    171 (193)
+ *            TILE 256 x 256             74.5 (65.4)    141 (121)     287 (232)     554 (454)
+ *   fp32     MID   32 x 128, 2 groups   17.8 (19.0)   32.9 (40.1)   63.3 (82.1)    124 (166)
+ *            MID   64 x 64, 4 groups    17.0 (17.2)   29.8 (34.7)   56.6 (69.6)    111 (140)
+ *            MID   64 x 128, 2 groups   25.4 (25.1)   47.5 (53.6)   92.7 (110)     180 (224)
+ *            MID  128 x 128, 2 groups   39.2 (37.6)   77.3 (80.0)    152 (165)     296 (334)
+ *            TILE  64 x 128             35.2 (29.0)   47.2 (50.8)   82.9 (94.4)    158 (181)
+ *            TILE 128 x 128             53.7 (46.2)   76.6 (82.8)    145 (156)     281 (302)
+ *
+ * TILE 256 x 256 takes 63 to 64 for 128 to 192 workgroups: with all units at work the clock
+ * falls.  By the rows of 4096 x 4096, 16 bits: 2304 rows 62.9 in it and 61.2 in TILE 128 x 128,
+ * 2816 63.4 and 63.4, 3584 67.9 and 82.2, 4096 75.3 and 87.1, 5120 (its 320 workgroups are two
+ * rounds) 122 and 110; it is taken in all of these.  Sizes alone would not do: calls of many
+ * rounds cost the same as larger tiles' calls of few.
  *
  * TILE's 64 x 128 by four waves with two stages, three workgroups a compute unit: eight
  * waves with three stages, two workgroups, took 46.3 and 86.7 us for 768 and 1536 (fp32
